@@ -83,12 +83,20 @@ def lib():
             "hsg_gemm": [P, I, I, P, P, I, I, P, P, P, I, I, P, P],
             "hsg_gemm_f32_noalloc": [P, I, I, P, I, P, P, P, I, I, P, P],
             "hsg_check_bounded_wait": [I, C.POINTER(C.c_double)],
+            # draft scoring: one argument struct each (hs_guard_b200.drafts packs it)
+            "hsg_advance_tables": [C.c_char_p],
+            "hsg_plan_tree": [C.c_char_p],
+            "hsg_norm_rope": [C.c_char_p],
+            "hsg_tree_attention": [C.c_char_p],
+            "hsg_store_rows": [C.c_char_p],
         }
         for name, args in sig.items():
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, C.c_int
         L.hsg_slot_state_bytes.argtypes, L.hsg_slot_state_bytes.restype = [P], C.c_size_t
         L.hsg_stream.argtypes, L.hsg_stream.restype = [P], P
+        L.hsg_tree_attention_workspace.argtypes, L.hsg_tree_attention_workspace.restype = [I], C.c_size_t
+        L.hsg_device_error_text.argtypes, L.hsg_device_error_text.restype = [I], C.c_char_p
         L.hsg_last_error.argtypes, L.hsg_last_error.restype = [], C.c_char_p
         L.hsg_version.argtypes, L.hsg_version.restype = [], C.c_char_p
         _LIB = L

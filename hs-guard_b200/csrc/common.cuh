@@ -44,6 +44,8 @@ enum : int {
   ERR_BAD_SLOT = 3,        // slot index outside [0, max_slots]
   ERR_BAD_TOKEN = 4,       // token id outside the vocabulary
   ERR_BAD_LEN = 5,         // row length outside [0, lb]
+  ERR_BAD_PAGE = 6,        // block-table entry outside the cache's pages
+  ERR_BAD_PARENT = 7,      // parent link of a drafted token that is not an earlier token of its tree
 };
 
 __device__ __forceinline__ void set_error(int* err, int code) {

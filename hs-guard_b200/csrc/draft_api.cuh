@@ -1,0 +1,200 @@
+// C entry points of draft scoring (hsg_advance_tables, hsg_plan_tree, hsg_norm_rope, hsg_tree_attention,
+// hsg_store_rows): argument checks and launches. Part of the one translation unit of the library.
+#pragma once
+#include "draft_attn.cuh"
+#include "draft_rows.cuh"
+#include "draft_tables.cuh"
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// `bytes`-wide elements: strides that keep every row on a 16-byte boundary
+bool rows16(int64_t a, int64_t b, int bytes) { return (a * bytes) % 16 == 0 && (b * bytes) % 16 == 0; }
+bool head_dim_ok(int d) { return d == 64 || d == 128 || d == 256; }
+
+int check_cache(const hsg_page_cache& c, int heads, int dim) {
+  if (!c.k || !c.v) return fail(HSG_ERR_INVALID, "the cache's k or v is NULL");
+  if (c.pages < 1 || c.page_size < 8 || c.page_size % 8)
+    return fail(HSG_ERR_INVALID, "a cache has at least one page of a multiple of 8 tokens, got %d of %d", c.pages,
+                c.page_size);
+  if ((int64_t)c.pages * c.page_size > INT32_MAX)
+    return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit slots", c.pages, c.page_size);
+  if (!aligned16(c.k) || !aligned16(c.v) || c.page_stride % 8 || c.token_stride % 8 || c.head_stride % 8 ||
+      c.page_stride < 0 || c.token_stride < 0 || c.head_stride < 0)
+    return fail(HSG_ERR_INVALID, "cache rows must lie on 16-byte boundaries, at strides that are not negative");
+  if ((c.page_size > 1 && c.token_stride < dim) || (heads > 1 && c.head_stride < dim))
+    return fail(HSG_ERR_INVALID, "cache rows of %d elements overlap (token stride %lld, head stride %lld)", dim,
+                (long long)c.token_stride, (long long)c.head_stride);
+  return HSG_OK;
+}
+
+PageCache page_cache(const hsg_page_cache& c) {
+  return PageCache{c.k, c.v, c.page_stride, c.token_stride, c.head_stride, c.pages, c.page_size};
+}
+
+static_assert(DT_MAX_ROWS == HSG_MAX_TABLE_ROWS, "the header states the kernel's limit");
+
+#define DRAFT_ARGS(a)                                                                                  \
+  do {                                                                                                 \
+    if (!(a)) return fail(HSG_ERR_INVALID, "args is NULL");                                            \
+    if ((a)->size != (int64_t)sizeof(*(a)))                                                            \
+      return fail(HSG_ERR_INVALID, "args has %lld bytes, this library expects %lld", (long long)(a)->size, \
+                  (long long)sizeof(*(a)));                                                            \
+  } while (0)
+
+template <int D, typename TI, typename TO>
+int launch_norm(const DraftNormArgs& n, cudaStream_t st) {
+  draft_norm_kernel<D, TI, TO><<<n.tokens, DN_THREADS, 0, st>>>(n);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+template <int D, typename TI>
+int launch_norm_out(const DraftNormArgs& n, int out, cudaStream_t st) {
+  return out == HSG_DT_F16 ? launch_norm<D, TI, __half>(n, st) : launch_norm<D, TI, __nv_bfloat16>(n, st);
+}
+template <int D>
+int launch_norm_in(const DraftNormArgs& n, int in, int out, cudaStream_t st) {
+  if (in == HSG_DT_F32) return launch_norm_out<D, float>(n, out, st);
+  return in == HSG_DT_F16 ? launch_norm_out<D, __half>(n, out, st) : launch_norm_out<D, __nv_bfloat16>(n, out, st);
+}
+
+template <int D, typename T>
+int launch_draft_attn(const DraftAttnArgs& d, cudaStream_t st) {
+  const int64_t jobs = (int64_t)d.tokens * d.hq, per = DA_THREADS / 32;
+  draft_attn_simple_kernel<D, T><<<(unsigned)((jobs + per - 1) / per), DA_THREADS, 0, st>>>(d);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+template <typename T>
+int launch_draft_attn_dim(const DraftAttnArgs& d, int dim, cudaStream_t st) {
+  return dim == 64 ? launch_draft_attn<64, T>(d, st)
+                   : dim == 128 ? launch_draft_attn<128, T>(d, st) : launch_draft_attn<256, T>(d, st);
+}
+
+}  // namespace
+
+extern "C" int hsg_advance_tables(const hsg_tables_args* a) {
+  DRAFT_ARGS(a);
+  if (a->rows < 0 || a->rows > DT_MAX_ROWS)
+    return fail(HSG_ERR_INVALID, "rows must be in [0, %d], got %d", DT_MAX_ROWS, a->rows);
+  if (a->width < 1 || a->ring_size < 1 || a->page_size < 1 || a->capacity < 0 || a->table_stride < a->width)
+    return fail(HSG_ERR_INVALID, "bad table shape (width %d, stride %lld, ring %d, page %d, capacity %d)", a->width,
+                (long long)a->table_stride, a->ring_size, a->page_size, a->capacity);
+  if ((int64_t)a->width * a->page_size > INT32_MAX || (int64_t)a->ring_size * a->page_size > INT32_MAX)
+    return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit positions or slots",
+                std::max(a->width, a->ring_size), a->page_size);
+  if (!a->ring || !a->counters || !a->counters_out || !a->cu ||
+      (a->rows && (!a->lens || !a->delta || !a->table || !a->lens_out)) ||
+      (a->capacity && (!a->slots || !a->token_rows || !a->positions)))
+    return fail(HSG_ERR_INVALID, "NULL argument");
+  if ((a->rows && a->lens_out == a->lens) || a->counters_out == a->counters)
+    return fail(HSG_ERR_INVALID, "lens_out and counters_out must not be the inputs");
+  DraftTablesArgs t{a->lens, a->delta, a->table, a->table_stride, a->ring, a->counters, a->rows, a->width,
+                    a->ring_size, a->page_size, a->lens_out, a->counters_out, a->cu, a->slots, a->token_rows,
+                    a->positions, a->capacity, a->err};
+  draft_tables_kernel<<<1, DT_THREADS, 0, (cudaStream_t)a->stream>>>(t);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+
+extern "C" int hsg_plan_tree(const hsg_tree_args* a) {
+  DRAFT_ARGS(a);
+  if (a->rows < 0 || a->tokens < 0 || a->words < 1 || a->words > HSG_MAX_TREE / 32)
+    return fail(HSG_ERR_INVALID, "bad tree shape (rows %d, tokens %d, words %d)", a->rows, a->tokens, a->words);
+  if (a->rows == 0 || a->tokens == 0) return HSG_OK;
+  if (!a->parents || !a->cu || !a->lens || !a->positions || !a->mask) return fail(HSG_ERR_INVALID, "NULL argument");
+  DraftTreeArgs t{a->parents, a->cu, a->lens, a->rows, a->tokens, a->words, a->positions, a->mask, a->err};
+  draft_tree_kernel<<<a->rows, DTREE_THREADS, 0, (cudaStream_t)a->stream>>>(t);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+
+extern "C" int hsg_norm_rope(const hsg_norm_rope_args* a) {
+  DRAFT_ARGS(a);
+  if (a->tokens < 0 || a->hq < 1 || a->hkv < 1) return fail(HSG_ERR_INVALID, "bad shape (tokens %d, heads %d / %d)",
+                                                            a->tokens, a->hq, a->hkv);
+  if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
+  if (a->rot < 16 || a->rot > a->dim || a->rot % 16)
+    return fail(HSG_ERR_INVALID, "the rotated dims must be a multiple of 16 up to head_dim, got %d", a->rot);
+  if (a->in_dtype < HSG_DT_F32 || a->in_dtype > HSG_DT_BF16 || (a->out_dtype != HSG_DT_F16 && a->out_dtype != HSG_DT_BF16))
+    return fail(HSG_ERR_INVALID, "inputs are fp32, fp16 or bf16, outputs fp16 or bf16");
+  if (a->tokens == 0) return HSG_OK;
+  if (!a->q || !a->k || !a->v || !a->q_weight || !a->k_weight || !a->inv_freq || !a->positions || !a->q_out)
+    return fail(HSG_ERR_INVALID, "NULL argument");
+  if (!a->slots && (!a->k_out || !a->v_out)) return fail(HSG_ERR_INVALID, "k_out and v_out, or slots, are needed");
+  const int bytes = a->in_dtype == HSG_DT_F32 ? 4 : 2;
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) ||
+      !rows16(a->q_token_stride, a->q_head_stride, bytes) || !rows16(a->k_token_stride, a->k_head_stride, bytes) ||
+      !rows16(a->v_token_stride, a->v_head_stride, bytes) || (!a->slots && (!aligned16(a->k_out) || !aligned16(a->v_out))))
+    return fail(HSG_ERR_INVALID, "q, k and v rows must lie on 16-byte boundaries");
+  int rc;
+  DraftNormArgs n{a->q, a->k, a->v, a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride,
+                  a->v_token_stride, a->v_head_stride, a->q_weight, a->k_weight, a->inv_freq, a->positions, a->tokens,
+                  a->hq, a->hkv, a->rot, a->eps, a->q_out, a->k_out, a->v_out, a->slots, PageCache{}, a->err};
+  if (a->slots) {
+    if ((rc = check_cache(a->cache, a->hkv, a->dim)) != HSG_OK) return rc;
+    n.cache = page_cache(a->cache);
+  }
+  cudaStream_t st = (cudaStream_t)a->stream;
+  if (a->dim == 64) return launch_norm_in<64>(n, a->in_dtype, a->out_dtype, st);
+  if (a->dim == 128) return launch_norm_in<128>(n, a->in_dtype, a->out_dtype, st);
+  return launch_norm_in<256>(n, a->in_dtype, a->out_dtype, st);
+}
+
+extern "C" size_t hsg_tree_attention_workspace(int head_dim) {
+  (void)head_dim;
+  return 0;
+}
+
+extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
+  DRAFT_ARGS(a);
+  if (a->rows < 0 || a->tokens < 0 || a->hq < 1 || a->hkv < 1 || a->hq % a->hkv)
+    return fail(HSG_ERR_INVALID, "bad shape (rows %d, tokens %d, heads %d / %d)", a->rows, a->tokens, a->hq, a->hkv);
+  if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
+  if (a->dtype != HSG_DT_F16 && a->dtype != HSG_DT_BF16) return fail(HSG_ERR_INVALID, "dtype must be fp16 or bf16");
+  if (a->max_tree < 1 || a->max_tree > HSG_MAX_TREE)
+    return fail(HSG_ERR_INVALID, "max_tree must be in [1, %d], got %d", HSG_MAX_TREE, a->max_tree);
+  if (a->mask && (int64_t)a->words * 32 < a->max_tree)
+    return fail(HSG_ERR_INVALID, "%d mask words hold fewer than max_tree = %d bits", a->words, a->max_tree);
+  if (a->window < 0) return fail(HSG_ERR_INVALID, "window must not be negative, got %d", a->window);
+  if (a->rows == 0 || a->tokens == 0) return HSG_OK;
+  if (!a->q || !a->k || !a->v || !a->table || !a->lens || !a->cu || !a->out) return fail(HSG_ERR_INVALID, "NULL argument");
+  if (a->width < 1 || a->table_stride < a->width)
+    return fail(HSG_ERR_INVALID, "bad table shape (width %d, stride %lld)", a->width, (long long)a->table_stride);
+  int rc;
+  if ((rc = check_cache(a->cache, a->hkv, a->dim)) != HSG_OK) return rc;
+  if ((int64_t)a->width * a->cache.page_size > INT32_MAX)
+    return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit positions", a->width, a->cache.page_size);
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||
+      !rows16(a->q_token_stride, a->q_head_stride, 2) || !rows16(a->k_token_stride, a->k_head_stride, 2) ||
+      !rows16(a->v_token_stride, a->v_head_stride, 2))
+    return fail(HSG_ERR_INVALID, "q, k and v rows must lie on 16-byte boundaries");
+  DraftAttnArgs d{a->q, a->k, a->v, a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride,
+                  a->v_token_stride, a->v_head_stride, page_cache(a->cache), a->table, a->table_stride, a->lens, a->cu,
+                  a->positions, a->mask, a->rows, a->width, a->tokens, a->words, a->max_tree, a->hq, a->hkv, a->window,
+                  a->scale, a->out, a->lse, a->err};
+  cudaStream_t st = (cudaStream_t)a->stream;
+  return a->dtype == HSG_DT_F16 ? launch_draft_attn_dim<__half>(d, a->dim, st)
+                                : launch_draft_attn_dim<__nv_bfloat16>(d, a->dim, st);
+}
+
+extern "C" int hsg_store_rows(const hsg_store_args* a) {
+  DRAFT_ARGS(a);
+  if (a->count < 0 || a->rows < 0 || a->heads < 1) return fail(HSG_ERR_INVALID, "bad shape (count %d, rows %d, heads %d)",
+                                                               a->count, a->rows, a->heads);
+  if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
+  if (a->count == 0) return HSG_OK;
+  if (!a->k || !a->v || !a->slots) return fail(HSG_ERR_INVALID, "NULL argument");
+  if (!aligned16(a->k) || !aligned16(a->v) || !rows16(a->k_token_stride, a->k_head_stride, 2) ||
+      !rows16(a->v_token_stride, a->v_head_stride, 2))
+    return fail(HSG_ERR_INVALID, "k and v rows must lie on 16-byte boundaries");
+  int rc;
+  if ((rc = check_cache(a->cache, a->heads, a->dim)) != HSG_OK) return rc;
+  DraftStoreArgs s{a->k, a->v, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->source,
+                   a->slots, a->count, a->rows, a->heads, a->dim, page_cache(a->cache), a->err};
+  draft_store_kernel<<<a->count, DS_THREADS, 0, (cudaStream_t)a->stream>>>(s);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+
+extern "C" const char* hsg_device_error_text(int code) { return code ? device_error_text(code) : "no error"; }

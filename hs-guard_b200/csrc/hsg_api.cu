@@ -57,6 +57,8 @@ static const char* device_error_text(int code) {
     case ERR_BAD_SLOT: return "a slot index was outside [0, max_slots]";
     case ERR_BAD_TOKEN: return "a token id was outside the vocabulary";
     case ERR_BAD_LEN: return "a row length was outside [0, lb]";
+    case ERR_BAD_PAGE: return "a block-table entry was outside the cache's pages";
+    case ERR_BAD_PARENT: return "a drafted token's parent was not an earlier token of its tree";
     default: return "unknown device error";
   }
 }
@@ -1274,3 +1276,5 @@ extern "C" int hsg_gemm_f32_noalloc(const void* w, int n, int k, const float* x,
   return launch_gemm(st, w, n, k, hi, lo, m, m, mode, y, n, static_cast<__nv_bfloat16*>(act_hi),
                      static_cast<__nv_bfloat16*>(act_lo), n / 2, err, splits);
 }
+
+#include "draft_api.cuh"

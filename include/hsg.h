@@ -191,6 +191,161 @@ int hsg_gemm_f32_noalloc(const void* w, int n, int k, const float* x, int m, flo
  * the wait ended without recording it. The GPU stays usable. */
 int hsg_check_bounded_wait(int device, double* seconds);
 
+/* ---- draft scoring: trees of drafted tokens over a paged cache (no counterpart in the reference) ----
+ *
+ * A host model that drafts several continuations of a conversation has all of them attended at once, without
+ * committing any: drafted keys and values stay outside the cache until a branch is accepted. Per tick:
+ *   hsg_plan_tree        parent links -> positions and ancestor masks
+ *   hsg_norm_rope        per-head RMSNorm and rotation of q and k, v converted
+ *   hsg_tree_attention   drafted tokens over their request's cached tokens and their own ancestors
+ *   hsg_advance_tables   accepted (or withdrawn) tokens per request -> pages, slots, positions
+ *   hsg_store_rows       accepted keys and values -> the cache
+ * All pointers are device pointers, all work is queued on `stream` (cudaStream_t, NULL: the default stream) of the
+ * current device and nothing waits for it. `size` is the struct's size in bytes (checked). `err` is a device int (0 on
+ * entry) or NULL: a kernel that meets an index outside its range skips it and records the reason there
+ * (hsg_device_error_text). Element types: HSG_DT_*. Strides count elements; rows (the last dimension) are contiguous
+ * and begin on 16-byte boundaries. A call with no rows or tokens does nothing. */
+#define HSG_DT_F32 0
+#define HSG_DT_F16 1
+#define HSG_DT_BF16 2
+#define HSG_MAX_TREE 1024     /* drafted tokens of one request */
+#define HSG_MAX_TABLE_ROWS 4096
+
+/* Keys and values in `pages` pages of `page_size` tokens (a multiple of 8): element (page, token, head, d) lies at
+ * page * page_stride + token * token_stride + head * head_stride + d, in k as in v. Pages may overlap in memory as
+ * long as the tokens in use do not. */
+typedef struct hsg_page_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, token_stride, head_stride;
+  int32_t pages, page_size;
+} hsg_page_cache;
+
+/* Request b holds lens[b] tokens in the first ceil(lens[b] / page_size) pages of its row of table [rows][width]; free
+ * pages are entries head .. tail - 1, modulo ring_size, of the ring, with counters = {head, tail} only growing.
+ * delta[b] > 0 appends that many tokens, taking pages from the head in request order; delta[b] < 0 takes back that
+ * many (all it has, if fewer), returning emptied pages at the tail. Pages returned by a call are free for the next
+ * one. An append that needs pages is served iff all needs up to and including its own, in request order, are within
+ * the pages free at entry, and an append past width * page_size is not served: lens_out[b] then stays lens[b] and no
+ * token of it is listed. The appended tokens are listed in request order: cu [rows + 1] their counts before each
+ * request, and for each its slot (page id * page_size + offset), request and position; entries from the last token to
+ * `capacity` are -1. Tokens beyond capacity are not listed (and err is set). Inputs and outputs must not alias; table
+ * and ring change in place, so that a repeated call with the same inputs gives the same result. rows <=
+ * HSG_MAX_TABLE_ROWS. */
+typedef struct hsg_tables_args {
+  int64_t size;
+  const int32_t* lens;
+  const int32_t* delta;
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* ring;
+  const int64_t* counters;
+  int32_t* lens_out;
+  int64_t* counters_out;
+  int32_t* cu;
+  int32_t* slots;
+  int32_t* token_rows;
+  int32_t* positions;
+  int32_t* err;
+  void* stream;
+  int32_t rows, width, ring_size, page_size, capacity;
+} hsg_tables_args;
+int hsg_advance_tables(const hsg_tables_args* args);
+
+/* Drafted tokens cu[b] .. cu[b+1] - 1 belong to request b; parents [tokens] holds each one's parent as an index within
+ * its request, an earlier token, or -1 (child of the last cached token). positions = lens[b] + depth; bit j of
+ * mask [tokens][words] (32 bits a word) is set iff j is the token or one of its ancestors. */
+typedef struct hsg_tree_args {
+  int64_t size;
+  const int32_t* parents;
+  const int32_t* cu;
+  const int32_t* lens;
+  int32_t* positions;
+  uint32_t* mask;
+  int32_t* err;
+  void* stream;
+  int32_t rows, tokens, words;
+} hsg_tree_args;
+int hsg_plan_tree(const hsg_tree_args* args);
+
+/* q [tokens][hq][dim], k and v [tokens][hkv][dim] in in_dtype: q and k become x * rsqrt(mean(x^2) + eps) * weight,
+ * their first `rot` dims rotated by positions[t] * inv_freq[i] (pairs d, d + rot / 2), v is only converted. q_out
+ * [tokens][hq][dim] contiguous in out_dtype; k and v go to k_out and v_out [tokens][hkv][dim], or, with slots
+ * [tokens], to those slots of the cache (a negative slot: nowhere). dim 64, 128 or 256; rot a multiple of 16. */
+typedef struct hsg_norm_rope_args {
+  int64_t size;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const float* q_weight;
+  const float* k_weight;
+  const float* inv_freq;
+  const int32_t* positions;
+  void* q_out;
+  void* k_out;
+  void* v_out;
+  const int32_t* slots;
+  hsg_page_cache cache;
+  int32_t* err;
+  void* stream;
+  int32_t tokens, hq, hkv, dim, rot, in_dtype, out_dtype;
+  float eps;
+} hsg_norm_rope_args;
+int hsg_norm_rope(const hsg_norm_rope_args* args);
+
+/* Drafted token t of request b, at position p_t, attends the cached tokens n < lens[b] with n > p_t - window (all of
+ * them when window is 0) and the drafted tokens j of its request whose bit in mask[t] is set (mask NULL: j <= t) and,
+ * with a window, p_j > p_t - window. out [tokens][hq][dim] = softmax(scale q.k) v in dtype (HSG_DT_F16 or _BF16, as q,
+ * k, v and the cache), lse [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing gets 0 and -inf;
+ * what is not seen, beyond a length included, does not enter a result whatever its bits. positions are read only with
+ * a window (NULL: lens[b] + index) and must be at least lens[b]. Requests may have no cached or no drafted tokens; none
+ * has more than max_tree drafted ones. Table entries of pages wholly outside the window are not read. `workspace`:
+ * hsg_tree_attention_workspace(dim) bytes on a 16-byte boundary, not shared by calls that overlap in time. */
+typedef struct hsg_tree_attention_args {
+  int64_t size;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  hsg_page_cache cache;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* cu;
+  const int32_t* positions;
+  const uint32_t* mask;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;
+  void* stream;
+  int32_t rows, width, tokens, words, max_tree, hq, hkv, dim, window, dtype;
+  float scale;
+} hsg_tree_attention_args;
+size_t hsg_tree_attention_workspace(int head_dim);
+int hsg_tree_attention(const hsg_tree_attention_args* args);
+
+/* For i < count: row source[i] (NULL: i) of k and v [rows][heads][dim] (16-bit elements, the cache's type) to slot
+ * slots[i] of the cache; a negative slot is skipped. Slots must differ. */
+typedef struct hsg_store_args {
+  int64_t size;
+  const void* k;
+  const void* v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int32_t* source;
+  const int32_t* slots;
+  hsg_page_cache cache;
+  int32_t* err;
+  void* stream;
+  int32_t count, rows, heads, dim;
+} hsg_store_args;
+int hsg_store_rows(const hsg_store_args* args);
+
+/* What the value of a device error word says. */
+const char* hsg_device_error_text(int code);
+
 const char* hsg_last_error(void);
 const char* hsg_version(void);
 
