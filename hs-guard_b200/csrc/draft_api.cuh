@@ -58,17 +58,75 @@ int launch_norm_in(const DraftNormArgs& n, int in, int out, cudaStream_t st) {
   return in == HSG_DT_F16 ? launch_norm_out<D, __half>(n, out, st) : launch_norm_out<D, __nv_bfloat16>(n, out, st);
 }
 
+// Tensor map of a paged cache's K or V: (d, token, head, page) read in boxes of 64 dims x `box` tokens. A stride whose
+// dimension has one element is never used; the encoder still wants a valid one.
+int make_cache_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, const PageCache& c, int heads, int dim,
+                   int box) {
+  if (get_encoder() != HSG_OK) return HSG_ERR_CUDA;
+  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)c.page, (cuuint64_t)heads, (cuuint64_t)c.pages};
+  cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)(heads > 1 ? c.head_stride : dim) * 2,
+                           (cuuint64_t)(c.pages > 1 ? c.page_stride : dim) * 2};
+  cuuint32_t box4[4] = {64, (cuuint32_t)box, 1, 1}, one[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(map, type, 4, const_cast<void*>(base), dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed (%d)", (int)r);
+  return HSG_OK;
+}
+
+// Tensor map of drafted K or V: (d, token, head) in boxes of 64 dims x 8 tokens.
+int make_drafted_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int tokens, int heads, int dim,
+                     int64_t token_stride, int64_t head_stride) {
+  if (get_encoder() != HSG_OK) return HSG_ERR_CUDA;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads};
+  cuuint64_t strides[2] = {(cuuint64_t)(tokens > 1 ? token_stride : dim) * 2, (cuuint64_t)(heads > 1 ? head_stride : dim) * 2};
+  cuuint32_t box[3] = {64, 8, 1}, one[3] = {1, 1, 1};
+  CUresult r = g_encode(map, type, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (drafted) failed (%d)", (int)r);
+  return HSG_OK;
+}
+
+// Q double-buffered while both buffers stay within 64 KB, the rest of shared memory for K and V tiles.
+DaPlan plan_draft_attn(int max_tree, int group, int dim, int page) {
+  DaPlan p;
+  p.q_rows = (int)std::min<int64_t>(DA_ROWS, ((int64_t)max_tree * group + 7) / 8 * 8);
+  const int q = p.q_rows * dim * 2;
+  p.q_bufs = q <= 32768 ? 2 : 1;
+  p.kv_bufs = std::min(12, (DA_SMEM_LIMIT - 1536 - p.q_bufs * q) / da_buffer_bytes(dim));
+  p.box = 8;
+  while (p.box < da_tile(dim) && page % (2 * p.box) == 0) p.box *= 2;
+  p.pieces = SM_COUNT;
+  return p;
+}
+
 template <int D, typename T>
-int launch_draft_attn(const DraftAttnArgs& d, cudaStream_t st) {
-  const int64_t jobs = (int64_t)d.tokens * d.hq, per = DA_THREADS / 32;
-  draft_attn_simple_kernel<D, T><<<(unsigned)((jobs + per - 1) / per), DA_THREADS, 0, st>>>(d);
+int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) {
+  constexpr CUtensorMapDataType type =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const DaPlan p = plan_draft_attn(d.max_tree, d.hq / d.hkv, D, d.cache.page);
+  CUtensorMap ck, cv, k, v;
+  int rc;
+  if ((rc = make_cache_map(&ck, d.cache.k, type, d.cache, d.hkv, D, p.box)) != HSG_OK ||
+      (rc = make_cache_map(&cv, d.cache.v, type, d.cache, d.hkv, D, p.box)) != HSG_OK ||
+      (rc = make_drafted_map(&k, d.k, type, d.tokens, d.hkv, D, d.k_ts, d.k_hs)) != HSG_OK ||
+      (rc = make_drafted_map(&v, d.v, type, d.tokens, d.hkv, D, d.v_ts, d.v_hs)) != HSG_OK)
+    return rc;
+  DaSplit* splits = static_cast<DaSplit*>(workspace);
+  float* partials = reinterpret_cast<float*>(splits + p.pieces);
+  CU(cudaFuncSetAttribute(draft_attn_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, DA_SMEM_LIMIT));
+  draft_attn_kernel<D, T><<<p.pieces, DA_THREADS, da_smem_bytes(p, D), st>>>(ck, cv, k, v, d, p, splits, partials);
   CU(cudaGetLastError());
+  const int rows = p.q_rows;
+  CU(launch_k(draft_join_kernel<D, T>, dim3(p.pieces, (rows + DJ_THREADS / 32 - 1) / (DJ_THREADS / 32)),
+              dim3(DJ_THREADS), 0, st, true, d, (const DaSplit*)splits, (const float*)partials));
   return HSG_OK;
 }
 template <typename T>
-int launch_draft_attn_dim(const DraftAttnArgs& d, int dim, cudaStream_t st) {
-  return dim == 64 ? launch_draft_attn<64, T>(d, st)
-                   : dim == 128 ? launch_draft_attn<128, T>(d, st) : launch_draft_attn<256, T>(d, st);
+int launch_draft_attn_dim(const DraftAttnArgs& d, int dim, void* ws, cudaStream_t st) {
+  return dim == 64 ? launch_draft_attn<64, T>(d, ws, st)
+                   : dim == 128 ? launch_draft_attn<128, T>(d, ws, st) : launch_draft_attn<256, T>(d, ws, st);
 }
 
 }  // namespace
@@ -142,8 +200,7 @@ extern "C" int hsg_norm_rope(const hsg_norm_rope_args* a) {
 }
 
 extern "C" size_t hsg_tree_attention_workspace(int head_dim) {
-  (void)head_dim;
-  return 0;
+  return head_dim_ok(head_dim) ? da_workspace_bytes(head_dim, SM_COUNT) : 0;
 }
 
 extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
@@ -156,9 +213,13 @@ extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
     return fail(HSG_ERR_INVALID, "max_tree must be in [1, %d], got %d", HSG_MAX_TREE, a->max_tree);
   if (a->mask && (int64_t)a->words * 32 < a->max_tree)
     return fail(HSG_ERR_INVALID, "%d mask words hold fewer than max_tree = %d bits", a->words, a->max_tree);
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(HSG_ERR_INVALID, "scale must be positive");
   if (a->window < 0) return fail(HSG_ERR_INVALID, "window must not be negative, got %d", a->window);
   if (a->rows == 0 || a->tokens == 0) return HSG_OK;
   if (!a->q || !a->k || !a->v || !a->table || !a->lens || !a->cu || !a->out) return fail(HSG_ERR_INVALID, "NULL argument");
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)hsg_tree_attention_workspace(a->dim))
+    return fail(HSG_ERR_INVALID, "the workspace must have %zu bytes on a 16-byte boundary",
+                hsg_tree_attention_workspace(a->dim));
   if (a->width < 1 || a->table_stride < a->width)
     return fail(HSG_ERR_INVALID, "bad table shape (width %d, stride %lld)", a->width, (long long)a->table_stride);
   int rc;
@@ -174,8 +235,8 @@ extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
                   a->positions, a->mask, a->rows, a->width, a->tokens, a->words, a->max_tree, a->hq, a->hkv, a->window,
                   a->scale, a->out, a->lse, a->err};
   cudaStream_t st = (cudaStream_t)a->stream;
-  return a->dtype == HSG_DT_F16 ? launch_draft_attn_dim<__half>(d, a->dim, st)
-                                : launch_draft_attn_dim<__nv_bfloat16>(d, a->dim, st);
+  return a->dtype == HSG_DT_F16 ? launch_draft_attn_dim<__half>(d, a->dim, a->workspace, st)
+                                : launch_draft_attn_dim<__nv_bfloat16>(d, a->dim, a->workspace, st);
 }
 
 extern "C" int hsg_store_rows(const hsg_store_args* a) {
