@@ -58,45 +58,35 @@ int launch_norm_in(const DraftNormArgs& n, int in, int out, cudaStream_t st) {
   return in == HSG_DT_F16 ? launch_norm_out<D, __half>(n, out, st) : launch_norm_out<D, __nv_bfloat16>(n, out, st);
 }
 
-// Tensor map of a paged cache's K or V: (d, token, head, page) read in boxes of 64 dims x `box` tokens. A stride whose
-// dimension has one element is never used; the encoder still wants a valid one.
-int make_cache_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, const PageCache& c, int heads, int dim,
-                   int box) {
+// Tensor map of 16-bit rows of `dim` elements, read 64 dims at a time in 128-byte swizzle: dimension 0 is 64 dims, the
+// others as given (element strides). A stride whose dimension has one element is never used, but the encoder wants a
+// valid one.
+int make_rows_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int rank, const int64_t* sizes,
+                  const int64_t* strides, const int* boxes) {
   if (get_encoder() != HSG_OK) return HSG_ERR_CUDA;
-  cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)c.page, (cuuint64_t)heads, (cuuint64_t)c.pages};
-  cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)(heads > 1 ? c.head_stride : dim) * 2,
-                           (cuuint64_t)(c.pages > 1 ? c.page_stride : dim) * 2};
-  cuuint32_t box4[4] = {64, (cuuint32_t)box, 1, 1}, one[4] = {1, 1, 1, 1};
-  CUresult r = g_encode(map, type, 4, const_cast<void*>(base), dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t dims[5], bytes[4];
+  cuuint32_t box[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = (cuuint64_t)sizes[i];
+    box[i] = (cuuint32_t)boxes[i];
+    one[i] = 1;
+    if (i) bytes[i - 1] = (cuuint64_t)(sizes[i] > 1 ? strides[i] : 64) * 2;
+  }
+  CUresult r = g_encode(map, type, rank, const_cast<void*>(base), dims, bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed (%d)", (int)r);
+  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (%d-d rows) failed (%d)", rank, (int)r);
   return HSG_OK;
 }
 
-// Tensor map of drafted K or V: (d, token, head) in boxes of 64 dims x 8 tokens.
-int make_drafted_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int tokens, int heads, int dim,
-                     int64_t token_stride, int64_t head_stride) {
-  if (get_encoder() != HSG_OK) return HSG_ERR_CUDA;
-  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads};
-  cuuint64_t strides[2] = {(cuuint64_t)(tokens > 1 ? token_stride : dim) * 2, (cuuint64_t)(heads > 1 ? head_stride : dim) * 2};
-  cuuint32_t box[3] = {64, 8, 1}, one[3] = {1, 1, 1};
-  CUresult r = g_encode(map, type, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (drafted) failed (%d)", (int)r);
-  return HSG_OK;
-}
-
-// Q double-buffered while both buffers stay within 64 KB, the rest of shared memory for K and V tiles.
-DaPlan plan_draft_attn(int max_tree, int group, int dim, int page) {
+// As many whole drafted tokens as fit 128 rows; Q double-buffered up to 64 KB, the rest of shared memory for K and V.
+DaPlan plan_draft_attn(int max_tree, int group, int dim) {
   DaPlan p;
-  p.q_rows = (int)std::min<int64_t>(DA_ROWS, ((int64_t)max_tree * group + 7) / 8 * 8);
+  p.block = std::min(max_tree, DA_ROWS / group);
+  p.q_rows = (p.block * group + 7) / 8 * 8;
   const int q = p.q_rows * dim * 2;
   p.q_bufs = q <= 32768 ? 2 : 1;
   p.kv_bufs = std::min(12, (DA_SMEM_LIMIT - 1536 - p.q_bufs * q) / da_buffer_bytes(dim));
-  p.box = 8;
-  while (p.box < da_tile(dim) && page % (2 * p.box) == 0) p.box *= 2;
   p.pieces = SM_COUNT;
   return p;
 }
@@ -105,22 +95,40 @@ template <int D, typename T>
 int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) {
   constexpr CUtensorMapDataType type =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const DaPlan p = plan_draft_attn(d.max_tree, d.hq / d.hkv, D, d.cache.page);
-  CUtensorMap ck, cv, k, v;
+  constexpr int NC = D / 64;
+  const int group = d.hq / d.hkv;
+  const DaPlan p = plan_draft_attn(d.max_tree, group, D);
+  const PageCache& c = d.cache;
+  CUtensorMap q, ck, cv, k, v;
   int rc;
-  if ((rc = make_cache_map(&ck, d.cache.k, type, d.cache, d.hkv, D, p.box)) != HSG_OK ||
-      (rc = make_cache_map(&cv, d.cache.v, type, d.cache, d.hkv, D, p.box)) != HSG_OK ||
-      (rc = make_drafted_map(&k, d.k, type, d.tokens, d.hkv, D, d.k_ts, d.k_hs)) != HSG_OK ||
-      (rc = make_drafted_map(&v, d.v, type, d.tokens, d.hkv, D, d.v_ts, d.v_hs)) != HSG_OK)
-    return rc;
+  {
+    const int64_t sizes[3] = {D, d.hq, d.tokens}, strides[3] = {1, d.q_hs, d.q_ts};
+    const int boxes[3] = {64, group, p.block};
+    if ((rc = make_rows_map(&q, d.q, type, 3, sizes, strides, boxes)) != HSG_OK) return rc;
+  }
+  {
+    const int64_t sizes[5] = {64, c.page, NC, d.hkv, c.pages}, strides[5] = {1, c.token_stride, 64, c.head_stride, c.page_stride};
+    const int boxes[5] = {64, 8, NC, 1, 1};
+    if ((rc = make_rows_map(&ck, c.k, type, 5, sizes, strides, boxes)) != HSG_OK ||
+        (rc = make_rows_map(&cv, c.v, type, 5, sizes, strides, boxes)) != HSG_OK)
+      return rc;
+  }
+  {
+    const int64_t sizes[4] = {64, d.tokens, NC, d.hkv};
+    const int64_t ks[4] = {1, d.k_ts, 64, d.k_hs}, vs[4] = {1, d.v_ts, 64, d.v_hs};
+    const int boxes[4] = {64, 8, NC, 1};
+    if ((rc = make_rows_map(&k, d.k, type, 4, sizes, ks, boxes)) != HSG_OK ||
+        (rc = make_rows_map(&v, d.v, type, 4, sizes, vs, boxes)) != HSG_OK)
+      return rc;
+  }
   DaSplit* splits = static_cast<DaSplit*>(workspace);
   float* partials = reinterpret_cast<float*>(splits + p.pieces);
   CU(cudaFuncSetAttribute(draft_attn_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, DA_SMEM_LIMIT));
-  draft_attn_kernel<D, T><<<p.pieces, DA_THREADS, da_smem_bytes(p, D), st>>>(ck, cv, k, v, d, p, splits, partials);
+  draft_attn_kernel<D, T><<<p.pieces, DA_THREADS, da_smem_bytes(p, D), st>>>(q, ck, cv, k, v, d, p, splits, partials);
   CU(cudaGetLastError());
   const int rows = p.q_rows;
   CU(launch_k(draft_join_kernel<D, T>, dim3(p.pieces, (rows + DJ_THREADS / 32 - 1) / (DJ_THREADS / 32)),
-              dim3(DJ_THREADS), 0, st, true, d, (const DaSplit*)splits, (const float*)partials));
+              dim3(DJ_THREADS), 0, st, true, d, p.block, (const DaSplit*)splits, (const float*)partials));
   return HSG_OK;
 }
 template <typename T>
@@ -207,6 +215,8 @@ extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
   DRAFT_ARGS(a);
   if (a->rows < 0 || a->tokens < 0 || a->hq < 1 || a->hkv < 1 || a->hq % a->hkv)
     return fail(HSG_ERR_INVALID, "bad shape (rows %d, tokens %d, heads %d / %d)", a->rows, a->tokens, a->hq, a->hkv);
+  if (a->hq / a->hkv > DA_ROWS)
+    return fail(HSG_ERR_INVALID, "at most %d query heads a key head, got %d", DA_ROWS, a->hq / a->hkv);
   if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
   if (a->dtype != HSG_DT_F16 && a->dtype != HSG_DT_BF16) return fail(HSG_ERR_INVALID, "dtype must be fp16 or bf16");
   if (a->max_tree < 1 || a->max_tree > HSG_MAX_TREE)

@@ -32,18 +32,22 @@ struct DraftAttnArgs {
 };
 
 // One kernel for every shape, on tcgen05. The drafted tokens of a request that share a key head are the rows of a matrix
-// product, row r = (token r / G, query head r % G of the group of G); 128 rows and all of a request's keys in tiles of
-// KT (128, or 64 at head dim 256) are an item (request, key head, block of 128 rows). All items' tiles, in order, are one
+// product, row r = (token r / G, query head r % G of the group of G); as many whole tokens as fit 128 rows and all of a
+// request's keys in tiles of KT (128, or 64 at head dim 256) are an item (request, key head, block of tokens). All items' tiles, in order, are one
 // line that is cut into equal pieces, one a thread block, whatever the requests' lengths, so a long cache is split over
 // many SMs and short ones share one; the lengths are read on the device. An item that lies in one piece is written
 // out; of one that is cut, each piece leaves its unnormalised sums, row maxima and row sums in the workspace and
 // draft_join_kernel joins them in piece order, so results do not depend on timing.
 //
 // Per tile: S = Q K^T (tcgen05, TMEM), softmax with a running maximum in registers (a row a thread), P in the type of V
-// written over S in TMEM, O += P V (A = P from TMEM, B = V as it lies in shared memory, N-major). Warp 0 brings K and
-// V tiles by TMA, page by page, 128-byte swizzle, through one ring of buffers in the order in which the products use
-// them; warp 1 issues the products, S of the next tile before P V of this one; warps 2-3 gather Q; warps 4-7 do the
-// softmax and the epilogue. Tiles of the next item are under way during an item's epilogue.
+// written over S in TMEM, O += P V (A = P from TMEM, B = V as it lies in shared memory, N-major). Warps 0 and 3 bring K
+// and V tiles by TMA, eight tokens of one page a box, through one ring of buffers in the order in which the products use
+// them; warp 1 issues the products, S of the next tile before P V of this one; warp 2 brings Q; warps 4-7 do the
+// softmax and the epilogue. A K or V tile lies in shared memory as [8 keys][dim / 64][8][128 B], 128-byte swizzle: boxes
+// of any page size then sit at one stride, which is all that a product's descriptor can say. Warp 1 runs as a whole warp
+// with one elected lane at each group of products, so that their descriptors stay in uniform registers: issued from a
+// branch on the lane, each took about 150 cycles. Copies are the other way round: 32 lanes with a box each take 64 to 95
+// cycles a box (1 to 4 KB), one elected lane in a loop over boxes 135 to 240, and one warp alone falls short of HBM. Tiles of the next item are under way during an item's epilogue.
 //
 // S, P and P V of a tile each have two barriers, for even and odd tiles: a wait tells a phase from its neighbours only,
 // and whoever waits for tile g of one of them knows tile g - 2 to be done and g + 2 to be impossible before it goes on
@@ -61,10 +65,10 @@ __host__ __device__ constexpr int da_tile(int dim) { return dim == 256 ? 64 : 12
 __host__ __device__ constexpr int da_buffer_bytes(int dim) { return da_tile(dim) * dim * 2; }
 
 struct DaPlan {  // launch shape, chosen by the host
-  int q_rows;    // rows a Q buffer holds: a multiple of 8 up to 128
+  int block;     // drafted tokens of an item: at most 128 rows
+  int q_rows;    // rows a Q buffer holds: block * G rounded up to a multiple of 8
   int q_bufs;
   int kv_bufs;
-  int box;       // tokens of one TMA box of the cache: the largest power of two that divides the page, at most KT
   int pieces;    // thread blocks
 };
 __host__ __device__ inline int da_smem_bytes(const DaPlan& p, int dim) {
@@ -89,7 +93,7 @@ struct DaReq {
   int len, t0, fresh, lo, first, cached, n, blocks;
 };
 template <int KT>
-__device__ __forceinline__ DaReq da_request(const DraftAttnArgs& a, int b, bool report) {
+__device__ __forceinline__ DaReq da_request(const DraftAttnArgs& a, int block, int b, bool report) {
   DaReq r;
   r.len = a.lens[b];
   r.t0 = a.cu[b];
@@ -104,7 +108,7 @@ __device__ __forceinline__ DaReq da_request(const DraftAttnArgs& a, int b, bool 
   r.first = r.lo / KT;
   r.cached = r.lo < r.len ? (r.len + KT - 1) / KT - r.first : 0;
   r.n = r.fresh ? r.cached + (r.fresh + KT - 1) / KT : 0;
-  r.blocks = (r.fresh * (a.hq / a.hkv) + DA_ROWS - 1) / DA_ROWS;
+  r.blocks = (r.fresh + block - 1) / block;
   return r;
 }
 
@@ -113,11 +117,13 @@ template <int KT>
 struct DaWalk {
   const DraftAttnArgs* a;
   DaReq r;
+  int size;  // tokens of a block
   int b, h, block, i;
-  __device__ __forceinline__ void start(const DraftAttnArgs& args, int b0, int64_t within) {
+  __device__ __forceinline__ void start(const DraftAttnArgs& args, int block_size, int b0, int64_t within) {
     a = &args;
+    size = block_size;
     b = b0;
-    r = da_request<KT>(args, b, false);
+    r = da_request<KT>(args, size, b, false);
     const int64_t item = within / r.n;
     i = (int)(within - item * r.n);
     h = (int)(item / r.blocks);
@@ -133,7 +139,7 @@ struct DaWalk {
     h = 0;
     do {
       if (++b >= a->rows) return;
-      r = da_request<KT>(*a, b, false);
+      r = da_request<KT>(*a, size, b, false);
     } while (r.n == 0);
   }
 };
@@ -150,11 +156,20 @@ template <> struct DaType<__nv_bfloat16> {
 };
 constexpr uint32_t DA_B_N_MAJOR = 1u << 16;
 
-// Shared-memory descriptor of an N-major operand in 128-byte swizzle: blocks of 64 n-elements (128 bytes) `block_bytes`
-// apart (leading byte offset), in each 8 k-rows are 1024 bytes (stride byte offset).
-__device__ __forceinline__ uint64_t sw128_n_major_desc(uint32_t saddr, uint32_t block_bytes) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(block_bytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+// Shared-memory descriptors of a tile that lies as [8 keys][NC][8][128 B] in 128-byte swizzle: as a K-major operand (S:
+// rows are keys, stride byte offset from 8 keys to the next 8) and as an N-major one (P V: leading byte offset from 64
+// dims to the next 64, stride byte offset from 8 keys to the next 8).
+template <int NC> __device__ __forceinline__ uint64_t da_k_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(NC * 1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+template <int NC> __device__ __forceinline__ uint64_t da_v_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(NC * 1024 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Byte offset of 16-byte piece ch of key k in such a tile.
+template <int NC> __device__ __forceinline__ uint32_t da_offset(int k, int ch) {
+  return (uint32_t)(((k >> 3) * NC + (ch >> 3)) * 1024) + sw128_off(k & 7, ch & 7);
 }
 
 // D[tmem] (+)= A[tmem] B[smem], kind::f16: A's 16-bit elements two a column, one lane a row.
@@ -168,6 +183,17 @@ __device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// true in one lane of a converged warp, always the same one
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint64_t* bar) {
   asm volatile(
@@ -176,8 +202,34 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w, int u,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(u), "r"(smem_u32(bar))
+      : "memory");
+}
 
-// 32 packed 32-bit values a thread into TMEM columns taddr .. taddr + 31 of its lane; completes with tmem_st_wait.
+// TMEM columns taddr .. taddr + 31 of a thread's lane, complete after tmem_ld_wait; da_pin keeps what uses them behind it.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void da_pin(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                 "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+// 32 packed 32-bit values a thread into TMEM columns taddr .. taddr + 31 of its lane; complete after tmem_st_wait.
 __device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -190,23 +242,54 @@ __device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t (
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-struct DaBox {  // one lane's TMA box of a K or V tile
-  int kind;     // 0: none, 1: cache, 2: drafted
-  int row, page, head;
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// Position in a ring of buffers and the parity of its use.
+struct DaRing {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++at == size) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// What a lane fetches of a K or V tile: eight keys.
+struct DaFetch {
+  int row, page;  // token within the page and page id, or drafted token
+  int drafted, head;
+  bool mine;      // some of them exist
 };
 
 template <int D, typename T>
 __global__ void __launch_bounds__(DA_THREADS, 1)
-draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_constant__ CUtensorMap tm_cv,
-                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ DraftAttnArgs a, const DaPlan plan, DaSplit* splits, float* partials) {
+draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_ck,
+                  const __grid_constant__ CUtensorMap tm_cv, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DraftAttnArgs a, const DaPlan plan,
+                  DaSplit* splits, float* partials) {
   constexpr int KT = da_tile(D), NC = D / 64, BUF = da_buffer_bytes(D);
   constexpr uint32_t O_COL = 2 * KT;
   extern __shared__ __align__(1024) uint8_t da_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(da_smem_raw) + 1023) & ~uintptr_t(1023));
   const int q_buf = plan.q_rows * D * 2, q_box = plan.q_rows * 128;
   uint8_t* qs = smem;                            // [q_bufs][NC][q_rows][128 B], SW128
-  uint8_t* kvs = qs + plan.q_bufs * q_buf;       // [kv_bufs][NC][KT][128 B], SW128
+  uint8_t* kvs = qs + plan.q_bufs * q_buf;       // [kv_bufs][KT / 8][NC][8][128 B], SW128
   uint64_t* bars = reinterpret_cast<uint64_t*>(kvs + plan.kv_bufs * BUF);
   uint64_t* full = bars;                         // [kv_bufs <= 12] a tile has landed
   uint64_t* empty = full + 12;                   // [kv_bufs] the products that read it are done
@@ -222,7 +305,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
   int64_t* s_scan = reinterpret_cast<int64_t*>(((uintptr_t)(low_max + 4) + 7) & ~uintptr_t(7));  // [8] warp sums, then
   int* s_start = reinterpret_cast<int*>(s_scan + 8);  // the piece's first request
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, piece = blockIdx.x;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
   const int G = a.hq / a.hkv;
   if (tid == 0) {
     for (int i = 0; i < plan.kv_bufs; ++i) {
@@ -230,14 +313,15 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 64);
+      mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(all_done, 1);
     fence_barrier_init();
+    prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_ck);
     prefetch_tmap(&tm_cv);
     prefetch_tmap(&tm_k);
@@ -251,7 +335,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
   // ---- this piece of the line: requests' tile counts summed over the block ----
   const int per = (a.rows + DA_THREADS - 1) / DA_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
   auto tiles_of = [&](int b, bool report) -> int64_t {
-    const DaReq r = da_request<KT>(a, b, report);
+    const DaReq r = da_request<KT>(a, plan.block, b, report);
     return (int64_t)r.n * r.blocks * a.hkv;
   };
   int64_t mine = 0;
@@ -288,150 +372,152 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
   }
   if (tid == 0) splits[piece].last = -1;
   __syncthreads();
-  const uint32_t tmem = *tmem_slot;
-  int issued = 0;  // warp 0: tiles requested
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  bool ok = true;  // no wait of this thread has given up
+  int issued = 0;  // warps 0 and 3: ring entries up to their last one; warp 2: Q tiles
   if (n_tiles > 0) {
     DaWalk<KT> walk;
-    walk.start(a, s_start[0], *reinterpret_cast<const int64_t*>(s_start + 2));
-    // K of tile g is the ring's entry 0 (g = 0) or 2 g - 1, V of tile g entry 2 g + 2, or 2 g + 1 for the last
-    auto v_entry = [&](int g) { return g + 1 < n_tiles ? 2 * g + 2 : 2 * g + 1; };
-    if (warp == 0) {
-      // ---- K and V tiles: every lane one box ----
-      const int rb = lane / NC, cb = lane % NC;
-      auto box_of = [&](const DaWalk<KT>& w) {
-        DaBox x{0, 0, 0, w.h};
+    walk.start(a, plan.block, s_start[0], *reinterpret_cast<const int64_t*>(s_start + 2));
+    // K and V of tile g are the ring's entries 2 g - 1 (0 for g = 0) and 2 g + 2 (2 g + 1 for the last)
+    if (warp == 0 || warp == 3) {
+      // ---- K tiles (warp 0) and V tiles (warp 3): lane i brings keys 8 i .. 8 i + 7 ----
+      const bool is_v = warp == 3;
+      const CUtensorMap *cache = is_v ? &tm_cv : &tm_ck, *drafted = is_v ? &tm_v : &tm_k;
+      auto fetch_of = [&](const DaWalk<KT>& w) {
+        DaFetch x{0, -1, 0, w.h, false};
         if (w.i < w.r.cached) {
-          const int pos = (w.r.first + w.i) * KT + rb * plan.box;
-          if (rb < KT / plan.box && pos < w.r.len && pos + plan.box > w.r.lo) {
+          const int base = (w.r.first + w.i) * KT, pos = base + lane * 8;
+          x.mine = lane < KT / 8 && pos < w.r.len && pos + 8 > w.r.lo;
+          if (x.mine) {
             const int p = pos / a.cache.page;
-            x.kind = 1;
             x.row = pos - p * a.cache.page;
             x.page = a.table[w.b * a.table_stride + p];
           }
         } else {
-          const int j = (w.i - w.r.cached) * KT + rb * 8;
-          if (rb < KT / 8 && j < w.r.fresh) {
-            x.kind = 2;
-            x.row = w.r.t0 + j;
-          }
+          const int j = (w.i - w.r.cached) * KT + lane * 8;
+          x.mine = lane < KT / 8 && j < w.r.fresh;
+          x.row = w.r.t0 + j;
+          x.drafted = 1;
         }
         return x;
       };
-      bool ok = true;
-      auto bring = [&](const DaBox& x, bool v) {
-        const int s = issued % plan.kv_bufs, turn = issued / plan.kv_bufs;
-        if (turn > 0) ok = mbar_wait(&empty[s], (turn - 1) & 1, a.err, ERR_TIMEOUT_MMA);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        const bool in_cache = x.kind == 1 && x.page >= 0 && x.page < a.cache.pages;
-        if (x.kind == 1 && !in_cache) set_error(a.err, ERR_BAD_PAGE);
-        const unsigned c = __ballot_sync(0xffffffffu, in_cache), d = __ballot_sync(0xffffffffu, x.kind == 2);
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], __popc(c) * plan.box * 128 + __popc(d) * 8 * 128);
-        __syncwarp();
-        uint8_t* dst = kvs + s * BUF + cb * KT * 128 + rb * (x.kind == 1 ? plan.box : 8) * 128;
-        if (in_cache) tma_load_4d(dst, v ? &tm_cv : &tm_ck, cb * 64, x.row, x.head, x.page, &full[s]);
-        if (x.kind == 2) tma_load_3d(dst, v ? &tm_v : &tm_k, cb * 64, x.row, x.head, &full[s]);
-        ++issued;
-      };
-      DaBox cur = box_of(walk), next = cur, later = cur;
-      if (n_tiles > 1) {
-        walk.skip(1);
-        next = box_of(walk);
-      }
-      bring(cur, false);
+      DaRing ring;
+      if (is_v) ring.next(plan.kv_bufs);
+      DaFetch cur = fetch_of(walk), next = cur;
       for (int g = 0; g < n_tiles && ok; ++g) {
-        if (g + 2 < n_tiles) {  // the table entries of the tile after the next, ahead of the waits
+        if (g + 1 < n_tiles) {  // the next tile's table entries, ahead of the wait
           walk.skip(1);
-          later = box_of(walk);
+          next = fetch_of(walk);
         }
-        if (g + 1 < n_tiles) bring(next, false);
-        if (ok) bring(cur, true);
+        if (is_v && g + 1 < n_tiles) ring.next(plan.kv_bufs);
+        const int e = is_v ? (g + 1 < n_tiles ? 2 * g + 2 : 2 * g + 1) : g ? 2 * g - 1 : 0;
+        if (e >= plan.kv_bufs) ok = __all_sync(0xffffffffu, mbar_wait(&empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+        if (!ok) break;
+        const bool good = cur.drafted || (cur.page >= 0 && cur.page < a.cache.pages);
+        if (cur.mine && !good) set_error(a.err, ERR_BAD_PAGE);
+        const bool bring = cur.mine && good;
+        const unsigned boxes = __ballot_sync(0xffffffffu, bring);
+        uint8_t* dst = kvs + ring.at * BUF + lane * NC * 1024;
+        if (lane == 0) mbar_arrive_expect_tx(&full[ring.at], __popc(boxes) * (NC * 1024));
+        __syncwarp();
+        if (bring) {
+          if (cur.drafted) tma_load_4d(dst, drafted, 0, cur.row, 0, cur.head, &full[ring.at]);
+          else tma_load_5d(dst, cache, 0, cur.row, 0, cur.head, cur.page, &full[ring.at]);
+        }
+        issued = e + 1;
+        ring.next(plan.kv_bufs);
+        if (!is_v && g > 0) ring.next(plan.kv_bufs);
         cur = next;
-        next = later;
       }
     } else if (warp == 1) {
       // ---- products ----
-      if (lane == 0) {
-        bool ok = true;
-        const uint32_t idesc_s = DaType<T>::idesc(KT), idesc_o = DaType<T>::idesc(D) | DA_B_N_MAJOR;
-        int entry = 0, item = -1;
-        bool begins = true;
-        auto score = [&](int g) {  // S of tile g (the walk's place), then the walk moves on
-          if (begins) {
-            ++item;
-            ok = mbar_wait(&q_full[item % plan.q_bufs], (item / plan.q_bufs) & 1, a.err, ERR_TIMEOUT_MMA);
-          }
-          if (ok) ok = mbar_wait(&full[entry % plan.kv_bufs], (entry / plan.kv_bufs) & 1, a.err, ERR_TIMEOUT_TMA);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t qb = smem_u32(qs + (item % plan.q_bufs) * q_buf), kb = smem_u32(kvs + (entry % plan.kv_bufs) * BUF);
-          const uint32_t d = tmem + (uint32_t)((g & 1) * KT);
+      const uint32_t idesc_s = DaType<T>::idesc(KT), idesc_o = DaType<T>::idesc(D) | DA_B_N_MAJOR;
+      DaRing ring, q_ring;
+      bool begins = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, code));
+      };
+      auto score = [&](int g) {  // S of tile g (the walk's place), then the walk moves on
+        if (begins) wait(&q_full[q_ring.at], q_ring.phase, ERR_TIMEOUT_TMA);
+        wait(&full[ring.at], ring.phase, ERR_TIMEOUT_TMA);
+        if (!ok) return;
+        tc_fence_after();
+        const bool ends = __shfl_sync(0xffffffffu, (int)(walk.i + 1 == walk.r.n), 0) || g + 1 == n_tiles;
+        const uint64_t qd = sw128_desc(smem_u32(qs + q_ring.at * q_buf)), kd = da_k_desc<NC>(smem_u32(kvs + ring.at * BUF));
+        const uint32_t d = tmem + (uint32_t)((g & 1) * KT);
+        if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              mma_bf16(d, sw128_desc(qb + c * q_box + kk * 32), sw128_desc(kb + c * KT * 128 + kk * 32), idesc_s,
+              mma_bf16(d, qd + (uint64_t)((c * q_box + kk * 32) >> 4), kd + (uint64_t)((c * 1024 + kk * 32) >> 4), idesc_s,
                        (c > 0 || kk > 0) ? 1u : 0u);
           mma_commit(&s_full[g & 1]);
-          mma_commit(&empty[entry % plan.kv_bufs]);
-          const bool ends = walk.i + 1 == walk.r.n || g + 1 == n_tiles;
-          if (ends) mma_commit(&q_empty[item % plan.q_bufs]);
-          begins = ends;
-          if (g + 1 < n_tiles) walk.skip(1);
-          ++entry;
-        };
-        bool first = true;  // of its item (or of this piece's part of it)
-        score(0);
-        for (int g = 0; g < n_tiles && ok; ++g) {
-          const bool ends = begins;  // the tile that was scored last is the last of its item: tile g
-          if (g + 1 < n_tiles) score(g + 1);
-          if (ok) ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
-          if (ok) ok = mbar_wait(&full[entry % plan.kv_bufs], (entry / plan.kv_bufs) & 1, a.err, ERR_TIMEOUT_TMA);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t vb = smem_u32(kvs + (entry % plan.kv_bufs) * BUF), p = tmem + (uint32_t)((g & 1) * KT);
+          mma_commit(&empty[ring.at]);
+          if (ends) mma_commit(&q_empty[q_ring.at]);
+        }
+        __syncwarp();
+        if (ends) q_ring.next(plan.q_bufs);
+        begins = ends;
+        if (g + 1 < n_tiles) walk.skip(1);
+        ring.next(plan.kv_bufs);
+      };
+      bool first = true;  // of its item (or of this piece's part of it)
+      score(0);
+      for (int g = 0; g < n_tiles && ok; ++g) {
+        const bool ends = begins;  // the tile that was scored last, tile g, is the last of its item
+        if (g + 1 < n_tiles) score(g + 1);
+        wait(&p_full[g & 1], (g >> 1) & 1, ERR_TIMEOUT_MMA);
+        wait(&full[ring.at], ring.phase, ERR_TIMEOUT_TMA);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = da_v_desc<NC>(smem_u32(kvs + ring.at * BUF));
+        const uint32_t p = tmem + (uint32_t)((g & 1) * KT);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk)
-            mma_tmem_a(tmem + O_COL, p + kk * 8, sw128_n_major_desc(vb + kk * 2048, KT * 128), idesc_o,
+            mma_tmem_a(tmem + O_COL, p + kk * 8, vd + (uint64_t)((kk * 2 * NC * 1024) >> 4), idesc_o,
                        (!first || kk > 0) ? 1u : 0u);
           mma_commit(&pv_done[g & 1]);
-          mma_commit(&empty[entry % plan.kv_bufs]);
-          ++entry;
-          first = ends;
+          mma_commit(&empty[ring.at]);
         }
+        __syncwarp();
+        ring.next(plan.kv_bufs);
+        first = ends;
       }
-    } else if (warp < 4) {
-      // ---- Q rows of every item into its buffer ----
-      bool ok = true;
+    } else if (warp == 2) {
+      // ---- Q of every item: block tokens x G heads, one box for each 64 dims ----
+      DaRing ring;
       int left = n_tiles;
-      for (int item = 0; left > 0; ++item) {
-        const int s = item % plan.q_bufs, turn = item / plan.q_bufs;
-        if (ok && turn > 0) ok = mbar_wait(&q_empty[s], (turn - 1) & 1, a.err, ERR_TIMEOUT_MMA);
-        const int rows = min(DA_ROWS, walk.r.fresh * G - walk.block * DA_ROWS);
-        for (int c = tid - 64; c < rows * (D / 8); c += 64) {
-          const int r = c / (D / 8), ch = c % (D / 8), all = walk.block * DA_ROWS + r;
-          const T* src = (const T*)a.q + (int64_t)(walk.r.t0 + all / G) * a.q_ts + (int64_t)(walk.h * G + all % G) * a.q_hs;
-          *reinterpret_cast<uint4*>(qs + s * q_buf + (ch >> 3) * q_box + sw128_off(r, ch & 7)) =
-              *reinterpret_cast<const uint4*>(src + ch * 8);
+      for (int item = 0; left > 0 && ok; ++item) {
+        if (item >= plan.q_bufs) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+        if (!ok) break;
+        const int token = __shfl_sync(0xffffffffu, walk.r.t0 + walk.block * plan.block, 0);
+        const int head = __shfl_sync(0xffffffffu, walk.h * G, 0);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&q_full[ring.at], plan.block * G * D * 2);
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            tma_load_3d(qs + ring.at * q_buf + c * q_box, &tm_q, c * 64, head, token, &q_full[ring.at]);
         }
-        fence_proxy_async();
-        mbar_arrive(&q_full[s]);
+        __syncwarp();
+        ++issued;
+        ring.next(plan.q_bufs);
         const int tiles = min(left, walk.r.n - walk.i);
         left -= tiles;
         walk.skip(tiles);
       }
-    } else {
+    } else if (warp >= 4) {
       // ---- softmax: thread = row = TMEM lane ----
-      bool ok = true;
       const int row = tid - 128;
       const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
       int g = 0;
       for (int item = 0; g < n_tiles; ++item) {
         const DaReq r = walk.r;
-        const int all = walk.block * DA_ROWS + row, tok = all / G;
-        const bool valid = tok < r.fresh;
-        const bool live = (walk.block * DA_ROWS + (row & ~31)) / G < r.fresh;  // some row of this warp is
+        const int tok = walk.block * plan.block + row / G;
+        const bool valid = row < plan.block * G && tok < r.fresh;
+        const bool live = __any_sync(0xffffffffu, valid);
         const int i0 = walk.i, i1 = min(r.n, i0 + n_tiles - g);
         // keys of this row are those at positions above `low`
         int low = r.lo - 1, lows = -1;
@@ -452,15 +538,19 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
           const int end = min(KT, (tree ? r.fresh : r.len) - base);          // keys that exist
           const int begin = tree ? 0 : max(0, r.lo - base);
           const bool some = tree || (a.window && base <= lows);              // not every row sees the same keys
+          const bool special = some || begin > 0 || end < KT;
           if (ok) ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
           tc_fence_after();
           __syncwarp();
           if (live) {
-            float sc[KT];
+            uint32_t sc[KT];
 #pragma unroll
-            for (int c = 0; c < KT; c += 32) tmem_ld32(lanes + (uint32_t)((g & 1) * KT + c), *reinterpret_cast<float(*)[32]>(sc + c));
-            if (some || begin > 0 || end < KT) {
-              uint32_t vis[KT / 32];
+            for (int c = 0; c < KT; c += 32) tmem_ld32_async(lanes + (uint32_t)((g & 1) * KT + c), sc + c);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < KT; c += 32) da_pin(sc + c);
+            auto at = [&](int j) { return __uint_as_float(sc[j]); };
+            if (special) {
 #pragma unroll
               for (int w = 0; w < KT / 32; ++w) {
                 const int from = tree ? 0 : max(0, low + 1 - base), z = min(32, max(0, end - 32 * w));
@@ -479,15 +569,18 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
                     }
                   }
                 }
-                vis[w] = bits;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sc[32 * w + j] = bits >> j & 1 ? sc[32 * w + j] : 0xff800000u;  // -inf
               }
-#pragma unroll
-              for (int j = 0; j < KT; ++j) sc[j] = vis[j >> 5] >> (j & 31) & 1 ? sc[j] : -INFINITY;
             }
-            float top = -INFINITY;
+            float tops[4] = {at(0), at(1), at(2), at(3)};
 #pragma unroll
-            for (int j = 0; j < KT; ++j) top = fmaxf(top, sc[j]);
-            top *= sl2;
+            for (int j = 4; j + 4 < KT; j += 8)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) tops[q] = fmaxf(fmaxf(tops[q], at(j + q)), at(j + 4 + q));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tops[q] = fmaxf(tops[q], at(KT - 4 + q));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sl2;
             // the maximum is raised only when a tile exceeds it by 2^8: weights stay below that, which fp16 holds
             const bool raise = valid && (top > m + 8.f || (m == -INFINITY && top > -INFINITY));
             const float alpha = raise && m > -INFINITY ? ex2_approx(m - top) : raise ? 0.f : 1.f;
@@ -508,30 +601,34 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
                 tmem_st32(lanes + O_COL + c, o);
               }
             }
-            const float base_m = m == -INFINITY ? 0.f : m;
+            const float2 mul = make_float2(sl2, sl2), off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m, -m);
+            float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < KT; c += 64) {
               uint32_t pk[32];
 #pragma unroll
               for (int j = 0; j < 64; j += 2) {
-                const float p0 = ex2_approx(fmaf(sc[c + j], sl2, -base_m)), p1 = ex2_approx(fmaf(sc[c + j + 1], sl2, -base_m));
-                l += p0 + p1;
-                pk[j >> 1] = pack2(p0, p1, (const T*)nullptr);
+                float2 x = fma2(make_float2(at(c + j), at(c + j + 1)), mul, off);
+                x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                sums[j >> 1 & 1] = add2(sums[j >> 1 & 1], x);
+                pk[j >> 1] = pack2(x.x, x.y, (const T*)nullptr);
               }
-              __syncwarp();
               tmem_st32_async(lanes + (uint32_t)((g & 1) * KT + c / 2), pk);
             }
+            sums[0] = add2(sums[0], sums[1]);
+            l += sums[0].x + sums[0].y;
             tmem_st_wait();
           }
-          if (some || begin > 0 || end < KT) {
+          if (special) {
             // V rows that nobody sees become 0 (0 times whatever lay there must not count); where rows differ in what
             // they see, so do V's infinities and NaN, which the epilogue puts back for the rows that see them
-            const int e = v_entry(g);
+            const int e = g + 1 < n_tiles ? 2 * g + 2 : 2 * g + 1;
             if (ok) ok = mbar_wait(&full[e % plan.kv_bufs], (e / plan.kv_bufs) & 1, a.err, ERR_TIMEOUT_TMA);
             uint8_t* vb = kvs + (e % plan.kv_bufs) * BUF;
             for (int c = row; c < KT * (D / 8); c += 128) {
               const int k = c / (D / 8), ch = c % (D / 8);
-              uint4* at = reinterpret_cast<uint4*>(vb + (ch >> 3) * KT * 128 + sw128_off(k, ch & 7));
+              uint4* at = reinterpret_cast<uint4*>(vb + da_offset<NC>(k, ch));
               if (k < begin || k >= end) {
                 *at = make_uint4(0u, 0u, 0u, 0u);
               } else if (some) {
@@ -554,7 +651,8 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
             fence_proxy_async();
           }
           tc_fence_before();
-          mbar_arrive(&p_full[g & 1]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[g & 1]);
         }
         // ---- epilogue of the item, or of this piece's part of it ----
         if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
@@ -565,7 +663,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
         const int slot = 2 * piece + (item > 0 ? 1 : 0);
         float* part = partials + slot * da_partial_floats(D);
         const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-        const int64_t orow = (int64_t)(r.t0 + tok) * a.hq + walk.h * G + all % G;
+        const int64_t orow = (int64_t)(r.t0 + tok) * a.hq + walk.h * G + row % G;
         if (live) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -630,18 +728,27 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_ck, const __grid_consta
       }
     }
   }
-  // ---- teardown: roles are done or have given up; products and copies in flight end before the memory goes ----
+  // ---- teardown. If every role went through, every copy and product has been waited for. If one gave up, those still
+  // in flight end before the memory goes. ----
   __syncwarp();
-  if (warp == 0) {
-    for (int e = max(0, issued - plan.kv_bufs); e < issued; ++e)
-      mbar_wait(&full[e % plan.kv_bufs], (e / plan.kv_bufs) & 1, nullptr, 0);
-  }
-  if (tid == 32) {
-    mma_commit(all_done);
-    mbar_wait(all_done, 0, a.err, ERR_TIMEOUT_MMA);
-  }
   tc_fence_before();
-  __syncthreads();
+  if (!__syncthreads_and(ok)) {
+    if (warp == 0 || warp == 3) {
+      for (int e = max(0, issued - plan.kv_bufs); e < issued; ++e) {
+        const bool v_entry = (e > 0 && e % 2 == 0) || e == 2 * n_tiles - 1;
+        if (v_entry == (warp == 3)) mbar_wait(&full[e % plan.kv_bufs], (e / plan.kv_bufs) & 1, nullptr, 0);
+      }
+    } else if (warp == 2) {
+      for (int e = max(0, issued - plan.q_bufs); e < issued; ++e)
+        mbar_wait(&q_full[e % plan.q_bufs], (e / plan.q_bufs) & 1, nullptr, 0);
+    } else if (warp == 1) {
+      if (elect_one()) mma_commit(all_done);
+      __syncwarp();
+      mbar_wait(all_done, 0, nullptr, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, DA_TMEM_COLS);
@@ -653,15 +760,15 @@ constexpr int DJ_THREADS = 256;
 // Joins the parts of an item that was cut: one warp a row, parts in piece order. Block (c, y): the item that begins in
 // piece c, rows 8 y .. 8 y + 7.
 template <int D, typename T>
-__global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_constant__ DraftAttnArgs a,
+__global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_constant__ DraftAttnArgs a, int block,
                                                                 const DaSplit* splits, const float* partials) {
   pdl_wait();
   const int c = blockIdx.x, lane = threadIdx.x & 31;
   const DaSplit s = splits[c];
   if (s.last < 0) return;
   const int row = blockIdx.y * (DJ_THREADS / 32) + (threadIdx.x >> 5), G = a.hq / a.hkv;
-  const int all = s.block * DA_ROWS + row, tok = all / G, t0 = a.cu[s.b];
-  if (tok >= a.cu[s.b + 1] - t0) return;
+  const int tok = s.block * block + row / G, t0 = a.cu[s.b];
+  if (row >= block * G || tok >= a.cu[s.b + 1] - t0) return;
   const size_t size = da_partial_floats(D);
   auto part = [&](int p) { return partials + (p == c ? (size_t)s.first_slot : 2 * (size_t)p) * size; };
   float m = -INFINITY;
@@ -683,7 +790,7 @@ __global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_con
     for (int e = 0; e < D / 32; ++e) o[e] += w * x[row * D + e * 32 + lane];
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-  const int64_t orow = (int64_t)(t0 + tok) * a.hq + s.h * G + all % G;
+  const int64_t orow = (int64_t)(t0 + tok) * a.hq + s.h * G + row % G;
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) ((T*)a.out)[orow * D + e * 32 + lane] = (T)(o[e] * inv);
   if (lane == 0 && a.lse) a.lse[orow] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
