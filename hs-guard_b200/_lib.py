@@ -83,7 +83,7 @@ def lib():
             "hsg_gemm": [P, I, I, P, P, I, I, P, P, P, I, I, P, P],
             "hsg_gemm_f32_noalloc": [P, I, I, P, I, P, P, P, I, I, P, P],
             "hsg_check_bounded_wait": [I, C.POINTER(C.c_double)],
-            # draft scoring: one argument struct each (hs_guard_b200.drafts packs it)
+            # draft scoring: one argument struct each
             "hsg_advance_tables": [C.c_char_p],
             "hsg_plan_tree": [C.c_char_p],
             "hsg_norm_rope": [C.c_char_p],

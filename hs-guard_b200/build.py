@@ -1,9 +1,10 @@
-"""Build libhsg.so (all CUDA kernels + the C ABI of include/hsg.h) in-tree for sm_100a with nvcc, and the host
-fast-path module _hsg_host (csrc/hsg_host.c, CPython C API) with the C compiler.
+"""Build libhsg.so (all CUDA kernels + the C ABI of include/hsg.h) in-tree for sm_100a with nvcc, the host fast-path
+module _hsg_host (csrc/hsg_host.c, CPython C API) with the C compiler, and the tensor module _hsg_torch
+(csrc/hsg_torch.cpp, torch's C++ tensors over libhsg.so) with the C++ compiler.
 
     python -m hs_guard_b200.build [--force] [--verbose]
 
-Both are written next to this file so they travel with the source tree; the library links the CUDA runtime
+All are written next to this file so they travel with the source tree; the library links the CUDA runtime
 statically and resolves the driver's tensor-map encoder at run time, so it needs no libcuda at link time.
 """
 from __future__ import annotations
@@ -24,6 +25,8 @@ MAIN = os.path.join(HERE, "csrc", "hsg_api.cu")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
          "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include")]
 HOST_SRC = os.path.join(HERE, "csrc", "hsg_host.c")
+TORCH_SRC = os.path.join(HERE, "csrc", "hsg_torch.cpp")
+TORCH_LIB = os.path.join(HERE, "_hsg_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 HOST_LIB = os.path.join(HERE, "_hsg_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
@@ -83,8 +86,49 @@ def host():
     return _HOST
 
 
+def build_torch(force=False):
+    """Compile the _hsg_torch extension module when it is missing or older than its sources. It finds libhsg.so beside
+    itself and torch's libraries where they are now."""
+    sources = (TORCH_SRC, os.path.join(ROOT, "include", "hsg.h"))
+    if not force and os.path.exists(TORCH_LIB) and all(os.path.getmtime(TORCH_LIB) >= os.path.getmtime(f) for f in sources):
+        return TORCH_LIB
+    build()
+    import torch
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("no C++ compiler for " + TORCH_SRC)
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    tmp = "%s.%d.tmp" % (TORCH_LIB, os.getpid())
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-isystem", os.path.join(home, "include"),
+           "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"), "-isystem", cuda,
+           "-isystem", sysconfig.get_paths()["include"], "-o", tmp, TORCH_SRC, "-L" + HERE, "-l:libhsg.so", "-Wl,-rpath,$ORIGIN",
+           "-L" + os.path.join(home, "lib"), "-Wl,-rpath," + os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("building _hsg_torch failed:\n" + res.stdout + res.stderr)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
+_TORCH = None
+
+
+def tensors():
+    """The _hsg_torch module (built first if needed); raises if it cannot be built or loaded."""
+    global _TORCH
+    if _TORCH is None:
+        build_torch()
+        _TORCH = importlib.import_module("hs_guard_b200._hsg_torch")
+    return _TORCH
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="--verbose" in sys.argv)
     build_host(force="--force" in sys.argv)
+    build_torch(force="--force" in sys.argv)
+    print(TORCH_LIB)
     print(LIB)
     print(HOST_LIB)

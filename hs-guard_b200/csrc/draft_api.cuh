@@ -44,7 +44,9 @@ static_assert(DT_MAX_ROWS == HSG_MAX_TABLE_ROWS, "the header states the kernel's
 
 template <int D, typename TI, typename TO>
 int launch_norm(const DraftNormArgs& n, cudaStream_t st) {
-  draft_norm_kernel<D, TI, TO><<<n.tokens, DN_THREADS, 0, st>>>(n);
+  // tokens a block: one unit of every head, as long as that leaves four blocks an SM
+  const int per = std::max(1, std::min(DN_LIVE, n.tokens / (4 * SM_COUNT)));
+  draft_norm_kernel<D, TI, TO><<<(n.tokens + per - 1) / per, DN_THREADS, per * (n.rot / 2) * sizeof(float2), st>>>(n, per);
   CU(cudaGetLastError());
   return HSG_OK;
 }
@@ -156,9 +158,15 @@ extern "C" int hsg_advance_tables(const hsg_tables_args* a) {
   if ((a->rows && a->lens_out == a->lens) || a->counters_out == a->counters)
     return fail(HSG_ERR_INVALID, "lens_out and counters_out must not be the inputs");
   DraftTablesArgs t{a->lens, a->delta, a->table, a->table_stride, a->ring, a->counters, a->rows, a->width,
-                    a->ring_size, a->page_size, a->lens_out, a->counters_out, a->cu, a->slots, a->token_rows,
-                    a->positions, a->capacity, a->err};
-  draft_tables_kernel<<<1, DT_THREADS, 0, (cudaStream_t)a->stream>>>(t);
+                    a->ring_size, FastDiv::of(a->page_size), a->lens_out, a->counters_out, a->cu, a->slots,
+                    a->token_rows, a->positions, a->capacity, a->err};
+  const int smem = 3 * a->rows * (int)sizeof(int);
+  if (smem > 48 * 1024 - 1024)
+    CU(cudaFuncSetAttribute(draft_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * DT_MAX_ROWS * 4));
+  // a block for 4,096 listed tokens or 8,192 table entries, any of which may change hands
+  const int64_t share = std::max<int64_t>(a->capacity / (4 * DT_THREADS), (int64_t)a->rows * a->width / (8 * DT_THREADS));
+  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(SM_COUNT, share));
+  draft_tables_kernel<<<blocks, DT_THREADS, smem, (cudaStream_t)a->stream>>>(t);
   CU(cudaGetLastError());
   return HSG_OK;
 }
@@ -189,6 +197,8 @@ extern "C" int hsg_norm_rope(const hsg_norm_rope_args* a) {
     return fail(HSG_ERR_INVALID, "NULL argument");
   if (!a->slots && (!a->k_out || !a->v_out)) return fail(HSG_ERR_INVALID, "k_out and v_out, or slots, are needed");
   const int bytes = a->in_dtype == HSG_DT_F32 ? 4 : 2;
+  if (!aligned16(a->q_weight) || !aligned16(a->k_weight))
+    return fail(HSG_ERR_INVALID, "q_weight and k_weight must lie on 16-byte boundaries");
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) ||
       !rows16(a->q_token_stride, a->q_head_stride, bytes) || !rows16(a->k_token_stride, a->k_head_stride, bytes) ||
       !rows16(a->v_token_stride, a->v_head_stride, bytes) || (!a->slots && (!aligned16(a->k_out) || !aligned16(a->v_out))))
@@ -262,8 +272,12 @@ extern "C" int hsg_store_rows(const hsg_store_args* a) {
   int rc;
   if ((rc = check_cache(a->cache, a->heads, a->dim)) != HSG_OK) return rc;
   DraftStoreArgs s{a->k, a->v, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->source,
-                   a->slots, a->count, a->rows, a->heads, a->dim, page_cache(a->cache), a->err};
-  draft_store_kernel<<<a->count, DS_THREADS, 0, (cudaStream_t)a->stream>>>(s);
+                   a->slots, a->count, a->rows, a->heads, page_cache(a->cache), a->err};
+  const int blocks = (a->count + DS_THREADS / 32 - 1) / (DS_THREADS / 32);
+  cudaStream_t st = (cudaStream_t)a->stream;
+  if (a->dim == 64) draft_store_kernel<64><<<blocks, DS_THREADS, 0, st>>>(s);
+  else if (a->dim == 128) draft_store_kernel<128><<<blocks, DS_THREADS, 0, st>>>(s);
+  else draft_store_kernel<256><<<blocks, DS_THREADS, 0, st>>>(s);
   CU(cudaGetLastError());
   return HSG_OK;
 }

@@ -75,72 +75,94 @@ __device__ __forceinline__ void rotation(int position, float freq, float& s, flo
   sincosf((float)fma(-kTurn, rint(angle * (1.0 / kTurn)), angle), &s, &c);
 }
 
-constexpr int DN_THREADS = 256;
+constexpr int DN_THREADS = 128;
+constexpr int DN_LIVE = 4;  // tokens a lane has under way
 
-// One thread block a token. dim / 8 lanes share a head, eight consecutive elements each, so a warp works on 256 / dim
-// heads at once; the rotation's partner (d and d + rot / 2) is rot / 16 lanes away.
+// dim / 8 lanes share a head, eight consecutive elements each, so a warp works on 256 / dim heads at once; the
+// rotation's partner (d and d + rot / 2) is rot / 16 lanes away. A block takes `per` tokens: their angles once into
+// shared memory, then units of (a warp's heads, DN_LIVE tokens) spread over its warps, so that what depends on the head
+// (kind, addresses, weights) is found once for DN_LIVE tokens. Measured at 22,528 tokens of 12 fp32 heads of 256 (415 MB):
+// 73 us, 5.7 TB/s, bound by HBM; units of one head and token, whose index is divided by the head count at every step,
+// took 110 us (instructions), blocks of 256 threads 81 us at 8 tokens and 86 us at 16 (a last wave partly empty).
 template <int D, typename TI, typename TO>
-__global__ void __launch_bounds__(DN_THREADS) draft_norm_kernel(const DraftNormArgs a) {
-  __shared__ float s_cos[D / 2], s_sin[D / 2];
-  constexpr int LPH = D / 8;
-  const int64_t t = blockIdx.x;
-  const int half = a.rot / 2;
-  for (int i = threadIdx.x; i < half; i += DN_THREADS) rotation(a.positions[t], a.inv_freq[i], s_sin[i], s_cos[i]);
-  __syncthreads();
-  const int heads = a.hq + 2 * a.hkv, j = threadIdx.x % LPH;
-  // every thread of a warp takes part in the shuffles: the loop's trip count is the warp's
-  for (int base = 0; base < heads; base += DN_THREADS / LPH) {
-    const int h = base + threadIdx.x / LPH;
-    const bool live = h < heads;
+__global__ void __launch_bounds__(DN_THREADS) draft_norm_kernel(const __grid_constant__ DraftNormArgs a, int per) {
+  extern __shared__ float2 s_turn[];  // [per][rot / 2] (cos, sin)
+  constexpr int LPH = D / 8, HPW = 32 / LPH, WARPS = DN_THREADS / 32;
+  const int t0 = blockIdx.x * per, tokens = min(per, a.tokens - t0), half = a.rot / 2;
+  const int heads = a.hq + 2 * a.hkv, groups = (heads + HPW - 1) / HPW;
+  const int units = groups * ((tokens + DN_LIVE - 1) / DN_LIVE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LPH * 8;
+  const bool first = d < half, in_rot = d < a.rot;
+  const int partner = in_rot ? (first ? lane + half / 8 : lane - half / 8) : lane, f = first ? d : d - half;
+  bool turned = false;  // the angles are there
+  for (int unit = warp; unit < units || !turned; unit += WARPS) {
+    const int chunk = unit / groups, h = (unit - chunk * groups) * HPW + lane / LPH, c0 = chunk * DN_LIVE;
+    const int live = unit < units && h < heads ? min(DN_LIVE, tokens - c0) : 0;
     const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.hkv;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const TI* src = is_q ? (const TI*)a.q + t * a.q_ts + h * a.q_hs
-                           : is_k ? (const TI*)a.k + t * a.k_ts + (h - a.hq) * a.k_hs
-                                  : (const TI*)a.v + t * a.v_ts + (h - a.hq - a.hkv) * a.v_hs;
-      load8(src + j * 8, x);
-    }
-    float ss = 0.f;
+    const int g = is_q ? h : is_k ? h - a.hq : h - a.hq - a.hkv;  // index among its kind
+    const int64_t ts = is_q ? a.q_ts : is_k ? a.k_ts : a.v_ts;
+    const TI* src = (const TI*)(is_q ? a.q : is_k ? a.k : a.v) + (t0 + c0) * ts + g * (is_q ? a.q_hs : is_k ? a.k_hs : a.v_hs) + d;
+    float x[DN_LIVE][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    for (int u = 0; u < DN_LIVE; ++u) {
+      if (u < live) {
+        load8(src + u * ts, x[u]);
+      } else {
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (is_q || is_k) {
-      const float r = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-      const float* w = (is_q ? a.qw : a.kw) + j * 8;
+        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+      }
+    }
+    float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    if (live && (is_q || is_k)) load8((is_q ? a.qw : a.kw) + d, w);
+    if (!turned) {  // while the first heads are on their way
+      for (int i = threadIdx.x; i < tokens * half; i += DN_THREADS) {
+        const int t = i / half;
+        rotation(a.positions[t0 + t], a.inv_freq[i - t * half], s_turn[i].y, s_turn[i].x);
+      }
+      __syncthreads();
+      turned = true;
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-    }
-    const int d = j * 8, lane = threadIdx.x & 31;
-    const bool first = d < half, turned = d < a.rot && (is_q || is_k);
-    const int partner = d < a.rot ? (first ? lane + half / 8 : lane - half / 8) : lane;
-    float y[8];
+    for (int u = 0; u < DN_LIVE; ++u) {
+      if (__any_sync(0xffffffffu, u < live && (is_q || is_k))) {  // every lane of the warp takes part in the shuffles
+        float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
-    if (turned) {
-      const int f = first ? d : d - half;
+        for (int i = 0; i < 8; ++i) ss += x[u][i] * x[u][i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = first ? x[i] * s_cos[f + i] - y[i] * s_sin[f + i] : x[i] * s_cos[f + i] + y[i] * s_sin[f + i];
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = is_q || is_k ? rsqrtf(ss * (1.0f / D) + a.eps) : 1.f;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * r * w[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[u][i], partner);
+        if (in_rot && u < live && (is_q || is_k)) {
+          const float4* cs = reinterpret_cast<const float4*>(s_turn + (c0 + u) * half + f);
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float4 v = cs[i / 2];
+            x[u][i] = fmaf(first ? -y[i] : y[i], v.y, x[u][i] * v.x);
+            x[u][i + 1] = fmaf(first ? -y[i + 1] : y[i + 1], v.w, x[u][i + 1] * v.z);
+          }
+        }
+      }
+      if (u >= live) continue;
+      const int64_t tok = t0 + c0 + u;
+      if (is_q) {
+        store8((TO*)a.q_out + (tok * a.hq + g) * D + d, x[u]);
+      } else if (!a.slots) {
+        store8((TO*)(is_k ? a.k_out : a.v_out) + (tok * a.hkv + g) * D + d, x[u]);
+      } else {
+        const int slot = a.slots[tok], page = slot / a.cache.page;
+        if (slot < 0) continue;
+        if (page >= a.cache.pages) {
+          if (d == 0) set_error(a.err, ERR_BAD_SLOT);
+          continue;
+        }
+        store8((TO*)(is_k ? a.cache.k : a.cache.v) + page * a.cache.page_stride +
+                   (slot - page * a.cache.page) * a.cache.token_stride + g * a.cache.head_stride + d, x[u]);
+      }
     }
-    if (!live) continue;
-    if (is_q) {
-      store8((TO*)a.q_out + (t * a.hq + h) * D + d, x);
-      continue;
-    }
-    const int g = is_k ? h - a.hq : h - a.hq - a.hkv;
-    if (!a.slots) {
-      store8((TO*)(is_k ? a.k_out : a.v_out) + (t * a.hkv + g) * D + d, x);
-      continue;
-    }
-    const int slot = a.slots[t], page = slot / a.cache.page;
-    if (slot < 0) continue;
-    if (page >= a.cache.pages) {
-      if (j == 0) set_error(a.err, ERR_BAD_SLOT);
-      continue;
-    }
-    store8((TO*)(is_k ? a.cache.k : a.cache.v) + page * a.cache.page_stride +
-               (slot - page * a.cache.page) * a.cache.token_stride + g * a.cache.head_stride + d, x);
   }
 }
 
@@ -149,32 +171,44 @@ struct DraftStoreArgs {
   int64_t k_ts, k_hs, v_ts, v_hs;
   const int32_t* source;  // [count] row of k and v for each entry, or NULL: row i
   const int32_t* slots;   // [count]; < 0: not kept
-  int count, rows, heads, dim;
+  int count, rows, heads;
   PageCache cache;
   int* err;
 };
 
 constexpr int DS_THREADS = 256;
+constexpr int DS_LIVE = 8;  // 16-byte pieces a lane has under way
 
-// One thread block an entry: its K and V rows in 16-byte pieces.
-__global__ void __launch_bounds__(DS_THREADS) draft_store_kernel(const DraftStoreArgs a) {
-  const int i = blockIdx.x;
+// One warp an entry: its K and V rows in 16-byte pieces, DS_LIVE requested by a lane before the first is written. Bound
+// by HBM: 30,000 entries of 2 x 2 KB (246 MB in and out) take 42 us, 5.9 TB/s; one block an entry took 59 us.
+template <int D>
+__global__ void __launch_bounds__(DS_THREADS) draft_store_kernel(const __grid_constant__ DraftStoreArgs a) {
+  constexpr int PER = D / 8;  // pieces a head
+  const int i = blockIdx.x * (DS_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= a.count) return;
   const int slot = a.slots[i], page = slot / a.cache.page;
   const int src = a.source ? a.source[i] : i;
   if (slot < 0) return;
   if (page >= a.cache.pages || src < 0 || src >= a.rows) {
-    if (threadIdx.x == 0) set_error(a.err, ERR_BAD_SLOT);
+    if (lane == 0) set_error(a.err, ERR_BAD_SLOT);
     return;
   }
   const int64_t to = page * a.cache.page_stride + (slot - page * a.cache.page) * a.cache.token_stride;
-  const int per = a.dim / 8, n = a.heads * per;
-  for (int c = threadIdx.x; c < 2 * n; c += DS_THREADS) {
-    const bool is_v = c >= n;
-    const int h = (is_v ? c - n : c) / per, d = (c % per) * 8;
-    const uint16_t* from = (const uint16_t*)(is_v ? a.v : a.k) + (int64_t)src * (is_v ? a.v_ts : a.k_ts) +
-                           h * (is_v ? a.v_hs : a.k_hs) + d;
-    *reinterpret_cast<uint4*>((uint16_t*)(is_v ? a.cache.v : a.cache.k) + to + h * a.cache.head_stride + d) =
-        *reinterpret_cast<const uint4*>(from);
+  const uint16_t *k = (const uint16_t*)a.k + src * a.k_ts, *v = (const uint16_t*)a.v + src * a.v_ts;
+  const int n = a.heads * PER;
+  for (int base = lane; base < 2 * n; base += 32 * DS_LIVE) {
+    uint4 x[DS_LIVE];
+#pragma unroll
+    for (int u = 0; u < DS_LIVE; ++u) {
+      const int c = base + 32 * u, p = c < n ? c : c - n, h = p / PER, d = p % PER * 8;
+      if (c < 2 * n) x[u] = *reinterpret_cast<const uint4*>(c < n ? k + h * a.k_hs + d : v + h * a.v_hs + d);
+    }
+#pragma unroll
+    for (int u = 0; u < DS_LIVE; ++u) {
+      const int c = base + 32 * u, p = c < n ? c : c - n, h = p / PER, d = p % PER * 8;
+      if (c < 2 * n)
+        *reinterpret_cast<uint4*>((uint16_t*)(c < n ? a.cache.k : a.cache.v) + to + h * a.cache.head_stride + d) = x[u];
+    }
   }
 }
 

@@ -1,8 +1,18 @@
 """Draft scoring on the host: argument checks of the C entry points and of the Python layer, no GPU."""
+import struct
+
 import pytest
 import torch
 
 from hs_guard_b200 import _lib, drafts
+
+# the argument structs of include/hsg.h as a host without a C compiler packs them ("0q" pads the end as C does)
+CACHE = "PPqqqii"
+TABLES = struct.Struct("@qPPPqPPPPPPPPPPiiiii0q")
+TREE = struct.Struct("@qPPPPPPPiii0q")
+NORM = struct.Struct("@qPPPqqqqqqPPPPPPPP" + CACHE + "PPiiiiiiif0q")
+ATTENTION = struct.Struct("@qPPPqqqqqq" + CACHE + "PqPPPPPPPqPPiiiiiiiiiif0q")
+STORE = struct.Struct("@qPPqqqqPP" + CACHE + "PPiiii0q")
 
 
 @pytest.fixture(scope="module")
@@ -12,8 +22,8 @@ def L():
     return _lib.lib()
 
 
-PACKS = [("hsg_advance_tables", drafts._TABLES), ("hsg_plan_tree", drafts._TREE), ("hsg_norm_rope", drafts._NORM),
-         ("hsg_tree_attention", drafts._ATTENTION), ("hsg_store_rows", drafts._STORE)]
+PACKS = [("hsg_advance_tables", TABLES), ("hsg_plan_tree", TREE), ("hsg_norm_rope", NORM),
+         ("hsg_tree_attention", ATTENTION), ("hsg_store_rows", STORE)]
 
 
 @pytest.mark.parametrize("name,pack", PACKS, ids=[n for n, _ in PACKS])
@@ -35,7 +45,7 @@ def _attention(**kw):
              page=16, table=16, tstride=2, lens=16, cu=16, mask=16, out=16, lse=16, ws=16, wsb=1 << 40, rows=1, width=2, tokens=3,
              words=1, max_tree=3, hq=8, hkv=2, dim=128, dtype=1, scale=1.0)
     a.update(kw)
-    return drafts._ATTENTION.pack(drafts._ATTENTION.size, *(a[f] for f in fields))
+    return ATTENTION.pack(ATTENTION.size, *(a[f] for f in fields))
 
 
 @pytest.mark.parametrize("bad", [
@@ -52,13 +62,13 @@ def test_tree_attention_refuses(L, bad):
 def test_a_call_without_work_does_nothing(L):
     assert L.hsg_tree_attention(_attention(tokens=0)) == _lib.HSG_OK
     assert L.hsg_tree_attention(_attention(rows=0)) == _lib.HSG_OK
-    assert L.hsg_plan_tree(drafts._TREE.pack(drafts._TREE.size, *[0] * 7, 4, 0, 1)) == _lib.HSG_OK
+    assert L.hsg_plan_tree(TREE.pack(TREE.size, *[0] * 7, 4, 0, 1)) == _lib.HSG_OK
 
 
 def test_advance_tables_refuses_aliased_outputs(L):
     def call(lens_out=48, counters_out=64, lens=16, counters=32, rows=1, ring=4, page=16, capacity=0):
-        return L.hsg_advance_tables(drafts._TABLES.pack(
-            drafts._TABLES.size, lens, 16, 16, 2, 16, counters, lens_out, counters_out, 16, 16, 16, 16, 0, 0, rows, 2, ring,
+        return L.hsg_advance_tables(TABLES.pack(
+            TABLES.size, lens, 16, 16, 2, 16, counters, lens_out, counters_out, 16, 16, 16, 16, 0, 0, rows, 2, ring,
             page, capacity))
     assert call(lens_out=16) == _lib.HSG_ERR_INVALID
     assert call(counters_out=32) == _lib.HSG_ERR_INVALID
