@@ -32,6 +32,7 @@ PageCache page_cache(const hsg_page_cache& c) {
   return PageCache{c.k, c.v, c.page_stride, c.token_stride, c.head_stride, c.pages, c.page_size};
 }
 
+static_assert(DA_PIECES == SM_COUNT, "one piece an SM");
 static_assert(DT_MAX_ROWS == HSG_MAX_TABLE_ROWS, "the header states the kernel's limit");
 
 #define DRAFT_ARGS(a)                                                                                  \
@@ -82,14 +83,25 @@ int make_rows_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, 
 }
 
 // As many whole drafted tokens as fit 128 rows; Q double-buffered up to 64 KB, the rest of shared memory for K and V.
-DaPlan plan_draft_attn(int max_tree, int group, int dim) {
+// Boxes of the cache: 8 tokens with page, head, 64-dim block, token and dim as the five dimensions that a map may have.
+// Several 8-token groups at a constant stride need a dimension of their own, which the heads give up where they continue
+// another: the 64-dim blocks, if a token's heads are contiguous (fold 1), or the groups, if a head's rows begin a whole
+// number of groups after the last head's (fold 2). Then a box takes up to 8 KB, as far as the page size divides.
+DaPlan plan_draft_attn(int max_tree, int group, int dim, int heads, const PageCache& c) {
   DaPlan p;
+  const int64_t eight = 8 * c.token_stride;
+  p.groups = 1;
+  while (p.groups * 2 * 16 * dim <= DA_BOX_BYTES && 16 * p.groups <= da_tile(dim) && c.page % (16 * p.groups) == 0) p.groups *= 2;
+  p.fold = p.groups == 1 ? 0 : heads == 1 || c.head_stride == dim ? 1 : c.head_stride % eight == 0 ? 2 : 0;
+  if (p.fold == 0) p.groups = 1;
+  p.head_step = p.fold == 1 ? dim / 64 : p.fold == 2 ? (int)(c.head_stride / eight) : 0;
   p.block = std::min(max_tree, DA_ROWS / group);
   p.q_rows = (p.block * group + 7) / 8 * 8;
   const int q = p.q_rows * dim * 2;
   p.q_bufs = q <= 32768 ? 2 : 1;
-  p.kv_bufs = std::min(12, (DA_SMEM_LIMIT - 1536 - p.q_bufs * q) / da_buffer_bytes(dim));
-  p.pieces = SM_COUNT;
+  const int bufs = std::min(2 * DA_MAX_BUFS, (DA_SMEM_LIMIT - 1024 - da_extra(dim, p.block) - p.q_bufs * q) / da_buffer_bytes(dim));
+  p.k_bufs = bufs / 2;
+  p.v_bufs = bufs - p.k_bufs;
   return p;
 }
 
@@ -99,8 +111,8 @@ int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) 
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   constexpr int NC = D / 64;
   const int group = d.hq / d.hkv;
-  const DaPlan p = plan_draft_attn(d.max_tree, group, D);
   const PageCache& c = d.cache;
+  const DaPlan p = plan_draft_attn(d.max_tree, group, D, d.hkv, c);
   CUtensorMap q, ck, cv, k, v;
   int rc;
   {
@@ -109,8 +121,12 @@ int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) 
     if ((rc = make_rows_map(&q, d.q, type, 3, sizes, strides, boxes)) != HSG_OK) return rc;
   }
   {
-    const int64_t sizes[5] = {64, c.page, NC, d.hkv, c.pages}, strides[5] = {1, c.token_stride, 64, c.head_stride, c.page_stride};
-    const int boxes[5] = {64, 8, NC, 1, 1};
+    const int64_t own[5] = {64, c.page, NC, d.hkv, c.pages}, own_strides[5] = {1, c.token_stride, 64, c.head_stride, c.page_stride};
+    const int64_t folded[5] = {64, 8, p.fold == 1 ? NC * d.hkv : NC,
+                               c.page / 8 + (p.fold == 2 ? (int64_t)(d.hkv - 1) * p.head_step : 0), c.pages};
+    const int64_t folded_strides[5] = {1, c.token_stride, 64, 8 * c.token_stride, c.page_stride};
+    const int64_t *sizes = p.fold ? folded : own, *strides = p.fold ? folded_strides : own_strides;
+    const int boxes[5] = {64, 8, NC, p.fold ? p.groups : 1, 1};
     if ((rc = make_rows_map(&ck, c.k, type, 5, sizes, strides, boxes)) != HSG_OK ||
         (rc = make_rows_map(&cv, c.v, type, 5, sizes, strides, boxes)) != HSG_OK)
       return rc;
@@ -124,12 +140,12 @@ int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) 
       return rc;
   }
   DaSplit* splits = static_cast<DaSplit*>(workspace);
-  float* partials = reinterpret_cast<float*>(splits + p.pieces);
+  float* partials = reinterpret_cast<float*>(splits + DA_PIECES);
   CU(cudaFuncSetAttribute(draft_attn_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, DA_SMEM_LIMIT));
-  draft_attn_kernel<D, T><<<p.pieces, DA_THREADS, da_smem_bytes(p, D), st>>>(q, ck, cv, k, v, d, p, splits, partials);
+  draft_attn_kernel<D, T><<<DA_PIECES, DA_THREADS, da_smem_bytes(p, D), st>>>(q, ck, cv, k, v, d, p, splits, partials);
   CU(cudaGetLastError());
   const int rows = p.q_rows;
-  CU(launch_k(draft_join_kernel<D, T>, dim3(p.pieces, (rows + DJ_THREADS / 32 - 1) / (DJ_THREADS / 32)),
+  CU(launch_k(draft_join_kernel<D, T>, dim3(DA_PIECES, (rows + DJ_THREADS / 32 - 1) / (DJ_THREADS / 32)),
               dim3(DJ_THREADS), 0, st, true, d, p.block, (const DaSplit*)splits, (const float*)partials));
   return HSG_OK;
 }
@@ -218,7 +234,7 @@ extern "C" int hsg_norm_rope(const hsg_norm_rope_args* a) {
 }
 
 extern "C" size_t hsg_tree_attention_workspace(int head_dim) {
-  return head_dim_ok(head_dim) ? da_workspace_bytes(head_dim, SM_COUNT) : 0;
+  return head_dim_ok(head_dim) ? da_workspace_bytes(head_dim) : 0;
 }
 
 extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {

@@ -33,46 +33,73 @@ struct DraftAttnArgs {
 
 // One kernel for every shape, on tcgen05. The drafted tokens of a request that share a key head are the rows of a matrix
 // product, row r = (token r / G, query head r % G of the group of G); as many whole tokens as fit 128 rows and all of a
-// request's keys in tiles of KT (128, or 64 at head dim 256) are an item (request, key head, block of tokens). All items' tiles, in order, are one
-// line that is cut into equal pieces, one a thread block, whatever the requests' lengths, so a long cache is split over
-// many SMs and short ones share one; the lengths are read on the device. An item that lies in one piece is written
+// request's keys in tiles of KT (128, or 64 at head dim 256) are an item (request, key head, block of tokens). All items,
+// in order, are one line, an item up to DA_ITEM_COST units (its set-up and epilogue) and then a unit a tile long, that is cut
+// into equal pieces, one a thread block, whatever the requests' lengths, so a long cache is split over many SMs and short
+// ones share one; the lengths are read on the device. (Without the units for items, pieces with many short ones ran up to
+// half as long again as the mean.) An item that lies in one piece is written
 // out; of one that is cut, each piece leaves its unnormalised sums, row maxima and row sums in the workspace and
 // draft_join_kernel joins them in piece order, so results do not depend on timing.
 //
 // Per tile: S = Q K^T (tcgen05, TMEM), softmax with a running maximum in registers (a row a thread), P in the type of V
-// written over S in TMEM, O += P V (A = P from TMEM, B = V as it lies in shared memory, N-major). Warps 0 and 3 bring K
-// and V tiles by TMA, eight tokens of one page a box, through one ring of buffers in the order in which the products use
-// them; warp 1 issues the products, S of the next tile before P V of this one; warp 2 brings Q; warps 4-7 do the
-// softmax and the epilogue. A K or V tile lies in shared memory as [8 keys][dim / 64][8][128 B], 128-byte swizzle: boxes
-// of any page size then sit at one stride, which is all that a product's descriptor can say. Warp 1 runs as a whole warp
-// with one elected lane at each group of products, so that their descriptors stay in uniform registers: issued from a
-// branch on the lane, each took about 150 cycles. Copies are the other way round: 32 lanes with a box each take 64 to 95
-// cycles a box (1 to 4 KB), one elected lane in a loop over boxes 135 to 240, and one warp alone falls short of HBM. Tiles of the next item are under way during an item's epilogue.
+// written over S in TMEM, O += P V (A = P from TMEM, B = V as it lies in shared memory, N-major). Warps:
+//   0   K tiles, and Q of each item; 3: V tiles: TMA, tokens of one page a box, each through a ring of buffers, with a word
+//       for each tile that says what the product has to know
+//   1   S, up to NS tiles ahead of P V;  2: P V
+//   4-7 the softmax of even tiles, 8-11 that of odd ones, one handing the rows' maxima on to the other before its
+//       exponentials; whichever has an item's last tile writes the result, while the other goes on to the next item.
+//       Warp 3 tells them what an item is, its tokens' positions and first mask words, an item ahead.
+// A K or V tile lies in shared memory as [8 keys][dim / 64][8][128 B], 128-byte swizzle: boxes of any page size then sit at
+// one stride, which is all that a product's descriptor can say.
 //
-// S, P and P V of a tile each have two barriers, for even and odd tiles: a wait tells a phase from its neighbours only,
-// and whoever waits for tile g of one of them knows tile g - 2 to be done and g + 2 to be impossible before it goes on
-// (S of tile g + 2 is issued after P of tile g has been waited for, and its commit covers every product before it).
+// What was measured on the way (cycles a tile of 128 rows and 128 keys at head dim 128):
+//  - products issued from a branch on the lane took about 150 each, since their descriptors are then not uniform; a whole
+//    warp that elects a lane for a tile's products issues them at the tensor cores' rate (64 a 128 x 128 x 16 step; issue
+//    blocks at that rate).
+//  - one warp for S and P V was the bottleneck: 1,600 of products and 1,400 of waits and bookkeeping between them in one
+//    line. Hence two warps, and words written by the copying warps instead of a walk over requests.
+//  - copies are the other way round: 32 lanes with a box each take 64 to 136 cycles a box (1 to 8 KB, 8 to 64 rows of 128
+//    bytes), one elected lane in a loop over boxes 135 to 240. Boxes of 8 tokens at head dim 128 (2 KB) bound a tile of K
+//    and V at 2,400 cycles, short of HBM: hence boxes of several 8-token groups where page size and strides allow one map to
+//    describe them (plan_draft_attn).
+//  - two buffers of S put softmax, P V and S of a group's next tile in one line; NS = 3 or 4 take S out of it.
 //
 // The weights are rounded to V's type for the second product (relative 2^-11 or 2^-8 each, as the result itself is);
 // scores, maxima, sums and O are fp32, and the row sum adds the weights before they are rounded.
-constexpr int DA_THREADS = 256;
+//
+// A wait tells a barrier's phase from its neighbours only. S, P and P V of tile g use barrier g % NS: S of tile g waits for
+// P V of tile g - NS, which waited for P of that tile, which its softmax wrote after it had read S; so whoever waits there
+// for tile g knows tile g - NS to be done and g + NS to be impossible before it goes on. The rows' maxima of tile g use the
+// barrier of its group: who waits for it has waited for g - 2 and is itself needed for g + 2. The rings of K, V and Q have
+// one warp that fills them and one that empties them, both in order.
+constexpr int DA_THREADS = 384;
 constexpr int DA_ROWS = 128;
-constexpr int DA_MIN_TILES = 2;       // a piece is at least this long
+constexpr int DA_PIECES = 148;        // one thread block an SM
+constexpr int DA_ITEM_COST = 3;       // what an item costs besides its tiles, in tiles, where pieces are long
 constexpr int DA_SMEM_LIMIT = 227 * 1024;
-constexpr uint32_t DA_TMEM_COLS = 512;  // S (later P) of even and odd tiles, then O
+constexpr int DA_MAX_BUFS = 6;
+constexpr int DA_BARS = 4 * DA_MAX_BUFS + 37;
+constexpr int DA_BOX_BYTES = 8192;     // of a TMA box of the cache, at most
+constexpr uint32_t DA_TMEM_COLS = 512;  // da_scores buffers of S (later P), then O
 
 __host__ __device__ constexpr int da_tile(int dim) { return dim == 256 ? 64 : 128; }
+__host__ __device__ constexpr int da_scores(int dim) { return dim == 256 ? 4 : 3; }
+// barriers, items, row maxima and sums, and for each token of two items its position and first mask words
+__host__ __device__ constexpr int da_extra(int dim, int block) { return 4608 + 8 * block * (1 + da_tile(dim) / 32); }
 __host__ __device__ constexpr int da_buffer_bytes(int dim) { return da_tile(dim) * dim * 2; }
 
 struct DaPlan {  // launch shape, chosen by the host
   int block;     // drafted tokens of an item: at most 128 rows
   int q_rows;    // rows a Q buffer holds: block * G rounded up to a multiple of 8
   int q_bufs;
-  int kv_bufs;
-  int pieces;    // thread blocks
+  int k_bufs, v_bufs;  // at most DA_MAX_BUFS each
+  int fold;      // how the cache's maps tell heads apart: 0 by a dimension of their own (boxes of 8 tokens), 1 by the dimension
+                 // of 64-dim blocks, 2 by the dimension of 8-token groups (boxes of `groups` of them)
+  int groups;    // 8-token groups of a box
+  int head_step; // fold 1 or 2: what a head adds to its coordinate
 };
 __host__ __device__ inline int da_smem_bytes(const DaPlan& p, int dim) {
-  return p.q_bufs * p.q_rows * dim * 2 + p.kv_bufs * da_buffer_bytes(dim) + 1024 + 512;
+  return p.q_bufs * p.q_rows * dim * 2 + (p.k_bufs + p.v_bufs) * da_buffer_bytes(dim) + 1024 + da_extra(dim, p.block);
 }
 
 // Workspace: per piece two partial results (its first and its last item) of 128 rows, O [128][dim], then (m, l) [128],
@@ -83,8 +110,8 @@ struct DaSplit {
   int pad[3];
 };
 __host__ __device__ inline size_t da_partial_floats(int dim) { return (size_t)DA_ROWS * (dim + 2); }
-__host__ __device__ inline size_t da_workspace_bytes(int dim, int pieces) {
-  return pieces * sizeof(DaSplit) + 2 * pieces * da_partial_floats(dim) * sizeof(float);
+__host__ __device__ inline size_t da_workspace_bytes(int dim) {
+  return DA_PIECES * sizeof(DaSplit) + 2 * DA_PIECES * da_partial_floats(dim) * sizeof(float);
 }
 
 // What a request asks for: its drafted tokens, first visible tile and tile counts; n = 0 if it drafts nothing or its
@@ -117,22 +144,30 @@ template <int KT>
 struct DaWalk {
   const DraftAttnArgs* a;
   DaReq r;
-  int size;  // tokens of a block
+  int size;      // tokens of a block
   int b, h, block, i;
-  __device__ __forceinline__ void start(const DraftAttnArgs& args, int block_size, int b0, int64_t within) {
+  int cost;      // units of an item before its tiles
+  int64_t unit;  // where the item begins
+  // `within` units into request b0, which begins at unit `begin`
+  __device__ __forceinline__ void start(const DraftAttnArgs& args, int block_size, int item_cost, int b0, int64_t begin,
+                                        int64_t within) {
     a = &args;
     size = block_size;
+    cost = item_cost;
     b = b0;
     r = da_request<KT>(args, size, b, false);
-    const int64_t item = within / r.n;
-    i = (int)(within - item * r.n);
-    h = (int)(item / r.blocks);
-    block = (int)(item - (int64_t)h * r.blocks);
+    const int len = r.n + cost;
+    const int64_t item = within <= INT32_MAX ? (int64_t)((uint32_t)within / (uint32_t)len) : within / len;
+    i = max(0, (int)(within - item * len) - cost);
+    h = (int)((uint32_t)item / (uint32_t)r.blocks);  // items of one request: heads x blocks
+    block = (int)item - h * r.blocks;
+    unit = begin + item * len;
   }
   __device__ __forceinline__ void skip(int tiles) {  // at most to the item's end
     i += tiles;
     if (i < r.n) return;
     i = 0;
+    unit += r.n + cost;
     if (++block < r.blocks) return;
     block = 0;
     if (++h < a->hkv) return;
@@ -229,15 +264,12 @@ __device__ __forceinline__ void da_pin(uint32_t* r) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                  "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
-// 32 packed 32-bit values a thread into TMEM columns taddr .. taddr + 31 of its lane; complete after tmem_st_wait.
-__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t (&v)[32]) {
+// 16 packed 32-bit values a thread into TMEM columns taddr .. taddr + 15 of its lane; complete after tmem_st_wait.
+__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -258,6 +290,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// mbar_wait with its loop out of line: the kernel waits in two dozen places.
+__device__ __noinline__ bool da_wait_on(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return mbar_wait(bar, parity, err, code);
+}
+__device__ __forceinline__ bool da_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return mbar_try_wait(bar, parity) || da_wait_on(bar, parity, err, code);
+}
+
 // Position in a ring of buffers and the parity of its use.
 struct DaRing {
   int at = 0;
@@ -270,10 +310,20 @@ struct DaRing {
   }
 };
 
-// What a lane fetches of a K or V tile: eight keys.
+// An item, or a piece's part of it, as warp 3 describes it to the softmax.
+struct DaItem {
+  int b, h, block, t0, fresh, len, lo, first, cached, n;  // as in DaReq and DaWalk
+  int i0, i1;  // this piece's tiles
+  int lows;    // with a window: the largest of its tokens' positions - window; else -1
+  int last;    // the piece in which it ends
+  int pad[2];
+};
+
+// What a lane fetches of a K or V tile: one box.
 struct DaFetch {
   int row, page;  // token within the page and page id, or drafted token
-  int drafted, head;
+  int drafted, head, block, t0;
+  uint32_t info;
   bool mine;      // some of them exist
 };
 
@@ -283,315 +333,431 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                   const __grid_constant__ CUtensorMap tm_cv, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DraftAttnArgs a, const DaPlan plan,
                   DaSplit* splits, float* partials) {
-  constexpr int KT = da_tile(D), NC = D / 64, BUF = da_buffer_bytes(D);
-  constexpr uint32_t O_COL = 2 * KT;
+  constexpr int KT = da_tile(D), NC = D / 64, BUF = da_buffer_bytes(D), NS = da_scores(D);
+  constexpr uint32_t O_COL = NS * KT;
+  static_assert(O_COL + D <= DA_TMEM_COLS, "S buffers and O fill TMEM");
   extern __shared__ __align__(1024) uint8_t da_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(da_smem_raw) + 1023) & ~uintptr_t(1023));
   const int q_buf = plan.q_rows * D * 2, q_box = plan.q_rows * 128;
   uint8_t* qs = smem;                            // [q_bufs][NC][q_rows][128 B], SW128
-  uint8_t* kvs = qs + plan.q_bufs * q_buf;       // [kv_bufs][KT / 8][NC][8][128 B], SW128
-  uint64_t* bars = reinterpret_cast<uint64_t*>(kvs + plan.kv_bufs * BUF);
-  uint64_t* full = bars;                         // [kv_bufs <= 12] a tile has landed
-  uint64_t* empty = full + 12;                   // [kv_bufs] the products that read it are done
-  uint64_t* q_full = empty + 12;                 // [2]
+  uint8_t* ks = qs + plan.q_bufs * q_buf;        // [k_bufs][KT / 8][NC][8][128 B], SW128
+  uint8_t* vs = ks + plan.k_bufs * BUF;          // [v_bufs], likewise
+  uint64_t* bars = reinterpret_cast<uint64_t*>(vs + plan.v_bufs * BUF);
+  uint64_t* k_full = bars;                       // [k_bufs] a tile has landed
+  uint64_t* k_empty = k_full + DA_MAX_BUFS;      // [k_bufs] the products that read it are done
+  uint64_t* v_full = k_empty + DA_MAX_BUFS;
+  uint64_t* v_empty = v_full + DA_MAX_BUFS;
+  uint64_t* q_full = v_empty + DA_MAX_BUFS;      // [2]
   uint64_t* q_empty = q_full + 2;                // [2]
-  uint64_t* s_full = q_empty + 2;                // [2] S of even / odd tiles
-  uint64_t* p_full = s_full + 2;                 // [2] P of a tile is written, O rescaled, V mended
-  uint64_t* pv_done = p_full + 2;                // [2] O includes the tile
-  uint64_t* all_done = pv_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
-  int* poison = reinterpret_cast<int*>(tmem_slot + 1);  // [2] of even / odd items: item + 1 if it met a non-finite V
-  int* low_max = poison + 2;                     // [4] a softmax warp's largest row bound
-  int64_t* s_scan = reinterpret_cast<int64_t*>(((uintptr_t)(low_max + 4) + 7) & ~uintptr_t(7));  // [8] warp sums, then
-  int* s_start = reinterpret_cast<int*>(s_scan + 8);  // the piece's first request
+  uint64_t* s_full = q_empty + 2;                // [NS] S of a tile is there
+  uint64_t* p_full = s_full + 4;                 // [NS] P of a tile is written, O rescaled, V mended
+  uint64_t* pv_done = p_full + 4;                // [NS] O includes the tile
+  uint64_t* v_there = pv_done + 4;               // [NS] V of the tile has landed
+  uint64_t* all_done = v_there + 4;              // [2] of warps 1 and 2, when a role has given up
+  uint64_t* m_full = all_done + 2;               // [2][4] a softmax warp's maxima
+  uint64_t* item_full = m_full + 8;              // [2] what an item is, for the softmax
+  uint64_t* item_empty = item_full + 2;          // [2]
+  uint64_t* ml_full = item_empty + 2;            // [2] the group without an item's last tile is through with it
+  uint64_t* o_free = ml_full + 2;                // O has been read
+  static_assert(DA_BARS == 4 * DA_MAX_BUFS + 4 + 4 * 4 + 2 + 8 + 2 + 2 + 2 + 1, "every barrier is initialised");
+  int64_t* s_scan = reinterpret_cast<int64_t*>(bars + DA_BARS);  // [12][2] warp sums of items and tiles
+  int64_t* s_begin = s_scan + 24;                // the unit at which the piece's first request begins
+  int64_t* s_tiles = s_begin + 1;                // [2] tiles before the piece and up to its end
+  int* s_start = reinterpret_cast<int*>(s_tiles + 2);        // the piece's first request
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_start + 1);
+  int* poison = s_start + 2;                     // [2] of even / odd items: item + 1 if it met a non-finite V
+  uint32_t* k_info = reinterpret_cast<uint32_t*>(poison + 2);  // [k_bufs], [v_bufs] of the tile in a buffer, see below
+  uint32_t* v_info = k_info + DA_MAX_BUFS;
+  DaItem* items = reinterpret_cast<DaItem*>(v_info + DA_MAX_BUFS);  // [2]
+  float2* ml_rows = reinterpret_cast<float2*>(items + 2);    // [2][128] (m, l) of that group
+  float* m_rows = reinterpret_cast<float*>(ml_rows + 256);   // [2][128] maxima after even / odd tiles
+  int* row_pos = reinterpret_cast<int*>(m_rows + 256);       // [2][block] an item's tokens: positions, with a window
+  uint32_t* row_words = reinterpret_cast<uint32_t*>(row_pos + 2 * plan.block);  // [2][block][KT / 32] first mask words
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
   const int G = a.hq / a.hkv;
-  if (tid == 0) {
-    for (int i = 0; i < plan.kv_bufs; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
-    }
-    mbar_init(all_done, 1);
+  // requests' items and tiles; their loads are on the way during the set-up
+  const int per = (a.rows + DA_THREADS - 1) / DA_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
+  struct Span {
+    int64_t items, tiles;
+  };
+  auto span_of = [&](int b, bool report) {
+    const DaReq r = da_request<KT>(a, plan.block, b, report);
+    const int64_t items = r.n ? (int64_t)r.blocks * a.hkv : 0;
+    return Span{items, items * r.n};
+  };
+  Span mine{0, 0};
+  for (int b = rb0; b < rb1; ++b) {
+    const Span x = span_of(b, piece == 0);
+    mine.items += x.items;
+    mine.tiles += x.tiles;
+  }
+  if (tid >= 32 && tid < 32 + DA_BARS) {  // one barrier a thread
+    const int i = tid - 32;
+    uint64_t* bar = bars + i;
+    mbar_init(bar, bar >= p_full && bar < pv_done ? 4 : bar >= m_full ? (bar < item_full ? 1 : bar < item_empty ? 1 : bar < ml_full ? 8 : 4) : 1);
     fence_barrier_init();
+  }
+  if (tid == 0) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_ck);
     prefetch_tmap(&tm_cv);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
     poison[0] = poison[1] = 0;
-    *s_start = -1;
+    splits[piece].last = -1;
   }
-  if (warp == 1) tmem_alloc(tmem_slot, DA_TMEM_COLS);
+  if (warp == 3) tmem_alloc(tmem_slot, DA_TMEM_COLS);
   pdl_trigger();
 
-  // ---- this piece of the line: requests' tile counts summed over the block ----
-  const int per = (a.rows + DA_THREADS - 1) / DA_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
-  auto tiles_of = [&](int b, bool report) -> int64_t {
-    const DaReq r = da_request<KT>(a, plan.block, b, report);
-    return (int64_t)r.n * r.blocks * a.hkv;
-  };
-  int64_t mine = 0;
-  for (int b = rb0; b < rb1; ++b) mine += tiles_of(b, piece == 0);
-  int64_t upto = mine;
+  // ---- this piece of the line ----
+  Span upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
+    const int64_t x = __shfl_up_sync(0xffffffffu, upto.items, o), y = __shfl_up_sync(0xffffffffu, upto.tiles, o);
+    if (lane >= o) {
+      upto.items += x;
+      upto.tiles += y;
+    }
   }
-  if (lane == 31) s_scan[warp] = upto;
+  if (lane == 31) {
+    s_scan[2 * warp] = upto.items;
+    s_scan[2 * warp + 1] = upto.tiles;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int64_t total = 0, before = upto - mine;
+  Span total{0, 0}, before{upto.items - mine.items, upto.tiles - mine.tiles};
   for (int w = 0; w < DA_THREADS / 32; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  const int64_t even = (total + plan.pieces - 1) / plan.pieces, step = even < DA_MIN_TILES ? DA_MIN_TILES : even;
-  const int64_t w0 = piece * step < total ? piece * step : total, w1 = w0 + step < total ? w0 + step : total;
-  const int n_tiles = (int)(w1 - w0);
-  if (n_tiles > 0 && w0 >= before && w0 < before + mine) {
-    int64_t at = before;
-    for (int b = rb0; b < rb1; ++b) {
-      const int64_t n = tiles_of(b, false);
-      if (w0 < at + n) {
-        s_start[0] = b;
-        *reinterpret_cast<int64_t*>(s_start + 2) = w0 - at;
-        break;
-      }
-      at += n;
+    if (w < warp) {
+      before.items += s_scan[2 * w];
+      before.tiles += s_scan[2 * w + 1];
     }
+    total.items += s_scan[2 * w];
+    total.tiles += s_scan[2 * w + 1];
   }
-  if (tid == 0) splits[piece].last = -1;
+  // where pieces have few tiles, latency counts and not the balance: an item is then as long as its tiles
+  const int64_t mean = (total.tiles + DA_PIECES - 1) / DA_PIECES;
+  const int cost = mean >= 4 * DA_ITEM_COST ? DA_ITEM_COST : 0;
+  const int64_t units = total.tiles + cost * total.items, step = max((int64_t)1, (units + DA_PIECES - 1) / DA_PIECES);
+  const int64_t w0 = min(units, piece * step), w1 = min(units, w0 + step);
+  // whose requests hold the piece's first unit, or the one past its last, says how many tiles lie before it
+  auto locate = [&](int64_t w, bool begins) {
+    const int64_t first = before.tiles + cost * before.items;
+    if (w < first || w >= first + mine.tiles + cost * mine.items) return;
+    Span at = before;
+    for (int b = rb0; b < rb1; ++b) {
+      const Span x = span_of(b, false);
+      const int64_t at_unit = at.tiles + cost * at.items;
+      if (w >= at_unit + x.tiles + cost * x.items) {
+        at.items += x.items;
+        at.tiles += x.tiles;
+        continue;
+      }
+      DaWalk<KT> there;
+      there.start(a, plan.block, cost, b, at_unit, w - at_unit);
+      s_tiles[begins ? 0 : 1] = at.tiles + (int64_t)(there.h * there.r.blocks + there.block) * there.r.n + there.i;
+      if (begins) {
+        s_start[0] = b;
+        *s_begin = at_unit;
+      }
+      return;
+    }
+  };
+  if (tid == 0 && w0 >= units) s_tiles[0] = s_tiles[1] = total.tiles;  // past the line's end
+  if (tid == 0 && w0 < units && w1 >= units) s_tiles[1] = total.tiles;
+  locate(w0, true);
+  locate(w1, false);
   __syncthreads();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int n_tiles = (int)(s_tiles[1] - s_tiles[0]);
   bool ok = true;  // no wait of this thread has given up
-  int issued = 0;  // warps 0 and 3: ring entries up to their last one; warp 2: Q tiles
+  int issued = 0, q_issued = 0;  // warps 0 and 3: K and V tiles requested; warp 0: Q tiles
   if (n_tiles > 0) {
     DaWalk<KT> walk;
-    walk.start(a, plan.block, s_start[0], *reinterpret_cast<const int64_t*>(s_start + 2));
-    // K and V of tile g are the ring's entries 2 g - 1 (0 for g = 0) and 2 g + 2 (2 g + 1 for the last)
+    walk.start(a, plan.block, cost, s_start[0], *s_begin, w0 - *s_begin);
+    // info: of a K tile bit 0: first of its item in this piece, bit 1: last; of a V tile bit 0 as well, then the steps of
+    // 16 keys that hold keys: bits 4-7 the first, bits 8-11 one past the last
     if (warp == 0 || warp == 3) {
-      // ---- K tiles (warp 0) and V tiles (warp 3): lane i brings keys 8 i .. 8 i + 7 ----
+      // ---- K tiles and Q (warp 0), V tiles (warp 3): lane i brings the i-th box ----
+      const int box = 8 * plan.groups;  // cached tokens of one
       const bool is_v = warp == 3;
       const CUtensorMap *cache = is_v ? &tm_cv : &tm_ck, *drafted = is_v ? &tm_v : &tm_k;
-      auto fetch_of = [&](const DaWalk<KT>& w) {
-        DaFetch x{0, -1, 0, w.h, false};
+      uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+      uint32_t* info = is_v ? v_info : k_info;
+      uint8_t* bufs = is_v ? vs : ks;
+      const int n_bufs = is_v ? plan.v_bufs : plan.k_bufs;
+      auto fetch_of = [&](const DaWalk<KT>& w, bool begins, bool ends) {
+        DaFetch x{0, -1, 0, w.h, w.block, w.r.t0, 0u, false};
+        int begin = 0, end;
         if (w.i < w.r.cached) {
-          const int base = (w.r.first + w.i) * KT, pos = base + lane * 8;
-          x.mine = lane < KT / 8 && pos < w.r.len && pos + 8 > w.r.lo;
+          const int base = (w.r.first + w.i) * KT, pos = base + lane * box;
+          begin = max(0, w.r.lo - base);
+          end = min(KT, w.r.len - base);
+          x.mine = lane * box < end && lane * box + box > begin;
           if (x.mine) {
             const int p = pos / a.cache.page;
             x.row = pos - p * a.cache.page;
             x.page = a.table[w.b * a.table_stride + p];
           }
         } else {
-          const int j = (w.i - w.r.cached) * KT + lane * 8;
-          x.mine = lane < KT / 8 && j < w.r.fresh;
-          x.row = w.r.t0 + j;
+          const int j = (w.i - w.r.cached) * KT;
+          end = min(KT, w.r.fresh - j);
+          x.mine = lane * 8 < end;
+          x.row = w.r.t0 + j + lane * 8;
           x.drafted = 1;
         }
+        x.info = (begins ? 1u : 0u) | (ends ? 2u : 0u) | (uint32_t)(begin >> 4) << 4 | (uint32_t)((end + 15) >> 4) << 8;
         return x;
       };
-      DaRing ring;
-      if (is_v) ring.next(plan.kv_bufs);
-      DaFetch cur = fetch_of(walk), next = cur;
+      DaRing ring, q_ring;
+      auto fetch = [&](int g) { return fetch_of(walk, g == 0 || walk.i == 0, g + 1 == n_tiles || walk.i + 1 == walk.r.n); };
+      auto item_of = [&](int g) {
+        const DaReq& r = walk.r;
+        return DaItem{walk.b, walk.h, walk.block, r.t0, r.fresh, r.len, r.lo, r.first, r.cached, r.n, walk.i,
+                      min(r.n, walk.i + n_tiles - g), -1, (int)((walk.unit + cost + r.n - 1) / step), {0, 0}};
+      };
+      DaFetch cur = fetch(0), next = cur;
+      DaItem cur_item = item_of(0), next_item = cur_item;
+      int item = 0;  // warp 3: items described
       for (int g = 0; g < n_tiles && ok; ++g) {
         if (g + 1 < n_tiles) {  // the next tile's table entries, ahead of the wait
           walk.skip(1);
-          next = fetch_of(walk);
+          next = fetch(g + 1);
+          if (is_v && (next.info & 1)) next_item = item_of(g + 1);
         }
-        if (is_v && g + 1 < n_tiles) ring.next(plan.kv_bufs);
-        const int e = is_v ? (g + 1 < n_tiles ? 2 * g + 2 : 2 * g + 1) : g ? 2 * g - 1 : 0;
-        if (e >= plan.kv_bufs) ok = __all_sync(0xffffffffu, mbar_wait(&empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+        if (is_v && (cur.info & 1)) {  // the item, for the softmax
+          if (item >= 2)
+            ok = __all_sync(0xffffffffu, da_wait(&item_empty[item & 1], ((item >> 1) - 1) & 1, a.err, ERR_TIMEOUT_MMA));
+          if (!ok) break;
+          const int size = plan.block, tokens = min(size, cur_item.fresh - cur_item.block * size);
+          const int t = cur_item.t0 + cur_item.block * size;
+          int lows = -1;
+          for (int k = lane; k < tokens; k += 32) {
+            if (a.window) {
+              const int pos = a.positions ? a.positions[t + k] : cur_item.len + cur_item.block * size + k;
+              row_pos[(item & 1) * size + k] = pos;
+              lows = max(lows, pos - a.window);
+            }
+            if (a.mask)
+              for (int w = 0; w < KT / 32; ++w)
+                row_words[((item & 1) * size + k) * (KT / 32) + w] = w < a.words ? a.mask[(int64_t)(t + k) * a.words + w] : 0u;
+          }
+          lows = __reduce_max_sync(0xffffffffu, lows);
+          if (lane == 0) {
+            cur_item.lows = max(lows, a.window ? cur_item.lo - 1 : -1);
+            items[item & 1] = cur_item;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&item_full[item & 1]);
+          ++item;
+        }
+        if (!is_v && (cur.info & 1)) {  // Q: block tokens x G heads, one box for each 64 dims
+          if (q_issued >= plan.q_bufs)
+            ok = __all_sync(0xffffffffu, da_wait(&q_empty[q_ring.at], q_ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[q_ring.at], plan.block * G * D * 2);
+          __syncwarp();
+          if (lane < NC)
+            tma_load_3d(qs + q_ring.at * q_buf + lane * q_box, &tm_q, lane * 64, cur.head * G, cur.t0 + cur.block * plan.block,
+                        &q_full[q_ring.at]);
+          ++q_issued;
+          q_ring.next(plan.q_bufs);
+        }
+        if (g >= n_bufs) ok = __all_sync(0xffffffffu, da_wait(&empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
         if (!ok) break;
         const bool good = cur.drafted || (cur.page >= 0 && cur.page < a.cache.pages);
         if (cur.mine && !good) set_error(a.err, ERR_BAD_PAGE);
         const bool bring = cur.mine && good;
         const unsigned boxes = __ballot_sync(0xffffffffu, bring);
-        uint8_t* dst = kvs + ring.at * BUF + lane * NC * 1024;
-        if (lane == 0) mbar_arrive_expect_tx(&full[ring.at], __popc(boxes) * (NC * 1024));
+        const int box_groups = cur.drafted ? 1 : plan.groups;
+        if (lane == 0) {
+          info[ring.at] = cur.info;
+          mbar_arrive_expect_tx(&full[ring.at], __popc(boxes) * box_groups * (NC * 1024));
+        }
         __syncwarp();
         if (bring) {
+          uint8_t* dst = bufs + ring.at * BUF + lane * box_groups * NC * 1024;
           if (cur.drafted) tma_load_4d(dst, drafted, 0, cur.row, 0, cur.head, &full[ring.at]);
-          else tma_load_5d(dst, cache, 0, cur.row, 0, cur.head, cur.page, &full[ring.at]);
+          else if (plan.fold == 0) tma_load_5d(dst, cache, 0, cur.row, 0, cur.head, cur.page, &full[ring.at]);
+          else if (plan.fold == 1) tma_load_5d(dst, cache, 0, 0, cur.head * plan.head_step, cur.row >> 3, cur.page, &full[ring.at]);
+          else tma_load_5d(dst, cache, 0, 0, 0, cur.head * plan.head_step + (cur.row >> 3), cur.page, &full[ring.at]);
         }
-        issued = e + 1;
-        ring.next(plan.kv_bufs);
-        if (!is_v && g > 0) ring.next(plan.kv_bufs);
+        issued = g + 1;
+        ring.next(n_bufs);
         cur = next;
+        cur_item = next_item;
       }
     } else if (warp == 1) {
-      // ---- products ----
-      const uint32_t idesc_s = DaType<T>::idesc(KT), idesc_o = DaType<T>::idesc(D) | DA_B_N_MAJOR;
-      DaRing ring, q_ring;
-      bool begins = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, code));
-      };
-      auto score = [&](int g) {  // S of tile g (the walk's place), then the walk moves on
-        if (begins) wait(&q_full[q_ring.at], q_ring.phase, ERR_TIMEOUT_TMA);
-        wait(&full[ring.at], ring.phase, ERR_TIMEOUT_TMA);
-        if (!ok) return;
+      // ---- S ----
+      const uint32_t idesc = DaType<T>::idesc(KT);
+      DaRing ring, q_ring, s_ring;
+      for (int g = 0; g < n_tiles && ok; ++g) {
+        ok = __all_sync(0xffffffffu, da_wait(&k_full[ring.at], ring.phase, a.err, ERR_TIMEOUT_TMA));
+        const uint32_t what = k_info[ring.at];
+        if (ok && (what & 1)) ok = __all_sync(0xffffffffu, da_wait(&q_full[q_ring.at], q_ring.phase, a.err, ERR_TIMEOUT_TMA));
+        if (ok && g >= NS) ok = __all_sync(0xffffffffu, da_wait(&pv_done[s_ring.at], s_ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+        if (!ok) break;
         tc_fence_after();
-        const bool ends = __shfl_sync(0xffffffffu, (int)(walk.i + 1 == walk.r.n), 0) || g + 1 == n_tiles;
-        const uint64_t qd = sw128_desc(smem_u32(qs + q_ring.at * q_buf)), kd = da_k_desc<NC>(smem_u32(kvs + ring.at * BUF));
-        const uint32_t d = tmem + (uint32_t)((g & 1) * KT);
+        const uint64_t qd = sw128_desc(smem_u32(qs + q_ring.at * q_buf)), kd = da_k_desc<NC>(smem_u32(ks + ring.at * BUF));
+        const uint32_t d = tmem + (uint32_t)(s_ring.at * KT);
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              mma_bf16(d, qd + (uint64_t)((c * q_box + kk * 32) >> 4), kd + (uint64_t)((c * 1024 + kk * 32) >> 4), idesc_s,
+              mma_bf16(d, qd + (uint64_t)((c * q_box + kk * 32) >> 4), kd + (uint64_t)((c * 1024 + kk * 32) >> 4), idesc,
                        (c > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&s_full[g & 1]);
-          mma_commit(&empty[ring.at]);
-          if (ends) mma_commit(&q_empty[q_ring.at]);
+          mma_commit(&s_full[s_ring.at]);
+          mma_commit(&k_empty[ring.at]);
+          if (what & 2) mma_commit(&q_empty[q_ring.at]);
         }
         __syncwarp();
-        if (ends) q_ring.next(plan.q_bufs);
-        begins = ends;
-        if (g + 1 < n_tiles) walk.skip(1);
-        ring.next(plan.kv_bufs);
-      };
-      bool first = true;  // of its item (or of this piece's part of it)
-      score(0);
+        ring.next(plan.k_bufs);
+        if (what & 2) q_ring.next(plan.q_bufs);
+        s_ring.next(NS);
+      }
+    } else if (warp == 2) {
+      // ---- P V ----
+      const uint32_t idesc = DaType<T>::idesc(D) | DA_B_N_MAJOR;
+      DaRing ring, p_ring;
+      int item = 0;
       for (int g = 0; g < n_tiles && ok; ++g) {
-        const bool ends = begins;  // the tile that was scored last, tile g, is the last of its item
-        if (g + 1 < n_tiles) score(g + 1);
-        wait(&p_full[g & 1], (g >> 1) & 1, ERR_TIMEOUT_MMA);
-        wait(&full[ring.at], ring.phase, ERR_TIMEOUT_TMA);
+        ok = __all_sync(0xffffffffu, da_wait(&v_full[ring.at], ring.phase, a.err, ERR_TIMEOUT_TMA));
+        const uint32_t what = v_info[ring.at];
+        if (ok && lane == 0) mbar_arrive(&v_there[p_ring.at]);
+        __syncwarp();
+        if (what & 1) {
+          if (ok && item > 0) ok = __all_sync(0xffffffffu, da_wait(o_free, (item - 1) & 1, a.err, ERR_TIMEOUT_MMA));
+          ++item;
+        }
+        if (ok) ok = __all_sync(0xffffffffu, da_wait(&p_full[p_ring.at], p_ring.phase, a.err, ERR_TIMEOUT_MMA));
         if (!ok) break;
         tc_fence_after();
-        const uint64_t vd = da_v_desc<NC>(smem_u32(kvs + ring.at * BUF));
-        const uint32_t p = tmem + (uint32_t)((g & 1) * KT);
+        const uint64_t vd = da_v_desc<NC>(smem_u32(vs + ring.at * BUF));
+        const uint32_t p = tmem + (uint32_t)(p_ring.at * KT);
+        // steps of 16 keys that exist: the others' V is whatever lay in the buffer
+        const int k0 = what >> 4 & 15, k1 = what >> 8 & 15;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk)
-            mma_tmem_a(tmem + O_COL, p + kk * 8, vd + (uint64_t)((kk * 2 * NC * 1024) >> 4), idesc_o,
-                       (!first || kk > 0) ? 1u : 0u);
-          mma_commit(&pv_done[g & 1]);
-          mma_commit(&empty[ring.at]);
+            if (kk >= k0 && kk < k1)
+              mma_tmem_a(tmem + O_COL, p + kk * 8, vd + (uint64_t)((kk * 2 * NC * 1024) >> 4), idesc,
+                         (!(what & 1) || kk > k0) ? 1u : 0u);
+          mma_commit(&pv_done[p_ring.at]);
+          mma_commit(&v_empty[ring.at]);
         }
         __syncwarp();
-        ring.next(plan.kv_bufs);
-        first = ends;
-      }
-    } else if (warp == 2) {
-      // ---- Q of every item: block tokens x G heads, one box for each 64 dims ----
-      DaRing ring;
-      int left = n_tiles;
-      for (int item = 0; left > 0 && ok; ++item) {
-        if (item >= plan.q_bufs) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
-        if (!ok) break;
-        const int token = __shfl_sync(0xffffffffu, walk.r.t0 + walk.block * plan.block, 0);
-        const int head = __shfl_sync(0xffffffffu, walk.h * G, 0);
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&q_full[ring.at], plan.block * G * D * 2);
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-            tma_load_3d(qs + ring.at * q_buf + c * q_box, &tm_q, c * 64, head, token, &q_full[ring.at]);
-        }
-        __syncwarp();
-        ++issued;
-        ring.next(plan.q_bufs);
-        const int tiles = min(left, walk.r.n - walk.i);
-        left -= tiles;
-        walk.skip(tiles);
+        ring.next(plan.v_bufs);
+        p_ring.next(NS);
       }
     } else if (warp >= 4) {
-      // ---- softmax: thread = row = TMEM lane ----
-      const int row = tid - 128;
-      const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
-      int g = 0;
-      for (int item = 0; g < n_tiles; ++item) {
-        const DaReq r = walk.r;
-        const int tok = walk.block * plan.block + row / G;
-        const bool valid = row < plan.block * G && tok < r.fresh;
-        const bool live = __any_sync(0xffffffffu, valid);
-        const int i0 = walk.i, i1 = min(r.n, i0 + n_tiles - g);
-        // keys of this row are those at positions above `low`
-        int low = r.lo - 1, lows = -1;
-        if (a.window) {
-          if (valid) low = max(low, (a.positions ? a.positions[r.t0 + tok] : r.len + tok) - a.window);
-          int x = valid ? low : -1;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
-          named_sync_id<2, 128>();  // the last item's readers are done
-          if (lane == 0) low_max[warp & 3] = x;
-          named_sync_id<2, 128>();
-          lows = max(max(low_max[0], low_max[1]), max(low_max[2], low_max[3]));
+      // ---- softmax: thread = row = TMEM lane; group 0 (warps 4-7) takes even tiles, group 1 (warps 8-11) odd ones ----
+      const int group = warp >= 8, row = tid & 127, quarter = warp & 3;
+      const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+      const float sl2 = a.scale * 1.4426950408889634f;        // scores in log2 units
+      const int row_tok = row / G;                            // token within the block
+      DaRing ring;  // of tile g's S and P
+      int reached = 0;
+      int g0 = 0;  // the item's first tile
+      for (int item = 0; g0 < n_tiles; ++item) {
+        if (ok) ok = da_wait(&item_full[item & 1], (item >> 1) & 1, a.err, ERR_TIMEOUT_TMA);
+        if (!__all_sync(0xffffffffu, ok)) {  // without the item there is nothing to go by
+          ok = false;
+          break;
         }
-        float m = -INFINITY, l = 0.f;
-        for (int i = i0; i < i1; ++i, ++g) {
-          const bool tree = i >= r.cached;
-          const int base = tree ? (i - r.cached) * KT : (r.first + i) * KT;  // first key: drafted index or position
-          const int end = min(KT, (tree ? r.fresh : r.len) - base);          // keys that exist
-          const int begin = tree ? 0 : max(0, r.lo - base);
-          const bool some = tree || (a.window && base <= lows);              // not every row sees the same keys
-          const bool special = some || begin > 0 || end < KT;
-          if (ok) ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
-          tc_fence_after();
-          __syncwarp();
-          if (live) {
-            uint32_t sc[KT];
-#pragma unroll
-            for (int c = 0; c < KT; c += 32) tmem_ld32_async(lanes + (uint32_t)((g & 1) * KT + c), sc + c);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < KT; c += 32) da_pin(sc + c);
-            auto at = [&](int j) { return __uint_as_float(sc[j]); };
-            if (special) {
-#pragma unroll
-              for (int w = 0; w < KT / 32; ++w) {
-                const int from = tree ? 0 : max(0, low + 1 - base), z = min(32, max(0, end - 32 * w));
-                const int f = min(32, max(0, from - 32 * w));
-                uint32_t bits = (z == 32 ? ~0u : (1u << z) - 1u) & (f == 32 ? 0u : ~0u << f);
-                if (tree && valid) {
-                  const int word = (base >> 5) + w;
-                  if (a.mask)
-                    bits &= word < a.words ? a.mask[(int64_t)(r.t0 + tok) * a.words + word] : 0u;
-                  else
-                    bits &= tok >= base + 32 * w + 31 ? ~0u : tok < base + 32 * w ? 0u : (2u << (tok - base - 32 * w)) - 1u;
-                  if (a.window) {
-                    for (uint32_t rest = bits; rest; rest &= rest - 1) {
-                      const int j = base + 32 * w + __ffs(rest) - 1;
-                      if ((a.positions ? a.positions[r.t0 + j] : r.len + j) <= low) bits &= ~(rest & -rest);
-                    }
-                  }
+        const DaItem& it = items[item & 1];
+        const int i0 = it.i0, i1 = it.i1, cached = it.cached, len = it.len, fresh = it.fresh, t0 = it.t0;
+        const int tok = it.block * plan.block + row_tok;
+        const bool valid = row < plan.block * G && tok < fresh;
+        const bool live = __any_sync(0xffffffffu, valid);
+        // keys of this row are those at positions above `low`; no row's bound is above it.lows
+        int low = it.lo - 1;
+        if (a.window && valid) low = max(low, row_pos[(item & 1) * plan.block + row_tok] - a.window);
+        const uint32_t* first_words = row_words + ((item & 1) * plan.block + row_tok) * (KT / 32);
+        float m = -INFINITY, l = 0.f;  // maximum of the last tile that this group took part in, sum of its own weights
+        for (int i = i0 + ((g0 ^ group) & 1); i < i1; i += 2) {
+          const int g = g0 + i - i0;
+          for (; reached < g; ++reached) ring.next(NS);
+          const uint32_t s_col = lanes + (uint32_t)(ring.at * KT);  // S, later P
+          const bool tree = i >= cached;
+          const int base = tree ? (i - cached) * KT : (it.first + i) * KT;  // first key: drafted index or position
+          const int end = min(KT, (tree ? fresh : len) - base);             // keys that exist
+          const int begin = tree ? 0 : max(0, it.lo - base);
+          // keys up to here are seen by some rows and not by others
+          const int mixed = tree ? end : a.window ? min(end, it.lows + 1 - base) : 0;
+          const bool special = mixed > 0 || begin > 0 || end < KT;
+          // which of keys 32 w .. 32 w + 31 of the tile this row sees
+          auto seen_keys = [&](int w) {
+            const int from = tree ? 0 : max(0, low + 1 - base), z = min(32, max(0, end - 32 * w));
+            const int f = min(32, max(0, from - 32 * w));
+            uint32_t bits = (z == 32 ? ~0u : (1u << z) - 1u) & (f == 32 ? 0u : ~0u << f);
+            if (tree && valid) {
+              const int word = (base >> 5) + w;
+              if (a.mask)
+                bits &= base == 0 ? first_words[w] : word < a.words ? a.mask[(int64_t)(t0 + tok) * a.words + word] : 0u;
+              else
+                bits &= tok >= base + 32 * w + 31 ? ~0u : tok < base + 32 * w ? 0u : (2u << (tok - base - 32 * w)) - 1u;
+              if (a.window && low >= len) {  // a window so short that it ends among the drafted tokens
+                for (uint32_t rest = bits; rest; rest &= rest - 1) {
+                  const int j = base + 32 * w + __ffs(rest) - 1;
+                  if ((a.positions ? a.positions[t0 + j] : len + j) <= low) bits &= ~(rest & -rest);
                 }
-#pragma unroll
-                for (int j = 0; j < 32; ++j) sc[32 * w + j] = bits >> j & 1 ? sc[32 * w + j] : 0xff800000u;  // -inf
               }
             }
-            float tops[4] = {at(0), at(1), at(2), at(3)};
+            return bits;
+          };
+          // 32 scores from TMEM, -inf where the row does not see the key
+          auto scores = [&](int c, uint32_t (&x)[32]) {
+            tmem_ld32_async(s_col + 32 * c, x);
+            const uint32_t bits = special ? seen_keys(c) : ~0u;
+            tmem_ld_wait();
+            da_pin(x);
+            if (special) {
 #pragma unroll
-            for (int j = 4; j + 4 < KT; j += 8)
+              for (int j = 0; j < 32; ++j) x[j] = bits >> j & 1 ? x[j] : 0xff800000u;
+            }
+          };
+          if (ok) ok = da_wait(&s_full[ring.at], ring.phase, a.err, ERR_TIMEOUT_MMA);
+          tc_fence_after();
+          __syncwarp();
+          float top = -INFINITY;
+          if (live) {
+            // S is read twice, for the maximum and for the weights, 32 columns at a time in loops that are not unrolled:
+            // twelve warps in seven places run best from a small program (a tile's softmax unrolled over its 128 columns,
+            // with a copy for masked ones, took twice the time)
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < KT / 32; ++c) {
+              uint32_t x[32];
+              scores(c, x);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) tops[q] = fmaxf(fmaxf(tops[q], at(j + q)), at(j + 4 + q));
+              for (int j = 0; j < 32; j += 8)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tops[q] = fmaxf(tops[q], at(KT - 4 + q));
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sl2;
-            // the maximum is raised only when a tile exceeds it by 2^8: weights stay below that, which fp16 holds
-            const bool raise = valid && (top > m + 8.f || (m == -INFINITY && top > -INFINITY));
-            const float alpha = raise && m > -INFINITY ? ex2_approx(m - top) : raise ? 0.f : 1.f;
-            if (raise) {
-              m = top;
-              l *= alpha;
+                for (int q = 0; q < 4; ++q)
+                  tops[q] = fmaxf(fmaxf(tops[q], __uint_as_float(x[j + q])), __uint_as_float(x[j + 4 + q]));
+            }
+            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sl2;
+          }
+          // the maximum so far, from the other group; it is raised only when a tile exceeds it by 2^8: weights stay
+          // below that, which fp16 holds
+          if (ok && g > 0) ok = da_wait(&m_full[4 * (group ^ 1) + quarter], ((g - 1) >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
+          const float seen = i > i0 ? m_rows[128 * (group ^ 1) + row] : -INFINITY;
+          const bool raise = valid && (top > seen + 8.f || (seen == -INFINITY && top > -INFINITY));
+          const float now = raise ? top : seen;
+          m_rows[128 * group + row] = now;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_full[4 * group + quarter]);
+          if (live) {
+            if (now != m) {  // m = -inf: l is 0
+              l *= m == -INFINITY ? 0.f : ex2_approx(m - now);
+              m = now;
             }
             if (i > i0 && __any_sync(0xffffffffu, raise)) {
-              if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
+              if (ok) ok = da_wait(&pv_done[(g - 1) % NS], ((g - 1) / NS) & 1, a.err, ERR_TIMEOUT_MMA);
               tc_fence_after();
               __syncwarp();
+              const float alpha = !raise ? 1.f : seen == -INFINITY ? 0.f : ex2_approx(seen - now);
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
                 float o[32];
@@ -604,66 +770,85 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const float2 mul = make_float2(sl2, sl2), off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m, -m);
             float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             __syncwarp();
+#pragma unroll 1
+            for (int c = 0; c < KT / 32; ++c) {
+              uint32_t x[32], pk[16];
+              scores(c, x);
 #pragma unroll
-            for (int c = 0; c < KT; c += 64) {
-              uint32_t pk[32];
-#pragma unroll
-              for (int j = 0; j < 64; j += 2) {
-                float2 x = fma2(make_float2(at(c + j), at(c + j + 1)), mul, off);
-                x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                sums[j >> 1 & 1] = add2(sums[j >> 1 & 1], x);
-                pk[j >> 1] = pack2(x.x, x.y, (const T*)nullptr);
+              for (int j = 0; j < 32; j += 2) {
+                float2 y = fma2(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul, off);
+                y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                sums[j >> 1 & 1] = add2(sums[j >> 1 & 1], y);
+                pk[j >> 1] = pack2(y.x, y.y, (const T*)nullptr);
               }
-              tmem_st32_async(lanes + (uint32_t)((g & 1) * KT + c / 2), pk);
+              tmem_st16_async(s_col + 16 * c, pk);  // over scores that have been read
             }
             sums[0] = add2(sums[0], sums[1]);
             l += sums[0].x + sums[0].y;
             tmem_st_wait();
           }
           if (special) {
-            // V rows that nobody sees become 0 (0 times whatever lay there must not count); where rows differ in what
-            // they see, so do V's infinities and NaN, which the epilogue puts back for the rows that see them
-            const int e = g + 1 < n_tiles ? 2 * g + 2 : 2 * g + 1;
-            if (ok) ok = mbar_wait(&full[e % plan.kv_bufs], (e / plan.kv_bufs) & 1, a.err, ERR_TIMEOUT_TMA);
-            uint8_t* vb = kvs + (e % plan.kv_bufs) * BUF;
-            for (int c = row; c < KT * (D / 8); c += 128) {
-              const int k = c / (D / 8), ch = c % (D / 8);
-              uint4* at = reinterpret_cast<uint4*>(vb + da_offset<NC>(k, ch));
-              if (k < begin || k >= end) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-              } else if (some) {
-                uint4 v = *at;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                bool bad = false;
+            // V rows that nobody sees become 0 (0 times whatever lay there must not count), as far as the product
+            // reaches: whole steps of 16 keys. Where rows differ in what they see, V's infinities and NaN become 0,
+            // and the epilogue puts them back for the rows that see them.
+            if (ok) ok = da_wait(&v_there[ring.at], ring.phase, a.err, ERR_TIMEOUT_TMA);
+            uint8_t* vb = vs + (g % plan.v_bufs) * BUF;
+            const int head_rows = begin & 15, z0 = begin - head_rows, tail_rows = -end & 15;
+            for (int c = row; c < (head_rows + tail_rows) * (D / 8); c += 128) {
+              const int k = c / (D / 8);
+              *reinterpret_cast<uint4*>(vb + da_offset<NC>(k < head_rows ? z0 + k : end + k - head_rows, c % (D / 8))) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            }
+            for (int c = begin * (D / 8) + row; c < mixed * (D / 8); c += 128) {
+              uint4* at = reinterpret_cast<uint4*>(vb + da_offset<NC>(c / (D / 8), c % (D / 8)));
+              uint4 v = *at;
+              uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+              bool bad = false;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  constexpr uint32_t E = DaType<T>::kExp;
-                  const bool lo_bad = (w[q] & E) == E, hi_bad = (w[q] >> 16 & E) == E;
-                  bad |= lo_bad | hi_bad;
-                  w[q] &= (lo_bad ? 0u : 0xffffu) | (hi_bad ? 0u : 0xffff0000u);
-                }
-                if (bad) {
-                  *at = v;
-                  poison[item & 1] = item + 1;
-                }
+              for (int q = 0; q < 4; ++q) {
+                constexpr uint32_t E = DaType<T>::kExp;
+                const bool lo_bad = (w[q] & E) == E, hi_bad = (w[q] >> 16 & E) == E;
+                bad |= lo_bad | hi_bad;
+                w[q] &= (lo_bad ? 0u : 0xffffu) | (hi_bad ? 0u : 0xffff0000u);
+              }
+              if (bad) {
+                *at = v;
+                poison[item & 1] = item + 1;
               }
             }
             fence_proxy_async();
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[g & 1]);
+          if (lane == 0) mbar_arrive(&p_full[ring.at]);
         }
-        // ---- epilogue of the item, or of this piece's part of it ----
-        if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
+        // ---- epilogue of the item, or of this piece's part of it: by the group that has its last tile, while the other
+        // goes on to the next item ----
+        const int last = g0 + i1 - i0 - 1;  // its last tile
+        g0 += i1 - i0;
+        if ((last & 1) != group) {
+          ml_rows[128 * (item & 1) + row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&ml_full[item & 1]);
+            mbar_arrive(&item_empty[item & 1]);
+          }
+          continue;
+        }
+        if (ok) ok = da_wait(&ml_full[item & 1], (item >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
+        {
+          const float2 theirs = ml_rows[128 * (item & 1) + row];  // their maximum is no larger than m, the last tile's
+          const float w = theirs.x == m ? 1.f : theirs.x == -INFINITY ? 0.f : ex2_approx(theirs.x - m);
+          l += theirs.y * w;
+        }
+        if (ok) ok = da_wait(&pv_done[last % NS], (last / NS) & 1, a.err, ERR_TIMEOUT_MMA);
         tc_fence_after();
-        named_sync_id<2, 128>();  // every warp's poison is written (the next item's goes to the other word)
-        const bool mend = poison[item & 1] == item + 1;
-        const bool whole = i0 == 0 && i1 == r.n;
-        const int slot = 2 * piece + (item > 0 ? 1 : 0);
+        const bool mend = poison[item & 1] == item + 1;  // every tile's P has been waited for, so its scan is done
+        const bool whole = i0 == 0 && i1 == it.n;
+        const int slot = 2 * piece + (item > 0 ? 1 : 0), h = it.h;
         float* part = partials + slot * da_partial_floats(D);
         const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-        const int64_t orow = (int64_t)(r.t0 + tok) * a.hq + walk.h * G + row % G;
+        const int64_t orow = (int64_t)(t0 + tok) * a.hq + h * G + row % G;
         if (live) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -673,21 +858,20 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (!valid) continue;
             if (mend) {  // rare, and slow: key after key
               for (int i = i0; i < i1; ++i) {
-                const bool tree = i >= r.cached;
-                const int base = tree ? (i - r.cached) * KT : (r.first + i) * KT;
-                if (!tree && !(a.window && base <= lows)) continue;
-                for (int j = base; j < base + KT && j < (tree ? r.fresh : r.len); ++j) {
+                const bool tree = i >= cached;
+                const int base = tree ? (i - cached) * KT : (it.first + i) * KT;
+                for (int j = base; j < min(base + KT, tree ? fresh : min(len, it.lows + 1)); ++j) {
                   const T* v;
                   if (tree) {
-                    if (a.mask ? (j >= 32 * a.words || !(a.mask[(int64_t)(r.t0 + tok) * a.words + (j >> 5)] >> (j & 31) & 1)) : j > tok) continue;
-                    if (a.window && (a.positions ? a.positions[r.t0 + j] : r.len + j) <= low) continue;
-                    v = (const T*)a.v + (int64_t)(r.t0 + j) * a.v_ts + (int64_t)walk.h * a.v_hs;
+                    if (a.mask ? (j >= 32 * a.words || !(a.mask[(int64_t)(t0 + tok) * a.words + (j >> 5)] >> (j & 31) & 1)) : j > tok) continue;
+                    if (a.window && (a.positions ? a.positions[t0 + j] : len + j) <= low) continue;
+                    v = (const T*)a.v + (int64_t)(t0 + j) * a.v_ts + (int64_t)h * a.v_hs;
                   } else {
                     if (j <= low) continue;
-                    const int pg = a.table[walk.b * a.table_stride + j / a.cache.page];
+                    const int pg = a.table[it.b * a.table_stride + j / a.cache.page];
                     if (pg < 0 || pg >= a.cache.pages) continue;
                     v = (const T*)a.cache.v + pg * a.cache.page_stride + j % a.cache.page * a.cache.token_stride +
-                        walk.h * a.cache.head_stride;
+                        h * a.cache.head_stride;
                   }
 #pragma unroll
                   for (int x = 0; x < 32; ++x) {
@@ -712,19 +896,19 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 *reinterpret_cast<float4*>(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
           }
-          if (valid) {
-            if (!whole)
-              *reinterpret_cast<float2*>(part + DA_ROWS * D + 2 * row) = make_float2(m, l);
-            else if (a.lse)
-              a.lse[orow] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-          }
-        }
-        if (row == 0 && i0 == 0 && i1 < r.n) {
-          const int64_t start = w0 + g - (i1 - i0);
-          splits[piece] = DaSplit{walk.b, walk.h, walk.block, (int)((start + r.n - 1) / step), slot, {0, 0, 0}};
         }
         tc_fence_before();
-        walk.skip(i1 - i0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_free);
+        if (valid) {
+          if (!whole)
+            *reinterpret_cast<float2*>(part + DA_ROWS * D + 2 * row) = make_float2(m, l);
+          else if (a.lse)
+            a.lse[orow] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        }
+        if (row == 0 && i0 == 0 && i1 < it.n) splits[piece] = DaSplit{it.b, h, it.block, it.last, slot, {0, 0, 0}};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[item & 1]);
       }
     }
   }
@@ -734,17 +918,15 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   tc_fence_before();
   if (!__syncthreads_and(ok)) {
     if (warp == 0 || warp == 3) {
-      for (int e = max(0, issued - plan.kv_bufs); e < issued; ++e) {
-        const bool v_entry = (e > 0 && e % 2 == 0) || e == 2 * n_tiles - 1;
-        if (v_entry == (warp == 3)) mbar_wait(&full[e % plan.kv_bufs], (e / plan.kv_bufs) & 1, nullptr, 0);
-      }
-    } else if (warp == 2) {
-      for (int e = max(0, issued - plan.q_bufs); e < issued; ++e)
-        mbar_wait(&q_full[e % plan.q_bufs], (e / plan.q_bufs) & 1, nullptr, 0);
-    } else if (warp == 1) {
-      if (elect_one()) mma_commit(all_done);
+      const int n_bufs = warp == 3 ? plan.v_bufs : plan.k_bufs;
+      for (int g = max(0, issued - n_bufs); g < issued; ++g)
+        da_wait(&(warp == 3 ? v_full : k_full)[g % n_bufs], (g / n_bufs) & 1, nullptr, 0);
+      for (int e = max(0, q_issued - plan.q_bufs); e < q_issued; ++e)
+        da_wait(&q_full[e % plan.q_bufs], (e / plan.q_bufs) & 1, nullptr, 0);
+    } else if (warp < 3) {
+      if (elect_one()) mma_commit(&all_done[warp - 1]);
       __syncwarp();
-      mbar_wait(all_done, 0, nullptr, 0);
+      da_wait(&all_done[warp - 1], 0, nullptr, 0);
     }
     tc_fence_before();
     __syncthreads();
