@@ -142,8 +142,8 @@ int launch_draft_attn(const DraftAttnArgs& d, void* workspace, cudaStream_t st) 
   DaSplit* splits = static_cast<DaSplit*>(workspace);
   float* partials = reinterpret_cast<float*>(splits + DA_PIECES);
   CU(cudaFuncSetAttribute(draft_attn_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, DA_SMEM_LIMIT));
-  draft_attn_kernel<D, T><<<DA_PIECES, DA_THREADS, da_smem_bytes(p, D), st>>>(q, ck, cv, k, v, d, p, splits, partials);
-  CU(cudaGetLastError());
+  CU(launch_k(draft_attn_kernel<D, T>, dim3(DA_PIECES), dim3(DA_THREADS), da_smem_bytes(p, D), st, true, q, ck, cv, k, v, d,
+              p, splits, partials));
   const int rows = p.q_rows;
   CU(launch_k(draft_join_kernel<D, T>, dim3(DA_PIECES, (rows + DJ_THREADS / 32 - 1) / (DJ_THREADS / 32)),
               dim3(DJ_THREADS), 0, st, true, d, p.block, (const DaSplit*)splits, (const float*)partials));
@@ -176,12 +176,12 @@ extern "C" int hsg_advance_tables(const hsg_tables_args* a) {
   DraftTablesArgs t{a->lens, a->delta, a->table, a->table_stride, a->ring, a->counters, a->rows, a->width,
                     a->ring_size, FastDiv::of(a->page_size), a->lens_out, a->counters_out, a->cu, a->slots,
                     a->token_rows, a->positions, a->capacity, a->err};
-  const int smem = 3 * a->rows * (int)sizeof(int);
-  if (smem > 48 * 1024 - 1024)
-    CU(cudaFuncSetAttribute(draft_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * DT_MAX_ROWS * 4));
-  // a block for 4,096 listed tokens or 8,192 table entries, any of which may change hands
+  const int smem = a->rows * DT_ROW_BYTES;
+  if (smem > 47 * 1024)
+    CU(cudaFuncSetAttribute(draft_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DT_MAX_ROWS * DT_ROW_BYTES));
+  // a block for 1,024 listed tokens or 2,048 table entries, any of which may change hands, at most two an SM
   const int64_t share = std::max<int64_t>(a->capacity / (4 * DT_THREADS), (int64_t)a->rows * a->width / (8 * DT_THREADS));
-  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(SM_COUNT, share));
+  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(2 * SM_COUNT, share));
   draft_tables_kernel<<<blocks, DT_THREADS, smem, (cudaStream_t)a->stream>>>(t);
   CU(cudaGetLastError());
   return HSG_OK;

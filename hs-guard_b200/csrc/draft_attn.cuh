@@ -139,6 +139,12 @@ __device__ __forceinline__ DaReq da_request(const DraftAttnArgs& a, int block, i
   return r;
 }
 
+// Where a piece begins.
+struct DaStart {
+  int b, h, block, i;  // request, head, block of tokens, tile
+  int64_t unit;        // where that item begins
+};
+
 // A place on the line of tiles.
 template <int KT>
 struct DaWalk {
@@ -148,20 +154,16 @@ struct DaWalk {
   int b, h, block, i;
   int cost;      // units of an item before its tiles
   int64_t unit;  // where the item begins
-  // `within` units into request b0, which begins at unit `begin`
-  __device__ __forceinline__ void start(const DraftAttnArgs& args, int block_size, int item_cost, int b0, int64_t begin,
-                                        int64_t within) {
+  __device__ __forceinline__ void start(const DraftAttnArgs& args, int block_size, int item_cost, const DaStart& at) {
     a = &args;
     size = block_size;
     cost = item_cost;
-    b = b0;
+    b = at.b;
+    h = at.h;
+    block = at.block;
+    i = at.i;
+    unit = at.unit;
     r = da_request<KT>(args, size, b, false);
-    const int len = r.n + cost;
-    const int64_t item = within <= INT32_MAX ? (int64_t)((uint32_t)within / (uint32_t)len) : within / len;
-    i = max(0, (int)(within - item * len) - cost);
-    h = (int)((uint32_t)item / (uint32_t)r.blocks);  // items of one request: heads x blocks
-    block = (int)item - h * r.blocks;
-    unit = begin + item * len;
   }
   __device__ __forceinline__ void skip(int tiles) {  // at most to the item's end
     i += tiles;
@@ -361,11 +363,10 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* o_free = ml_full + 2;                // O has been read
   static_assert(DA_BARS == 4 * DA_MAX_BUFS + 4 + 4 * 4 + 2 + 8 + 2 + 2 + 2 + 1, "every barrier is initialised");
   int64_t* s_scan = reinterpret_cast<int64_t*>(bars + DA_BARS);  // [12][2] warp sums of items and tiles
-  int64_t* s_begin = s_scan + 24;                // the unit at which the piece's first request begins
-  int64_t* s_tiles = s_begin + 1;                // [2] tiles before the piece and up to its end
-  int* s_start = reinterpret_cast<int*>(s_tiles + 2);        // the piece's first request
+  int64_t* s_tiles = s_scan + 24;                // [2] tiles before the piece and up to its end
+  DaStart* s_start = reinterpret_cast<DaStart*>(s_tiles + 2);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_start + 1);
-  int* poison = s_start + 2;                     // [2] of even / odd items: item + 1 if it met a non-finite V
+  int* poison = reinterpret_cast<int*>(tmem_slot + 2);       // [2] of even / odd items: item + 1 if it met a non-finite V
   uint32_t* k_info = reinterpret_cast<uint32_t*>(poison + 2);  // [k_bufs], [v_bufs] of the tile in a buffer, see below
   uint32_t* v_info = k_info + DA_MAX_BUFS;
   DaItem* items = reinterpret_cast<DaItem*>(v_info + DA_MAX_BUFS);  // [2]
@@ -376,7 +377,25 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
   const int G = a.hq / a.hkv;
-  // requests' items and tiles; their loads are on the way during the set-up
+  if (tid >= 32 && tid < 32 + DA_BARS) {  // one barrier a thread
+    const int i = tid - 32;
+    uint64_t* bar = bars + i;
+    mbar_init(bar, bar >= p_full && bar < pv_done ? 4 : bar >= m_full ? (bar < item_full ? 1 : bar < item_empty ? 1 : bar < ml_full ? 8 : 4) : 1);
+    fence_barrier_init();
+  }
+  if (tid == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_ck);
+    prefetch_tmap(&tm_cv);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    poison[0] = poison[1] = 0;
+  }
+  if (warp == 3) tmem_alloc(tmem_slot, DA_TMEM_COLS);
+  pdl_wait();  // nothing above reads or writes what an earlier kernel may use
+  if (tid == 0) splits[piece].last = -1;
+
+  // requests' items and tiles
   const int per = (a.rows + DA_THREADS - 1) / DA_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
   struct Span {
     int64_t items, tiles;
@@ -392,24 +411,6 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     mine.items += x.items;
     mine.tiles += x.tiles;
   }
-  if (tid >= 32 && tid < 32 + DA_BARS) {  // one barrier a thread
-    const int i = tid - 32;
-    uint64_t* bar = bars + i;
-    mbar_init(bar, bar >= p_full && bar < pv_done ? 4 : bar >= m_full ? (bar < item_full ? 1 : bar < item_empty ? 1 : bar < ml_full ? 8 : 4) : 1);
-    fence_barrier_init();
-  }
-  if (tid == 0) {
-    prefetch_tmap(&tm_q);
-    prefetch_tmap(&tm_ck);
-    prefetch_tmap(&tm_cv);
-    prefetch_tmap(&tm_k);
-    prefetch_tmap(&tm_v);
-    poison[0] = poison[1] = 0;
-    splits[piece].last = -1;
-  }
-  if (warp == 3) tmem_alloc(tmem_slot, DA_TMEM_COLS);
-  pdl_trigger();
-
   // ---- this piece of the line ----
   Span upto = mine;
 #pragma unroll
@@ -442,32 +443,34 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int64_t units = total.tiles + cost * total.items, step = max((int64_t)1, (units + DA_PIECES - 1) / DA_PIECES);
   const int64_t w0 = min(units, piece * step), w1 = min(units, w0 + step);
   // whose requests hold the piece's first unit, or the one past its last, says how many tiles lie before it
-  auto locate = [&](int64_t w, bool begins) {
-    const int64_t first = before.tiles + cost * before.items;
-    if (w < first || w >= first + mine.tiles + cost * mine.items) return;
+  const int64_t first = before.tiles + cost * before.items, past = first + mine.tiles + cost * mine.items;
+  const bool has0 = w0 >= first && w0 < past, has1 = w1 >= first && w1 < past;
+  if (has0 || has1) {
     Span at = before;
     for (int b = rb0; b < rb1; ++b) {
-      const Span x = span_of(b, false);
-      const int64_t at_unit = at.tiles + cost * at.items;
-      if (w >= at_unit + x.tiles + cost * x.items) {
-        at.items += x.items;
-        at.tiles += x.tiles;
-        continue;
+      const DaReq r = da_request<KT>(a, plan.block, b, false);
+      const int64_t items = r.n ? (int64_t)r.blocks * a.hkv : 0, at_unit = at.tiles + cost * at.items;
+      const int64_t end = at_unit + items * (r.n + cost);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t w = e ? w1 : w0;
+        if (!(e ? has1 : has0) || w < at_unit || w >= end) continue;
+        const int64_t within = w - at_unit;
+        const int len = r.n + cost;
+        const int64_t item = within <= INT32_MAX ? (int64_t)((uint32_t)within / (uint32_t)len) : within / len;
+        const int i = max(0, (int)(within - item * len) - cost);
+        s_tiles[e] = at.tiles + item * r.n + i;
+        if (e == 0) {
+          const int h = (int)((uint32_t)item / (uint32_t)r.blocks);  // items of a request: heads x blocks
+          *s_start = DaStart{b, h, (int)item - h * r.blocks, i, at_unit + item * len};
+        }
       }
-      DaWalk<KT> there;
-      there.start(a, plan.block, cost, b, at_unit, w - at_unit);
-      s_tiles[begins ? 0 : 1] = at.tiles + (int64_t)(there.h * there.r.blocks + there.block) * there.r.n + there.i;
-      if (begins) {
-        s_start[0] = b;
-        *s_begin = at_unit;
-      }
-      return;
+      at.items += items;
+      at.tiles += items * r.n;
     }
-  };
+  }
   if (tid == 0 && w0 >= units) s_tiles[0] = s_tiles[1] = total.tiles;  // past the line's end
   if (tid == 0 && w0 < units && w1 >= units) s_tiles[1] = total.tiles;
-  locate(w0, true);
-  locate(w1, false);
   __syncthreads();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int n_tiles = (int)(s_tiles[1] - s_tiles[0]);
@@ -475,7 +478,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   int issued = 0, q_issued = 0;  // warps 0 and 3: K and V tiles requested; warp 0: Q tiles
   if (n_tiles > 0) {
     DaWalk<KT> walk;
-    walk.start(a, plan.block, cost, s_start[0], *s_begin, w0 - *s_begin);
+    walk.start(a, plan.block, cost, *s_start);
     // info: of a K tile bit 0: first of its item in this piece, bit 1: last; of a V tile bit 0 as well, then the steps of
     // 16 keys that hold keys: bits 4-7 the first, bits 8-11 one past the last
     if (warp == 0 || warp == 3) {
@@ -588,6 +591,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         cur = next;
         cur_item = next_item;
       }
+      if (lane == 0 && !is_v) pdl_trigger();  // (at the kernel's begin it costs a microsecond)
     } else if (warp == 1) {
       // ---- S ----
       const uint32_t idesc = DaType<T>::idesc(KT);
@@ -945,6 +949,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_constant__ DraftAttnArgs a, int block,
                                                                 const DaSplit* splits, const float* partials) {
   pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();  // the next call's set-up
   const int c = blockIdx.x, lane = threadIdx.x & 31;
   const DaSplit s = splits[c];
   if (s.last < 0) return;

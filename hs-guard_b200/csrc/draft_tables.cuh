@@ -9,17 +9,18 @@
 // reads what it writes nor needs an order between thread blocks, and running it again on the same inputs gives the
 // same result.
 //
-// Every block sums over all requests by itself (two block scans, a few microseconds at most: cheaper than a second
-// launch or a wait between blocks) and then takes its share of the pages and tokens, found by bisection in the prefix
-// sums. Bound by launch and scan latency up to some 100,000 tokens, by the 12 bytes written a token beyond.
+// Every block sums over all requests by itself (two block scans: cheaper than a second launch or a wait between blocks)
+// and then takes its share of the pages and tokens, found by bisection in the prefix sums. Bound by launch and latency up
+// to some 100,000 tokens, by the 12 bytes written a token beyond: TABLES_US for 352 requests that accept or withdraw a few
+// tokens, PROMPTS_US for 870,000 tokens of 1,000 prompts. Blocks of 1,024 threads took 10.6 us for the first: their warps
+// issue the same few scalar steps four times as often.
 #pragma once
 #include "common.cuh"
 
 namespace hsg {
 
-constexpr int DT_THREADS = 1024;
+constexpr int DT_THREADS = 256;
 constexpr int DT_MAX_ROWS = 4096;
-constexpr int DT_PER = DT_MAX_ROWS / DT_THREADS;  // requests a thread
 
 // Division of 0 <= n < 2^31 by d: n * m >> (31 + s) with m = floor(2^(31 + s) / d) + 1, 2^(s - 1) < d <= 2^s.
 struct FastDiv {
@@ -53,30 +54,38 @@ struct DraftTablesArgs {
   int* err;
 };
 
+// Sums that stay at 2^32 - 1 when they would pass it: counts of pages and tokens are compared with less than 2^31.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  const uint32_t s = a + b;
+  return s < a ? 0xffffffffu : s;
+}
+
 // Exclusive prefix sums of two values at once over the block's threads; the totals go to tot.
-__device__ __forceinline__ longlong2 block_scan2(longlong2 v, longlong2* warp_sums, longlong2& tot) {
+__device__ __forceinline__ uint2 block_scan2(uint2 v, uint2* warp_sums, uint2& tot) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto scan = [&](longlong2 s) {
+  uint2 s = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, s.x, o), y = __shfl_up_sync(0xffffffffu, s.y, o);
-      if (lane >= o) { s.x += x; s.y += y; }
-    }
-    return s;
-  };
-  const longlong2 s = scan(v);
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, s.x, o), y = __shfl_up_sync(0xffffffffu, s.y, o);
+    if (lane >= o) s = make_uint2(add_sat(s.x, x), add_sat(s.y, y));
+  }
   __syncthreads();  // an earlier scan's readers of warp_sums are done
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  if (warp == 0) warp_sums[lane] = scan(warp_sums[lane]);
-  __syncthreads();
-  tot = warp_sums[DT_THREADS / 32 - 1];
-  const longlong2 before = warp ? warp_sums[warp - 1] : make_longlong2(0, 0);
-  return make_longlong2(before.x + s.x - v.x, before.y + s.y - v.y);
+  const uint32_t px = __shfl_up_sync(0xffffffffu, s.x, 1), py = __shfl_up_sync(0xffffffffu, s.y, 1);
+  uint2 before = lane ? make_uint2(px, py) : make_uint2(0, 0);
+  tot = make_uint2(0, 0);
+#pragma unroll
+  for (int w = 0; w < DT_THREADS / 32; ++w) {
+    const uint2 t = warp_sums[w];
+    if (w < warp) before = make_uint2(add_sat(before.x, t.x), add_sat(before.y, t.y));
+    tot = make_uint2(add_sat(tot.x, t.x), add_sat(tot.y, t.y));
+  }
+  return before;
 }
 
 // The last entry of the ascending first[0 .. n) that is at most i; first[0] <= i.
-__device__ __forceinline__ int last_at_most(const int* first, int n, int i) {
+__device__ __forceinline__ int last_at_most(const uint32_t* first, int n, uint32_t i) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -86,135 +95,153 @@ __device__ __forceinline__ int last_at_most(const int* first, int n, int i) {
   return lo;
 }
 
+constexpr int DT_ROW_BYTES = 20;  // of shared memory a request
+
 __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_constant__ DraftTablesArgs a) {
-  extern __shared__ int dt_smem[];
-  __shared__ longlong2 warp_sums[DT_THREADS / 32];
-  int* s_cu = dt_smem;            // [rows] tokens before the request, at most capacity
-  int* s_take = s_cu + a.rows;    // [rows] pages taken before it
-  int* s_give = s_take + a.rows;  // [rows] pages given back before it
+  extern __shared__ uint32_t dt_smem[];
+  __shared__ uint2 warp_sums[DT_THREADS / 32];
+  __shared__ int s_ring[3];       // head and tail modulo the ring's size, free pages
+  uint32_t* s_cu = dt_smem;       // [rows] tokens before the request
+  uint32_t* s_take = s_cu + a.rows;  // [rows] pages taken before it
+  uint32_t* s_give = s_take + a.rows;  // [rows] pages given back before it
+  int* s_len = reinterpret_cast<int*>(s_give + a.rows);  // [rows] its length
+  int* s_to = s_len + a.rows;     // [rows] and what that becomes
   const int tid = threadIdx.x;
   const bool writes = blockIdx.x == 0;
-  const int64_t head = a.counters[0], tail = a.counters[1];
-  const bool sane = head >= 0 && tail >= head && tail - head <= a.ring_size;
-  if (!sane && writes && tid == 0) set_error(a.err, ERR_BAD_LEN);
-  const int64_t avail = sane ? tail - head : 0;
-  const int head_at = sane ? (int)(head % a.ring_size) : 0, tail_at = sane ? (int)(tail % a.ring_size) : 0;
   const int most = a.width * (int)a.page.d;  // tokens a table row can hold (checked to be below 2^31)
   auto pages = [&](int n) { return n <= 0 ? 0 : (int)a.page.div((uint32_t)(n - 1)) + 1; };
-  auto ring_at = [&](int from, int i) {
-    const uint32_t x = (uint32_t)from + (uint32_t)i;
+  auto ring_at = [&](int from, uint32_t i) {
+    const uint32_t x = (uint32_t)from + i;
     return (int)(x < (uint32_t)a.ring_size ? x : x % (uint32_t)a.ring_size);
   };
-  const int per = (a.rows + DT_THREADS - 1) / DT_THREADS, b0 = tid * per;
-  int len[DT_PER], to[DT_PER];
-  longlong2 sum = make_longlong2(0, 0), tot;
-#pragma unroll
-  for (int k = 0; k < DT_PER; ++k) {
-    len[k] = to[k] = 0;
-    if (k >= per || b0 + k >= a.rows) continue;
-    len[k] = to[k] = a.lens[b0 + k];
-    if (len[k] < 0 || len[k] > most) {
-      if (writes) set_error(a.err, ERR_BAD_LEN);
-      continue;
-    }
-    const int64_t want = (int64_t)len[k] + a.delta[b0 + k];
-    if (want <= most) to[k] = want < 0 ? 0 : (int)want;
-    const int d = pages(to[k]) - pages(len[k]);
-    sum.x += max(d, 0);
-    sum.y += max(-d, 0);
+  for (int b = tid; b < a.rows; b += DT_THREADS) {
+    const int len = a.lens[b];
+    const int64_t want = (int64_t)len + a.delta[b];
+    const bool good = len >= 0 && len <= most;
+    if (!good && writes) set_error(a.err, ERR_BAD_LEN);
+    s_len[b] = len;
+    s_to[b] = !good || want > most ? len : want < 0 ? 0 : (int)want;
   }
-  const longlong2 at = block_scan2(sum, warp_sums, tot);
-  // more pages than the ring has cannot come back: lengths that say so are wrong
-  const bool returns = tot.y <= a.ring_size;
-  if (!returns && writes && tid == 0) set_error(a.err, ERR_BAD_LEN);
-  const int given = returns ? (int)tot.y : 0;
-  longlong2 grown = make_longlong2(0, 0);  // tokens, pages
-  int64_t need = at.x;
-#pragma unroll
-  for (int k = 0; k < DT_PER; ++k) {
-    const int d = pages(to[k]) - pages(len[k]);
-    need += max(d, 0);
-    if (d > 0 && need > avail) to[k] = len[k];  // not served
-    grown.x += max(to[k] - len[k], 0);
-    if (to[k] > len[k]) grown.y += d;
-  }
-  const longlong2 put = block_scan2(grown, warp_sums, tot);
-  const int total = (int)(tot.x < a.capacity ? tot.x : a.capacity), taken = (int)tot.y;
-  {
-    int64_t tokens = put.x;
-    int take = (int)put.y, give = (int)at.y;
-#pragma unroll
-    for (int k = 0; k < DT_PER; ++k) {
-      const int b = b0 + k;
-      if (k >= per || b >= a.rows) continue;
-      const int d = pages(to[k]) - pages(len[k]);
-      s_cu[b] = (int)(tokens < a.capacity ? tokens : a.capacity);
-      s_take[b] = take;
-      s_give[b] = give;
-      if (writes) {
-        a.lens_out[b] = to[k];
-        a.cu[b] = (int)(tokens < INT32_MAX ? tokens : INT32_MAX);
-      }
-      tokens += max(to[k] - len[k], 0);
-      take += max(d, 0);
-      give += max(-d, 0);
-    }
-  }
-  if (writes && tid == 0) {
-    a.cu[a.rows] = (int)(tot.x < INT32_MAX ? tot.x : INT32_MAX);
-    a.counters_out[0] = head + taken;
-    a.counters_out[1] = tail + given;
-    if (tot.x > a.capacity) set_error(a.err, ERR_BAD_LEN);
+  if (tid == DT_THREADS - 1) {
+    const int64_t head = a.counters[0], tail = a.counters[1];
+    const bool sane = head >= 0 && tail >= head && tail - head <= a.ring_size;
+    if (!sane && writes) set_error(a.err, ERR_BAD_LEN);
+    s_ring[0] = sane ? (int)(head % a.ring_size) : 0;
+    s_ring[1] = sane ? (int)(tail % a.ring_size) : 0;
+    s_ring[2] = sane ? (int)(tail - head) : 0;
   }
   __syncthreads();
-  const int me = blockIdx.x * DT_THREADS + tid, all = gridDim.x * DT_THREADS;
-  for (int i = me; i < taken; i += all) {
+  const int head_at = s_ring[0], tail_at = s_ring[1];
+  const uint32_t avail = (uint32_t)s_ring[2];
+  const int per = (a.rows + DT_THREADS - 1) / DT_THREADS, b0 = min(a.rows, tid * per), b1 = min(a.rows, b0 + per);
+  uint2 sum = make_uint2(0, 0), tot;  // pages wanted, pages given back
+  for (int b = b0; b < b1; ++b) {
+    const int d = pages(s_to[b]) - pages(s_len[b]);
+    sum = make_uint2(add_sat(sum.x, max(d, 0)), add_sat(sum.y, max(-d, 0)));
+  }
+  const uint2 at = block_scan2(sum, warp_sums, tot);
+  // more pages than the ring has cannot come back: lengths that say so are wrong
+  const bool returns = tot.y <= (uint32_t)a.ring_size;
+  if (!returns && writes && tid == 0) set_error(a.err, ERR_BAD_LEN);
+  const uint32_t given = returns ? tot.y : 0;
+  uint2 grown = make_uint2(0, 0);  // tokens, pages
+  uint32_t need = at.x;
+  for (int b = b0; b < b1; ++b) {
+    const int len = s_len[b], d = pages(s_to[b]) - pages(len);
+    need = add_sat(need, max(d, 0));
+    if (d > 0 && need > avail) s_to[b] = len;  // not served
+    if (s_to[b] > len) grown = make_uint2(add_sat(grown.x, s_to[b] - len), add_sat(grown.y, d));
+  }
+  const uint2 put = block_scan2(grown, warp_sums, tot);
+  const uint32_t total = min(tot.x, (uint32_t)a.capacity), taken = tot.y;
+  uint32_t tokens = put.x, take = put.y, give = at.y;
+  for (int b = b0; b < b1; ++b) {
+    const int len = s_len[b], to = s_to[b], d = pages(to) - pages(len);
+    s_cu[b] = tokens;
+    s_take[b] = take;
+    s_give[b] = give;
+    if (writes) {
+      a.lens_out[b] = to;
+      a.cu[b] = (int)min(tokens, 0x7fffffffu);
+    }
+    if (to > len) {
+      tokens = add_sat(tokens, to - len);
+      take = add_sat(take, d);
+    }
+    give = add_sat(give, max(-d, 0));
+  }
+  if (writes && tid == 0) {
+    a.cu[a.rows] = (int)min(tot.x, 0x7fffffffu);
+    a.counters_out[0] = a.counters[0] + taken;
+    a.counters_out[1] = a.counters[1] + given;
+    if (tot.x > (uint32_t)a.capacity) set_error(a.err, ERR_BAD_LEN);
+  }
+  __syncthreads();
+  // warps of all blocks in turn, so that a few entries spread over the SMs
+  const uint32_t me = ((tid >> 5) * gridDim.x + blockIdx.x) * 32 + (tid & 31), all = gridDim.x * DT_THREADS;
+  for (uint32_t i = me; i < taken; i += all) {
     const int b = last_at_most(s_take, a.rows, i);
-    a.table[b * a.table_stride + pages(a.lens[b]) + i - s_take[b]] = a.ring[ring_at(head_at, i)];
+    a.table[b * a.table_stride + pages(s_len[b]) + (i - s_take[b])] = a.ring[ring_at(head_at, i)];
   }
-  for (int i = me; i < given; i += all) {
-    // the last pages of a request that keeps its first pages(to): to is lens_out's value, found again
+  for (uint32_t i = me; i < given; i += all) {
     const int b = last_at_most(s_give, a.rows, i);
-    const int64_t want = (int64_t)a.lens[b] + a.delta[b];
-    a.ring[ring_at(tail_at, i)] = a.table[b * a.table_stride + pages(want < 0 ? 0 : (int)want) + i - s_give[b]];
+    a.ring[ring_at(tail_at, i)] = a.table[b * a.table_stride + pages(s_to[b]) + (i - s_give[b])];
   }
-  // four tokens at a time; a token in a page of this call's finds its page in the ring, whether or not another block
-  // has already written it to the table
+  // a token in a page of this call's finds its page in the ring, whether or not another block has already written it to
+  // the table
+  auto page_of = [&](int b, int no, int held) {
+    return no < held ? a.table[b * a.table_stride + no] : a.ring[ring_at(head_at, s_take[b] + (no - held))];
+  };
   const bool wide = ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.token_rows) |
                       reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
-  const int quads = a.capacity / 4 + (a.capacity % 4 != 0);
-  for (int q = me; q < quads; q += all) {
+  if (!wide || (uint32_t)a.capacity <= 4 * all) {  // few: a token a thread, for the shortest chain of loads
+    for (uint32_t i = me; i < (uint32_t)a.capacity; i += all) {
+      int slot = -1, row = -1, pos = -1;
+      if (i < total) {
+        row = last_at_most(s_cu, a.rows, i);
+        pos = s_len[row] + (int)(i - s_cu[row]);
+        const int no = (int)a.page.div((uint32_t)pos);
+        slot = page_of(row, no, pages(s_len[row])) * (int)a.page.d + pos - no * (int)a.page.d;
+      }
+      a.slots[i] = slot;
+      a.token_rows[i] = row;
+      a.positions[i] = pos;
+    }
+    return;
+  }
+  const uint32_t quads = ((uint32_t)a.capacity + 3) / 4;  // many: four at a time
+  for (uint32_t q = me; q < quads; q += all) {
     int slot[4], row[4], pos[4];
-    int b = -1, next = 0, n = 0, held = 0, page_id = 0, page_no = -1;  // page_id: of page page_no of request b
+    int b = -1, held = 0, page_id = 0, page_no = -1;  // page_id: of page page_no of request b
+    uint32_t next = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = 4 * q + k;
+      const uint32_t i = 4 * q + k;
       slot[k] = row[k] = pos[k] = -1;
       if (i >= total) continue;
-      if (i >= next || b < 0) {
+      if (i >= next) {
         b = last_at_most(s_cu, a.rows, i);
         next = b + 1 < a.rows ? s_cu[b + 1] : total;
-        n = a.lens[b];
-        held = pages(n);
+        held = pages(s_len[b]);
         page_no = -1;
       }
-      const int p = n + i - s_cu[b], no = (int)a.page.div((uint32_t)p);
+      const int p = s_len[b] + (int)(i - s_cu[b]), no = (int)a.page.div((uint32_t)p);
       if (no != page_no) {
         page_no = no;
-        page_id = no < held ? a.table[b * a.table_stride + no] : a.ring[ring_at(head_at, s_take[b] + no - held)];
+        page_id = page_of(b, no, held);
       }
       slot[k] = page_id * (int)a.page.d + p - no * (int)a.page.d;
       row[k] = b;
       pos[k] = p;
     }
-    if (wide && 4 * q + 4 <= a.capacity) {
+    if (4 * q + 4 <= (uint32_t)a.capacity) {
       reinterpret_cast<int4*>(a.slots)[q] = make_int4(slot[0], slot[1], slot[2], slot[3]);
       reinterpret_cast<int4*>(a.token_rows)[q] = make_int4(row[0], row[1], row[2], row[3]);
       reinterpret_cast<int4*>(a.positions)[q] = make_int4(pos[0], pos[1], pos[2], pos[3]);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (4 * q + k >= a.capacity) break;
+        if (4 * q + k >= (uint32_t)a.capacity) break;
         a.slots[4 * q + k] = slot[k];
         a.token_rows[4 * q + k] = row[k];
         a.positions[4 * q + k] = pos[k];
