@@ -329,6 +329,59 @@ struct DaFetch {
   bool mine;      // some of them exist
 };
 
+// The kernel's program is kept small: what is rare, or common to several places, is out of line.
+
+// Which of keys w .. w + 31 of a tile the drafted token `tok` of a request sees. The tile begins at key `base` (a cached
+// position or a drafted index) and has `end` keys; cached keys are seen from position low + 1 on. word: the mask's word
+// for these keys if it is at hand.
+__device__ __noinline__ uint32_t da_seen(const DraftAttnArgs& a, bool tree, int t0, int fresh, int len, int base, int w, int end,
+                                         int low, int tok, const uint32_t* word) {
+  const int from = tree ? 0 : max(0, low + 1 - base), z = min(32, max(0, end - w)), f = min(32, max(0, from - w));
+  uint32_t bits = (z == 32 ? ~0u : (1u << z) - 1u) & (f == 32 ? 0u : ~0u << f);
+  if (!tree || tok >= fresh) return bits;
+  if (a.mask) {
+    const int at = (base + w) >> 5;
+    bits &= word ? *word : at < a.words ? a.mask[(int64_t)(t0 + tok) * a.words + at] : 0u;
+  } else {
+    bits &= tok >= base + w + 31 ? ~0u : tok < base + w ? 0u : (2u << (tok - base - w)) - 1u;
+  }
+  if (a.window && low >= len) {  // a window so short that it ends among the drafted tokens
+    for (uint32_t rest = bits; rest; rest &= rest - 1) {
+      const int j = base + w + __ffs(rest) - 1;
+      if ((a.positions ? a.positions[t0 + j] : len + j) <= low) bits &= ~(rest & -rest);
+    }
+  }
+  return bits;
+}
+
+// Adds the non-finite elements of the V rows that token `tok` of `it` sees, among those that not every row sees, to its
+// written result: they were 0 in the product. Rare, and slow: key after key. Y: the type of `row`.
+template <int KT, int D, typename T, typename Y>
+__device__ __noinline__ void da_restore(const DraftAttnArgs& a, const DaItem& it, int tok, int low, Y* row) {
+  for (int i = it.i0; i < it.i1; ++i) {
+    const bool tree = i >= it.cached;
+    const int base = tree ? (i - it.cached) * KT : (it.first + i) * KT;
+    for (int j = base; j < min(base + KT, tree ? it.fresh : min(it.len, it.lows + 1)); ++j) {
+      const T* v;
+      if (tree) {
+        if (!(da_seen(a, true, it.t0, it.fresh, it.len, base, (j - base) & ~31, it.fresh - base, low, tok, nullptr) >> (j & 31) & 1))
+          continue;
+        v = (const T*)a.v + (int64_t)(it.t0 + j) * a.v_ts + (int64_t)it.h * a.v_hs;
+      } else {
+        if (j <= low) continue;
+        const int pg = a.table[it.b * a.table_stride + j / a.cache.page];
+        if (pg < 0 || pg >= a.cache.pages) continue;
+        v = (const T*)a.cache.v + pg * a.cache.page_stride + j % a.cache.page * a.cache.token_stride + it.h * a.cache.head_stride;
+      }
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) {
+        const float x = (float)v[d];
+        if (!(fabsf(x) < INFINITY)) row[d] = (Y)((float)row[d] + x);
+      }
+    }
+  }
+}
+
 template <int D, typename T>
 __global__ void __launch_bounds__(DA_THREADS, 1)
 draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_ck,
@@ -520,14 +573,19 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         return DaItem{walk.b, walk.h, walk.block, r.t0, r.fresh, r.len, r.lo, r.first, r.cached, r.n, walk.i,
                       min(r.n, walk.i + n_tiles - g), -1, (int)((walk.unit + cost + r.n - 1) / step), {0, 0}};
       };
-      DaFetch cur = fetch(0), next = cur;
-      DaItem cur_item = item_of(0), next_item = cur_item;
+      DaFetch cur{}, next{};
+      DaItem cur_item{}, next_item{};
       int item = 0;  // warp 3: items described
-      for (int g = 0; g < n_tiles && ok; ++g) {
+      for (int g = -1; g < n_tiles && ok; ++g) {
         if (g + 1 < n_tiles) {  // the next tile's table entries, ahead of the wait
-          walk.skip(1);
+          if (g >= 0) walk.skip(1);
           next = fetch(g + 1);
           if (is_v && (next.info & 1)) next_item = item_of(g + 1);
+        }
+        if (g < 0) {
+          cur = next;
+          cur_item = next_item;
+          continue;
         }
         if (is_v && (cur.info & 1)) {  // the item, for the softmax
           if (item >= 2)
@@ -691,30 +749,10 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           // keys up to here are seen by some rows and not by others
           const int mixed = tree ? end : a.window ? min(end, it.lows + 1 - base) : 0;
           const bool special = mixed > 0 || begin > 0 || end < KT;
-          // which of keys 32 w .. 32 w + 31 of the tile this row sees
-          auto seen_keys = [&](int w) {
-            const int from = tree ? 0 : max(0, low + 1 - base), z = min(32, max(0, end - 32 * w));
-            const int f = min(32, max(0, from - 32 * w));
-            uint32_t bits = (z == 32 ? ~0u : (1u << z) - 1u) & (f == 32 ? 0u : ~0u << f);
-            if (tree && valid) {
-              const int word = (base >> 5) + w;
-              if (a.mask)
-                bits &= base == 0 ? first_words[w] : word < a.words ? a.mask[(int64_t)(t0 + tok) * a.words + word] : 0u;
-              else
-                bits &= tok >= base + 32 * w + 31 ? ~0u : tok < base + 32 * w ? 0u : (2u << (tok - base - 32 * w)) - 1u;
-              if (a.window && low >= len) {  // a window so short that it ends among the drafted tokens
-                for (uint32_t rest = bits; rest; rest &= rest - 1) {
-                  const int j = base + 32 * w + __ffs(rest) - 1;
-                  if ((a.positions ? a.positions[t0 + j] : len + j) <= low) bits &= ~(rest & -rest);
-                }
-              }
-            }
-            return bits;
-          };
           // 32 scores from TMEM, -inf where the row does not see the key
           auto scores = [&](int c, uint32_t (&x)[32]) {
             tmem_ld32_async(s_col + 32 * c, x);
-            const uint32_t bits = special ? seen_keys(c) : ~0u;
+            const uint32_t bits = special ? da_seen(a, tree, t0, fresh, len, base, 32 * c, end, low, tok, base == 0 ? &first_words[c] : nullptr) : ~0u;
             tmem_ld_wait();
             da_pin(x);
             if (special) {
@@ -860,31 +898,6 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             __syncwarp();
             tmem_ld32(lanes + O_COL + c, o);
             if (!valid) continue;
-            if (mend) {  // rare, and slow: key after key
-              for (int i = i0; i < i1; ++i) {
-                const bool tree = i >= cached;
-                const int base = tree ? (i - cached) * KT : (it.first + i) * KT;
-                for (int j = base; j < min(base + KT, tree ? fresh : min(len, it.lows + 1)); ++j) {
-                  const T* v;
-                  if (tree) {
-                    if (a.mask ? (j >= 32 * a.words || !(a.mask[(int64_t)(t0 + tok) * a.words + (j >> 5)] >> (j & 31) & 1)) : j > tok) continue;
-                    if (a.window && (a.positions ? a.positions[t0 + j] : len + j) <= low) continue;
-                    v = (const T*)a.v + (int64_t)(t0 + j) * a.v_ts + (int64_t)h * a.v_hs;
-                  } else {
-                    if (j <= low) continue;
-                    const int pg = a.table[it.b * a.table_stride + j / a.cache.page];
-                    if (pg < 0 || pg >= a.cache.pages) continue;
-                    v = (const T*)a.cache.v + pg * a.cache.page_stride + j % a.cache.page * a.cache.token_stride +
-                        h * a.cache.head_stride;
-                  }
-#pragma unroll
-                  for (int x = 0; x < 32; ++x) {
-                    const float f = (float)v[c + x];
-                    if (!(fabsf(f) < INFINITY)) o[x] += f;
-                  }
-                }
-              }
-            }
             if (whole) {
               T* dst = (T*)a.out + orow * D + c;
 #pragma unroll
@@ -904,6 +917,10 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(o_free);
+        if (mend && valid) {
+          if (whole) da_restore<KT, D, T, T>(a, it, tok, low, (T*)a.out + orow * D);
+          else da_restore<KT, D, T, float>(a, it, tok, low, part + row * D);
+        }
         if (valid) {
           if (!whole)
             *reinterpret_cast<float2*>(part + DA_ROWS * D + 2 * row) = make_float2(m, l);
