@@ -12,7 +12,8 @@ and once a branch is accepted:
     t = advance_tables(lens, delta, table, ring, counters, page_size, capacity)    # once a tick
     store_rows(k, v, k_cache, v_cache, t.slots, source)                            # every layer
 
-``DraftCache`` holds the pages, tables and counters of several layers and calls the last two. Every function queues
+``DraftCache`` holds the pages, tables and counters of several layers and calls the last two; ``ring_cache`` shows a live
+engine's 512-token rings as such a cache. Every function queues
 work on torch's current stream of its tensors' device and waits for nothing; outputs are new tensors unless they are
 said to change in place. Arguments of a wrong shape, type, device or alignment raise ``ValueError`` before anything
 is queued. Values on the device are checked by the kernels, which skip an index outside its range and record the
@@ -108,6 +109,35 @@ def store_rows(k, v, k_cache, v_cache, slots, source=None, err=None):
     """Copy rows of k and v [rows, hkv, dim] into cache slots, in place: row source[i] (None: i) to slots[i], both
     [count] int32; a negative slot is skipped. The slots must differ. fp16 or bf16, as the cache."""
     tensors().store_rows(k, v, k_cache, v_cache, slots, source, err)
+
+
+def ring_cache(engine, layer, slots):
+    """A live engine's rings of softmax layer ``layer`` (0 .. 5) as the paged cache of ``tree_attention``: (k_cache, v_cache,
+    table, lens) for requests ``slots``, to be used with window <= 512 and positions from the slots' lengths on.
+
+    Nothing is copied: the rings [slots + 1, kv heads, 513, dim] are seen as pages of 64 columns that may begin at any
+    row, and logical page j of a slot is columns 64 (j mod 8) on. The engine writes its rings on its own stream: drafted
+    tokens may be attended between its ticks, and the next tick must not begin before the calls that read the rings have
+    ended."""
+    cfg = engine.cfg
+    pools = engine.pools()
+    ring_k, ring_v = pools["ring_k"], pools["ring_v"]
+    if not 0 <= layer < ring_k.shape[0]:
+        raise ValueError(f"layer must be in [0, {ring_k.shape[0]})")
+    slots = [int(x) for x in slots]
+    if not slots or min(slots) < 0 or max(slots) >= engine.max_slots:
+        raise ValueError(f"slots must be in [0, {engine.max_slots})")
+    page, cols, heads, dim = 64, cfg.window + 1, cfg.kv_heads, cfg.attn_head_dim
+    rows = ring_k[layer].numel() // dim - (heads - 1) * cols - (page - 1)
+    if rows * page > 2 ** 31 - 1:
+        raise ValueError("the engine's rings are beyond 32-bit page slots: use fewer slots")
+    views = [r[layer].as_strided((rows, page, heads, dim), (dim, dim, cols * dim, 1)) for r in (ring_k, ring_v)]
+    device = engine.device
+    lens = torch.as_tensor(engine.length[slots], dtype=torch.int32, device=device)
+    width = max(1, -(-int(engine.length[slots].max()) // page))
+    logical = torch.arange(width, device=device) % (cfg.window // page) * page
+    table = torch.as_tensor(slots, device=device)[:, None] * (heads * cols) + logical
+    return views[0], views[1], table.to(torch.int32), lens
 
 
 class DraftCache:
