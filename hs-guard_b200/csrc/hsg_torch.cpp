@@ -10,6 +10,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -141,6 +142,8 @@ PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F body) {
     return nullptr;
   }
   try {
+    // the outputs have no gradients: their creation skips autograd's dispatch
+    const at::AutoDispatchBelowADInplaceOrView below;
     return body();
   } catch (const Refused& r) {
     PyErr_SetString(PyExc_ValueError, r.text);
