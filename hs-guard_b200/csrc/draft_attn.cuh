@@ -274,6 +274,17 @@ __device__ __forceinline__ void da_pin(uint32_t* r) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                  "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
+// 32 32-bit values a thread into TMEM columns taddr .. taddr + 31 of its lane; complete after tmem_st_wait.
+__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
 // 16 packed 32-bit values a thread into TMEM columns taddr .. taddr + 15 of its lane; complete after tmem_st_wait.
 __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
@@ -757,17 +768,6 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           // keys up to here are seen by some rows and not by others
           const int mixed = tree ? end : a.window ? min(end, it.lows + 1 - base) : 0;
           const bool special = mixed > 0 || begin > 0 || end < KT;
-          // 32 scores from TMEM, -inf where the row does not see the key
-          auto scores = [&](int c, uint32_t (&x)[32]) {
-            tmem_ld32_async(s_col + 32 * c, x);
-            const uint32_t bits = special ? da_seen(a, tree, t0, fresh, len, base, 32 * c, end, low, tok, base == 0 ? &first_words[c] : nullptr) : ~0u;
-            tmem_ld_wait();
-            da_pin(x);
-            if (special) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = bits >> j & 1 ? x[j] : 0xff800000u;
-            }
-          };
           if (ok) ok = da_wait(&s_full[ring.at], ring.phase, a.err, ERR_TIMEOUT_MMA);
           tc_fence_after();
           __syncwarp();
@@ -780,13 +780,22 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll 1
             for (int c = 0; c < KT / 32; ++c) {
               uint32_t x[32];
-              scores(c, x);
+              tmem_ld32_async(s_col + 32 * c, x);
+              tmem_ld_wait();
+              da_pin(x);
+              if (special) {  // -inf where the row does not see the key, for the second reading as well
+                const uint32_t bits = da_seen(a, tree, t0, fresh, len, base, 32 * c, end, low, tok, base == 0 ? &first_words[c] : nullptr);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = bits >> j & 1 ? x[j] : 0xff800000u;
+                tmem_st32_async(s_col + 32 * c, x);
+              }
 #pragma unroll
               for (int j = 0; j < 32; j += 8)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                   tops[q] = fmaxf(fmaxf(tops[q], __uint_as_float(x[j + q])), __uint_as_float(x[j + 4 + q]));
             }
+            if (special) tmem_st_wait();
             top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sl2;
           }
           // the maximum so far, from the other group; it is raised only when a tile exceeds it by 2^8: weights stay
@@ -823,7 +832,9 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll 1
             for (int c = 0; c < KT / 32; ++c) {
               uint32_t x[32], pk[16];
-              scores(c, x);
+              tmem_ld32_async(s_col + 32 * c, x);
+              tmem_ld_wait();
+              da_pin(x);
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 float2 y = fma2(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul, off);
