@@ -22,6 +22,7 @@ int check_cache(const hsg_page_cache& c, int heads, int dim) {
   if (!aligned16(c.k) || !aligned16(c.v) || c.page_stride % 8 || c.token_stride % 8 || c.head_stride % 8 ||
       c.page_stride < 0 || c.token_stride < 0 || c.head_stride < 0)
     return fail(HSG_ERR_INVALID, "cache rows must lie on 16-byte boundaries, at strides that are not negative");
+  if (c.pages > 1 && c.page_stride == 0) return fail(HSG_ERR_INVALID, "the cache's pages must differ");
   if ((c.page_size > 1 && c.token_stride < dim) || (heads > 1 && c.head_stride < dim))
     return fail(HSG_ERR_INVALID, "cache rows of %d elements overlap (token stride %lld, head stride %lld)", dim,
                 (long long)c.token_stride, (long long)c.head_stride);
@@ -266,6 +267,10 @@ extern "C" int hsg_tree_attention(const hsg_tree_attention_args* a) {
       !rows16(a->q_token_stride, a->q_head_stride, 2) || !rows16(a->k_token_stride, a->k_head_stride, 2) ||
       !rows16(a->v_token_stride, a->v_head_stride, 2))
     return fail(HSG_ERR_INVALID, "q, k and v rows must lie on 16-byte boundaries");
+  // tiles are read through tensor maps, which know no stride of 0 (a broadcast dimension)
+  if ((a->tokens > 1 && (a->q_token_stride <= 0 || a->k_token_stride <= 0 || a->v_token_stride <= 0)) ||
+      (a->hq > 1 && a->q_head_stride <= 0) || (a->hkv > 1 && (a->k_head_stride <= 0 || a->v_head_stride <= 0)))
+    return fail(HSG_ERR_INVALID, "q, k and v must have positive strides: a broadcast dimension has to be written out");
   DraftAttnArgs d{a->q, a->k, a->v, a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride,
                   a->v_token_stride, a->v_head_stride, page_cache(a->cache), a->table, a->table_stride, a->lens, a->cu,
                   a->positions, a->mask, a->rows, a->width, a->tokens, a->words, a->max_tree, a->hq, a->hkv, a->window,

@@ -67,10 +67,11 @@ struct DraftAttnArgs {
 //    or two warps a scheduler wait for latency, not for the special-function unit.
 //  - an L2 policy that keeps a share of the keys for a request's next block of rows changed neither time nor HBM bytes.
 //
-// Measured on B200: five requests of up to 50,001 cached tokens, 13 drafts, 32 / 8 heads of 128: 488 MB in 86 us, 5.7 TB/s,
-// bound by HBM. 352 requests, 512-token window, up to 9 drafts, 8 / 2 heads of 256: 393 MB in 82 us, 4.7 TB/s: ten tiles an
-// item, so items' set-up and epilogues and masked tiles count. 40 requests of up to 6,000 tokens, 64 drafts, 32 / 4 heads of
-// 128: four blocks of rows read a head's keys, of which 1.05 GB come from HBM and 2.3 GB through L2 in 207 us.
+// Measured on B200, short loops (sustained ones are 10 to 15% slower, the clock falls): five requests of up to 50,001 cached
+// tokens, 13 drafts, 32 / 8 heads of 128: 488 MB in 85 us, 5.7 TB/s, bound by HBM. 352 requests, 512-token window, up to 9
+// drafts, 8 / 2 heads of 256: 393 MB in 80 us, 4.9 TB/s: ten tiles an item, so items' set-up and epilogues and masked tiles
+// count. 40 requests of up to 6,000 tokens, 64 drafts, 32 / 4 heads of 128: four blocks of rows read a head's keys, of which
+// 1.06 GB come from HBM and 2.3 GB through L2 in 190 us. One token: 10 us of latencies and 3 for the join.
 //
 // The weights are rounded to V's type for the second product (relative 2^-11 or 2^-8 each, as the result itself is);
 // scores, maxima, sums and O are fp32, and the row sum adds the weights before they are rounded.
@@ -463,9 +464,10 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     prefetch_tmap(&tm_v);
     poison[0] = poison[1] = 0;
   }
-  if (warp == 3) tmem_alloc(tmem_slot, DA_TMEM_COLS);
   pdl_wait();  // nothing above reads or writes what an earlier kernel may use
   if (tid == 0) splits[piece].last = -1;
+  // not before the wait: a block that held tensor memory there could keep it from the kernel that it waits for
+  if (warp == 3) tmem_alloc(tmem_slot, DA_TMEM_COLS);
 
   // requests' items and tiles
   const int per = (a.rows + DA_THREADS - 1) / DA_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);

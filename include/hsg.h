@@ -203,7 +203,7 @@ int hsg_check_bounded_wait(int device, double* seconds);
  * All pointers are device pointers, all work is queued on `stream` (cudaStream_t, NULL: the default stream) of the
  * current device and nothing waits for it. `size` is the struct's size in bytes (checked). `err` is a device int (0 on
  * entry) or NULL: a kernel that meets an index outside its range skips it and records the reason there
- * (hsg_device_error_text). Element types: HSG_DT_*. Strides count elements; rows (the last dimension) are contiguous
+ * (hsg_device_error_text); what the request concerned gets is then not defined. Element types: HSG_DT_*. Strides count elements; rows (the last dimension) are contiguous
  * and begin on 16-byte boundaries. A call with no rows or tokens does nothing. */
 #define HSG_DT_F32 0
 #define HSG_DT_F16 1

@@ -54,7 +54,8 @@ def _attention(**kw):
     dict(page=4), dict(pages=1 << 30, page=16), dict(rows=-1), dict(tokens=-1), dict(hq=0), dict(hkv=0), dict(hkv=3), dict(dim=96),
     dict(dtype=0), dict(dtype=3), dict(max_tree=0), dict(max_tree=1025), dict(max_tree=33), dict(window=-1), dict(width=0),
     dict(tstride=1), dict(width=1 << 28, tstride=1 << 28), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
-    dict(scale=float("nan")), dict(hq=258), dict(ws=0), dict(ws=8), dict(wsb=1000)])
+    dict(scale=float("nan")), dict(hq=258), dict(qt=0), dict(qh=0), dict(kt=0),
+    dict(vh=0), dict(vt=-8), dict(ps=0), dict(ws=0), dict(ws=8), dict(wsb=1000)])
 def test_tree_attention_refuses(L, bad):
     assert L.hsg_tree_attention(_attention(**bad)) == _lib.HSG_ERR_INVALID
     assert L.hsg_last_error()
