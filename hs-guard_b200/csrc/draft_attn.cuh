@@ -36,10 +36,10 @@ struct DraftAttnArgs {
 // request's keys in tiles of KT (128, or 64 at head dim 256) are an item (request, key head, block of tokens). All items,
 // in order, are one line, an item up to DA_ITEM_COST units (its set-up and epilogue) and then a unit a tile long, that is cut
 // into equal pieces, one a thread block, whatever the requests' lengths, so a long cache is split over many SMs and short
-// ones share one; the lengths are read on the device. (Without the units for items, pieces with many short ones ran up to
-// half as long again as the mean.) An item that lies in one piece is written
-// out; of one that is cut, each piece leaves its unnormalised sums, row maxima and row sums in the workspace and
-// draft_join_kernel joins them in piece order, so results do not depend on timing.
+// ones share one; a few long items are cut into fewer (what a part costs their join is said at the cut). The lengths are
+// read on the device. (Without the units for items, pieces with many short ones ran up to half as long again as the mean.)
+// An item that lies in one piece is written out; of one that is cut, each piece leaves its unnormalised sums, row maxima
+// and row sums in the workspace and draft_join_kernel joins them in piece order, so results do not depend on timing.
 //
 // Per tile: S = Q K^T (tcgen05, TMEM), softmax with a running maximum in registers (a row a thread), P in the type of V
 // written over S in TMEM, O += P V (A = P from TMEM, B = V as it lies in shared memory, N-major). Warps:
@@ -514,7 +514,14 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // where pieces have few tiles, latency counts and not the balance: an item is then as long as its tiles
   const int64_t mean = (total.tiles + DA_PIECES - 1) / DA_PIECES;
   const int cost = mean >= 4 * DA_ITEM_COST ? DA_ITEM_COST : 0;
-  const int64_t units = total.tiles + cost * total.items, step = max((int64_t)1, (units + DA_PIECES - 1) / DA_PIECES);
+  // An item of n tiles cut into pieces of s costs about 2 us for each of a piece's tiles and 0.37 us for each of the n / s
+  // parts that its join reads: s + 1 tiles a piece pay from n = 5 s (s + 1) on. That bounds the pieces from below where
+  // items are few and long. One request, one key head of 16 rows, head dim 128, without this and with it: 9,000 keys 31.6
+  // and 20.8 us, 17,000 keys 48.9 and 24.0, 40,000 keys 52.7 and 31.7; four key heads: 4,400 keys 20.9 and 17.5, 1,000 keys
+  // (one tile a piece either way) 15.7 and 15.6. A fixed two tiles a piece: two tiles an item 13.9 to 15.5.
+  const float item_tiles = (float)total.tiles / (float)max((int64_t)1, total.items);
+  const int64_t least = max(1, (int)(sqrtf(0.2f * item_tiles + 0.25f) + 0.5f));
+  const int64_t units = total.tiles + cost * total.items, step = max(least, (units + DA_PIECES - 1) / DA_PIECES);
   const int64_t w0 = min(units, piece * step), w1 = min(units, w0 + step);
   // whose requests hold the piece's first unit, or the one past its last, says how many tiles lie before it
   const int64_t first = before.tiles + cost * before.items, past = first + mine.tiles + cost * mine.items;

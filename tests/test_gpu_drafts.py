@@ -401,6 +401,17 @@ def test_tree_attention_flat_and_peaked_scores(D, spread):
     Case([1500, 37], [6, 11], 8, 2, 256, 16, F16, spread=min(spread, 3.0), seed=6).check(D)
 
 
+@pytest.mark.parametrize("lens,counts,hq,hkv,dim,page,dtype,window", [
+    ([1279], [1], 4, 1, 128, 16, BF16, 0), ([1281], [1], 4, 1, 128, 16, BF16, 0), ([639], [3], 2, 1, 256, 16, F16, 0),
+    ([3845], [2], 16, 2, 64, 64, F16, 0), ([8000], [5], 2, 1, 128, 32, F16, 0), ([9001], [1], 8, 1, 256, 64, BF16, 0),
+    ([14000, 0, 1], [1, 0, 2], 2, 1, 128, 48, BF16, 0), ([5, 9000, 300], [2, 70, 1], 4, 1, 128, 16, F16, 0),
+    ([30000], [4], 3, 3, 64, 40, BF16, 20000)])
+def test_tree_attention_pieces_of_few_long_items(D, lens, counts, hq, hkv, dim, page, dtype, window):
+    """Few items of many tiles: a piece holds several of an item's tiles although more thread blocks are free, the last
+    pieces of the line are empty, and an item's last part is shorter than the others."""
+    Case(lens, counts, hq, hkv, dim, page, dtype, window, mask="holes" if dim == 64 else "tree", seed=sum(lens)).check(D)
+
+
 def test_tree_attention_rising_scores(D):
     """Keys sorted so that the running maximum rises all along a long cache, by more than any fixed slack."""
     c = Case([3000], [2], 4, 1, 128, 8, F16, mask=None, seed=8)
