@@ -73,8 +73,12 @@ struct DraftAttnArgs {
 // count. 40 requests of up to 6,000 tokens, 64 drafts, 32 / 4 heads of 128: four blocks of rows read a head's keys, of which
 // 1.06 GB come from HBM and 2.3 GB through L2 in 190 us. One token: 10 us of latencies and 3 for the join.
 //
-// The weights are rounded to V's type for the second product (relative 2^-11 or 2^-8 each, as the result itself is);
-// scores, maxima, sums and O are fp32, and the row sum adds the weights before they are rounded.
+// The weights are rounded to V's type for the second product (tcgen05 takes both factors of one 16-bit type; a second
+// product with what the rounding left would double that product): relative 2^-11 or 2^-8 each, as the result itself is. For
+// fp16 that needs its whole range: weights are 2^(s - m + 11) with m at most 2^4 short of the maximum, so that the largest
+// lies between 2^11 and 2^15 and one of 2^-25 of it, 17 nats below, is still a normal number; what is smaller yet is rounded
+// to multiples of 2^-35 of the largest. The factor 2^11 is in O and in the row sums alike. bf16 has fp32's range and takes
+// none. Scores, maxima, sums and O are fp32, and the row sum adds the weights before they are rounded.
 //
 // A wait tells a barrier's phase from its neighbours only. S, P and P V of tile g use barrier g % NS: S of tile g waits for
 // P V of tile g - NS, which waited for P of that tile, which its softmax wrote after it had read S; so whoever waits there
@@ -190,15 +194,19 @@ struct DaWalk {
   }
 };
 
-// fp16 / bf16: instruction descriptors with B K-major (S) and N-major (P V), packing, and the bits of a non-finite value
+// fp16 / bf16: instruction descriptors with B K-major (S) and N-major (P V), the bits of a non-finite value, and of the
+// softmax weights 2^(s - m + kLift): m rises when a score exceeds it by more than kSlack. A larger kSlack rescales O less often,
+// kSlack + kLift is what the type holds above 1.
 template <typename T> struct DaType;
 template <> struct DaType<__half> {
   static __host__ __device__ constexpr uint32_t idesc(int n) { return idesc_f16(DA_ROWS, n); }
   static constexpr uint32_t kExp = 0x7c00u;
+  static constexpr float kSlack = 4.f, kLift = 11.f;
 };
 template <> struct DaType<__nv_bfloat16> {
   static __host__ __device__ constexpr uint32_t idesc(int n) { return idesc_bf16(DA_ROWS, n); }
   static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr float kSlack = 8.f, kLift = 0.f;
 };
 constexpr uint32_t DA_B_N_MAJOR = 1u << 16;
 
@@ -409,6 +417,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ DraftAttnArgs a, const DaPlan plan,
                   DaSplit* splits, float* partials) {
   constexpr int KT = da_tile(D), NC = D / 64, BUF = da_buffer_bytes(D), NS = da_scores(D);
+  constexpr float LIFT = DaType<T>::kLift;
   constexpr uint32_t O_COL = NS * KT;
   static_assert(O_COL + D <= DA_TMEM_COLS, "S buffers and O fill TMEM");
   extern __shared__ __align__(1024) uint8_t da_smem_raw[];
@@ -807,11 +816,10 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (special) tmem_st_wait();
             top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sl2;
           }
-          // the maximum so far, from the other group; it is raised only when a tile exceeds it by 2^8: weights stay
-          // below that, which fp16 holds
+          // the maximum so far, from the other group; it is raised only when a tile exceeds it by 2^kSlack
           if (ok && g > 0) ok = da_wait(&m_full[4 * (group ^ 1) + quarter], ((g - 1) >> 1) & 1, a.err, ERR_TIMEOUT_MMA);
           const float seen = i > i0 ? m_rows[128 * (group ^ 1) + row] : -INFINITY;
-          const bool raise = valid && (top > seen + 8.f || (seen == -INFINITY && top > -INFINITY));
+          const bool raise = valid && (top > seen + DaType<T>::kSlack || (seen == -INFINITY && top > -INFINITY));
           const float now = raise ? top : seen;
           m_rows[128 * group + row] = now;
           __syncwarp();
@@ -835,7 +843,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tmem_st32(lanes + O_COL + c, o);
               }
             }
-            const float2 mul = make_float2(sl2, sl2), off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(-m, -m);
+            const float2 mul = make_float2(sl2, sl2), off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(LIFT - m, LIFT - m);
             float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             __syncwarp();
 #pragma unroll 1
@@ -953,7 +961,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           if (!whole)
             *reinterpret_cast<float2*>(part + DA_ROWS * D + 2 * row) = make_float2(m, l);
           else if (a.lse)
-            a.lse[orow] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            a.lse[orow] = l > 0.f || l != l ? (m - LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
         }
         if (row == 0 && i0 == 0 && i1 < it.n) splits[piece] = DaSplit{it.b, h, it.block, it.last, slot, {0, 0, 0}};
         __syncwarp();
@@ -1025,7 +1033,7 @@ __global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_con
   const int64_t orow = (int64_t)(t0 + tok) * a.hq + s.h * G + row % G;
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) ((T*)a.out)[orow * D + e * 32 + lane] = (T)(o[e] * inv);
-  if (lane == 0 && a.lse) a.lse[orow] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  if (lane == 0 && a.lse) a.lse[orow] = l > 0.f || l != l ? (m - DaType<T>::kLift + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 }  // namespace hsg
