@@ -5,9 +5,10 @@
 // Pages. Request b holds len_b tokens in ceil(len_b / page) pages, listed in order in its row of the table. Free pages
 // wait in a ring: counters = (head, tail), both only ever growing, entries head .. tail - 1 (modulo the ring's size)
 // are free. A request that grows takes entries from the head in request order, one that shrinks puts its last pages
-// back at the tail. Takes read entries below the tail at entry and returns write from that tail on, so a call neither
-// reads what it writes nor needs an order between thread blocks, and running it again on the same inputs gives the
-// same result.
+// back at the tail. Takes read entries below the tail at entry and returns write from that tail on, as far as the ring has
+// places that hold no free page at entry (a ring with an entry for every page always has); returns beyond them are not
+// made. So a call neither reads what it writes nor needs an order between thread blocks, and running it again on the same
+// inputs gives the same result.
 //
 // Every block sums over all requests by itself (two block scans: cheaper than a second launch or a wait between blocks)
 // and then takes its share of the pages and tokens, found by bisection in the prefix sums. Bound by launch and latency up
@@ -100,7 +101,8 @@ constexpr int DT_ROW_BYTES = 20;  // of shared memory a request
 __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_constant__ DraftTablesArgs a) {
   extern __shared__ uint32_t dt_smem[];
   __shared__ uint2 warp_sums[DT_THREADS / 32];
-  __shared__ int s_ring[3];       // head and tail modulo the ring's size, free pages
+  __shared__ int s_ring[4];       // head and tail modulo the ring's size, free pages, places without one
+  __shared__ uint32_t s_given;    // pages given back, where not all can be
   uint32_t* s_cu = dt_smem;       // [rows] tokens before the request
   uint32_t* s_take = s_cu + a.rows;  // [rows] pages taken before it
   uint32_t* s_give = s_take + a.rows;  // [rows] pages given back before it
@@ -129,10 +131,12 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
     s_ring[0] = sane ? (int)(head % a.ring_size) : 0;
     s_ring[1] = sane ? (int)(tail % a.ring_size) : 0;
     s_ring[2] = sane ? (int)(tail - head) : 0;
+    s_ring[3] = sane ? a.ring_size - (int)(tail - head) : 0;
+    s_given = 0;
   }
   __syncthreads();
   const int head_at = s_ring[0], tail_at = s_ring[1];
-  const uint32_t avail = (uint32_t)s_ring[2];
+  const uint32_t avail = (uint32_t)s_ring[2], room = (uint32_t)s_ring[3];
   const int per = (a.rows + DT_THREADS - 1) / DT_THREADS, b0 = min(a.rows, tid * per), b1 = min(a.rows, b0 + per);
   uint2 sum = make_uint2(0, 0), tot;  // pages wanted, pages given back
   for (int b = b0; b < b1; ++b) {
@@ -140,19 +144,21 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
     sum = make_uint2(add_sat(sum.x, max(d, 0)), add_sat(sum.y, max(-d, 0)));
   }
   const uint2 at = block_scan2(sum, warp_sums, tot);
-  // more pages than the ring has cannot come back: lengths that say so are wrong
-  const bool returns = tot.y <= (uint32_t)a.ring_size;
-  if (!returns && writes && tid == 0) set_error(a.err, ERR_BAD_LEN);
-  const uint32_t given = returns ? tot.y : 0;
+  // a place may hold a page that this call takes, so a return into it would have to come after the take
+  const uint32_t returned = tot.y;
+  if (returned > room && writes && tid == 0) set_error(a.err, ERR_BAD_LEN);
   uint2 grown = make_uint2(0, 0);  // tokens, pages
-  uint32_t need = at.x;
+  uint32_t need = at.x, back = at.y;
   for (int b = b0; b < b1; ++b) {
     const int len = s_len[b], d = pages(s_to[b]) - pages(len);
     need = add_sat(need, max(d, 0));
-    if (d > 0 && need > avail) s_to[b] = len;  // not served
+    back = add_sat(back, max(-d, 0));
+    if ((d > 0 && need > avail) || (d < 0 && back > room)) s_to[b] = len;  // not served
+    else if (d < 0 && returned > room) atomicMax(&s_given, back);
     if (s_to[b] > len) grown = make_uint2(add_sat(grown.x, s_to[b] - len), add_sat(grown.y, d));
   }
   const uint2 put = block_scan2(grown, warp_sums, tot);
+  const uint32_t given = returned > room ? s_given : returned;
   const uint32_t total = min(tot.x, (uint32_t)a.capacity), taken = tot.y;
   uint32_t tokens = put.x, take = put.y, give = at.y;
   for (int b = b0; b < b1; ++b) {

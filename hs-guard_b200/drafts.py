@@ -54,7 +54,8 @@ def advance_tables(lens, delta, table, ring, counters, page_size, capacity, err=
     ``Tables(lens, counters, cu, slots, rows, positions)``: the new lengths and counters, and for the appended tokens in
     request order their offsets cu [rows + 1] and, each [capacity] with -1 past the last token, cache slot
     (page id * page_size + offset), request and position. An append that the free pages or the table's width cannot
-    hold is not made: its length stays as it was. The inputs lens and counters are kept, so the same call again gives
+    hold is not made: its length stays as it was. So is a return that the ring has no room for beside the pages free at
+    entry, which is recorded in ``err`` as well: a ring should have an entry for every page. The inputs lens and counters are kept, so the same call again gives
     the same result."""
     return Tables(*tensors().advance_tables(lens, delta, table, ring, counters, page_size, capacity, err))
 

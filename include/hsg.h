@@ -227,7 +227,10 @@ typedef struct hsg_page_cache {
  * many (all it has, if fewer), returning emptied pages at the tail. Pages returned by a call are free for the next
  * one. An append that needs pages is served iff all needs up to and including its own, in request order, are within
  * the pages free at entry, and an append past width * page_size is not served: lens_out[b] then stays lens[b] and no
- * token of it is listed. The appended tokens are listed in request order: cu [rows + 1] their counts before each
+ * token of it is listed. Returned pages need a place each beside the pages free at entry: a ring of at least as many
+ * entries as there are pages always has it. In a smaller one, a return is served iff all returned pages up to and
+ * including its own, in request order, fit ring_size - (tail - head); else lens_out[b] stays lens[b] and err is set.
+ * Counters that are negative, out of order or further apart than ring_size serve neither. The appended tokens are listed in request order: cu [rows + 1] their counts before each
  * request, and for each its slot (page id * page_size + offset), request and position; entries from the last token to
  * `capacity` are -1. Tokens beyond capacity are not listed (and err is set). Inputs and outputs must not alias; table
  * and ring change in place, so that a repeated call with the same inputs gives the same result. rows <=

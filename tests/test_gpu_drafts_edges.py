@@ -49,3 +49,89 @@ def test_tree_attention_many_small_weights_beside_a_large_one(D, dim, dtype, nat
     assert worst <= 1, f"{worst:.1f} times the tolerance"
     want = nats + math.log1p(small)
     assert float((lse.double() - want).abs().max()) <= ds + 4e-6 * (1 + want) + steps
+
+
+# ---- advance_tables: rings without room, counters out of range ------------------------------------------------------
+@pytest.mark.parametrize("lens,delta,ring,counters,new,new_counters,new_ring,code", [
+    # four free entries of four: nothing can come back, the append takes two
+    ([32, 0], [-32, 32], [5, 6, 7, 8], [8, 12], [32, 32], [10, 12], [5, 6, 7, 8], 5),
+    # two places: the first return fits, the second does not, the third is behind it
+    ([32, 32, 16], [-32, -17, -16], [5, 6, -1, -1], [4, 6], [0, 32, 16], [4, 8], [5, 6, 0, 1], 5),
+    # exactly full afterwards
+    ([32, 32], [-32, 0], [5, 6, -1, -1], [4, 6], [0, 32], [4, 8], [5, 6, 0, 1], 0),
+    # taking back within a page needs no place
+    ([32, 30], [-3, -13], [5, 6], [6, 8], [29, 17], [6, 8], [5, 6], 0),
+    # returns behind an append that is not served, in a ring that goes round
+    ([20, 40], [100, -40], [5, -1, -1, -1, 6], [4, 6], [20, 0], [4, 9], [5, 2, 3, 4, 6], 0),
+    # counters that cannot be: no page moves, what needs none is served
+    ([32, 0, 20, 3], [-32, 32, 5, -3], [5, 6, 7, 8], [-1, 3], [32, 0, 25, 3], [-1, 3], [5, 6, 7, 8], 5),
+    ([32, 0, 20, 3], [-32, 32, 5, -3], [5, 6, 7, 8], [3, 2], [32, 0, 25, 3], [3, 2], [5, 6, 7, 8], 5),
+    ([32, 0, 20, 3], [-32, 32, 5, -3], [5, 6, 7, 8], [0, 5], [32, 0, 25, 3], [0, 5], [5, 6, 7, 8], 5)])
+def test_advance_tables_ring_without_room(D, lens, delta, ring, counters, new, new_counters, new_ring, code):
+    page, width = 16, 12
+    table, at = torch.full((len(lens), width), -1, dtype=torch.int32), 0
+    for b, n in enumerate(lens):
+        held = -(-n // page)
+        table[b, :held] = torch.arange(at, at + held, dtype=torch.int32)
+        at += held
+    want, taken, listed = table.clone(), 0, []
+    for b, n in enumerate(new):
+        for p in range(-(-lens[b] // page), -(-n // page)):
+            want[b, p] = ring[(counters[0] + taken) % len(ring)]
+            taken += 1
+        listed += [(int(want[b, p // page]) * page + p % page, b, p) for p in range(lens[b], n)]
+    d_table, d_ring = table.cuda(), dev(ring)
+    for _ in range(2):  # the same call again gives the same result
+        err = err_word()
+        t = D.advance_tables(dev(lens), dev(delta), d_table, d_ring, dev(counters, torch.int64), page, 64, err)
+        assert int(err.item()) == code
+        assert t.lens.tolist() == new and t.counters.tolist() == new_counters
+        assert d_ring.tolist() == new_ring and torch.equal(d_table.cpu(), want)
+        none = [(-1, -1, -1)] * (64 - len(listed))
+        assert list(zip(t.slots.tolist(), t.rows.tolist(), t.positions.tolist())) == listed + none
+
+
+@pytest.mark.parametrize("rows,places", [(4000, 9000), (4000, 0), (3000, 1), (700, 10 ** 6)])
+def test_advance_tables_many_returns_into_few_places(D, rows, places):
+    """Several requests a thread and several thread blocks: served up to the first return without a place."""
+    page = 8
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, 60, (rows,), generator=g).tolist()
+    delta = torch.randint(-60, 20, (rows,), generator=g).tolist()
+    held = [-(-n // page) for n in lens]
+    width, used = 12, sum(held)
+    free = used // 3
+    size = free + min(places, used)
+    head = 7 * size + size // 2
+    order = torch.randperm(used + free, generator=g).tolist()
+    table, at = torch.full((rows, width), -1, dtype=torch.int32), 0
+    for b, h in enumerate(held):
+        table[b, :h] = torch.tensor(order[at:at + h], dtype=torch.int32)
+        at += h
+    ring = [-9] * size
+    for i in range(free):
+        ring[(head + i) % size] = order[used + i]
+    new, want, want_ring = [], table.clone(), list(ring)
+    wanted = back = taken = given = 0
+    for b, (n, d) in enumerate(zip(lens, delta)):
+        to = max(0, n + d)
+        have, then = held[b], -(-to // page)
+        wanted, back = wanted + max(0, then - have), back + max(0, have - then)
+        if (then > have and wanted > free) or (then < have and back > size - free):
+            to = n
+        for p in range(have, -(-to // page)):
+            want[b, p] = ring[(head + taken) % size]
+            taken += 1
+        for p in range(-(-to // page), have):
+            want_ring[(head + free + given) % size] = int(table[b, p])
+            given += 1
+        new.append(to)
+    d_table, d_ring, err = table.cuda(), dev(ring), err_word()
+    capacity = sum(max(0, n - m) for n, m in zip(new, lens))
+    t = D.advance_tables(dev(lens), dev(delta), d_table, d_ring, dev([head, head + free], torch.int64), page, capacity, err)
+    assert int(err.item()) == (5 if back > size - free else 0)
+    assert t.lens.tolist() == new and t.counters.tolist() == [head + taken, head + free + given]
+    assert d_ring.tolist() == want_ring and torch.equal(d_table.cpu(), want)
+    pos = t.positions.tolist()
+    assert t.slots.tolist() == [int(want[b, p // page]) * page + p % page for b, p in zip(t.rows.tolist(), pos)]
+    assert pos == [p for n, m in zip(lens, new) for p in range(n, m)]
