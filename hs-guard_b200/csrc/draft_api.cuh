@@ -175,8 +175,8 @@ extern "C" int hsg_advance_tables(const hsg_tables_args* a) {
   if ((a->rows && a->lens_out == a->lens) || a->counters_out == a->counters)
     return fail(HSG_ERR_INVALID, "lens_out and counters_out must not be the inputs");
   DraftTablesArgs t{a->lens, a->delta, a->table, a->table_stride, a->ring, a->counters, a->rows, a->width,
-                    a->ring_size, FastDiv::of(a->page_size), a->lens_out, a->counters_out, a->cu, a->slots,
-                    a->token_rows, a->positions, a->capacity, a->err};
+                    a->ring_size, FastDiv::of(a->page_size), (uint32_t)((1ll << 31) / a->page_size), a->lens_out,
+                    a->counters_out, a->cu, a->slots, a->token_rows, a->positions, a->capacity, a->err};
   const int smem = a->rows * DT_ROW_BYTES;
   if (smem > 47 * 1024)
     CU(cudaFuncSetAttribute(draft_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DT_MAX_ROWS * DT_ROW_BYTES));

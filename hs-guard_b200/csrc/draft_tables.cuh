@@ -8,7 +8,8 @@
 // back at the tail. Takes read entries below the tail at entry and returns write from that tail on, as far as the ring has
 // places that hold no free page at entry (a ring with an entry for every page always has); returns beyond them are not
 // made. So a call neither reads what it writes nor needs an order between thread blocks, and running it again on the same
-// inputs gives the same result.
+// inputs gives the same result. A page id that is negative, or whose slots are beyond 32 bits, is none: it moves on as -1, so
+// that no other page is handed out in its place, its tokens have slot -1, and the error word says so.
 //
 // Every block sums over all requests by itself (two block scans: cheaper than a second launch or a wait between blocks)
 // and then takes its share of the pages and tokens, found by bisection in the prefix sums. Bound by launch and latency up
@@ -45,6 +46,7 @@ struct DraftTablesArgs {
   const int64_t* counters;   // head, tail
   int rows, width, ring_size;
   FastDiv page;
+  uint32_t page_ids;         // ids below this have slots below 2^31
   int32_t* lens_out;         // [rows]
   int64_t* counters_out;
   int32_t* cu;               // [rows + 1] appended tokens before each request
@@ -183,21 +185,29 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
     if (tot.x > (uint32_t)a.capacity) set_error(a.err, ERR_BAD_LEN);
   }
   __syncthreads();
+  bool bad = false;  // this thread has met an id that is none (recorded at the end: a branch here would wait for each load)
+  auto id_of = [&](int id) {
+    const bool is = (uint32_t)id < a.page_ids;
+    bad |= !is;
+    return is ? id : -1;
+  };
   // warps of all blocks in turn, so that a few entries spread over the SMs
   const uint32_t me = ((tid >> 5) * gridDim.x + blockIdx.x) * 32 + (tid & 31), all = gridDim.x * DT_THREADS;
   for (uint32_t i = me; i < taken; i += all) {
     const int b = last_at_most(s_take, a.rows, i);
-    a.table[b * a.table_stride + pages(s_len[b]) + (i - s_take[b])] = a.ring[ring_at(head_at, i)];
+    a.table[b * a.table_stride + pages(s_len[b]) + (i - s_take[b])] = id_of(a.ring[ring_at(head_at, i)]);
   }
   for (uint32_t i = me; i < given; i += all) {
     const int b = last_at_most(s_give, a.rows, i);
-    a.ring[ring_at(tail_at, i)] = a.table[b * a.table_stride + pages(s_to[b]) + (i - s_give[b])];
+    a.ring[ring_at(tail_at, i)] = id_of(a.table[b * a.table_stride + pages(s_to[b]) + (i - s_give[b])]);
   }
-  // a token in a page of this call's finds its page in the ring, whether or not another block has already written it to
-  // the table
+  // the page's first slot, or -1 if its id is none. A token in a page of this call's finds its page in the ring, whether or
+  // not another block has already written it to the table
   auto page_of = [&](int b, int no, int held) {
-    return no < held ? a.table[b * a.table_stride + no] : a.ring[ring_at(head_at, s_take[b] + (no - held))];
+    const int id = id_of(no < held ? a.table[b * a.table_stride + no] : a.ring[ring_at(head_at, s_take[b] + (no - held))]);
+    return id < 0 ? -1 : id * (int)a.page.d;
   };
+  auto slot_in = [&](int first, int offset) { return (first + offset) | first >> 31; };
   const bool wide = ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.token_rows) |
                       reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
   if (!wide || (uint32_t)a.capacity <= 4 * all) {  // few: a token a thread, for the shortest chain of loads
@@ -207,18 +217,19 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
         row = last_at_most(s_cu, a.rows, i);
         pos = s_len[row] + (int)(i - s_cu[row]);
         const int no = (int)a.page.div((uint32_t)pos);
-        slot = page_of(row, no, pages(s_len[row])) * (int)a.page.d + pos - no * (int)a.page.d;
+        slot = slot_in(page_of(row, no, pages(s_len[row])), pos - no * (int)a.page.d);
       }
       a.slots[i] = slot;
       a.token_rows[i] = row;
       a.positions[i] = pos;
     }
+    if (bad) set_error(a.err, ERR_BAD_PAGE);
     return;
   }
   const uint32_t quads = ((uint32_t)a.capacity + 3) / 4;  // many: four at a time
   for (uint32_t q = me; q < quads; q += all) {
     int slot[4], row[4], pos[4];
-    int b = -1, held = 0, page_id = 0, page_no = -1;  // page_id: of page page_no of request b
+    int b = -1, held = 0, first = 0, page_no = -1;  // first: slot of page page_no of request b
     uint32_t next = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -234,9 +245,9 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
       const int p = s_len[b] + (int)(i - s_cu[b]), no = (int)a.page.div((uint32_t)p);
       if (no != page_no) {
         page_no = no;
-        page_id = page_of(b, no, held);
+        first = page_of(b, no, held);
       }
-      slot[k] = page_id * (int)a.page.d + p - no * (int)a.page.d;
+      slot[k] = slot_in(first, p - no * (int)a.page.d);
       row[k] = b;
       pos[k] = p;
     }
@@ -254,6 +265,7 @@ __global__ void __launch_bounds__(DT_THREADS) draft_tables_kernel(const __grid_c
       }
     }
   }
+  if (bad) set_error(a.err, ERR_BAD_PAGE);
 }
 
 struct DraftTreeArgs {

@@ -230,7 +230,8 @@ typedef struct hsg_page_cache {
  * token of it is listed. Returned pages need a place each beside the pages free at entry: a ring of at least as many
  * entries as there are pages always has it. In a smaller one, a return is served iff all returned pages up to and
  * including its own, in request order, fit ring_size - (tail - head); else lens_out[b] stays lens[b] and err is set.
- * Counters that are negative, out of order or further apart than ring_size serve neither. The appended tokens are listed in request order: cu [rows + 1] their counts before each
+ * Counters that are negative, out of order or further apart than ring_size serve neither. A page id met in the ring or
+ * the table that is negative or has slots beyond 32 bits sets err, is passed on as -1 and gives its tokens slot -1. The appended tokens are listed in request order: cu [rows + 1] their counts before each
  * request, and for each its slot (page id * page_size + offset), request and position; entries from the last token to
  * `capacity` are -1. Tokens beyond capacity are not listed (and err is set). Inputs and outputs must not alias; table
  * and ring change in place, so that a repeated call with the same inputs gives the same result. rows <=

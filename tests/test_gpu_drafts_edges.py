@@ -135,3 +135,48 @@ def test_advance_tables_many_returns_into_few_places(D, rows, places):
     pos = t.positions.tolist()
     assert t.slots.tolist() == [int(want[b, p // page]) * page + p % page for b, p in zip(t.rows.tolist(), pos)]
     assert pos == [p for n, m in zip(lens, new) for p in range(n, m)]
+
+
+@pytest.mark.parametrize("bad", [-1, -9, -2 ** 31, 2 ** 27, 2 ** 31 - 1])
+def test_advance_tables_page_ids_out_of_range(D, bad):
+    """They are recorded, passed on as -1 and never become another page's slot. 2^27 pages of 16 are beyond 32-bit slots."""
+    # an append into a page that the table does not have, and one that takes a bad entry of the ring
+    table, ring, err = dev([[bad, 7, 7], [1, 7, 7]]), dev([bad, 4, -5, -5, -5]), err_word()
+    t = D.advance_tables(dev([10, 16]), dev([3, 20]), table, ring, dev([0, 2], torch.int64), 16, 30, err)
+    assert int(err.item()) == 6
+    assert t.lens.tolist() == [13, 36] and t.counters.tolist() == [2, 2] and t.cu.tolist() == [0, 3, 23]
+    assert t.slots.tolist() == [-1] * 3 + [-1] * 16 + [64 + i for i in range(4)] + [-1] * 7
+    assert t.positions.tolist() == list(range(10, 13)) + list(range(16, 36)) + [-1] * 7
+    assert table.tolist() == [[bad, 7, 7], [1, -1, 4]] and ring.tolist() == [bad, 4, -5, -5, -5]
+    # pages given back
+    table, ring, err = dev([[3, bad, 2], [bad, 7, 7]]), dev([-5] * 5), err_word()
+    t = D.advance_tables(dev([40, 1]), dev([-40, 0]), table, ring, dev([5, 5], torch.int64), 16, 0, err)
+    assert int(err.item()) == 6
+    assert t.lens.tolist() == [0, 1] and t.counters.tolist() == [5, 8] and ring.tolist() == [3, -1, 2, -5, -5]
+    # the largest id there is
+    top = 2 ** 27 - 1
+    err = err_word()
+    t = D.advance_tables(dev([14]), dev([2]), dev([[top]]), dev([0]), dev([0, 0], torch.int64), 16, 2, err)
+    assert int(err.item()) == 0 and t.slots.tolist() == [2 ** 31 - 2, 2 ** 31 - 1]
+
+
+def test_advance_tables_page_ids_out_of_range_in_long_lists(D):
+    """Four tokens a thread."""
+    rows, page, width = 512, 16, 130
+    table = torch.arange(rows * width, dtype=torch.int32).view(rows, width)
+    table[5, 0], table[77, 0], table[400, 0] = -3, 2 ** 30, -1
+    d_table, err = table.cuda(), err_word()
+    ring = torch.arange(10 ** 6, 10 ** 6 + rows * 125, dtype=torch.int32)
+    ring[17], ring[40000] = -4, 2 ** 27
+    d_ring = torch.cat([ring, torch.full((rows,), -5, dtype=torch.int32)]).cuda()
+    t = D.advance_tables(dev([3] * rows), dev([2000] * rows), d_table, d_ring, dev([0, len(ring)], torch.int64), page,
+                         2000 * rows + 5, err)
+    assert int(err.item()) == 6 and t.lens.tolist() == [2003] * rows
+    ring = torch.where((ring < 0) | (ring >= 2 ** 27), torch.tensor(-1, dtype=torch.int32), ring)
+    want = table.clone()
+    want[:, 1:126] = ring.view(rows, 125)
+    assert torch.equal(d_table.cpu(), want)
+    pos = torch.arange(3, 2003)
+    ids = want.long()[:, pos // page]
+    slots = torch.where((ids < 0) | (ids >= 2 ** 27), torch.tensor(-1), ids * page + pos % page)
+    assert torch.equal(t.slots.cpu(), torch.cat([slots.flatten(), torch.full((5,), -1)]).to(torch.int32))
