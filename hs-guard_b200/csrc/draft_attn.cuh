@@ -996,8 +996,18 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
 constexpr int DJ_THREADS = 256;
 
+// Tokens from .. to - 1 as if they saw nothing, by `count` threads of which this is number `me`.
+template <int D, typename T>
+__device__ __noinline__ void da_blank(const DraftAttnArgs& a, int64_t from, int64_t to, int64_t me, int64_t count) {
+  constexpr int PER = D / 8;
+  for (int64_t i = from * a.hq * PER + me; i < to * a.hq * PER; i += count) reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (a.lse)
+    for (int64_t i = from * a.hq + me; i < to * a.hq; i += count) a.lse[i] = -INFINITY;
+}
+
 // Joins the parts of an item that was cut: one warp a row, parts in piece order. Block (c, y): the item that begins in
-// piece c, rows 8 y .. 8 y + 7.
+// piece c, rows 8 y .. 8 y + 7. And writes the tokens that no item has: those before cu_0 and from cu_rows on, by all blocks,
+// and those of requests whose lengths are out of range, by the blocks (request mod pieces, 0).
 template <int D, typename T>
 __global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_constant__ DraftAttnArgs a, int block,
                                                                 const DaSplit* splits, const float* partials) {
@@ -1005,6 +1015,22 @@ __global__ void __launch_bounds__(DJ_THREADS) draft_join_kernel(const __grid_con
   if (threadIdx.x == 0) pdl_trigger();  // the next call's set-up
   const int c = blockIdx.x, lane = threadIdx.x & 31;
   const DaSplit s = splits[c];
+  const int lead = a.cu[0], trail = a.cu[a.rows];
+  if (lead > 0 || trail < a.tokens) {
+    const int64_t me = ((int64_t)blockIdx.y * DA_PIECES + c) * DJ_THREADS + threadIdx.x, all = (int64_t)gridDim.y * DA_PIECES * DJ_THREADS;
+    da_blank<D, T>(a, 0, min(lead, a.tokens), me, all);
+    da_blank<D, T>(a, max(trail, 0), a.tokens, me, all);
+  }
+  if (blockIdx.y == 0) {
+    for (int b0 = c + DA_PIECES * (threadIdx.x & ~31); b0 < a.rows; b0 += DA_PIECES * DJ_THREADS) {
+      const int b = b0 + DA_PIECES * lane;
+      const bool out = b < a.rows && a.cu[b + 1] > a.cu[b] && da_request<da_tile(D)>(a, block, b, false).n == 0;
+      for (unsigned rest = __ballot_sync(0xffffffffu, out); rest; rest &= rest - 1) {
+        const int r = b0 + DA_PIECES * (__ffs(rest) - 1);
+        da_blank<D, T>(a, max(a.cu[r], 0), min(a.cu[r + 1], a.tokens), lane, 32);
+      }
+    }
+  }
   if (s.last < 0) return;
   const int row = blockIdx.y * (DJ_THREADS / 32) + (threadIdx.x >> 5), G = a.hq / a.hkv;
   const int tok = s.block * block + row / G, t0 = a.cu[s.b];

@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <limits>
 
 #include "../../include/hsg.h"
 
@@ -371,7 +372,12 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.dtype = code_of(dtype);
     s.stream = stream_of(device);
     const c10::cuda::CUDAGuard guard(device);
-    done(hsg_tree_attention(&s));
+    if (s.rows == 0) {  // the library has nothing to do: no token sees anything
+      out.zero_();
+      lse.fill_(-std::numeric_limits<float>::infinity());
+    } else {
+      done(hsg_tree_attention(&s));
+    }
     return tuple_of(out, lse);
   });
 }

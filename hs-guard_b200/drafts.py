@@ -100,7 +100,8 @@ def tree_attention(q, k, v, k_cache, v_cache, table, lens, cu, scale, max_tree, 
     ``plan_tree`` makes it (any bits may be set or not; None: a chain). With window > 0 only keys at positions above
     the query's own minus window are seen; positions [tokens] int32 (None: length + index) are read only then.
     Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets 0
-    and -inf. ``workspace`` (a uint8 tensor of ``attention_workspace(dim)`` bytes, for one call at a time) is allocated
+    and -inf, as do tokens outside cu[0] .. cu[rows] - 1 and those of a request whose lengths are out of range (which
+    ``err`` records). ``workspace`` (a uint8 tensor of ``attention_workspace(dim)`` bytes, for one call at a time) is allocated
     when it is not given."""
     return tensors().tree_attention(q, k, v, k_cache, v_cache, table, lens, cu, scale, max_tree, mask, positions, window,
                                     workspace, err)

@@ -203,7 +203,7 @@ int hsg_check_bounded_wait(int device, double* seconds);
  * All pointers are device pointers, all work is queued on `stream` (cudaStream_t, NULL: the default stream) of the
  * current device and nothing waits for it. `size` is the struct's size in bytes (checked). `err` is a device int (0 on
  * entry) or NULL: a kernel that meets an index outside its range skips it and records the reason there
- * (hsg_device_error_text); what the request concerned gets is then not defined. Element types: HSG_DT_*. Strides count elements; rows (the last dimension) are contiguous
+ * (hsg_device_error_text); what the request concerned gets is then not defined, unless said below. Element types: HSG_DT_*. Strides count elements; rows (the last dimension) are contiguous
  * and begin on 16-byte boundaries. A call with no rows or tokens does nothing. */
 #define HSG_DT_F32 0
 #define HSG_DT_F16 1
@@ -303,7 +303,9 @@ int hsg_norm_rope(const hsg_norm_rope_args* args);
  * with a window, p_j > p_t - window. out [tokens][hq][dim] = softmax(scale q.k) v in dtype (HSG_DT_F16 or _BF16, as q,
  * k, v and the cache), lse [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing gets 0 and -inf;
  * what is not seen, beyond a length included, does not enter a result whatever its bits. positions are read only with
- * a window (NULL: lens[b] + index) and must be at least lens[b]. Requests may have no cached or no drafted tokens; none
+ * a window (NULL: lens[b] + index) and must be at least lens[b]. cu must not descend. Tokens of no request (before cu[0], from
+ * cu[rows] on: a buffer of a fixed size may be longer than what is drafted) see nothing, and so do those of a request whose
+ * lengths are out of range. Requests may have no cached or no drafted tokens; none
  * has more than max_tree drafted ones. Table entries of pages wholly outside the window are not read. `workspace`:
  * hsg_tree_attention_workspace(dim) bytes on a 16-byte boundary, not shared by calls that overlap in time. */
 typedef struct hsg_tree_attention_args {

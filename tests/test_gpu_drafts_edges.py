@@ -180,3 +180,61 @@ def test_advance_tables_page_ids_out_of_range_in_long_lists(D):
     ids = want.long()[:, pos // page]
     slots = torch.where((ids < 0) | (ids >= 2 ** 27), torch.tensor(-1), ids * page + pos % page)
     assert torch.equal(t.slots.cpu(), torch.cat([slots.flatten(), torch.full((5,), -1)]).to(torch.int32))
+
+
+# ---- tokens that no request claims, and requests that are refused ---------------------------------------------------
+def dirty(*shape, dtype):
+    """Leaves memory of NaN for the next allocation of this size."""
+    x = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+    y = torch.full(shape[:2], float("nan"), device="cuda")
+    del x, y
+
+
+def blank(out, lse):
+    return bool((out == 0).all()) and bool((lse == float("-inf")).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_tree_attention_tokens_of_no_request(D, dim):
+    """A buffer longer than the requests' tokens (a fixed size in a graph): what lies around them is 0 and -inf, no error."""
+    c = Case([300, 0, 2000], [4, 3, 9], 8, 2, dim, 16, F16, seed=3)
+    out, lse = c.check(D)
+    lead, trail = 5, 1000
+    pad = lambda x: torch.cat([x.new_full((lead, *x.shape[1:]), 7), x, x.new_full((trail, *x.shape[1:]), 7)])  # noqa: E731
+    c.q, c.k, c.v, c.mask, c.positions = (pad(x) for x in (c.q, c.k, c.v, c.mask, c.positions))
+    c.cu = [lead + x for x in c.cu]
+    dirty(*c.q.shape, dtype=F16)
+    err = err_word()
+    more, more_lse = c.call(D, err=err)
+    assert int(err.item()) == 0
+    mine = slice(lead, lead + len(out))
+    assert torch.equal(more[mine], out) and torch.equal(more_lse[mine], lse)
+    assert blank(more[:lead], more_lse[:lead]) and blank(more[-trail:], more_lse[-trail:])
+
+
+def test_tree_attention_without_requests(D):
+    c = Case([40], [6], 8, 2, 128, 16, F16, seed=3)
+    c.lens, c.cu, c.table = [], [0], c.table[:0]
+    dirty(*c.q.shape, dtype=F16)
+    assert blank(*c.call(D))
+
+
+@pytest.mark.parametrize("lens,cu,max_tree,refused", [
+    ([100, -1, 50], [0, 4, 9, 12], 16, [(4, 9)]), ([100, 10 ** 6, 50], [0, 4, 9, 12], 16, [(4, 9)]),
+    ([100, 60, 50], [0, 4, 9, 12], 4, [(4, 9)]), ([100, 60, 50], [0, 4, 9, 14], 16, [(9, 12)]),
+    ([100, 60, 50], [-2, 4, 9, 12], 16, [(0, 4)]), ([-5, -5, -5], [1, 4, 4, 12], 16, [(0, 12)])])
+def test_tree_attention_refused_requests_see_nothing(D, lens, cu, max_tree, refused):
+    """The others are what they are without them."""
+    c = Case([100, 60, 50], [4, 5, 3], 8, 2, 128, 16, F16, seed=4, max_tree=16)
+    out, lse = c.check(D)
+    c.lens, c.cu, c.max_tree = lens, cu, max_tree
+    dirty(*c.q.shape, dtype=F16)
+    err = err_word()
+    got, got_lse = c.call(D, err=err)
+    assert int(err.item()) == 5
+    rest = torch.ones(12, dtype=torch.bool)
+    for a, b in refused:
+        assert blank(got[a:b], got_lse[a:b])
+        rest[a:b] = False
+    rest = rest.cuda()
+    assert torch.equal(got[rest], out[rest]) and torch.equal(got_lse[rest], lse[rest])
