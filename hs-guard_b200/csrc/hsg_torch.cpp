@@ -237,7 +237,12 @@ PyObject* plan_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.mask = static_cast<uint32_t*>(mask.data_ptr());
     s.stream = stream_of(device);
     const c10::cuda::CUDAGuard guard(device);
-    done(hsg_plan_tree(&s));
+    if (s.rows == 0) {  // the library has nothing to do: every token is one of no request
+      positions.fill_(-1);
+      mask.zero_();
+    } else {
+      done(hsg_plan_tree(&s));
+    }
     return tuple_of(positions, mask);
   });
 }

@@ -65,7 +65,8 @@ def plan_tree(parents, cu, lens, max_tree, err=None):
 
     parents [tokens] int32: each token's parent as an index within its request (an earlier token) or -1; cu [rows + 1]
     and lens [rows] int32. A token's position is its request's length plus its depth; bit j of its mask is set iff j is
-    the token itself or one of its ancestors."""
+    the token itself or one of its ancestors. Tokens outside cu[0] .. cu[rows] - 1, and those of a request whose offsets are
+    out of range or which has more tokens than its masks have bits (recorded in ``err``), have position -1 and no bits."""
     return tensors().plan_tree(parents, cu, lens, max_tree, err)
 
 

@@ -258,7 +258,9 @@ int hsg_advance_tables(const hsg_tables_args* args);
 
 /* Drafted tokens cu[b] .. cu[b+1] - 1 belong to request b; parents [tokens] holds each one's parent as an index within
  * its request, an earlier token, or -1 (child of the last cached token). positions = lens[b] + depth; bit j of
- * mask [tokens][words] (32 bits a word) is set iff j is the token or one of its ancestors. */
+ * mask [tokens][words] (32 bits a word) is set iff j is the token or one of its ancestors. cu must not descend; tokens of no
+ * request (before cu[0], from cu[rows] on), and those of a request whose offsets are out of range or which has more than
+ * 32 * words tokens, have position -1 and no bits. */
 typedef struct hsg_tree_args {
   int64_t size;
   const int32_t* parents;

@@ -238,3 +238,32 @@ def test_tree_attention_refused_requests_see_nothing(D, lens, cu, max_tree, refu
         rest[a:b] = False
     rest = rest.cuda()
     assert torch.equal(got[rest], out[rest]) and torch.equal(got_lse[rest], lse[rest])
+
+
+@pytest.mark.parametrize("cu,max_tree,refused,code", [
+    ([3, 5, 9], 64, [], 0), ([0, 5, 9], 64, [], 0), ([3, 5, 40], 32, [(5, 40)], 5), ([-1, 5, 9], 64, [(0, 5)], 5),
+    ([0, 40, 90], 64, [(40, 60)], 5)])
+def test_plan_tree_tokens_of_no_request(D, cu, max_tree, refused, code):
+    """They, and those of refused requests, have position -1 and no bits."""
+    tokens, words = 60, (max_tree + 31) // 32
+    parents = dev([-1] * tokens)
+    torch.full((tokens,), 77, dtype=torch.int32, device="cuda"), torch.full((tokens, words), 77, dtype=torch.int32, device="cuda")
+    err = err_word()
+    positions, mask = D.plan_tree(parents, dev(cu), dev([10, 20]), max_tree, err)
+    assert int(err.item()) == code
+    want = torch.full((tokens,), -1, dtype=torch.int32)
+    bits = torch.zeros(tokens, words, dtype=torch.int64)
+    for b in range(2):
+        for t in range(max(cu[b], 0), min(cu[b + 1], tokens)):
+            if not any(x <= t < y for x, y in refused):
+                want[t] = (10, 20)[b]
+                bits[t, (t - cu[b]) // 32] = 1 << (t - cu[b]) % 32
+    bits = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).to(torch.int32)
+    assert torch.equal(positions.cpu(), want) and torch.equal(mask.cpu(), bits)
+
+
+def test_plan_tree_without_requests(D):
+    torch.full((6,), 77, dtype=torch.int32, device="cuda")
+    e = torch.empty(0, dtype=torch.int32, device="cuda")
+    positions, mask = D.plan_tree(dev([-1] * 6), dev([0]), e, 4)
+    assert positions.tolist() == [-1] * 6 and not bool(mask.any())
