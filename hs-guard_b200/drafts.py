@@ -166,7 +166,6 @@ class DraftCache:
         self.ring = torch.arange(pages, dtype=torch.int32, device=device)
         self.counters = torch.tensor([0, pages], dtype=torch.int64, device=device)
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        self.workspace = torch.empty(attention_workspace(dim), dtype=torch.uint8, device=device)
 
     def advance(self, delta, capacity):
         """``advance_tables`` by delta [rows]; the cache's lengths and counters become the new ones."""
@@ -179,9 +178,10 @@ class DraftCache:
         store_rows(k, v, self.k[layer], self.v[layer], slots, source, self.err)
 
     def attend(self, layer, q, k, v, cu, scale, max_tree, mask=None, positions=None, window=0):
-        """``tree_attention`` over a layer's pages: (out, lse)."""
+        """``tree_attention`` over a layer's pages: (out, lse). Each call has a workspace of its own, so calls on several
+        streams may overlap."""
         return tree_attention(q, k, v, self.k[layer], self.v[layer], self.table, self.lens, cu, scale, max_tree, mask,
-                              positions, window, self.workspace, self.err)
+                              positions, window, None, self.err)
 
     def raise_device_error(self):
         """Wait for the device and raise HsgError if a kernel met an index outside its range."""

@@ -267,3 +267,28 @@ def test_plan_tree_without_requests(D):
     e = torch.empty(0, dtype=torch.int32, device="cuda")
     positions, mask = D.plan_tree(dev([-1] * 6), dev([0]), e, 4)
     assert positions.tolist() == [-1] * 6 and not bool(mask.any())
+
+
+# ---- a cache used on several streams --------------------------------------------------------------------------------
+def test_cache_attends_on_two_streams_at_once(D):
+    """Items that are cut leave partial results in a workspace: calls that overlap must not share one."""
+    layers, rows, page, hq, hkv, dim, n = 2, 3, 16, 16, 4, 128, 5
+    cache = D.DraftCache(layers, rows, 3000, page, 16000, hkv, dim, BF16)
+    cache.advance(dev([15000, 9000, 12001]), 0)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for x in (cache.k, cache.v):
+        x.normal_(generator=g)
+    cu = dev([0, n, 2 * n, 3 * n])
+    new = [[torch.randn(3 * n, h, dim, generator=g, device="cuda").to(BF16) for h in (hq, hkv, hkv)] for _ in range(layers)]
+    want = [cache.attend(layer, *new[layer], cu, 0.09, n) for layer in range(layers)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(layers)]
+    got = []
+    for _ in range(40):
+        for layer, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append((layer, cache.attend(layer, *new[layer], cu, 0.09, n)))
+    torch.cuda.synchronize()
+    for layer, (out, lse) in got:
+        assert torch.equal(out, want[layer][0]) and torch.equal(lse, want[layer][1])
+    cache.err.zero_()  # advance listed none of its tokens
