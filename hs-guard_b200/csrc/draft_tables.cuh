@@ -280,26 +280,26 @@ struct DraftTreeArgs {
 
 constexpr int DTREE_THREADS = 128;
 
+// Nodes from .. to - 1, as far as they exist, as those of no request. Rare, so out of line.
+__device__ __noinline__ void dtree_blank(const DraftTreeArgs& a, int64_t from, int64_t to) {
+  for (int64_t t = max(from, (int64_t)0) + threadIdx.x; t < min(to, (int64_t)a.tokens); t += DTREE_THREADS) {
+    a.positions[t] = -1;
+    for (int w = 0; w < a.words; ++w) a.mask[t * a.words + w] = 0;
+  }
+}
+
 // One thread block a request, one thread a node: the node's chain of parents, which ends because every link goes to
 // an earlier node. The indexes along it fall, so a mask word is complete once the chain has passed below it. Nodes of no
-// request (before cu_0 and from cu_rows on, by all blocks) and of a request that is refused have position -1 and no bits.
-__global__ void __launch_bounds__(DTREE_THREADS) draft_tree_kernel(const DraftTreeArgs a) {
+// request (before cu_0 and from cu_rows on, by the first and the last block) and of a request that is refused have position -1 and no bits.
+__global__ void __launch_bounds__(DTREE_THREADS) draft_tree_kernel(const __grid_constant__ DraftTreeArgs a) {
   const int b = blockIdx.x;
-  const int64_t t0 = a.cu[b], t1 = a.cu[b + 1], lead = a.cu[0], trail = a.cu[a.rows];
-  auto blank = [&](int64_t from, int64_t to, int64_t me, int64_t count) {
-    for (int64_t t = from + me; t < to; t += count) {
-      a.positions[t] = -1;
-      for (int w = 0; w < a.words; ++w) a.mask[t * a.words + w] = 0;
-    }
-  };
-  if (lead > 0 || trail < a.tokens) {
-    const int64_t me = (int64_t)threadIdx.x * a.rows + b, all = (int64_t)DTREE_THREADS * a.rows;
-    blank(0, min(lead, (int64_t)a.tokens), me, all);
-    blank(max(trail, (int64_t)0), a.tokens, me, all);
-  }
-  if (t0 < 0 || t1 < t0 || t1 > a.tokens || t1 - t0 > 32 * a.words) {
+  const int64_t t0 = a.cu[b], t1 = a.cu[b + 1];
+  const bool refused = t0 < 0 || t1 < t0 || t1 > a.tokens || t1 - t0 > 32 * a.words;
+  if (b == 0 && t0 > 0) dtree_blank(a, 0, t0);
+  if (b == a.rows - 1 && t1 < a.tokens) dtree_blank(a, t1, a.tokens);
+  if (refused) {
     if (threadIdx.x == 0) set_error(a.err, ERR_BAD_LEN);
-    blank(max(t0, (int64_t)0), min(t1, (int64_t)a.tokens), threadIdx.x, DTREE_THREADS);
+    dtree_blank(a, t0, t1);
     return;
   }
   for (int i = threadIdx.x; i < t1 - t0; i += DTREE_THREADS) {
