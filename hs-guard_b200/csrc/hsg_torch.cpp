@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -47,7 +48,17 @@ const char* name_of(at::ScalarType t) { return c10::toString(t); }
 
 const Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse("%s must be a tensor", name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  // outputs are made below autograd: a gradient would be lost in silence
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse("%s requires a gradient and there is no backward pass: call under torch.no_grad()", name);
+  return t;
+}
+
+// What a call changes in place, for those who compare version counters.
+void changed(PyObject* o) {
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // A tensor on the calls' device, of these dimensions and this type, its last dimension contiguous.
@@ -214,6 +225,8 @@ PyObject* advance_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.stream = stream_of(device);
     const c10::cuda::CUDAGuard guard(device);
     done(hsg_advance_tables(&s));
+    changed(a[2]);
+    changed(a[3]);
     return tuple_of(out.narrow(0, 0, rows), counters, out.narrow(0, rows, rows + 1), out.narrow(0, lists, s.capacity),
                     out.narrow(0, lists + room, s.capacity), out.narrow(0, lists + 2 * room, s.capacity));
   });
@@ -317,6 +330,8 @@ PyObject* norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.err = error_word(a[11], device);
     const c10::cuda::CUDAGuard guard(device);
     done(hsg_norm_rope(&s));
+    changed(a[8]);
+    changed(a[9]);
     return THPVariable_Wrap(q_out);
   });
 }
@@ -416,6 +431,8 @@ PyObject* store_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.stream = stream_of(device);
     const c10::cuda::CUDAGuard guard(device);
     done(hsg_store_rows(&s));
+    changed(a[2]);
+    changed(a[3]);
     Py_RETURN_NONE;
   });
 }

@@ -16,7 +16,8 @@ and once a branch is accepted:
 engine's 512-token rings as such a cache. Every function queues
 work on torch's current stream of its tensors' device and waits for nothing; outputs are new tensors unless they are
 said to change in place. Arguments of a wrong shape, type, device or alignment raise ``ValueError`` before anything
-is queued. Values on the device are checked by the kernels, which skip an index outside its range and record the
+is queued, and so do tensors that require gradients outside ``torch.no_grad()``: there are no backward passes. Values on
+the device are checked by the kernels, which skip an index outside its range and record the
 reason in ``err`` (an int32 tensor of one element, 0 at first; see ``raise_device_error``).
 
 Arguments are checked and outputs allocated by the extension module _hsg_torch (csrc/hsg_torch.cpp), which calls

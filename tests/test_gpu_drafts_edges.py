@@ -292,3 +292,49 @@ def test_cache_attends_on_two_streams_at_once(D):
     for layer, (out, lse) in got:
         assert torch.equal(out, want[layer][0]) and torch.equal(lse, want[layer][1])
     cache.err.zero_()  # advance listed none of its tokens
+
+
+# ---- autograd -------------------------------------------------------------------------------------------------------
+def test_inputs_that_want_gradients_are_refused(D):
+    """There are no backward passes: such a call must not lose a gradient in silence."""
+    c = Case([40], [3], 8, 2, 128, 16, F16, seed=1)
+    w, inv = torch.ones(128, device="cuda"), torch.ones(32, device="cuda")
+    learned = torch.nn.Parameter(torch.ones(128, device="cuda"))
+
+    def norm(weight):
+        return D.norm_rope(c.q, c.k, c.v, weight, w, inv, c.positions, 1e-6, F16)
+
+    want = norm(w)
+    with pytest.raises(ValueError, match="gradient"):
+        norm(learned)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(norm(learned), want))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(norm(learned), want))
+    plain = c.call(D)
+    c.q = c.q.detach().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        c.call(D)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(c.call(D), plain))
+    with pytest.raises(ValueError, match="gradient"):
+        D.store_rows(c.k.detach().requires_grad_(), c.v, c.kc, c.vc, dev([0, 1, 2]))
+
+
+def test_what_changes_in_place_says_so(D):
+    """autograd, and others that compare version counters, see the change."""
+    c = Case([40], [3], 8, 2, 128, 16, F16, seed=1)
+    before = c.kc._version, c.vc._version
+    D.store_rows(c.k, c.v, c.kc, c.vc, dev([0, 1, 2]))
+    assert c.kc._version > before[0] and c.vc._version > before[1]
+    w, inv, before = torch.ones(128, device="cuda"), torch.ones(32, device="cuda"), (c.kc._version, c.vc._version)
+    D.norm_rope_store(c.q, c.k, c.v, w, w, inv, c.positions, 1e-6, c.kc, c.vc, dev([0, 1, 2]))
+    assert c.kc._version > before[0] and c.vc._version > before[1]
+    table, ring = dev([[0, -1]]), dev([1, 2])
+    before = table._version, ring._version
+    D.advance_tables(dev([16]), dev([1]), table, ring, dev([0, 2], torch.int64), 16, 1)
+    assert table._version > before[0] and ring._version > before[1]
+    with torch.inference_mode():
+        cache = torch.zeros(2, 16, 2, 128, device="cuda", dtype=F16)
+    D.store_rows(c.k, c.v, cache, cache.clone(), dev([0, 1, 2]))  # without a version counter
+    assert torch.equal(cache[0, :3], c.k)
