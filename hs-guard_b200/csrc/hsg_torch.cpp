@@ -87,11 +87,15 @@ at::Device device_of(const Tensor& t, const char* name) {
   return t.device();
 }
 
+// A Python integer, or what converts to one without loss as numpy's do. Not a tensor, whose conversion would wait for the GPU.
 int32_t whole(PyObject* o, const char* name, int64_t lo, int64_t hi) {
+  PyObject* index = PyLong_Check(o) ? (Py_INCREF(o), o) : THPVariable_Check(o) ? nullptr : PyNumber_Index(o);
   int overflow = 0;
-  const long long v = PyLong_Check(o) ? PyLong_AsLongLongAndOverflow(o, &overflow) : 0;
-  if (!PyLong_Check(o) || overflow || v < lo || v > hi)
-    refuse("%s must be an integer in [%lld, %lld]", name, (long long)lo, (long long)hi);
+  const long long v = index ? PyLong_AsLongLongAndOverflow(index, &overflow) : 0;
+  const bool good = index && !overflow && v >= lo && v <= hi;
+  Py_XDECREF(index);
+  PyErr_Clear();
+  if (!good) refuse("%s must be an integer in [%lld, %lld]", name, (long long)lo, (long long)hi);
   return (int32_t)v;
 }
 

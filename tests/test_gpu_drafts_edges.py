@@ -4,6 +4,7 @@ room, page ids outside their range, caches used on several streams, gradients, a
 Tolerances are those of test_gpu_drafts.py unless a test says otherwise; all were derived before the first run."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -338,3 +339,14 @@ def test_what_changes_in_place_says_so(D):
         cache = torch.zeros(2, 16, 2, 128, device="cuda", dtype=F16)
     D.store_rows(c.k, c.v, cache, cache.clone(), dev([0, 1, 2]))  # without a version counter
     assert torch.equal(cache[0, :3], c.k)
+
+
+# ---- arguments and storage ------------------------------------------------------------------------------------------
+def test_numpy_integers_are_integers(D):
+    parents, cu, lens = dev([-1, 0]), dev([0, 2]), dev([5])
+    for kind in (np.int32, np.int64, np.uint8):
+        positions, _ = D.plan_tree(parents, cu, lens, kind(2))
+        assert positions.tolist() == [5, 6]
+    for wrong in (np.float32(2), torch.tensor(2), torch.tensor(2, device="cuda"), 2.0, "2", None, np.int64(0), np.int64(1 << 40)):
+        with pytest.raises(ValueError):
+            D.plan_tree(parents, cu, lens, wrong)
