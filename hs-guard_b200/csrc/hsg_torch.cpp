@@ -140,6 +140,16 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, at::Device device) {
   return at::empty(sizes, at::TensorOptions().dtype(dtype).device(device));
 }
 
+// n elements of `base`'s storage from the offset-th on (both counted in elements of this type) as a vector: a view operator
+// costs several times as much.
+Tensor part(const Tensor& base, at::ScalarType dtype, int64_t offset, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(),
+                                                      c10::scalarTypeToTypeMeta(dtype));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 void* stream_of(at::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
 
 struct LibraryError {
@@ -216,23 +226,25 @@ PyObject* advance_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.capacity = whole(a[6], "capacity", 0, INT32_MAX - 3);
     s.err = error_word(a[7], device);
     s.rows = (int32_t)rows;
-    // one allocation for the int32 outputs; the three lists each begin on a 16-byte boundary
-    const int64_t lists = (2 * rows + 1 + 3) / 4 * 4, room = ((int64_t)s.capacity + 3) / 4 * 4;
-    const Tensor out = empty({lists + 3 * room}, at::kInt, device), counters = empty({2}, at::kLong, device);
-    int32_t* base = static_cast<int32_t*>(out.data_ptr());
-    s.lens_out = base;
-    s.cu = base + rows;
-    s.slots = base + lists;
+    // one allocation for what a caller keeps until the next call (counters, lengths, offsets) and one for the three lists,
+    // each of which begins on a 16-byte boundary
+    const int64_t room = ((int64_t)s.capacity + 3) / 4 * 4;
+    const Tensor kept = empty({4 + 2 * rows + 1}, at::kInt, device), lists = empty({3 * room}, at::kInt, device);
+    int32_t* base = static_cast<int32_t*>(kept.data_ptr());
+    s.counters_out = reinterpret_cast<int64_t*>(base);
+    s.lens_out = base + 4;
+    s.cu = s.lens_out + rows;
+    s.slots = static_cast<int32_t*>(lists.data_ptr());
     s.token_rows = s.slots + room;
     s.positions = s.token_rows + room;
-    s.counters_out = static_cast<int64_t*>(counters.data_ptr());
     s.stream = stream_of(device);
     const c10::cuda::CUDAGuard guard(device);
     done(hsg_advance_tables(&s));
     changed(a[2]);
     changed(a[3]);
-    return tuple_of(out.narrow(0, 0, rows), counters, out.narrow(0, rows, rows + 1), out.narrow(0, lists, s.capacity),
-                    out.narrow(0, lists + room, s.capacity), out.narrow(0, lists + 2 * room, s.capacity));
+    return tuple_of(part(kept, at::kInt, 4, rows), part(kept, at::kLong, 0, 2), part(kept, at::kInt, 4 + rows, rows + 1),
+                    part(lists, at::kInt, 0, s.capacity), part(lists, at::kInt, room, s.capacity),
+                    part(lists, at::kInt, 2 * room, s.capacity));
   });
 }
 

@@ -350,3 +350,14 @@ def test_numpy_integers_are_integers(D):
     for wrong in (np.float32(2), torch.tensor(2), torch.tensor(2, device="cuda"), 2.0, "2", None, np.int64(0), np.int64(1 << 40)):
         with pytest.raises(ValueError):
             D.plan_tree(parents, cu, lens, wrong)
+
+
+def test_lengths_do_not_keep_the_lists(D):
+    """What a cache keeps from call to call (lengths, counters) shares no memory with the lists of a call's tokens."""
+    t = D.advance_tables(dev([0, 3]), dev([1000, 2]), dev([[-1] * 70, [0] + [-1] * 69]), dev(list(range(1, 101))),
+                         dev([0, 100], torch.int64), 16, 100000)
+    assert t.lens.tolist() == [1000, 5] and t.counters.tolist() == [63, 100] and t.cu.tolist() == [0, 1000, 1002]
+    assert t.slots.shape == t.rows.shape == t.positions.shape == (100000,)
+    for kept in (t.lens, t.counters, t.cu):
+        assert kept.untyped_storage().nbytes() < 4096
+    assert t.counters.dtype == torch.int64 and t.lens.is_contiguous() and t.cu.is_contiguous()
