@@ -159,7 +159,11 @@ class DraftCache:
             raise ValueError("page_size must be a multiple of 8, dim 64, 128 or 256")
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("the cache must be fp16 or bf16")
-        device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError("the cache lives on a CUDA device, got %s" % device)
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         pool = torch.zeros(2, layers, pages, page_size, kv_heads, dim, dtype=dtype, device=device)
         self.k, self.v, self.page_size = pool[0], pool[1], page_size
         self.table = torch.full((rows, (max_len + page_size - 1) // page_size), -1, dtype=torch.int32, device=device)

@@ -361,3 +361,13 @@ def test_lengths_do_not_keep_the_lists(D):
     for kept in (t.lens, t.counters, t.cu):
         assert kept.untyped_storage().nbytes() < 4096
     assert t.counters.dtype == torch.int64 and t.lens.is_contiguous() and t.cu.is_contiguous()
+
+
+@pytest.mark.parametrize("device", [None, 0, "cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0)])
+def test_cache_devices(D, device):
+    cache = D.DraftCache(1, 2, 4, 8, 16, 1, 64, device=device)
+    assert {x.device for x in (cache.k, cache.table, cache.lens, cache.counters, cache.err)} == {torch.device("cuda", 0)}
+    cache.advance(dev([3, 9]), 12)
+    assert cache.lens.tolist() == [3, 9]
+    with pytest.raises(ValueError):
+        D.DraftCache(1, 2, 4, 8, 16, 1, 64, device="cpu")
