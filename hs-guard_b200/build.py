@@ -27,6 +27,7 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std
 HOST_SRC = os.path.join(HERE, "csrc", "hsg_host.c")
 TORCH_SRC = os.path.join(HERE, "csrc", "hsg_torch.cpp")
 TORCH_LIB = os.path.join(HERE, "_hsg_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
+TORCH_STAMP = os.path.join(HERE, "_build", "_hsg_torch.torch")  # the torch that it was built against
 HOST_LIB = os.path.join(HERE, "_hsg_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
@@ -86,11 +87,27 @@ def host():
     return _HOST
 
 
-def build_torch(force=False):
-    """Compile the _hsg_torch extension module when it is missing or older than its sources. It finds libhsg.so beside
-    itself and torch's libraries where they are now."""
+def torch_stamp():
+    """What an _hsg_torch is bound to besides its sources: the installed torch and where it lies."""
+    import torch
+    return "%s %s\n" % (torch.__version__, os.path.dirname(torch.__file__))
+
+
+def torch_stale():
     sources = (TORCH_SRC, os.path.join(ROOT, "include", "hsg.h"))
-    if not force and os.path.exists(TORCH_LIB) and all(os.path.getmtime(TORCH_LIB) >= os.path.getmtime(f) for f in sources):
+    if not os.path.exists(TORCH_LIB) or any(os.path.getmtime(TORCH_LIB) < os.path.getmtime(f) for f in sources):
+        return True
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read() != torch_stamp()
+    except OSError:
+        return True
+
+
+def build_torch(force=False):
+    """Compile the _hsg_torch extension module when it is missing, older than its sources or built against another torch. It
+    finds libhsg.so beside itself and torch's libraries where they are now."""
+    if not force and not torch_stale():
         return TORCH_LIB
     build()
     import torch
@@ -110,6 +127,11 @@ def build_torch(force=False):
     if res.returncode != 0:
         raise RuntimeError("building _hsg_torch failed:\n" + res.stdout + res.stderr)
     os.replace(tmp, TORCH_LIB)
+    os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
+    stamp = "%s.%d.tmp" % (TORCH_STAMP, os.getpid())
+    with open(stamp, "w") as f:
+        f.write(torch_stamp())
+    os.replace(stamp, TORCH_STAMP)
     return TORCH_LIB
 
 
