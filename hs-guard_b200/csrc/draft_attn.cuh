@@ -115,6 +115,19 @@ __host__ __device__ inline int da_smem_bytes(const DaPlan& p, int dim) {
   return p.q_bufs * p.q_rows * dim * 2 + (p.k_bufs + p.v_bufs) * da_buffer_bytes(dim) + 1024 + da_extra(dim, p.block);
 }
 
+// Whose mask words, of an item's block of tokens, a row reads: its own token's, or the last one's if it has none (it then
+// counts for nothing, but reads like the others of its warp).
+__host__ __device__ constexpr int da_row_token(int row, int group, int block) {
+  return row / group < block ? row / group : block - 1;
+}
+constexpr bool da_row_tokens_fit() {
+  for (int group = 1; group <= DA_ROWS; ++group)
+    for (int row = 0; row < DA_ROWS; ++row)
+      if (da_row_token(row, group, DA_ROWS / group) >= DA_ROWS / group || da_row_token(row, group, 1) > 0) return false;
+  return true;
+}
+static_assert(da_row_tokens_fit(), "rows read mask words of their block's tokens only");
+
 // Workspace: per piece two partial results (its first and its last item) of 128 rows, O [128][dim], then (m, l) [128],
 // and the item that begins in it and ends in a later piece.
 struct DaSplit {
@@ -773,7 +786,7 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // keys of this row are those at positions above `low`; no row's bound is above it.lows
         int low = it.lo - 1;
         if (a.window && valid) low = max(low, row_pos[(item & 1) * plan.block + row_tok] - a.window);
-        const uint32_t* first_words = row_words + ((item & 1) * plan.block + row_tok) * (KT / 32);
+        const uint32_t* first_words = row_words + ((item & 1) * plan.block + da_row_token(row, G, plan.block)) * (KT / 32);
         float m = -INFINITY, l = 0.f;  // maximum of the last tile that this group took part in, sum of its own weights
         for (int i = i0 + ((g0 ^ group) & 1); i < i1; i += 2) {
           const int g = g0 + i - i0;
