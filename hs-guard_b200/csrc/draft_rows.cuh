@@ -86,7 +86,7 @@ constexpr int DN_LIVE = 4;  // tokens a lane has under way
 // took 110 us (instructions), blocks of 256 threads 81 us at 8 tokens and 86 us at 16 (a last wave partly empty).
 template <int D, typename TI, typename TO>
 __global__ void __launch_bounds__(DN_THREADS) draft_norm_kernel(const __grid_constant__ DraftNormArgs a, int per) {
-  extern __shared__ float2 s_turn[];  // [per][rot / 2] (cos, sin)
+  extern __shared__ __align__(16) float2 s_turn[];  // [per][rot / 2] (cos, sin), read two at a time
   constexpr int LPH = D / 8, HPW = 32 / LPH, WARPS = DN_THREADS / 32;
   const int t0 = blockIdx.x * per, tokens = min(per, a.tokens - t0), half = a.rot / 2;
   const int heads = a.hq + 2 * a.hkv, groups = (heads + HPW - 1) / HPW;

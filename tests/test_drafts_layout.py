@@ -36,3 +36,10 @@ def test_rows_read_mask_words_of_their_items_tokens(index, KT):
                     assert item * block * words <= first and first + words <= (item + 1) * block * words, (G, block, item, row)
                     if row < block * G:
                         assert first == (item * block + row // G) * words
+
+
+def test_rotations_are_read_from_where_two_fit():
+    """draft_norm_kernel reads its (cos, sin) pairs two at a time, 16 bytes: more than float2 is aligned to by itself."""
+    text = open(os.path.join(os.path.dirname(SOURCE), "draft_rows.cuh")).read()
+    assert "reinterpret_cast<const float4*>(s_turn + " in text
+    assert re.search(r"extern __shared__ __align__\(16\) float2 s_turn\[\];", text)
