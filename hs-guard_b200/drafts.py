@@ -120,11 +120,10 @@ def ring_cache(engine, layer, slots):
     table, lens) for requests ``slots``, to be used with window <= 512 and positions from the slots' lengths on.
 
     Nothing is copied: the rings [slots + 1, kv heads, 513, dim] are seen as pages of 64 columns that may begin at any
-    row, and logical page j of a slot is columns 64 (j mod 8) on. The engine writes its rings on its own stream: drafted
-    tokens may be attended between its ticks, and the next tick must not begin before the calls that read the rings have
-    ended."""
-    cfg = engine.cfg
-    pools = engine.pools()
+    row, and logical page j of a slot is columns 64 (j mod 8) on. The engine writes its rings on its own stream, and its
+    calls return when they have ended: drafted tokens may be attended between its ticks. ``ring_done`` after the last call
+    that reads the rings makes the next tick wait for it."""
+    cfg, pools = engine.cfg, engine.pools()
     ring_k, ring_v = pools["ring_k"], pools["ring_v"]
     if not 0 <= layer < ring_k.shape[0]:
         raise ValueError(f"layer must be in [0, {ring_k.shape[0]})")
@@ -142,6 +141,13 @@ def ring_cache(engine, layer, slots):
     logical = torch.arange(width, device=device) % (cfg.window // page) * page
     table = torch.as_tensor(slots, device=device)[:, None] * (heads * cols) + logical
     return views[0], views[1], table.to(torch.int32), lens
+
+
+def ring_done(engine):
+    """Order the engine's next tick, reset or restore behind what torch's current stream holds by now (calls over its
+    ``ring_cache``). Nothing waits on the host; calls on other streams need a call of their own."""
+    stream = engine._lib.hsg_stream(engine.handle)
+    torch.cuda.ExternalStream(stream, engine.device).wait_stream(torch.cuda.current_stream(engine.device))
 
 
 class DraftCache:

@@ -371,3 +371,33 @@ def test_cache_devices(D, device):
     assert cache.lens.tolist() == [3, 9]
     with pytest.raises(ValueError):
         D.DraftCache(1, 2, 4, 8, 16, 1, 64, device="cpu")
+
+
+def test_the_next_tick_waits_for_reads_of_the_rings(weights_seed0):
+    """Attention that is still queued when the engine's next tick is called reads the rings as they were."""
+    from hs_guard_b200 import drafts
+    from hs_guard_b200.engine import SlotEngine
+    eng = SlotEngine(weights_seed0, 2)
+    rng = np.random.default_rng(9)
+    eng.step([(s, rng.integers(0, 1000, 600).tolist()) for s in range(2)])
+    k_cache, v_cache, table, lens = drafts.ring_cache(eng, 4, [0, 1])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(6, h, 256, generator=g, device="cuda").half() for h in (8, 2, 2))
+    cu = torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")
+
+    def attend():
+        return drafts.tree_attention(q, k, v, k_cache, v_cache, table, lens, cu, 1.0 / 16, 3, window=512)
+
+    want, want_lse = attend()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second: the tick would be through long before
+        out, lse = attend()
+        drafts.ring_done(eng)
+    eng.step([(s, rng.integers(0, 1000, 64).tolist()) for s in range(2)])
+    assert side.query()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert not torch.equal(attend()[0], want)  # the rings have moved on
+    torch.cuda.synchronize()
+    eng.close()
