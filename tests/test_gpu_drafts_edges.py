@@ -401,3 +401,44 @@ def test_the_next_tick_waits_for_reads_of_the_rings(weights_seed0):
     assert not torch.equal(attend()[0], want)  # the rings have moved on
     torch.cuda.synchronize()
     eng.close()
+
+
+# ---- the widest shapes ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lens,counts,hq,hkv,dim,page,dtype,window", [
+    ([300, 31], [3, 2], 128, 1, 64, 16, F16, 0), ([129], [5], 128, 1, 128, 16, BF16, 0), ([70, 600], [2, 3], 256, 2, 256, 16, F16, 200),
+    ([200, 9], [4, 7], 100, 1, 64, 8, BF16, 0), ([1000], [3], 65, 1, 128, 32, F16, 0), ([257, 40], [9, 4], 66, 2, 64, 16, F16, 30),
+    ([500], [11], 24, 1, 256, 48, BF16, 0), ([50, 0, 700], [1, 6, 2], 33, 3, 128, 16, F16, 0)])
+def test_tree_attention_many_query_heads_a_key_head(D, lens, counts, hq, hkv, dim, page, dtype, window):
+    """Groups of 11 to 128 query heads, most of which leave rows of a block without a token."""
+    Case(lens, counts, hq, hkv, dim, page, dtype, window, seed=hq).check(D)
+
+
+@pytest.mark.parametrize("mask,window", [("tree", 0), ("holes", 0), (None, 0), ("tree", 300), (None, 300)])
+def test_tree_attention_largest_trees(D, mask, window):
+    """1,024 drafted tokens: all 32 mask words, drafts of many tiles, and windows that end among them."""
+    Case([90, 700], [1024, 1000], 2, 1, 64, 16, F16, window, mask=mask, seed=5).check(D)
+
+
+@pytest.mark.parametrize("tokens", [1, 37])
+def test_norm_rope_is_the_models(D, tokens):
+    """The classifier's own norm and rotation (32-bit, written for the oracle) of its fused projection, at positions where a
+    32-bit angle is exact enough: 4,000 x 2^-24 x |y| below an fp16 result's rounding."""
+    from hs_guard_b200 import DEFAULT as cfg
+    from oracle import stream
+    g = torch.Generator().manual_seed(tokens)
+    hq, hkv, dim, rot = cfg.attn_heads, cfg.kv_heads, cfg.attn_head_dim, cfg.rotary_dim
+    proj = torch.randn(tokens, (2 * hq + 2 * hkv) * dim, generator=g)
+    q = proj[:, :2 * hq * dim].view(tokens, hq, 2 * dim)[..., :dim]
+    k = proj[:, 2 * hq * dim:(2 * hq + hkv) * dim].view(tokens, hkv, dim)
+    v = proj[:, (2 * hq + hkv) * dim:].view(tokens, hkv, dim)
+    wq, wk = (1 + 0.2 * torch.randn(dim, generator=g) for _ in range(2))
+    inv = 1.0 / cfg.rope_theta ** (torch.arange(0, rot, 2, dtype=torch.int64).float() / rot)
+    pos = torch.randint(0, 4000, (tokens,), generator=g)
+    angle = torch.cat([pos[:, None].float() * inv] * 2, -1)
+    cos, sin = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    gq, gk, gv = D.norm_rope(*(x.cuda() for x in (q, k, v, wq, wk, inv)), dev(pos), cfg.rms_eps, F16)
+    for got, x, w in ((gq, q, wq), (gk, k, wk)):
+        ref = stream.rope(stream.rms_norm(x, w, cfg.rms_eps), cos, sin, rot)
+        tol = U[F16] * ref.abs() + (1e-5 + 4000 * 2.0 ** -24) * ref.abs().amax(-1, keepdim=True) + TINY[F16]
+        assert bool(((got.cpu() - ref).abs() <= tol).all())
+    assert torch.equal(gv.cpu(), v.half())
