@@ -533,14 +533,20 @@ draft_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     total.items += s_scan[2 * w];
     total.tiles += s_scan[2 * w + 1];
   }
-  // where pieces have few tiles, latency counts and not the balance: an item is then as long as its tiles
+  // An item counts DA_ITEM_COST tiles more than it has, but not where a piece has hardly more tiles than that. Without and
+  // with it, at about 4, 8, 12 and 24 tiles a piece: head dim 256, window 512, 21.7 and 19.8 us, 29.2 and 27.2, 35.0 and
+  // 31.8, 49.9 and 47.4; head dim 128, caches of 200, 26.1 and 22.9, 32.7 and 29.5, 43.8 and 38.2, 76.2 and 67.5; of 5,000,
+  // 22.8 and 19.3, 28.1 and 23.3, 33.0 and 26.4, 45.8 and 42.5; head dim 64, caches of 600, 20.7 and 18.9, 31.9 and 27.0,
+  // 39.6 and 33.5, 64.5 and 55.2.
   const int64_t mean = (total.tiles + DA_PIECES - 1) / DA_PIECES;
-  const int cost = mean >= 4 * DA_ITEM_COST ? DA_ITEM_COST : 0;
+  const int cost = mean > DA_ITEM_COST ? DA_ITEM_COST : 0;
   // An item of n tiles cut into pieces of s costs about 2 us for each of a piece's tiles and 0.37 us for each of the n / s
   // parts that its join reads: s + 1 tiles a piece pay from n = 5 s (s + 1) on. That bounds the pieces from below where
   // items are few and long. One request, one key head of 16 rows, head dim 128, without this and with it: 9,000 keys 31.6
   // and 20.8 us, 17,000 keys 48.9 and 24.0, 40,000 keys 52.7 and 31.7; four key heads: 4,400 keys 20.9 and 17.5, 1,000 keys
-  // (one tile a piece either way) 15.7 and 15.6. A fixed two tiles a piece: two tiles an item 13.9 to 15.5.
+  // (one tile a piece either way) 15.7 and 15.6; head dim 64, four key heads, 2,500 keys 16.2 and 15.4; head dim 256, two key
+  // heads, 2,200 keys 28.1 and 21.3. A fixed two tiles a piece: two tiles an item 13.9 to 15.5. The mean over all items
+  // decides, so a long one among many short ones is cut like those.
   const float item_tiles = (float)total.tiles / (float)max((int64_t)1, total.items);
   const int64_t least = max(1, (int)(sqrtf(0.2f * item_tiles + 0.25f) + 0.5f));
   const int64_t units = total.tiles + cost * total.items, step = max(least, (units + DA_PIECES - 1) / DA_PIECES);
