@@ -67,11 +67,13 @@ struct DraftAttnArgs {
 //    or two warps a scheduler wait for latency, not for the special-function unit.
 //  - an L2 policy that keeps a share of the keys for a request's next block of rows changed neither time nor HBM bytes.
 //
-// Measured on B200, short loops (sustained ones are 10 to 15% slower, the clock falls): five requests of up to 50,001 cached
-// tokens, 13 drafts, 32 / 8 heads of 128: 488 MB in 85 us, 5.7 TB/s, bound by HBM. 352 requests, 512-token window, up to 9
-// drafts, 8 / 2 heads of 256: 393 MB in 80 us, 4.9 TB/s: ten tiles an item, so items' set-up and epilogues and masked tiles
-// count. 40 requests of up to 6,000 tokens, 64 drafts, 32 / 4 heads of 128: four blocks of rows read a head's keys, of which
-// 1.06 GB come from HBM and 2.3 GB through L2 in 190 us. One token: 10 us of latencies and 3 for the join.
+// Measured on B200, means of three sets of inputs in short loops (in sustained ones the clock falls: 2 to 16% longer, by size
+// and GPU): four requests of up to 50,001 cached tokens, 13 drafts, 32 / 8 heads of 128: 534 MB in 99 us, 5.4 TB/s, bound by
+// HBM. 352 requests, 512-token window, up to 9 drafts, 8 / 2 heads of 256: 384 MB in 85 us, 4.5 TB/s: ten tiles an item, so
+// items' set-up and epilogues and masked tiles count. 40 requests of up to 6,000 tokens, 64 drafts, 32 / 4 heads of 128: 210 us;
+// four blocks of rows read a head's keys, and of 362 MB that one set has, 1.06 GB come from HBM and 2.3 GB through L2. One
+// token: 11 us of latencies and 3 for the join. 352 requests of up to 100 cached tokens, one draft, 8 / 8 heads of 64 or 128:
+// 113 and 117 us for 51 and 101 MB: 2,816 items of two tiles, one after the other in each thread block.
 //
 // The weights are rounded to V's type for the second product (tcgen05 takes both factors of one 16-bit type; a second
 // product with what the rounding left would double that product): relative 2^-11 or 2^-8 each, as the result itself is. For

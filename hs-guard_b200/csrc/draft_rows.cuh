@@ -82,7 +82,7 @@ constexpr int DN_LIVE = 4;  // tokens a lane has under way
 // rotation's partner (d and d + rot / 2) is rot / 16 lanes away. A block takes `per` tokens: their angles once into
 // shared memory, then units of (a warp's heads, DN_LIVE tokens) spread over its warps, so that what depends on the head
 // (kind, addresses, weights) is found once for DN_LIVE tokens. Measured at 22,528 tokens of 12 fp32 heads of 256 (415 MB):
-// 73 us, 5.7 TB/s, bound by HBM; units of one head and token, whose index is divided by the head count at every step,
+// 74 us, 5.6 TB/s, bound by HBM; units of one head and token, whose index is divided by the head count at every step,
 // took 110 us (instructions), blocks of 256 threads 81 us at 8 tokens and 86 us at 16 (a last wave partly empty).
 template <int D, typename TI, typename TO>
 __global__ void __launch_bounds__(DN_THREADS) draft_norm_kernel(const __grid_constant__ DraftNormArgs a, int per) {

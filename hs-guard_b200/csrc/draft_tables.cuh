@@ -13,8 +13,8 @@
 //
 // Every block sums over all requests by itself (two block scans: cheaper than a second launch or a wait between blocks)
 // and then takes its share of the pages and tokens, found by bisection in the prefix sums. Bound by launch and latency up
-// to some 100,000 tokens, by the 12 bytes written a token beyond: 5.5 us for 352 requests that accept or withdraw a few
-// tokens, 12.6 us for 870,000 tokens of 1,000 prompts (10 MB, 0.8 TB/s). Blocks of 1,024 threads took 10.6 us for the first: their warps
+// to some 100,000 tokens, by the 12 bytes written a token beyond: 5.9 us for 352 requests that accept or withdraw a few
+// tokens, 13.1 us for 870,000 tokens of 1,000 prompts (10 MB, 0.8 TB/s). Blocks of 1,024 threads took 10.6 us for the first: their warps
 // issue the same few scalar steps four times as often.
 #pragma once
 #include "common.cuh"

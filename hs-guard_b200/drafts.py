@@ -13,15 +13,17 @@ and once a branch is accepted:
     store_rows(k, v, k_cache, v_cache, t.slots, source)                            # every layer
 
 ``DraftCache`` holds the pages, tables and counters of several layers and calls the last two; ``ring_cache`` shows a live
-engine's 512-token rings as such a cache. Every function queues
-work on torch's current stream of its tensors' device and waits for nothing; outputs are new tensors unless they are
-said to change in place. Arguments of a wrong shape, type, device or alignment raise ``ValueError`` before anything
-is queued, and so do tensors that require gradients outside ``torch.no_grad()``: there are no backward passes. Values on
-the device are checked by the kernels, which skip an index outside its range and record the
-reason in ``err`` (an int32 tensor of one element, 0 at first; see ``raise_device_error``).
+engine's 512-token rings as such a cache. All of this is one softmax layer's part: the layer's projections come from the
+host's model, and what its attention gives goes back there. Every function queues work on torch's current stream of its
+tensors' device and waits for nothing; outputs are new tensors unless they are said to change in place. Arguments of a
+wrong shape, type, device or alignment raise ``ValueError`` before anything is queued, and so do tensors that require
+gradients outside ``torch.no_grad()``: there are no backward passes. Values on the device are checked by the kernels, which
+skip an index outside its range and record the reason in ``err`` (an int32 tensor of one element, 0 at first; see
+``raise_device_error``); without ``err`` nothing says that one was met.
 
 Arguments are checked and outputs allocated by the extension module _hsg_torch (csrc/hsg_torch.cpp), which calls
-hsg_plan_tree, hsg_norm_rope, hsg_tree_attention, hsg_advance_tables and hsg_store_rows of include/hsg.h. The reference has no counterpart: its ticks are chains and its caches 512-token rings.
+hsg_plan_tree, hsg_norm_rope, hsg_tree_attention, hsg_advance_tables and hsg_store_rows of include/hsg.h. The reference has
+no counterpart: its ticks are chains and its caches 512-token rings.
 """
 from __future__ import annotations
 
@@ -62,7 +64,7 @@ def advance_tables(lens, delta, table, ring, counters, page_size, capacity, err=
 
 
 def plan_tree(parents, cu, lens, max_tree, err=None):
-    """Positions [tokens] int32 and ancestor masks [tokens, words] int32 of drafted trees of at most max_tree tokens.
+    """Positions [tokens] int32 and ancestor masks [tokens, words] int32 of drafted trees; words hold max_tree bits.
 
     parents [tokens] int32: each token's parent as an index within its request (an earlier token) or -1; cu [rows + 1]
     and lens [rows] int32. A token's position is its request's length plus its depth; bit j of its mask is set iff j is
@@ -155,7 +157,8 @@ class DraftCache:
 
     ``k[layer]``, ``v[layer]`` [pages, page_size, kv_heads, dim]; ``table`` [rows, width], ``lens`` [rows], free-page
     ``ring`` [pages] and ``counters`` as ``advance_tables`` takes them: ``advance`` moves them on. Rows are the callers'
-    requests; a finished one gives its pages back with a delta of minus its length."""
+    requests; a finished one gives its pages back with a delta of minus its length. Calls that change the cache (advance,
+    store) and calls that read it are ordered by their stream; on several streams that order is the caller's."""
 
     def __init__(self, layers, rows, pages, page_size, max_len, kv_heads, dim, dtype=torch.float16, device=None):
         if min(layers, rows, pages, max_len, kv_heads) < 1 or rows > MAX_TABLE_ROWS:

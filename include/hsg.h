@@ -303,7 +303,8 @@ int hsg_norm_rope(const hsg_norm_rope_args* args);
 /* Drafted token t of request b, at position p_t, attends the cached tokens n < lens[b] with n > p_t - window (all of
  * them when window is 0) and the drafted tokens j of its request whose bit in mask[t] is set (mask NULL: j <= t) and,
  * with a window, p_j > p_t - window. out [tokens][hq][dim] = softmax(scale q.k) v in dtype (HSG_DT_F16 or _BF16, as q,
- * k, v and the cache), lse [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing gets 0 and -inf;
+ * k, v and the cache), lse [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing, or only scores of -inf,
+ * gets 0 and -inf;
  * what is not seen, beyond a length included, does not enter a result whatever its bits. positions are read only with
  * a window (NULL: lens[b] + index) and must be at least lens[b]. cu must not descend. Tokens of no request (before cu[0], from
  * cu[rows] on: a buffer of a fixed size may be longer than what is drafted) see nothing, and so do those of a request whose
