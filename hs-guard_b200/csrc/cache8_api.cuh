@@ -1,0 +1,160 @@
+// C entry points of the 8-bit cache and of token log-probabilities (hsg_append8, hsg_attention8, hsg_token_logprobs): argument
+// checks and launches. Part of the one translation unit of the library.
+#pragma once
+#include "cache8_attn.cuh"
+#include "draft_api.cuh"
+#include "logprobs.cuh"
+
+namespace {
+
+int check_cache8(const hsg_cache8& c, int heads, int dim) {
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale) return fail(HSG_ERR_INVALID, "the cache's k, v or scales are NULL");
+  if (c.pages < 1 || c.page_size < 8 || c.page_size % 8)
+    return fail(HSG_ERR_INVALID, "a cache has at least one page of a multiple of 8 tokens, got %d of %d", c.pages, c.page_size);
+  if (c.block < 8 || c.block % 8 || c.page_size % c.block)
+    return fail(HSG_ERR_INVALID, "blocks must be a multiple of 8 tokens that divides a page's %d, got %d", c.page_size, c.block);
+  if ((int64_t)c.pages * c.page_size > INT32_MAX)
+    return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit slots", c.pages, c.page_size);
+  if (!aligned16(c.k) || !aligned16(c.v) || c.page_stride % 16 || c.token_stride % 16 || c.head_stride % 16 ||
+      c.page_stride < 0 || c.token_stride < 0 || c.head_stride < 0)
+    return fail(HSG_ERR_INVALID, "cache rows must lie on 16-byte boundaries, at strides that are not negative");
+  if ((reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale)) & 3)
+    return fail(HSG_ERR_INVALID, "scales must lie on 4-byte boundaries");
+  if (c.pages > 1 && c.page_stride == 0) return fail(HSG_ERR_INVALID, "the cache's pages must differ");
+  if (c.token_stride < dim || (heads > 1 && c.head_stride < dim))
+    return fail(HSG_ERR_INVALID, "cache rows of %d bytes overlap (token stride %lld, head stride %lld)", dim,
+                (long long)c.token_stride, (long long)c.head_stride);
+  return HSG_OK;
+}
+
+Cache8 cache8(const hsg_cache8& c) {
+  return Cache8{static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_scale, c.v_scale, c.page_stride, c.token_stride,
+                c.head_stride, c.pages, c.page_size, c.block};
+}
+
+template <int D, typename T>
+int launch_append8(const Append8Args& p, cudaStream_t st) {
+  // entries a thread block: one where that leaves few blocks idle, else eight, of which most continue a run
+  const int per = p.count <= 16 * SM_COUNT ? 1 : 8;
+  const int smem = A8R_CHUNK * (p.rot / 2) * (int)sizeof(float2) + 2 * p.hkv * (int)sizeof(float);
+  if (smem > 48 * 1024) return fail(HSG_ERR_INVALID, "too many key heads (%d)", p.hkv);
+  append8_kernel<D, T><<<(p.count + per - 1) / per, A8R_THREADS, smem, st>>>(p, per);
+  CU(cudaGetLastError());
+  return HSG_OK;
+}
+template <typename T>
+int launch_append8_dim(const Append8Args& p, int dim, cudaStream_t st) {
+  return dim == 64 ? launch_append8<64, T>(p, st) : dim == 128 ? launch_append8<128, T>(p, st) : launch_append8<256, T>(p, st);
+}
+
+template <int D, typename T>
+int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
+  A8Split* splits = static_cast<A8Split*>(workspace);
+  float* partials = reinterpret_cast<float*>(splits + A8_PIECES);
+  CU(cudaFuncSetAttribute(attn8_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
+  CU(launch_k(attn8_kernel<D, T>, dim3(A8_PIECES), dim3(A8_THREADS), a8_smem(D), st, true, p, splits, partials));
+  CU(launch_k(attn8_join_kernel<D, T>, dim3(A8_PIECES, A8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
+              (const A8Split*)splits, (const float*)partials));
+  return HSG_OK;
+}
+template <typename T>
+int launch_attn8_dim(const Attn8Args& p, int dim, void* ws, cudaStream_t st) {
+  return dim == 64 ? launch_attn8<64, T>(p, ws, st) : dim == 128 ? launch_attn8<128, T>(p, ws, st) : launch_attn8<256, T>(p, ws, st);
+}
+
+template <typename T>
+int launch_logprobs(const LogprobsArgs& p, cudaStream_t st) {
+  // blocks a row: as many as it takes to give every SM two, up to a cluster's eight
+  int size = 1;
+  while (size < LP_CLUSTER && (int64_t)p.rows * size < 2 * SM_COUNT) size *= 2;
+  CU(launch_cluster(logprobs_kernel<T>, dim3((unsigned)(p.rows * size)), dim3(LP_THREADS), size, 0, st, false, p));
+  return HSG_OK;
+}
+
+}  // namespace
+
+extern "C" int hsg_append8(const hsg_append8_args* a) {
+  DRAFT_ARGS(a);
+  if (a->count < 0 || a->rows < 0 || a->hkv < 1 || a->hq < 0)
+    return fail(HSG_ERR_INVALID, "bad shape (count %d, rows %d, heads %d / %d)", a->count, a->rows, a->hq, a->hkv);
+  if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
+  if (a->rot < 0 || a->rot > a->dim || a->rot % 16)
+    return fail(HSG_ERR_INVALID, "the rotated dims must be a multiple of 16 up to head_dim, got %d", a->rot);
+  if (a->dtype != HSG_DT_F16 && a->dtype != HSG_DT_BF16) return fail(HSG_ERR_INVALID, "q, k and v must be fp16 or bf16");
+  if (!(fabsf(a->rope_scale) < INFINITY)) return fail(HSG_ERR_INVALID, "rope_scale must be finite");
+  if (a->count == 0) return HSG_OK;
+  if (!a->slots || (a->rows && (!a->k || !a->v)) || (a->hq && (!a->q || !a->q_out)) || (a->rot && (!a->positions || !a->inv_freq)))
+    return fail(HSG_ERR_INVALID, "NULL argument");
+  if (a->hq && a->source) return fail(HSG_ERR_INVALID, "q goes with entries in order: source must be NULL");
+  if (!aligned16(a->k) || !aligned16(a->v) || !rows16(a->k_token_stride, a->k_head_stride, 2) ||
+      !rows16(a->v_token_stride, a->v_head_stride, 2) ||
+      (a->hq && (!aligned16(a->q) || !aligned16(a->q_out) || !rows16(a->q_token_stride, a->q_head_stride, 2))))
+    return fail(HSG_ERR_INVALID, "q, k and v rows must lie on 16-byte boundaries");
+  int rc;
+  if ((rc = check_cache8(a->cache, a->hkv, a->dim)) != HSG_OK) return rc;
+  Append8Args p{a->q, a->k, a->v, a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride,
+                a->v_head_stride, a->source, a->slots, a->positions, a->inv_freq, a->count, a->rows, a->hq, a->hkv, a->rot,
+                a->interleaved != 0, a->rope_scale, a->q_out, cache8(a->cache), a->err};
+  cudaStream_t st = (cudaStream_t)a->stream;
+  return a->dtype == HSG_DT_F16 ? launch_append8_dim<__half>(p, a->dim, st) : launch_append8_dim<__nv_bfloat16>(p, a->dim, st);
+}
+
+extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? a8_workspace_bytes(head_dim) : 0; }
+
+extern "C" int hsg_attention8(const hsg_attention8_args* a) {
+  DRAFT_ARGS(a);
+  if (a->rows < 0 || a->tokens < 0 || a->hq < 1 || a->hkv < 1 || a->hq % a->hkv)
+    return fail(HSG_ERR_INVALID, "bad shape (rows %d, tokens %d, heads %d / %d)", a->rows, a->tokens, a->hq, a->hkv);
+  if (a->hq / a->hkv > DA_ROWS)
+    return fail(HSG_ERR_INVALID, "at most %d query heads a key head, got %d", DA_ROWS, a->hq / a->hkv);
+  if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
+  if (a->dtype != HSG_DT_F16 && a->dtype != HSG_DT_BF16) return fail(HSG_ERR_INVALID, "dtype must be fp16 or bf16");
+  if (a->max_new < 1 || a->max_new > HSG_MAX_NEW)
+    return fail(HSG_ERR_INVALID, "max_new must be in [1, %d], got %d", HSG_MAX_NEW, a->max_new);
+  if (a->mask && (int64_t)a->words * 32 < a->max_new)
+    return fail(HSG_ERR_INVALID, "%d mask words hold fewer than max_new = %d bits", a->words, a->max_new);
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(HSG_ERR_INVALID, "scale must be positive");
+  if (a->window < 0 || a->sinks < 0) return fail(HSG_ERR_INVALID, "window and sinks must not be negative, got %d and %d", a->window, a->sinks);
+  if (a->rows == 0 || a->tokens == 0) return HSG_OK;
+  if (!a->q || !a->table || !a->lens || !a->cu || !a->out) return fail(HSG_ERR_INVALID, "NULL argument");
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)hsg_attention8_workspace(a->dim))
+    return fail(HSG_ERR_INVALID, "the workspace must have %zu bytes on a 16-byte boundary", hsg_attention8_workspace(a->dim));
+  if (a->width < 1 || a->table_stride < a->width)
+    return fail(HSG_ERR_INVALID, "bad table shape (width %d, stride %lld)", a->width, (long long)a->table_stride);
+  int rc;
+  if ((rc = check_cache8(a->cache, a->hkv, a->dim)) != HSG_OK) return rc;
+  if ((int64_t)a->width * a->cache.page_size > INT32_MAX)
+    return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit positions", a->width, a->cache.page_size);
+  if (!aligned16(a->q) || !aligned16(a->out) || !rows16(a->q_token_stride, a->q_head_stride, 2))
+    return fail(HSG_ERR_INVALID, "q rows must lie on 16-byte boundaries");
+  if ((int64_t)a->max_new * (a->hq / a->hkv) > INT32_MAX / 2) return fail(HSG_ERR_INVALID, "too many rows a key head");
+  Attn8Args p{a->q, a->q_token_stride, a->q_head_stride, cache8(a->cache), a->table, a->table_stride, a->lens, a->cu,
+              a->positions, a->mask, a->rows, a->width, a->tokens, a->words, a->max_new, a->hq, a->hkv, a->window, a->sinks,
+              a->scale, a->out, a->lse, a->err};
+  cudaStream_t st = (cudaStream_t)a->stream;
+  return a->dtype == HSG_DT_F16 ? launch_attn8_dim<__half>(p, a->dim, a->workspace, st)
+                                : launch_attn8_dim<__nv_bfloat16>(p, a->dim, a->workspace, st);
+}
+
+extern "C" int hsg_token_logprobs(const hsg_logprobs_args* a) {
+  DRAFT_ARGS(a);
+  if (a->rows < 0 || a->vocab < 1 || a->n_given < 0)
+    return fail(HSG_ERR_INVALID, "bad shape (rows %d, vocabulary %d, given %d)", a->rows, a->vocab, a->n_given);
+  if (a->dtype < HSG_DT_F32 || a->dtype > HSG_DT_BF16) return fail(HSG_ERR_INVALID, "logits must be fp32, fp16 or bf16");
+  if (a->top < 0 || a->top > HSG_MAX_TOP || a->top > a->vocab)
+    return fail(HSG_ERR_INVALID, "top must be in [0, %d] and at most the vocabulary, got %d", HSG_MAX_TOP, a->top);
+  if (!(a->temperature >= 1e-4f) || !(a->temperature <= 1e4f))
+    return fail(HSG_ERR_INVALID, "temperature must be in [1e-4, 1e4], got %g", a->temperature);
+  if (a->rows == 0) return HSG_OK;
+  if (!a->logits || !a->entropy || !a->lse || (a->n_given && (!a->given || !a->logprobs)) || (a->top && (!a->top_logprobs || !a->top_ids)))
+    return fail(HSG_ERR_INVALID, "NULL argument");
+  if (a->rows > 1 && a->row_stride < 0) return fail(HSG_ERR_INVALID, "rows of logits must not descend");
+  if (reinterpret_cast<uintptr_t>(a->logits) % (a->dtype == HSG_DT_F32 ? 4 : 2))
+    return fail(HSG_ERR_INVALID, "logits must lie on an element's boundary");
+  if (a->rows > INT32_MAX / LP_CLUSTER) return fail(HSG_ERR_INVALID, "too many rows (%d)", a->rows);
+  LogprobsArgs p{a->logits, a->row_stride, a->given, a->rows, a->vocab, a->n_given, a->top, 1.0f / a->temperature, a->logprobs,
+                 a->entropy, a->lse, a->top_logprobs, a->top_ids, a->err};
+  cudaStream_t st = (cudaStream_t)a->stream;
+  return a->dtype == HSG_DT_F32 ? launch_logprobs<float>(p, st)
+                                : a->dtype == HSG_DT_F16 ? launch_logprobs<__half>(p, st) : launch_logprobs<__nv_bfloat16>(p, st);
+}

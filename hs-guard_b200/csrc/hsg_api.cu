@@ -1279,3 +1279,4 @@ extern "C" int hsg_gemm_f32_noalloc(const void* w, int n, int k, const float* x,
 }
 
 #include "draft_api.cuh"
+#include "cache8_api.cuh"

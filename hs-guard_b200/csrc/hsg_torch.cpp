@@ -1,4 +1,4 @@
-// Tensor side of draft scoring (CPython extension module _hsg_torch over libhsg.so and torch's C++ tensors).
+// Tensor side of draft scoring and of the 8-bit cache (CPython extension module _hsg_torch over libhsg.so and torch's C++ tensors).
 //
 // hs_guard_b200.drafts documents these functions; here their arguments are checked, their outputs allocated and the
 // argument structs of include/hsg.h filled. The same steps in Python cost 6 to 15 us a call, several times what the
@@ -140,14 +140,17 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, at::Device device) {
   return at::empty(sizes, at::TensorOptions().dtype(dtype).device(device));
 }
 
-// n elements of `base`'s storage from the offset-th on (both counted in elements of this type) as a vector: a view operator
-// costs several times as much.
-Tensor part(const Tensor& base, at::ScalarType dtype, int64_t offset, int64_t n) {
+// A contiguous tensor of these sizes over `base`'s storage from the offset-th element (of this type) on: a view operator costs
+// several times as much.
+Tensor part(const Tensor& base, at::ScalarType dtype, int64_t offset, at::IntArrayRef sizes) {
   Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(),
                                                       c10::scalarTypeToTypeMeta(dtype));
   t.unsafeGetTensorImpl()->set_storage_offset(offset);
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   return t;
+}
+Tensor part(const Tensor& base, at::ScalarType dtype, int64_t offset, int64_t n) {
+  return part(base, dtype, offset, at::IntArrayRef(&n, 1));
 }
 
 void* stream_of(at::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
@@ -453,6 +456,189 @@ PyObject* store_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// k_cache and v_cache [pages, page_size, heads, dim] e4m3, alike in strides, and their scales [pages, blocks, heads].
+hsg_cache8 cache8(PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso, int64_t heads, int64_t dim, at::Device device) {
+  const Tensor &k = shaped(ko, "k_cache", 4, at::kFloat8_e4m3fn, device), &v = shaped(vo, "v_cache", 4, at::kFloat8_e4m3fn, device);
+  const Tensor &ks = shaped(kso, "k_scale", 3, at::kFloat, device), &vs = shaped(vso, "v_scale", 3, at::kFloat, device);
+  if (v.sizes() != k.sizes() || v.strides() != k.strides() || k.size(2) != heads || k.size(3) != dim)
+    refuse("k_cache and v_cache must be alike, [pages, page_size, %lld, %lld]", (long long)heads, (long long)dim);
+  const int64_t blocks = ks.size(1);
+  if (vs.sizes() != ks.sizes() || !ks.is_contiguous() || !vs.is_contiguous() || ks.size(0) != k.size(0) || ks.size(2) != heads ||
+      blocks < 1 || k.size(1) % blocks)
+    refuse("k_scale and v_scale must be contiguous, [pages, blocks of a page, %lld]", (long long)heads);
+  return hsg_cache8{k.data_ptr(), v.data_ptr(), static_cast<float*>(ks.data_ptr()), static_cast<float*>(vs.data_ptr()),
+                    k.stride(0), k.stride(1), k.stride(2), small(k.size(0), "pages"), small(k.size(1), "page_size"),
+                    small(k.size(1) / blocks, "block"), 0};
+}
+
+bool truth(PyObject* o, const char* name) {
+  if (o != Py_True && o != Py_False) refuse("%s must be True or False", name);
+  return o == Py_True;
+}
+
+// append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source, positions, inv_freq, interleaved, rope_scale, q, err)
+//   -> q or None
+PyObject* append_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 14, [&]() -> PyObject* {
+    const Tensor& k0 = tensor(a[0], "k");
+    const at::Device device = device_of(k0, "k");
+    const at::ScalarType dtype = k0.scalar_type();
+    if (!is_16(dtype)) refuse("q, k and v must be fp16 or bf16");
+    const Tensor &k = shaped(a[0], "k", 3, dtype, device), &v = shaped(a[1], "v", 3, dtype, device);
+    if (k.sizes() != v.sizes()) refuse("k and v must be alike, [rows, kv heads, dim]");
+    hsg_append8_args s{};
+    s.size = sizeof(s);
+    s.k = k.data_ptr();
+    s.v = v.data_ptr();
+    s.k_token_stride = k.stride(0);
+    s.k_head_stride = k.stride(1);
+    s.v_token_stride = v.stride(0);
+    s.v_head_stride = v.stride(1);
+    s.rows = small(k.size(0), "rows");
+    s.hkv = small(k.size(1), "kv heads");
+    s.dim = small(k.size(2), "dim");
+    s.dtype = code_of(dtype);
+    s.cache = cache8(a[2], a[3], a[4], a[5], s.hkv, s.dim, device);
+    s.slots = vector<int32_t>(a[6], "slots", at::kInt, device);
+    s.count = small(THPVariable_Unpack(a[6]).size(0), "slots");
+    if (a[7] != Py_None) s.source = vector<int32_t>(a[7], "source", at::kInt, device, s.count);
+    else if (s.count > s.rows) refuse("%d slots for %d rows", s.count, s.rows);
+    if ((a[8] == Py_None) != (a[9] == Py_None)) refuse("positions and inv_freq go together");
+    if (a[9] != Py_None) {
+      s.positions = vector<int32_t>(a[8], "positions", at::kInt, device, s.count);
+      s.inv_freq = vector<float>(a[9], "inv_freq", at::kFloat, device);
+      s.rot = small(2 * THPVariable_Unpack(a[9]).size(0), "inv_freq");
+    }
+    s.interleaved = truth(a[10], "interleaved");
+    s.rope_scale = real(a[11], "rope_scale");
+    s.err = error_word(a[13], device);
+    Tensor q_out;
+    if (a[12] != Py_None) {
+      if (a[7] != Py_None) refuse("q goes with entries in order, not with a source");
+      const Tensor& q = shaped(a[12], "q", 3, dtype, device);
+      if (q.size(0) != s.count || q.size(2) != s.dim) refuse("q must be [%d, heads, %d]", s.count, s.dim);
+      s.hq = small(q.size(1), "heads");
+      if (s.hq < 1) refuse("q must have heads");
+      s.q = q.data_ptr();
+      s.q_token_stride = q.stride(0);
+      s.q_head_stride = q.stride(1);
+      q_out = empty({s.count, s.hq, s.dim}, dtype, device);
+      s.q_out = q_out.data_ptr();
+    }
+    s.stream = stream_of(device);
+    const c10::cuda::CUDAGuard guard(device);
+    done(hsg_append8(&s));
+    for (int i = 2; i < 6; ++i) changed(a[i]);
+    if (a[12] == Py_None) Py_RETURN_NONE;
+    return THPVariable_Wrap(q_out);
+  });
+}
+
+// attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask, positions, window, sinks, workspace,
+//   err) -> (out, lse)
+PyObject* attention_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 16, [&]() -> PyObject* {
+    const Tensor& q0 = tensor(a[0], "q");
+    const at::Device device = device_of(q0, "q");
+    const at::ScalarType dtype = q0.scalar_type();
+    if (!is_16(dtype)) refuse("q must be fp16 or bf16");
+    const Tensor& q = shaped(a[0], "q", 3, dtype, device);
+    hsg_attention8_args s{};
+    s.size = sizeof(s);
+    s.q = q.data_ptr();
+    s.q_token_stride = q.stride(0);
+    s.q_head_stride = q.stride(1);
+    s.tokens = small(q.size(0), "tokens");
+    s.hq = small(q.size(1), "heads");
+    s.dim = small(q.size(2), "dim");
+    const Tensor& codes = tensor(a[1], "k_cache");
+    if (codes.dim() != 4) refuse("k_cache must be a 4-d tensor");
+    s.hkv = small(codes.size(2), "kv heads");
+    s.cache = cache8(a[1], a[2], a[3], a[4], s.hkv, s.dim, device);
+    const Tensor& table = shaped(a[5], "table", 2, at::kInt, device);
+    s.rows = small(table.size(0), "rows");
+    s.width = small(table.size(1), "the table's width");
+    s.table = static_cast<const int32_t*>(table.data_ptr());
+    s.table_stride = s.rows > 1 ? table.stride(0) : s.width;
+    s.lens = vector<int32_t>(a[6], "lens", at::kInt, device, s.rows);
+    s.cu = vector<int32_t>(a[7], "cu", at::kInt, device, (int64_t)s.rows + 1);
+    s.scale = real(a[8], "scale");
+    s.max_new = whole(a[9], "max_new", 1, HSG_MAX_NEW);
+    if (a[10] != Py_None) {
+      const Tensor& mask = shaped(a[10], "mask", 2, at::kInt, device);
+      if (mask.size(0) != s.tokens || !mask.is_contiguous()) refuse("mask must be contiguous, [%d, words]", s.tokens);
+      s.words = small(mask.size(1), "the mask's words");
+      s.mask = static_cast<const uint32_t*>(mask.data_ptr());
+    }
+    if (a[11] != Py_None) s.positions = vector<int32_t>(a[11], "positions", at::kInt, device, s.tokens);
+    s.window = whole(a[12], "window", 0, INT32_MAX);
+    s.sinks = whole(a[13], "sinks", 0, INT32_MAX);
+    Tensor workspace;
+    if (a[14] == Py_None) workspace = empty({(int64_t)hsg_attention8_workspace(s.dim)}, at::kByte, device);
+    else workspace = shaped(a[14], "workspace", 1, at::kByte, device);
+    s.workspace = workspace.data_ptr();
+    s.workspace_bytes = workspace.numel();
+    s.err = error_word(a[15], device);
+    const Tensor out = empty({s.tokens, s.hq, s.dim}, dtype, device), lse = empty({s.tokens, s.hq}, at::kFloat, device);
+    s.out = out.data_ptr();
+    s.lse = static_cast<float*>(lse.data_ptr());
+    s.dtype = code_of(dtype);
+    s.stream = stream_of(device);
+    const c10::cuda::CUDAGuard guard(device);
+    if (s.rows == 0) {  // the library has nothing to do: no token sees anything
+      out.zero_();
+      lse.fill_(-std::numeric_limits<float>::infinity());
+    } else {
+      done(hsg_attention8(&s));
+    }
+    return tuple_of(out, lse);
+  });
+}
+
+// token_logprobs(logits, given, top, temperature, err) -> the five tensors of Logprobs
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    const Tensor& x0 = tensor(a[0], "logits");
+    const at::Device device = device_of(x0, "logits");
+    hsg_logprobs_args s{};
+    s.size = sizeof(s);
+    s.dtype = code_of(x0.scalar_type());
+    if (s.dtype < 0) refuse("logits must be fp32, fp16 or bf16");
+    const Tensor& x = shaped(a[0], "logits", 2, x0.scalar_type(), device);
+    s.logits = x.data_ptr();
+    s.row_stride = x.stride(0);
+    s.rows = small(x.size(0), "rows");
+    s.vocab = small(x.size(1), "the vocabulary");
+    bool flat = false;
+    if (a[1] != Py_None) {
+      flat = tensor(a[1], "given").dim() == 1;
+      const Tensor& given = shaped(a[1], "given", flat ? 1 : 2, at::kInt, device);
+      if (given.size(0) != s.rows || !given.is_contiguous()) refuse("given must be contiguous, [%d] or [%d, tokens]", s.rows, s.rows);
+      s.n_given = flat ? 1 : small(given.size(1), "given");
+      s.given = static_cast<const int32_t*>(given.data_ptr());
+    }
+    s.top = whole(a[2], "top", 0, HSG_MAX_TOP);
+    s.temperature = real(a[3], "temperature");
+    s.err = error_word(a[4], device);
+    const int64_t rows = s.rows, at_lse = rows, at_given = 2 * rows, at_top = at_given + rows * s.n_given, at_ids = at_top + rows * s.top;
+    const Tensor all = empty({at_ids + rows * s.top}, at::kFloat, device);
+    float* base = static_cast<float*>(all.data_ptr());
+    s.entropy = base;
+    s.lse = base + at_lse;
+    s.logprobs = base + at_given;
+    s.top_logprobs = base + at_top;
+    s.top_ids = reinterpret_cast<int32_t*>(base + at_ids);
+    s.stream = stream_of(device);
+    const c10::cuda::CUDAGuard guard(device);
+    done(hsg_token_logprobs(&s));
+    const int64_t n_given = s.n_given, top = s.top;
+    return tuple_of(flat ? part(all, at::kFloat, at_given, rows) : part(all, at::kFloat, at_given, at::IntArrayRef({rows, n_given})),
+                    part(all, at::kFloat, 0, rows), part(all, at::kFloat, at_lse, rows),
+                    part(all, at::kFloat, at_top, at::IntArrayRef({rows, top})),
+                    part(all, at::kInt, at_ids, at::IntArrayRef({rows, top})));
+  });
+}
+
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f))
 PyMethodDef methods[] = {{"advance_tables", FAST(advance_tables), METH_FASTCALL, nullptr},
                          {"plan_tree", FAST(plan_tree), METH_FASTCALL, nullptr},
@@ -460,6 +646,9 @@ PyMethodDef methods[] = {{"advance_tables", FAST(advance_tables), METH_FASTCALL,
                          {"norm_rope_store", FAST(norm_rope_store), METH_FASTCALL, nullptr},
                          {"tree_attention", FAST(tree_attention), METH_FASTCALL, nullptr},
                          {"store_rows", FAST(store_rows), METH_FASTCALL, nullptr},
+                         {"append_8bit", FAST(append_8bit), METH_FASTCALL, nullptr},
+                         {"attention_8bit", FAST(attention_8bit), METH_FASTCALL, nullptr},
+                         {"token_logprobs", FAST(token_logprobs), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hsg_torch", nullptr, -1, methods};
 

@@ -21,9 +21,20 @@ gradients outside ``torch.no_grad()``: there are no backward passes. Values on t
 skip an index outside its range and record the reason in ``err`` (an int32 tensor of one element, 0 at first; see
 ``raise_device_error``); without ``err`` nothing says that one was met.
 
+The same over a cache in 8 bits, half the memory and half the reading: keys and values as e4m3 codes with a scale for each block
+of tokens and key head. There the newest tokens (one, a chunk of a prompt, a drafted tree) are appended first and then attended
+where they lie; what is not accepted is taken back with ``advance_tables``:
+
+    t = advance_tables(...)
+    q = append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, t.slots, positions=t.positions, inv_freq=inv_freq, q=q)   # rotates
+    out, lse = attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, t.lens, t.cu, scale, max_new, window=512, sinks=4)
+
+``DraftCache8`` holds such pages. ``token_logprobs`` says from a host's logits how likely the drafted tokens were, how sure the
+model is and which tokens it likes best.
+
 Arguments are checked and outputs allocated by the extension module _hsg_torch (csrc/hsg_torch.cpp), which calls
-hsg_plan_tree, hsg_norm_rope, hsg_tree_attention, hsg_advance_tables and hsg_store_rows of include/hsg.h. The reference has
-no counterpart: its ticks are chains and its caches 512-token rings.
+hsg_plan_tree, hsg_norm_rope, hsg_tree_attention, hsg_advance_tables, hsg_store_rows, hsg_append8, hsg_attention8 and
+hsg_token_logprobs of include/hsg.h. The reference has no counterpart: its ticks are chains and its caches 512-token rings.
 """
 from __future__ import annotations
 
@@ -36,8 +47,11 @@ from .build import tensors
 
 MAX_TREE = 1024        # drafted tokens of one request
 MAX_TABLE_ROWS = 4096  # requests of one advance_tables call
+MAX_NEW = 1 << 20      # newest tokens of one request in attention_8bit
+MAX_TOP = 64           # alternatives of token_logprobs
 
 Tables = namedtuple("Tables", "lens counters cu slots rows positions")
+Logprobs = namedtuple("Logprobs", "logprobs entropy lse top top_ids")
 
 
 def raise_device_error(err):
@@ -117,6 +131,60 @@ def store_rows(k, v, k_cache, v_cache, slots, source=None, err=None):
     tensors().store_rows(k, v, k_cache, v_cache, slots, source, err)
 
 
+def append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source=None, positions=None, inv_freq=None, interleaved=False,
+                rope_scale=1.0, q=None, err=None):
+    """Write rows of k and v [rows, hkv, dim] (fp16 or bf16) into slots [count] int32 of an 8-bit cache, in place: row source[i]
+    (None: i) to slots[i]; a negative slot is skipped.
+
+    k_cache, v_cache [pages, page_size, hkv, dim] float8_e4m3fn views, alike in strides, rows on 16-byte boundaries; k_scale, v_scale
+    [pages, page_size // block, hkv] fp32, contiguous, block a multiple of 8. With inv_freq [rot / 2] fp32 and positions [count]
+    int32, the first rot dims of k (a multiple of 16) turn by positions * inv_freq and are multiplied by rope_scale, as rotations stretched for long
+    contexts want it: dims (j, j + rot / 2), or (2 j, 2 j + 1) if ``interleaved``. Then q [count, hq, dim] may be given too: its turned
+    rows are returned, those of skipped slots among them.
+
+    Entries of one block must stand together (but for skipped ones), in ascending slots (as ``advance_tables`` lists them). A block's scale becomes the
+    power of two that its largest appended element asks for (a pair that turns counts with the sum of its magnitudes, so that
+    rounding decides nothing); unless its first token is among the entries it does not fall, and when it rises the tokens that
+    were there are rounded again. Elements that are not finite become NaN. Slots that do not ascend within a block or lie beyond
+    the pages, and sources outside the rows, are skipped and recorded in ``err``."""
+    return tensors().append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source, positions, inv_freq, interleaved,
+                                 rope_scale, q, err)
+
+
+def attention_8bit_workspace(dim):
+    """Bytes of workspace an ``attention_8bit`` call of this head dim uses."""
+    return int(_lib.lib().hsg_attention8_workspace(dim))
+
+
+def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask=None, positions=None, window=0,
+                   sinks=0, workspace=None, err=None):
+    """Attention of each request's newest tokens over its pages of an 8-bit cache.
+
+    q [tokens, hq, dim] (fp16 or bf16, hq a multiple of hkv, at most 128 query heads a key head, dim 64, 128 or 256; any strides
+    that keep rows on 16-byte boundaries); cache and scales as in ``append_8bit`` (any positive scales); table [rows, width], lens
+    [rows], cu [rows + 1] int32. Request b has lens[b] tokens in its pages, the last cu[b + 1] - cu[b] (at most max_new) being
+    those of q. They see all tokens before them, and among themselves the earlier ones and their own, or the ones whose bits
+    mask [tokens, words] int32 has set (as ``plan_tree`` makes it). With window > 0 only tokens at positions above the query's own
+    minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (None: their places in the cache) are
+    read only then. Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets
+    0 and -inf, as do tokens outside cu[0] .. cu[rows] - 1 and those of a request whose lengths are out of range (which ``err``
+    records). ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim)`` bytes, for one call at a time) is allocated when it
+    is not given."""
+    return tensors().attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask, positions, window,
+                                    sinks, workspace, err)
+
+
+def token_logprobs(logits, given=None, top=0, temperature=1.0, err=None):
+    """Log-probabilities of given tokens under softmax(logits / temperature), its entropy and its most likely tokens.
+
+    logits [rows, vocab] fp32, fp16 or bf16, rows at any stride; given [rows] or [rows, n] int32, -1: none; top at most MAX_TOP.
+    Returns ``Logprobs(logprobs, entropy, lse, top, top_ids)``: logprobs in given's shape (0 for none; NaN, and recorded in
+    ``err``, for a token beyond the vocabulary), entropy and log-sum-exp of logits / temperature [rows], and [rows, top] the
+    log-probabilities and ids (int32) of the most likely tokens, of equally likely ones the lowest first. Logits of -inf have no
+    probability; a row of nothing else, or with NaN or +inf, has NaN everywhere (but lse -inf for the former) and ids -1."""
+    return Logprobs(*tensors().token_logprobs(logits, given, top, temperature, err))
+
+
 def ring_cache(engine, layer, slots):
     """A live engine's rings of softmax layer ``layer`` (0 .. 5) as the paged cache of ``tree_attention``: (k_cache, v_cache,
     table, lens) for requests ``slots``, to be used with window <= 512 and positions from the slots' lengths on.
@@ -160,14 +228,16 @@ class DraftCache:
     requests; a finished one gives its pages back with a delta of minus its length. Calls that change the cache (advance,
     store) and calls that read it are ordered by their stream; on several streams that order is the caller's."""
 
+    _dtypes = (torch.float16, torch.bfloat16)
+
     def __init__(self, layers, rows, pages, page_size, max_len, kv_heads, dim, dtype=torch.float16, device=None):
         if min(layers, rows, pages, max_len, kv_heads) < 1 or rows > MAX_TABLE_ROWS:
             raise ValueError("layers, rows, pages, max_len and kv_heads must be positive, rows at most %d" %
                              MAX_TABLE_ROWS)
         if page_size < 8 or page_size % 8 or dim not in (64, 128, 256):
             raise ValueError("page_size must be a multiple of 8, dim 64, 128 or 256")
-        if dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError("the cache must be fp16 or bf16")
+        if dtype not in self._dtypes:
+            raise ValueError("the cache must be %s" % " or ".join(str(d)[6:] for d in self._dtypes))
         device = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
         if device.type != "cuda":
             raise ValueError("the cache lives on a CUDA device, got %s" % device)
@@ -200,3 +270,29 @@ class DraftCache:
     def raise_device_error(self):
         """Wait for the device and raise HsgError if a kernel met an index outside its range."""
         raise_device_error(self.err)
+
+
+class DraftCache8(DraftCache):
+    """``DraftCache`` in 8 bits: ``k[layer]``, ``v[layer]`` are e4m3 codes and ``k_scale[layer]``, ``v_scale[layer]`` [pages,
+    page_size // block, kv_heads] their scales. New tokens are stored before they are attended: ``advance`` makes room (and takes
+    back what was not accepted), ``store`` appends, ``attend`` lets the newest tokens of each request see its pages."""
+
+    _dtypes = (torch.float8_e4m3fn,)
+
+    def __init__(self, layers, rows, pages, page_size, max_len, kv_heads, dim, block=None, device=None):
+        block = page_size if block is None else block
+        if block < 8 or block % 8 or page_size % block:
+            raise ValueError("block must be a multiple of 8 that divides page_size")
+        super().__init__(layers, rows, pages, page_size, max_len, kv_heads, dim, torch.float8_e4m3fn, device)
+        scales = torch.ones(2, layers, pages, page_size // block, kv_heads, dtype=torch.float32, device=self.k.device)
+        self.k_scale, self.v_scale = scales[0], scales[1]
+
+    def store(self, layer, k, v, slots, source=None, positions=None, inv_freq=None, interleaved=False, rope_scale=1.0, q=None):
+        """``append_8bit`` into a layer's pages; returns the turned q, if it was given."""
+        return append_8bit(k, v, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], slots, source, positions,
+                           inv_freq, interleaved, rope_scale, q, self.err)
+
+    def attend(self, layer, q, cu, scale, max_new, mask=None, positions=None, window=0, sinks=0):
+        """``attention_8bit`` of each request's newest tokens over a layer's pages: (out, lse)."""
+        return attention_8bit(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], self.table, self.lens, cu,
+                              scale, max_new, mask, positions, window, sinks, None, self.err)

@@ -352,6 +352,107 @@ typedef struct hsg_store_args {
 } hsg_store_args;
 int hsg_store_rows(const hsg_store_args* args);
 
+/* ---- a cache in 8 bits, and what the logits of drafted tokens say (no counterpart in the reference) ----
+ *
+ * Keys and values as e4m3 codes with a scale for each block of `block` consecutive tokens of a page and key head: code (page,
+ * token, head, d) lies at page * page_stride + token * token_stride + head * head_stride + d (bytes), in k as in v, and stands for
+ * code * scale [page][token / block][head]. page_size is a multiple of block, block of 8; rows begin on 16-byte boundaries. Tables
+ * and slots are those of hsg_advance_tables. The conventions above (size, err, stream) hold here as well. */
+#define HSG_MAX_NEW (1 << 20) /* newest tokens of one request */
+#define HSG_MAX_TOP 64        /* alternatives of a row of logits */
+typedef struct hsg_cache8 {
+  void* k;
+  void* v;
+  float* k_scale; /* [pages][page_size / block][heads], contiguous, positive and finite */
+  float* v_scale;
+  int64_t page_stride, token_stride, head_stride;
+  int32_t pages, page_size, block, reserved;
+} hsg_cache8;
+
+/* For i < count: row source[i] (NULL: i) of k and v [rows][hkv][dim] in dtype (fp16 or bf16) to slot slots[i]; a negative slot
+ * is skipped. With rot > 0 the first rot dims of k turn by positions[i] * inv_freq[j] and are multiplied by rope_scale: pairs
+ * (j, j + rot / 2), or (2 j, 2 j + 1) if interleaved. With hq > 0, q [count][hq][dim] is turned likewise into q_out
+ * [count][hq][dim], contiguous, whatever its slot (source is NULL then). Entries of one block must stand together (but for
+ * skipped ones) with ascending slots; the block's scales become 2^e, e the smallest integer (in [-100, 120]) with b <= 448 * 2^e, b the largest of: |x| of V's
+ * elements and of K's that do not turn, (|x| + |y|) |rope_scale| of K's pairs that do, computed in fp32 without those that are not finite; but if the
+ * block's first token is not among the entries, at least the scale that it had, and if that rises, tokens before the first
+ * entry are rounded again. Codes are x / scale to nearest even, NaN for what is not finite. A slot that does not ascend beyond
+ * the entry before it within a block, or beyond the pages, or a source outside the rows, is skipped and sets err. An entry of
+ * a block that other entries, apart from these, have been listed for gives that block's tokens and scales some value. */
+typedef struct hsg_append8_args {
+  int64_t size;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int32_t* source;
+  const int32_t* slots;
+  const int32_t* positions;
+  const float* inv_freq;
+  void* q_out;
+  hsg_cache8 cache;
+  int32_t* err;
+  void* stream;
+  int32_t count, rows, hq, hkv, dim, rot, interleaved, dtype;
+  float rope_scale;
+} hsg_append8_args;
+int hsg_append8(const hsg_append8_args* args);
+
+/* Request b holds lens[b] tokens in the pages of its table row, the last cu[b+1] - cu[b] of which are its query tokens, in order:
+ * one, a chunk of a prompt, or a drafted tree that was appended. Query token t (at position p_t) sees the tokens before the
+ * query tokens, and query token u iff bit u of mask[t] is set (mask NULL: u <= t); with a window only those at positions
+ * above p_t - window or below sinks. positions [tokens] of the query tokens (NULL: their places in the cache) are read only with a
+ * window and must be at least lens[b] - n. out [tokens][hq][dim] = softmax(scale q.k) v in dtype (q's: HSG_DT_F16 or _BF16), lse
+ * [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing, or only scores of -inf, gets 0 and -inf, and so do
+ * tokens of no request and those of a request whose lengths are out of range; what is not seen does not enter a result whatever
+ * its codes and scales. cu must not descend; no request has more than max_new query tokens. Table entries of pages that no query
+ * token sees are not read. `workspace`: hsg_attention8_workspace(dim) bytes on a 16-byte boundary, not shared by calls that
+ * overlap in time. */
+typedef struct hsg_attention8_args {
+  int64_t size;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  hsg_cache8 cache;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* cu;
+  const int32_t* positions;
+  const uint32_t* mask;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* err;
+  void* stream;
+  int32_t rows, width, tokens, words, max_new, hq, hkv, dim, window, sinks, dtype;
+  float scale;
+} hsg_attention8_args;
+size_t hsg_attention8_workspace(int head_dim);
+int hsg_attention8(const hsg_attention8_args* args);
+
+/* For each row x of logits [rows][vocab] in dtype (rows row_stride elements apart, beginning on any element): p = softmax(x /
+ * temperature), logprobs [rows][n_given] = log p of the given tokens (a negative one: 0; one beyond the vocabulary: NaN, and
+ * err is set), entropy [rows] = -sum p log p, lse [rows] the log-sum-exp of x / temperature, and the `top` most likely tokens,
+ * the lowest of equally likely ones first: top_logprobs and top_ids [rows][top]. Logits of -inf have no probability. A row without
+ * any, or with NaN or +inf, has NaN everywhere (but lse = -inf without any) and ids -1. */
+typedef struct hsg_logprobs_args {
+  int64_t size;
+  const void* logits;
+  int64_t row_stride;
+  const int32_t* given;
+  float* logprobs;
+  float* entropy;
+  float* lse;
+  float* top_logprobs;
+  int32_t* top_ids;
+  int32_t* err;
+  void* stream;
+  int32_t rows, vocab, n_given, top, dtype;
+  float temperature;
+} hsg_logprobs_args;
+int hsg_token_logprobs(const hsg_logprobs_args* args);
+
 /* What the value of a device error word says. */
 const char* hsg_device_error_text(int code);
 
