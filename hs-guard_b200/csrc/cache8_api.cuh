@@ -1,7 +1,7 @@
 // C entry points of the 8-bit cache and of token log-probabilities (hsg_append8, hsg_attention8, hsg_token_logprobs): argument
 // checks and launches. Part of the one translation unit of the library.
 #pragma once
-#include "cache8_attn.cuh"
+#include "cache8_wide.cuh"
 #include "draft_api.cuh"
 #include "logprobs.cuh"
 
@@ -32,6 +32,9 @@ Cache8 cache8(const hsg_cache8& c) {
                 c.head_stride, c.pages, c.page_size, c.block};
 }
 
+static_assert(A8_PIECES == SM_COUNT, "one piece an SM");
+constexpr int A8_WIDE_ROWS = 32;  // rows of a key head up to which warp-level products are taken
+
 template <int D, typename T>
 int launch_append8(const Append8Args& p, cudaStream_t st) {
   // entries a thread block: one where that leaves few blocks idle, else eight, of which most continue a run
@@ -51,9 +54,18 @@ template <int D, typename T>
 int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   A8Split* splits = static_cast<A8Split*>(workspace);
   float* partials = reinterpret_cast<float*>(splits + A8_PIECES);
+  // rows of a key head, as far as the host can tell: no request has more than max_new tokens, all have `tokens` together
+  const int64_t rows = std::min<int64_t>(p.max_new, (p.tokens + p.rows - 1) / p.rows) * (p.hq / p.hkv);
+  if (rows > A8_WIDE_ROWS) {
+    CU(cudaFuncSetAttribute(attn8_wide_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, w8_smem(D)));
+    CU(launch_k(attn8_wide_kernel<D, T>, dim3(A8_PIECES), dim3(W8_THREADS), w8_smem(D), st, true, p, splits, partials));
+    CU(launch_k(attn8_join_kernel<D, W8_ROWS, T>, dim3(A8_PIECES, W8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
+                (const A8Split*)splits, (const float*)partials));
+    return HSG_OK;
+  }
   CU(cudaFuncSetAttribute(attn8_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
   CU(launch_k(attn8_kernel<D, T>, dim3(A8_PIECES), dim3(A8_THREADS), a8_smem(D), st, true, p, splits, partials));
-  CU(launch_k(attn8_join_kernel<D, T>, dim3(A8_PIECES, A8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
+  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3(A8_PIECES, A8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
               (const A8Split*)splits, (const float*)partials));
   return HSG_OK;
 }
@@ -99,7 +111,7 @@ extern "C" int hsg_append8(const hsg_append8_args* a) {
   return a->dtype == HSG_DT_F16 ? launch_append8_dim<__half>(p, a->dim, st) : launch_append8_dim<__nv_bfloat16>(p, a->dim, st);
 }
 
-extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? a8_workspace_bytes(head_dim) : 0; }
+extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? a8_workspace_bytes(head_dim, W8_ROWS) : 0; }
 
 extern "C" int hsg_attention8(const hsg_attention8_args* a) {
   DRAFT_ARGS(a);

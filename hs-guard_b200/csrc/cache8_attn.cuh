@@ -62,20 +62,21 @@ __host__ __device__ constexpr int a8_stages(int dim) { return A8_RING / a8_stage
 __host__ __device__ constexpr int a8_smem(int dim) {
   return A8_WARPS * (A8_RING + a8_stages(dim) * 16) + A8_ROWS * dim * 2 + A8_ROWS * dim * 4 + 4096;
 }
-__host__ __device__ constexpr size_t a8_partial_floats(int dim) { return (size_t)A8_ROWS * (dim + 2); }
+__host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows = A8_ROWS) { return (size_t)rows * (dim + 2); }
 struct A8Split {  // an item that begins in a piece and ends in a later one
   int b, h, block, last;
   int first_slot;
   int pad[3];
 };
-__host__ __device__ constexpr size_t a8_workspace_bytes(int dim) {
-  return A8_PIECES * sizeof(A8Split) + 2 * A8_PIECES * a8_partial_floats(dim) * sizeof(float);
+__host__ __device__ constexpr size_t a8_workspace_bytes(int dim, int rows) {
+  return A8_PIECES * sizeof(A8Split) + 2 * A8_PIECES * a8_partial_floats(dim, rows) * sizeof(float);
 }
 
-// A request; n = 0 if its lengths are out of range.
+// A request, its rows in blocks of ROWS; n = 0 if its lengths are out of range.
 struct A8Req {
   int len, t0, n, blocks;
 };
+template <int ROWS>
 __device__ __forceinline__ A8Req a8_request(const Attn8Args& a, int G, int b, bool report) {
   A8Req r;
   r.len = a.lens[b];
@@ -87,27 +88,28 @@ __device__ __forceinline__ A8Req a8_request(const Attn8Args& a, int G, int b, bo
     if (report) set_error(a.err, ERR_BAD_LEN);
     r.n = 0;
   }
-  r.blocks = (int)(((int64_t)r.n * G + A8_ROWS - 1) / A8_ROWS);
+  r.blocks = (int)(((int64_t)r.n * G + ROWS - 1) / ROWS);
   return r;
 }
 
-// What a block of rows can see: tokens [0, ahead) and [lo, hi), in tiles [0, lead) and [first, first + n - lead).
+// What a block of rows can see, in tiles of TILE keys: tokens [0, ahead) and [lo, hi), in tiles [0, lead) and [first, first + n - lead).
 struct A8Span {
   int ahead, lo, hi, lead, first, n;
 };
+template <int ROWS, int TILE>
 __device__ __forceinline__ A8Span a8_span(const Attn8Args& a, const A8Req& r, int G, int block) {
   A8Span s;
   const int old = r.len - r.n;
-  const int t_lo = block * A8_ROWS / G, t_hi = min(r.n - 1, (block * A8_ROWS + A8_ROWS - 1) / G);
+  const int t_lo = block * ROWS / G, t_hi = min(r.n - 1, (block * ROWS + ROWS - 1) / G);
   s.hi = a.mask ? r.len : old + t_hi + 1;
   s.lo = s.ahead = 0;
   if (a.window) {
     s.lo = max(0, old + (a.mask || a.positions ? 0 : t_lo) - a.window + 1);
     s.ahead = min(a.sinks, s.lo);
   }
-  s.lead = (s.ahead + A8_TILE - 1) / A8_TILE;
-  s.first = max(s.lead, s.lo / A8_TILE);
-  s.n = s.lead + max(0, (s.hi - 1) / A8_TILE + 1 - s.first);  // a length may be close to 2^31
+  s.lead = (s.ahead + TILE - 1) / TILE;
+  s.first = max(s.lead, s.lo / TILE);
+  s.n = s.lead + max(0, (s.hi - 1) / TILE + 1 - s.first);  // a length may be close to 2^31
   return s;
 }
 
@@ -115,14 +117,15 @@ __device__ __forceinline__ A8Span a8_span(const Attn8Args& a, const A8Req& r, in
 struct A8At {
   int b, h, block, i;
 };
+template <int ROWS, int TILE>
 struct A8Walk {
   A8At at;
   A8Req r;
   A8Span s;
   __device__ __forceinline__ void start(const Attn8Args& a, int G, const A8At& from) {
     at = from;
-    r = a8_request(a, G, at.b, false);
-    s = a8_span(a, r, G, at.block);
+    r = a8_request<ROWS>(a, G, at.b, false);
+    s = a8_span<ROWS, TILE>(a, r, G, at.block);
   }
   __device__ __forceinline__ void next_item(const Attn8Args& a, int G) {
     at.i = 0;
@@ -136,14 +139,76 @@ struct A8Walk {
             s.n = 0;
             return;
           }
-          r = a8_request(a, G, at.b, false);
+          r = a8_request<ROWS>(a, G, at.b, false);
         } while (r.n == 0);
       }
     }
-    s = a8_span(a, r, G, at.block);
+    s = a8_span<ROWS, TILE>(a, r, G, at.block);
   }
-  __device__ __forceinline__ int base(int tile) const { return (tile < s.lead ? tile : s.first + tile - s.lead) * A8_TILE; }
+  __device__ __forceinline__ int base(int tile) const { return (tile < s.lead ? tile : s.first + tile - s.lead) * TILE; }
 };
+
+// Where a thread block's piece of the line begins: item and tile (`from`), where that item begins on the line (`begin`), where the
+// piece ends (w1) and how long pieces are (step). An item is its tiles and `cost` more; a piece holds at least one tile. Every
+// thread of the block calls it, with room for THREADS / 32 + 3 numbers; false: nothing is left for this piece.
+template <int ROWS, int TILE, int THREADS>
+__device__ __forceinline__ bool a8_piece(const Attn8Args& a, int G, int cost, int piece, int64_t* room, A8At& from, int64_t& begin,
+                                         int64_t& w1, int64_t& step) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (a.rows + THREADS - 1) / THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
+  auto units_of = [&](const A8Req& r) {  // of one key head
+    int64_t u = 0;
+    for (int k = 0; k < r.blocks; ++k) u += a8_span<ROWS, TILE>(a, r, G, k).n + cost;
+    return u;
+  };
+  int64_t mine = 0;
+  for (int b = rb0; b < rb1; ++b) mine += units_of(a8_request<ROWS>(a, G, b, piece == 0)) * a.hkv;
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  if (lane == 31) room[warp] = upto;
+  __syncthreads();
+  int64_t before = upto - mine, units = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += room[w];
+    units += room[w];
+  }
+  step = max((int64_t)(cost + 1), (units + A8_PIECES - 1) / A8_PIECES);
+  const int64_t w0 = min(units, piece * step);
+  w1 = min(units, w0 + step);
+  if (w0 >= w1) return false;
+  int64_t* found = room + THREADS / 32;
+  A8At* at_found = reinterpret_cast<A8At*>(found + 1);
+  if (w0 >= before && w0 < before + mine) {
+    int64_t at = before;
+    for (int b = rb0; b < rb1; ++b) {
+      const A8Req r = a8_request<ROWS>(a, G, b, false);
+      const int64_t one = units_of(r), all = one * a.hkv;
+      if (w0 >= at && w0 < at + all) {
+        const int h = (int)((w0 - at) / one);
+        int64_t u = at + h * one;
+        for (int k = 0; k < r.blocks; ++k) {
+          const int n = a8_span<ROWS, TILE>(a, r, G, k).n + cost;
+          if (w0 < u + n) {
+            *at_found = A8At{b, h, k, (int)max((int64_t)0, w0 - u - cost)};
+            *found = u;
+            break;
+          }
+          u += n;
+        }
+        break;
+      }
+      at += all;
+    }
+  }
+  __syncthreads();
+  from = *at_found;
+  begin = *found;
+  return true;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -169,6 +234,13 @@ template <int D> __device__ __forceinline__ uint32_t a8_v_at(int k, int ch) {
 __device__ __forceinline__ uint32_t f8_half2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// What brings a row whose largest element is `most` to [2^14, 2^15), and back. A row of zeros, or of values below 2^-100, stays.
+__device__ __forceinline__ void a8_row_scale(float most, float& up, float& back) {
+  const int e = (__float_as_int(most) >> 23) - 127, by = e < -100 ? 0 : min(14 - e, 100);
+  up = __int_as_float((by + 127) << 23);
+  back = __int_as_float((127 - by) << 23);
 }
 
 template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -203,71 +275,23 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
   float* s_m = s_o + A8_ROWS * D;                                       // [warps][16]
   float* s_l = s_m + A8_WARPS * A8_ROWS;                                // [warps][16]
   float* s_rowscale = s_l + A8_WARPS * A8_ROWS;                         // [16]
-  int64_t* s_scan = reinterpret_cast<int64_t*>(s_rowscale + 16);        // [warps][1]
-  int64_t* s_units = s_scan + A8_WARPS;                                 // [2]
-  A8At* s_start = reinterpret_cast<A8At*>(s_units + 2);
+  int64_t* s_scan = reinterpret_cast<int64_t*>(s_rowscale + 16);        // a8_piece's
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
   const int G = a.hq / a.hkv, quad = lane & 3, x8 = lane >> 2;
   pdl_wait();
   if (tid == 0) splits[piece].last = -1;
 
-  // ---- this piece of the line: an item is its tiles and A8_COST more ----
-  const int per = (a.rows + A8_THREADS - 1) / A8_THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
-  auto units_of = [&](const A8Req& r) {  // of one key head
-    int64_t u = 0;
-    for (int k = 0; k < r.blocks; ++k) u += a8_span(a, r, G, k).n + A8_COST;
-    return u;
-  };
-  int64_t mine = 0;
-  for (int b = rb0; b < rb1; ++b) mine += units_of(a8_request(a, G, b, piece == 0)) * a.hkv;
-  int64_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += y;
-  }
-  if (lane == 31) s_scan[warp] = upto;
-  __syncthreads();
-  int64_t before = upto - mine, units = 0;
-  for (int w = 0; w < A8_WARPS; ++w) {
-    if (w < warp) before += s_scan[w];
-    units += s_scan[w];
-  }
-  const int64_t step = max((int64_t)(A8_COST + 1), (units + A8_PIECES - 1) / A8_PIECES);
-  const int64_t w0 = min(units, piece * step), w1 = min(units, w0 + step);
-  if (w0 >= w1) return;  // nobody waits for this block
-  if (w0 >= before && w0 < before + mine) {
-    int64_t at = before;
-    for (int b = rb0; b < rb1; ++b) {
-      const A8Req r = a8_request(a, G, b, false);
-      const int64_t one = units_of(r), all = one * a.hkv;
-      if (w0 >= at && w0 < at + all) {
-        const int h = (int)((w0 - at) / one);
-        int64_t u = at + h * one;
-        for (int k = 0; k < r.blocks; ++k) {
-          const int n = a8_span(a, r, G, k).n + A8_COST;
-          if (w0 < u + n) {
-            *s_start = A8At{b, h, k, (int)max((int64_t)0, w0 - u - A8_COST)};
-            s_units[0] = u;  // where the item begins
-            break;
-          }
-          u += n;
-        }
-        break;
-      }
-      at += all;
-    }
-  }
-  __syncthreads();
-  const int64_t begin = s_units[0];
+  int64_t begin, w1, step;
+  A8At from;
+  if (!a8_piece<A8_ROWS, A8_TILE, A8_THREADS>(a, G, A8_COST, piece, s_scan, from, begin, w1, step)) return;  // nobody waits for this block
 
   // What of an item lies in this piece, from where the item begins on the line: tiles [i0, i1).
   auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, w1 - unit - A8_COST)); };
 
   // ---- the copying side of a warp: a walk of its own, ahead by ST stages ----
-  A8Walk put;
-  put.start(a, G, *s_start);
+  A8Walk<A8_ROWS, A8_TILE> put;
+  put.start(a, G, from);
   int64_t put_unit = begin;
   int put_i = put.at.i, put_i1 = part_end(put_unit, put.s.n);
   bool put_more = true;
@@ -342,8 +366,8 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
   for (int s = 0; s < ST; ++s) copy();
 
   // ---- items ----
-  A8Walk get;
-  get.start(a, G, *s_start);
+  A8Walk<A8_ROWS, A8_TILE> get;
+  get.start(a, G, from);
   int64_t unit = begin;
   int slot = 0;
   const float to_log2 = a.scale * 1.4426950408889634f;
@@ -369,11 +393,8 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
         for (int e = 0; e < N; ++e) most = fmaxf(most, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        // to [2^14, 2^15): 2^(14 - e); a row of zeros, or of values below 2^-100, stays as it is
-        const int e2 = (__float_as_int(most) >> 23) - 127;
-        const int by = e2 < -100 ? 0 : min(14 - e2, 100);
-        const float up = __int_as_float((min(max(by, -120), 120) + 127) << 23);
-        back = __int_as_float((127 - min(max(by, -120), 120)) << 23);
+        float up;
+        a8_row_scale(most, up, back);
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= up;
       }
@@ -669,7 +690,7 @@ __device__ __noinline__ void a8_blank(const Attn8Args& a, int64_t from, int64_t 
 // rows 8 y .. 8 y + 7. And writes the tokens that no item has: those of no request, by all blocks, and those of requests whose
 // lengths are out of range.
 constexpr int A8J_THREADS = 256;
-template <int D, typename T>
+template <int D, int ROWS, typename T>
 __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_constant__ Attn8Args a, const A8Split* splits,
                                                                 const float* partials) {
   pdl_wait();
@@ -685,7 +706,7 @@ __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_co
   if (blockIdx.y == 0) {
     for (int b0 = c + A8_PIECES * (threadIdx.x & ~31); b0 < a.rows; b0 += A8_PIECES * A8J_THREADS) {
       const int b = b0 + A8_PIECES * lane;
-      const bool out = b < a.rows && a.cu[b + 1] > a.cu[b] && a8_request(a, G, b, false).n == 0;
+      const bool out = b < a.rows && a.cu[b + 1] > a.cu[b] && a8_request<ROWS>(a, G, b, false).n == 0;
       for (unsigned rest = __ballot_sync(0xffffffffu, out); rest; rest &= rest - 1) {
         const int r = b0 + A8_PIECES * (__ffs(rest) - 1);
         a8_blank<D, T>(a, max(a.cu[r], 0), min(a.cu[r + 1], a.tokens), lane, 32);
@@ -693,19 +714,19 @@ __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_co
     }
   }
   if (s.last < 0) return;
-  const int row = blockIdx.y * (A8J_THREADS / 32) + (threadIdx.x >> 5), at = s.block * A8_ROWS + row, tok = at / G, t0 = a.cu[s.b];
+  const int row = blockIdx.y * (A8J_THREADS / 32) + (threadIdx.x >> 5), at = s.block * ROWS + row, tok = at / G, t0 = a.cu[s.b];
   if (tok >= a.cu[s.b + 1] - t0) return;
-  const size_t size = a8_partial_floats(D);
+  const size_t size = a8_partial_floats(D, ROWS);
   auto part = [&](int p) { return partials + (p == c ? (size_t)s.first_slot : 2 * (size_t)p) * size; };
   float m = -INFINITY;
-  for (int p = c + lane; p <= s.last; p += 32) m = fmaxf(m, part(p)[A8_ROWS * D + 2 * row]);
+  for (int p = c + lane; p <= s.last; p += 32) m = fmaxf(m, part(p)[ROWS * D + 2 * row]);
   m = warp_max(m);
   float l = 0.f, o[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
   for (int p = c; p <= s.last; ++p) {
     const float* x = part(p);
-    const float2 ml = *reinterpret_cast<const float2*>(x + A8_ROWS * D + 2 * row);
+    const float2 ml = *reinterpret_cast<const float2*>(x + ROWS * D + 2 * row);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
     const float w = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - m);  // -inf with a sum: NaN, which stays
     l += ml.y * w;
