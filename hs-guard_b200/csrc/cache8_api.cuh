@@ -29,7 +29,7 @@ int check_cache8(const hsg_cache8& c, int heads, int dim) {
 
 Cache8 cache8(const hsg_cache8& c) {
   return Cache8{static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_scale, c.v_scale, c.page_stride, c.token_stride,
-                c.head_stride, c.pages, c.page_size, c.block};
+                c.head_stride, c.pages, c.page_size, c.block, c.page_size / c.block, FastDiv::of(c.page_size), FastDiv::of(c.block)};
 }
 
 static_assert(A8_PIECES == SM_COUNT, "one piece an SM");

@@ -317,7 +317,7 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
     put_page = -1;
     const int j = put_base + (lane & 1) * 8;
     put_asked = lane < 2 && j < put.s.hi && (j > put.s.lo - 8 || j < put.s.ahead);
-    if (put_asked) put_page = a.table[put.at.b * a.table_stride + j / a.cache.page];
+    if (put_asked) put_page = a.table[put.at.b * a.table_stride + a.cache.page_div.div(j)];
   };
   settle();
   auto copy = [&]() {
@@ -334,7 +334,7 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
         const int j = put_base + 8 * g;
         pages[g] = page;
         good[g] = page >= 0 && page < c.pages;
-        off[g] = j % c.page;
+        off[g] = j - (int)c.page_div.div(j) * c.page;
         const int64_t at = good[g] ? (int64_t)page * c.page_stride + off[g] * c.token_stride + put.at.h * c.head_stride : 0;
         kb[g] = c.k + at;
         vb[g] = c.v + at;
@@ -353,7 +353,7 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
         const int page = g ? pages[1] : pages[0], from_row = g ? off[1] : off[0];
         const bool there = g ? good[1] : good[0];
         const float* from = lane < 2 ? c.ks : c.vs;
-        const int64_t at = there ? ((int64_t)page * (c.page / c.block) + from_row / c.block) * a.hkv + put.at.h : 0;
+        const int64_t at = there ? ((int64_t)page * c.blocks + c.block_div.div(from_row)) * a.hkv + put.at.h : 0;
         cp_async4(scales_u + (put_slot * 4 + lane) * 4, from + at, there);
       }
       if (++put_slot == ST) put_slot = 0;

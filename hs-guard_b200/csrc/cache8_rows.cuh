@@ -14,6 +14,7 @@
 #include <cuda_fp8.h>
 
 #include "draft_rows.cuh"
+#include "draft_tables.cuh"  // FastDiv
 
 namespace hsg {
 
@@ -23,7 +24,8 @@ struct Cache8 {
   uint8_t *k, *v;
   float *ks, *vs;
   int64_t page_stride, token_stride, head_stride;
-  int pages, page, block;
+  int pages, page, block, blocks;  // blocks of a page
+  FastDiv page_div, block_div;
 };
 
 struct Append8Args {

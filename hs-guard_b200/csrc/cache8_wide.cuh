@@ -5,8 +5,7 @@
 // can see are an item; all items are one line, cut into equal pieces, one a thread block. Per tile S = Q K^T (TMEM), softmax with
 // a running maximum in registers (a row a thread), P in fp16 over S in TMEM, O += P V (A = P from TMEM, B = V, N-major).
 //
-// Codes become fp16 on the way into shared memory, which is exact: four warps read a tile's codes from global memory into
-// registers while the tile before is at work, convert them and write them in the swizzled layout of the products. (e4m3
+// Codes become fp16 on the way into shared memory, which is exact. (e4m3
 // products could take the codes as they are, but a bf16 query is two e4m3 numbers and an fp16 query or weight three: as much or
 // more product time, and the softmax would have to split its weights.) Keys that the item cannot see are written as zeros and not
 // read. A NaN of V in a tile that not every row sees alike is written as zero as well, and put back for the rows that see it at
@@ -18,7 +17,7 @@
 //   1      S, up to NS tiles ahead of P V;  2: P V
 //   4-7    softmax of even tiles, 8-11 of odd ones, one handing the rows' maxima on to the other before its exponentials;
 //          whichever has an item's last tile writes the result
-//   12-15  K and V tiles
+//   12-15  K and V tiles: four warps copy codes three tiles of K or V ahead and convert them
 // A K or V tile lies in shared memory as [8 keys][dim / 64][8][128 B], 128-byte swizzle.
 //
 // A wait tells a barrier's phase from its neighbours only. S, P and P V of tile g use barrier g % NS, maxima that of their group
@@ -40,11 +39,13 @@ constexpr int W8_COPY = 128;       // threads that bring K and V
 
 __host__ __device__ constexpr int w8_tile(int dim) { return dim == 256 ? 64 : 128; }
 __host__ __device__ constexpr int w8_scores(int dim) { return dim == 256 ? 4 : 3; }
-__host__ __device__ constexpr int w8_q_bufs(int dim) { return dim == 256 ? 1 : 2; }
-__host__ __device__ constexpr int w8_bufs(int dim) { return dim == 64 ? 3 : 2; }  // of K, and of V
+__host__ __device__ constexpr int w8_q_bufs(int dim) { return dim == 64 ? 2 : 1; }
+__host__ __device__ constexpr int w8_k_bufs(int dim) { return dim == 64 ? 3 : 2; }
+__host__ __device__ constexpr int w8_v_bufs(int dim) { return dim == 64 ? 3 : dim == 128 ? 2 : 1; }
 __host__ __device__ constexpr int w8_buffer(int dim) { return w8_tile(dim) * dim * 2; }
 __host__ __device__ constexpr int w8_smem(int dim) {
-  return 1024 + w8_q_bufs(dim) * W8_ROWS * dim * 2 + 2 * w8_bufs(dim) * w8_buffer(dim) + 10240;
+  return 1024 + w8_q_bufs(dim) * W8_ROWS * dim * 2 + (w8_k_bufs(dim) + w8_v_bufs(dim)) * w8_buffer(dim) +
+         3 * w8_tile(dim) * dim + 9216;
 }
 
 struct W8Item {
@@ -105,7 +106,7 @@ __device__ __noinline__ void w8_restore(const Attn8Args& a, const W8Item& it, in
 template <int D, typename T>
 __global__ void __launch_bounds__(W8_THREADS, 1)
 attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partials) {
-  constexpr int KT = w8_tile(D), NC = D / 64, BUF = w8_buffer(D), NS = w8_scores(D), QB = w8_q_bufs(D), NB = w8_bufs(D);
+  constexpr int KT = w8_tile(D), NC = D / 64, BUF = w8_buffer(D), NS = w8_scores(D), QB = w8_q_bufs(D), NB = w8_k_bufs(D), NBV = w8_v_bufs(D);
   constexpr int Q_BUF = W8_ROWS * D * 2, Q_BOX = W8_ROWS * 128, GROUPS = KT / 8;
   constexpr uint32_t O_COL = NS * KT;
   static_assert(O_COL + D <= 512, "S buffers and O fill TMEM");
@@ -114,8 +115,9 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(w8_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* qs = smem;                            // [QB][NC][128 rows][128 B], SW128
   uint8_t* ks = qs + QB * Q_BUF;                 // [NB][KT / 8][NC][8][128 B], SW128
-  uint8_t* vs = ks + NB * BUF;                   // [NB], likewise
-  float4* group_scales = reinterpret_cast<float4*>(vs + NB * BUF);  // [8][GROUPS] K scale, log2 and reciprocal of V's
+  uint8_t* vs = ks + NB * BUF;                   // [NBV], likewise
+  uint8_t* codes = vs + NBV * BUF;               // [3][pieces a thread][128 threads][16 B]
+  float4* group_scales = reinterpret_cast<float4*>(codes + 3 * KT * D);  // [8][GROUPS] K scale, log2 and reciprocal of V's
   float* row_scale = reinterpret_cast<float*>(group_scales + W8_PLACES * 16);  // [2][128] of even / odd items
   float2* ml_rows = reinterpret_cast<float2*>(row_scale + 256);     // [2][128] (m, l) of the group without the last tile
   float* m_rows = reinterpret_cast<float*>(ml_rows + 256);          // [2][128] maxima after even / odd tiles
@@ -144,6 +146,8 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
   int* poison = reinterpret_cast<int*>(tmem_slot + 2);              // [4] of item & 3: item + 1 if a NaN of V was zeroed
   uint32_t* k_info = reinterpret_cast<uint32_t*>(poison + 4);       // [NB], [NB] bit 0: first of its item here, 1: last, 2: the piece's last
   uint32_t* v_info = k_info + 3;
+  uint32_t* tile_info = v_info + 3;                                 // [4 warps][4] likewise, and bit 3: keys that not all rows see, 4-19: item
+  float* raw_scales = reinterpret_cast<float*>(tile_info + 16);     // [4][K 16, V 16]
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
   const int G = a.hq / a.hkv;
@@ -172,115 +176,109 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
   auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, w1 - unit - W8_COST)); };
 
   if (warp >= 12) {
-    // ---- K and V: each thread the same 16 bytes of every few keys ----
-    constexpr int PIECES = D / 16, STRIDE = W8_COPY / PIECES, N = KT / STRIDE;  // keys apart, pieces a thread
-    const int me = tid - 384, ch = me % PIECES, key0 = me / PIECES;
+    // ---- K and V in turn. A thread copies 16-byte pieces of codes into places of its own (cp.async), three tiles of K or V
+    // ahead, and converts what it copied itself, so that only the products wait for other threads' work. ----
+    constexpr int PIECES = D / 16, AT_ONCE = 32 / PIECES, STRIDE = 4 * AT_ONCE, N = KT / STRIDE;  // keys a warp, all; pieces a thread
+    static_assert(STRIDE % 8 == 0, "a thread's keys have one place among eight");
+    const int me = tid - 384, wc = warp - 12;
+    // eight lanes take four pieces of two keys: written, they meet no bank twice
+    const int ch = (lane & 3) + 4 * ((lane >> 3) % (PIECES / 4));
+    const int key0 = wc * AT_ONCE + ((lane >> 2) & 1) + 2 * ((lane >> 3) / (PIECES / 4));
+    const uint32_t at0 = da_offset<NC>(key0, 2 * ch), at1 = da_offset<NC>(key0, 2 * ch + 1);
     const Cache8& c = a.cache;
+    const int64_t own = (key0 & 7) * c.token_stride + ch * 16;
+    uint8_t* my_codes = codes + me * 16;
     A8Walk<W8_ROWS, KT> walk;
     walk.start(a, G, from);
     int64_t unit = begin;
     int i = walk.at.i, i1 = part_end(unit, walk.s.n), item = 0;
-    // the next tile's pages, and where in the pages its keys begin: lane l has that of keys 8 l .. 8 l + 7; -1: not asked for
-    int page = -1, within = 0;
-    int64_t start = 0;
+    // the walk's tile: lane l has the page of keys 8 l .. 8 l + 7, which is asked for a tile before it is needed
+    bool more = true, asked = false;
+    int page = 0, within = 0;
     auto ask = [&]() {
       const int j = walk.base(i) + 8 * lane;
-      page = -1;
-      if (lane < GROUPS && j < walk.s.hi && (j > walk.s.lo - 8 || j < walk.s.ahead)) {
-        const int p = j / c.page;
-        page = a.table[walk.at.b * a.table_stride + p];
-        if (page < 0 || page >= c.pages) {
-          set_error(a.err, ERR_BAD_PAGE);
-          page = -1;
-        }
+      asked = lane < GROUPS && j < walk.s.hi && (j > walk.s.lo - 8 || j < walk.s.ahead);
+      if (asked) {
+        const int p = c.page_div.div(j);
         within = j - p * c.page;
-        start = (int64_t)page * c.page_stride + within * c.token_stride + walk.at.h * c.head_stride;
+        page = a.table[walk.at.b * a.table_stride + p];
       }
     };
-    auto fetch = [&](const uint8_t* codes, uint4 (&x)[N]) {
-      const int base = walk.base(i);
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int k = key0 + n * STRIDE, j = base + k;
-        const int pg = __shfl_sync(0xffffffffu, page, k >> 3);
-        const int64_t at = __shfl_sync(0xffffffffu, start, k >> 3);
-        x[n] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg >= 0 && j < walk.s.hi && (j >= walk.s.lo || j < walk.s.ahead))
-          x[n] = *reinterpret_cast<const uint4*>(codes + at + (k & 7) * c.token_stride + ch * 16);
-      }
-    };
-    auto put = [&](uint8_t* buf, const uint4 (&x)[N]) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int k = key0 + n * STRIDE;
-        const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-        uint32_t y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] = f8_half2(w[e] & 0xffffu);
-          y[2 * e + 1] = f8_half2(w[e] >> 16);
-        }
-        // lanes of the upper 64 dims write their pieces the other way round: banks
-        const int flip = ch >> 2 & 1;
-        const uint4 p0 = make_uint4(y[0], y[1], y[2], y[3]), p1 = make_uint4(y[4], y[5], y[6], y[7]);
-        *reinterpret_cast<uint4*>(buf + da_offset<NC>(k, 2 * ch + flip)) = flip ? p1 : p0;
-        *reinterpret_cast<uint4*>(buf + da_offset<NC>(k, 2 * ch + 1 - flip)) = flip ? p0 : p1;
-      }
-    };
-    uint4 kr[N], vr[N];
     ask();
-    fetch(c.k, kr);
-    DaRing ring;
-    for (int g = 0;; ++g) {
-      fetch(c.v, vr);
-      // this tile's scales, by the first of the four warps
-      float ksc = 0.f, vsc = 1.f;
-      if (warp == 12 && lane < GROUPS && page >= 0) {
-        const int64_t at = ((int64_t)page * (c.page / c.block) + within / c.block) * a.hkv + walk.at.h;
-        ksc = c.ks[at];
-        vsc = c.vs[at];
-      }
-      const int base = walk.base(i), old = walk.r.len - walk.r.n;
-      const int sure = a.mask ? old : old + walk.at.block * W8_ROWS / G + 1;
-      // (with a window, where rows differ is said by the item; here any tile that may hold such keys counts)
-      const bool mixed = base > sure - KT || a.window;
-      const bool first = g == 0 || i == 0;
-      const int this_item = item;
-      // on to the next tile
-      bool more = true;
-      uint32_t what = first ? 1u : 0u;
-      if (++i >= i1) {
-        what |= 2u;
-        unit += walk.s.n + W8_COST;
-        ++item;
-        if (unit + W8_COST >= w1) {
+    int64_t start = -1;  // where those keys begin in the pages; < 0: nowhere
+    int base = 0, hi = 0, lo = 0, ahead = 0;  // of the tile that is being copied
+    auto copy = [&](int b) {  // b even: K of the walk's tile, odd: V, and on to the next
+      if (more) {
+        if (!(b & 1)) {
+          const bool good = asked && page >= 0 && page < c.pages;
+          if (asked && !good) set_error(a.err, ERR_BAD_PAGE);
+          start = good ? (int64_t)page * c.page_stride + within * c.token_stride + walk.at.h * c.head_stride : -1;
+          base = walk.base(i);
+          hi = walk.s.hi;
+          lo = walk.s.lo;
+          ahead = walk.s.ahead;
+          if (wc == 0 && lane < GROUPS) {
+            const int64_t at = good ? ((int64_t)page * c.blocks + c.block_div.div(within)) * a.hkv + walk.at.h : 0;
+            const uint32_t to = smem_u32(raw_scales + (b / 2 % 4) * 32 + lane);
+            cp_async4(to, c.ks + at, good);
+            cp_async4(to + 64, c.vs + at, good);
+          }
+          const int old = walk.r.len - walk.r.n, sure = a.mask ? old : old + walk.at.block * W8_ROWS / G + 1;
+          uint32_t what = (b == 0 || i == 0 ? 1u : 0u) | (base > sure - KT || a.window ? 8u : 0u) | (uint32_t)(item & 0xffff) << 4;
+          if (++i >= i1) {
+            what |= 2u;
+            unit += walk.s.n + W8_COST;
+            ++item;
+            if (unit + W8_COST >= w1) {
+              what |= 4u;
+            } else {
+              walk.next_item(a, G);
+              i = 0;
+              i1 = part_end(unit, walk.s.n);
+            }
+          }
+          if (lane == 0) tile_info[wc * 4 + b / 2 % 4] = what;
+          if (!(what & 4u)) ask();
+          else i = -1;
+        } else if (i < 0) {
           more = false;
-          what |= 4u;
-        } else {
-          walk.next_item(a, G);
-          i = 0;
-          i1 = part_end(unit, walk.s.n);
         }
-      }
-      if (more) ask();
-      if (g >= NB) ok = __all_sync(0xffffffffu, da_wait(&k_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
-      if (!ok) break;
-      put(ks + ring.at * BUF, kr);
-      if (me == 0) k_info[ring.at] = what;
-      if (warp == 12) {
-        const float v = vsc != vsc ? vsc : fminf(fmaxf(vsc, 0x1p-100f), 0x1p120f);
-        if (lane < GROUPS) group_scales[(g % W8_PLACES) * 16 + lane] = make_float4(ksc, __log2f(v), 1.0f / v, 0.f);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[ring.at]);
-      if (warp == 12 && lane == 0) mbar_arrive(&sc_full[g % W8_PLACES]);
-      if (more) fetch(c.k, kr);
-      if (mixed) {
-        uint32_t bad = 0;
+        const uint8_t* from_codes = (b & 1 ? c.v : c.k) + own;
+        const uint32_t to = smem_u32(my_codes + (b % 3) * (KT * D));
+        const bool whole = base >= lo && base <= hi - KT;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&vr[n]);
+          const int k = key0 + n * STRIDE, j = base + k;
+          const int64_t at = __shfl_sync(0xffffffffu, start, k >> 3);
+          const bool there = at >= 0 && (whole || (j < hi && (j >= lo || j < ahead)));
+          cp_async16(to + n * (W8_COPY * 16), there ? from_codes + at : c.k, there);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int b = 0; b < 3; ++b) copy(b);
+    DaRing ring;
+#pragma unroll 1
+    for (int b = 0;; ++b) {
+      const bool is_v = b & 1;
+      const int g = b >> 1;
+      cp_async_wait<2>();
+      __syncwarp();
+      const uint32_t what = tile_info[wc * 4 + g % 4];
+      const int nb = is_v ? NBV : NB, slot = g % nb;
+      if (g >= nb)
+        ok = __all_sync(0xffffffffu, da_wait(&(is_v ? v_empty : k_empty)[slot], (g / nb - 1) & 1, a.err, ERR_TIMEOUT_MMA));
+      if (!ok) break;
+      uint8_t* to = (is_v ? vs : ks) + slot * BUF;
+      const uint8_t* x = my_codes + (b % 3) * (KT * D);
+      uint32_t bad = 0;
+      const bool mend = is_v && (what & 8u);
+#pragma unroll 4
+      for (int n = 0; n < N; ++n) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + n * (W8_COPY * 16));
+        uint32_t w[4] = {v.x, v.y, v.z, v.w}, y[8];
+        if (mend) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t hit = (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
@@ -288,24 +286,37 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
             w[e] &= ~(hit * 0xffu);
           }
         }
-        if (bad) poison[this_item & 3] = this_item + 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = f8_half2(w[e] & 0xffffu);
+          y[2 * e + 1] = f8_half2(w[e] >> 16);
+        }
+        *reinterpret_cast<uint4*>(to + at0 + n * (STRIDE / 8 * NC * 1024)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(to + at1 + n * (STRIDE / 8 * NC * 1024)) = make_uint4(y[4], y[5], y[6], y[7]);
       }
-      if (g >= NB) ok = __all_sync(0xffffffffu, da_wait(&v_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
-      if (!ok) break;
-      put(vs + ring.at * BUF, vr);
-      if (me == 0) v_info[ring.at] = what;
+      const int it = (int)(what >> 4 & 0xffff);
+      if (bad) poison[it & 3] = it + 1;
+      if (me == 0) (is_v ? v_info : k_info)[slot] = what;
+      if (!is_v && wc == 0 && lane < GROUPS) {
+        // scales of 0 or beyond what append_8bit writes are taken as the nearest that it would write
+        const float* raw = raw_scales + (g % 4) * 32 + lane;
+        const float v = fminf(fmaxf(raw[16], 0x1p-100f), 0x1p120f);
+        group_scales[(g % W8_PLACES) * 16 + lane] = make_float4(raw[0], __log2f(v), 1.0f / v, 0.f);
+      }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&v_full[ring.at]);
-        mbar_arrive(&v_seen[g % W8_PLACES]);
+        mbar_arrive(&(is_v ? v_full : k_full)[slot]);
+        if (is_v) mbar_arrive(&v_seen[g % W8_PLACES]);
+        else if (wc == 0) mbar_arrive(&sc_full[g % W8_PLACES]);
       }
-      ring.next(NB);
-      if (!more) break;
+      if (is_v && (what & 4u)) break;
+      copy(b + 3);
     }
+    cp_async_wait<0>();
   } else if (warp == 0 || warp == 3) {
     // ---- queries: LPR lanes a row, 16 bytes each; and what each item is ----
-    constexpr int LPR = D / 8, RPW = 32 / LPR, N = W8_ROWS / 2 / RPW, LIVE = N < 8 ? N : 8;
+    constexpr int LPR = D / 8, RPW = 32 / LPR, N = W8_ROWS / 2 / RPW, LIVE = 16;
     A8Walk<W8_ROWS, KT> walk;
     walk.start(a, G, from);
     int64_t unit = begin;
@@ -314,9 +325,6 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
     for (int item = 0;; ++item) {
       const int i0 = walk.at.i, i1 = part_end(unit, walk.s.n), row0 = walk.at.block * W8_ROWS;
       const bool end = unit + walk.s.n + 2 * W8_COST >= w1;
-      if (item >= 2) ok = __all_sync(0xffffffffu, da_wait(&item_empty[item & 1], ((item >> 1) - 1) & 1, a.err, ERR_TIMEOUT_MMA));
-      if (ok && item >= QB) ok = __all_sync(0xffffffffu, da_wait(&q_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
-      if (!ok) break;
       uint8_t* q = qs + ring.at * Q_BUF;
 #pragma unroll 1
       for (int n0 = 0; n0 < N; n0 += LIVE) {
@@ -328,6 +336,11 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
           if (t < walk.r.n)
             x[n] = *reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(walk.r.t0 + t) * a.q_ts +
                                                    (int64_t)(walk.at.h * G + at - t * G) * a.q_hs + ch * 8);
+        }
+        if (n0 == 0) {  // the first rows are on their way
+          if (item >= 2) ok = __all_sync(0xffffffffu, da_wait(&item_empty[item & 1], ((item >> 1) - 1) & 1, a.err, ERR_TIMEOUT_MMA));
+          if (ok && item >= QB) ok = __all_sync(0xffffffffu, da_wait(&q_empty[ring.at], ring.phase ^ 1u, a.err, ERR_TIMEOUT_MMA));
+          if (!ok) break;
         }
 #pragma unroll
         for (int n = 0; n < LIVE; ++n) {
@@ -354,6 +367,7 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
           if (ch == 0) row_scale[(item & 1) * W8_ROWS + row] = back * a.scale * 1.4426950408889634f;
         }
       }
+      if (!ok) break;
       if (warp == 3) {
         const int old = walk.r.len - walk.r.n;
         int lows = -1;
@@ -436,7 +450,7 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
         mma_commit(&v_empty[ring.at]);
       }
       __syncwarp();
-      ring.next(NB);
+      ring.next(NBV);
       p_ring.next(NS);
       if (what & 4) break;
     }
@@ -494,8 +508,7 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
 #pragma unroll
               for (int j = 1; j < 8; ++j) t = fmaxf(t, __uint_as_float(x[8 * e + j]));
               const float4 s = sc[4 * c + e];
-              const float y = fmaf(t, rs * s.x, s.y);
-              top = fmaxf(top, t == -INFINITY ? t : y);
+              top = fmaxf(top, fmaf(t, fmaxf(rs * s.x, 0x1p-126f), s.y));  // (-inf times 0 would not be -inf)
             }
           }
           if (special) tmem_st_wait();
@@ -540,22 +553,17 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
             da_pin(x);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float2 mul = make_float2(rs * s[e].x, rs * s[e].x), off = make_float2(s[e].y + less, s[e].y + less);
+              const float by = fmaxf(rs * s[e].x, 0x1p-126f);
+              const float2 mul = make_float2(by, by), off = make_float2(s[e].y + less, s[e].y + less);
               float2 sum = make_float2(0.f, 0.f);
-              bool none = special;  // a block that the row sees nothing of must not count by its scales either
 #pragma unroll
               for (int j = 8 * e; j < 8 * e + 8; j += 2) {
                 float2 y = fma2(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), mul, off);
                 y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                if (special) {
-                  if (x[j] == 0xff800000u) y.x = 0.f;
-                  if (x[j + 1] == 0xff800000u) y.y = 0.f;
-                  none = none && x[j] == 0xff800000u && x[j + 1] == 0xff800000u;
-                }
                 sum = add2(sum, y);
                 pk[j >> 1] = pack_half2(y.x, y.y);
               }
-              if (!none) l = fmaf(sum.x + sum.y, s[e].z, l);
+              l = fmaf(sum.x + sum.y, s[e].z, l);
             }
             tmem_st16_async(s_col + 16 * c, pk);  // over scores that have been read
           }
@@ -587,7 +595,7 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
       }
       if (ok) ok = da_wait(&pv_done[last % NS], (last / NS) & 1, a.err, ERR_TIMEOUT_MMA);
       tc_fence_after();
-      const bool mend = *(volatile int*)&poison[item & 3] == item + 1;
+      const bool mend = *(volatile int*)&poison[item & 3] == (item & 0xffff) + 1;
       const bool whole = i0 == 0 && i1 == it.s.n;
       const int slot = 2 * piece + (item > 0 ? 1 : 0), h = it.h;
       float* part = partials + slot * a8_partial_floats(D, W8_ROWS);
