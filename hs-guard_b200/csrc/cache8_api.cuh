@@ -32,7 +32,7 @@ Cache8 cache8(const hsg_cache8& c) {
                 c.head_stride, c.pages, c.page_size, c.block, c.page_size / c.block, FastDiv::of(c.page_size), FastDiv::of(c.block)};
 }
 
-static_assert(A8_PIECES == SM_COUNT, "one piece an SM");
+static_assert(A8_BLOCKS == SM_COUNT, "one piece an SM");
 constexpr int A8_WIDE_ROWS = 32;  // rows of a key head up to which warp-level products are taken
 
 template <int D, typename T>
@@ -50,23 +50,49 @@ int launch_append8_dim(const Append8Args& p, int dim, cudaStream_t st) {
   return dim == 64 ? launch_append8<64, T>(p, st) : dim == 128 ? launch_append8<128, T>(p, st) : launch_append8<256, T>(p, st);
 }
 
+// Tensor map of a cache's codes: `keys` tokens of one page and head a box, blocks of 128 bytes a token (64 at head dim 64), all
+// `cols` of them.
+int make_codes_map(CUtensorMap* map, const uint8_t* base, const Cache8& c, int dim, int heads, int keys, int cols) {
+  if (get_encoder() != HSG_OK) return HSG_ERR_CUDA;
+  const int wide = std::min(dim, 128);
+  const cuuint64_t dims[5] = {(cuuint64_t)wide, (cuuint64_t)c.page, (cuuint64_t)(dim / wide), (cuuint64_t)heads, (cuuint64_t)c.pages};
+  // a stride whose dimension has one element is never used, but the encoder wants a valid one
+  const cuuint64_t strides[4] = {(cuuint64_t)c.token_stride, 128, (cuuint64_t)(heads > 1 ? c.head_stride : 128),
+                                 (cuuint64_t)(c.pages > 1 ? c.page_stride : 128)};
+  const cuuint32_t box[5] = {(cuuint32_t)wide, (cuuint32_t)keys, (cuuint32_t)cols, 1, 1}, one[5] = {1, 1, 1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<uint8_t*>(base), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (codes) failed (%d)", (int)r);
+  return HSG_OK;
+}
+
 template <int D, typename T>
 int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   A8Split* splits = static_cast<A8Split*>(workspace);
-  float* partials = reinterpret_cast<float*>(splits + A8_PIECES);
   // rows of a key head, as far as the host can tell: no request has more than max_new tokens, all have `tokens` together
   const int64_t rows = std::min<int64_t>(p.max_new, (p.tokens + p.rows - 1) / p.rows) * (p.hq / p.hkv);
   if (rows > A8_WIDE_ROWS) {
+    float* partials = reinterpret_cast<float*>(splits + A8_BLOCKS);
     CU(cudaFuncSetAttribute(attn8_wide_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, w8_smem(D)));
-    CU(launch_k(attn8_wide_kernel<D, T>, dim3(A8_PIECES), dim3(W8_THREADS), w8_smem(D), st, true, p, splits, partials));
-    CU(launch_k(attn8_join_kernel<D, W8_ROWS, T>, dim3(A8_PIECES, W8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
+    CU(launch_k(attn8_wide_kernel<D, T>, dim3(A8_BLOCKS), dim3(W8_THREADS), w8_smem(D), st, true, p, splits, partials));
+    CU(launch_k(attn8_join_kernel<D, W8_ROWS, T>, dim3(A8_BLOCKS, W8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
                 (const A8Split*)splits, (const float*)partials));
     return HSG_OK;
   }
+  constexpr int PIECES = A8_BLOCKS * A8_WARPS;
+  float* partials = reinterpret_cast<float*>(splits + PIECES);
+  const int box = p.cache.page % A8_SLICE == 0 ? A8_SLICE : 8, cols = D == 256 && box == A8_SLICE ? 2 : 1;
+  CUtensorMap k, v;
+  int rc;
+  if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||
+      (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
+    return rc;
   CU(cudaFuncSetAttribute(attn8_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
-  CU(launch_k(attn8_kernel<D, T>, dim3(A8_PIECES), dim3(A8_THREADS), a8_smem(D), st, true, p, splits, partials));
-  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3(A8_PIECES, A8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
-              (const A8Split*)splits, (const float*)partials));
+  CU(launch_k(attn8_kernel<D, T>, dim3(A8_BLOCKS), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box, splits, partials));
+  const int64_t most = std::min<int64_t>(A8_ROWS, (int64_t)p.max_new * (p.hq / p.hkv));  // rows of an item
+  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3(PIECES, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),
+              dim3(A8J_THREADS), 0, st, true, p, (const A8Split*)splits, (const float*)partials));
   return HSG_OK;
 }
 template <typename T>
@@ -111,7 +137,7 @@ extern "C" int hsg_append8(const hsg_append8_args* a) {
   return a->dtype == HSG_DT_F16 ? launch_append8_dim<__half>(p, a->dim, st) : launch_append8_dim<__nv_bfloat16>(p, a->dim, st);
 }
 
-extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? a8_workspace_bytes(head_dim, W8_ROWS) : 0; }
+extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? std::max(a8_workspace_bytes(head_dim, A8_WARPS, A8_ROWS), a8_workspace_bytes(head_dim, 1, W8_ROWS)) : 0; }
 
 extern "C" int hsg_attention8(const hsg_attention8_args* a) {
   DRAFT_ARGS(a);

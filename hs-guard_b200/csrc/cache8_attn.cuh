@@ -33,11 +33,11 @@ struct Attn8Args {
 
 // This kernel is for few rows a key head, where reading the cache is all that counts; products are warp-level (16 rows by 8
 // keys by 16 dims), since the 128 rows of a tcgen05 product would be padding. A request's rows of a key head, row r = (token
-// r / G, query head r % G), in blocks of 16, and the 128-key tiles that such a block can see are an item; all items are one
-// line that is cut into equal pieces, one a thread block, as the 16-bit attention does. Warp w of a block takes keys
-// 16 w .. 16 w + 15 of each tile of its piece: it copies them into its own ring of stages (cp.async, 16 bytes a lane; keys
-// outside what the item can see are filled with zeros and not read), and keeps its own running maximum, sums and
-// accumulators, so warps meet only at an item's end.
+// r / G, query head r % G), in blocks of 16, and the slices of 16 keys that such a block can see are an item; all items are one
+// line that is cut into equal pieces, one a warp, eight warps an SM, whatever the requests' lengths. Warps do not meet: each has
+// its ring of slices, which it fills itself ahead of its use (TMA, one box of 16 keys, or two of 8 where pages divide into nothing
+// longer), its own running maximum, sums and accumulators. An item that lies in one piece is written out; of one that is cut, each
+// piece leaves its sums in the workspace, and attn8_join_kernel joins them in piece order, so results do not depend on timing.
 //
 // Codes become fp16 exactly in registers. Queries are fp16 as well: an fp16 q as it is, a bf16 q times a power of two for
 // each row that brings its largest element to 2^14 (what then falls below fp16's range is under 2^-38 of it). A V scale would
@@ -45,31 +45,34 @@ struct Attn8Args {
 // that sum, so that weights use fp16's range however the scales differ, and the row sum takes w_j / vs_j. Weights are rounded to
 // fp16 (2^-11, the largest between 2^11 and 2^15, as in the 16-bit attention); sums, maxima and accumulators are fp32.
 //
-// The order of dims within a product is free as long as both factors agree: a lane reads 16 consecutive bytes of a key, which
-// are its elements of four steps of 16 dims, and for P V consecutive dims of two keys, interleaved bytewise.
+// The order of dims and keys within a product is free as long as both factors agree: a lane reads 16 consecutive bytes of a key,
+// which are its elements of four steps of 16 dims, and for P V consecutive dims of two keys, interleaved bytewise. Which keys
+// (a8_key) and which dims (a8_piece_of) a lane takes is chosen so that reading the swizzled slices meets no bank twice at head dims
+// 128 and 256 (twice at 64, for V).
 constexpr int A8_THREADS = 256;
 constexpr int A8_WARPS = 8;
 constexpr int A8_ROWS = 16;
-constexpr int A8_TILE = 128;        // keys: 16 a warp
-constexpr int A8_PIECES = 148;      // one thread block an SM
-constexpr int A8_COST = 2;          // what an item costs besides its tiles, in tiles
-constexpr int A8_RING = 24576;      // bytes of a warp's ring
+constexpr int A8_SLICE = 16;        // keys
+constexpr int A8_BLOCKS = 148;      // one thread block an SM
+constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
 constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
 
-__host__ __device__ constexpr int a8_stage(int dim) { return 2 * 16 * dim; }
-__host__ __device__ constexpr int a8_stages(int dim) { return A8_RING / a8_stage(dim); }
-// rings, scales, query fragments, accumulators, maxima and sums
+__host__ __device__ constexpr int a8_stage(int dim) { return 2 * A8_SLICE * dim; }
+__host__ __device__ constexpr int a8_stages(int dim) { return dim == 64 ? 12 : dim == 128 ? 6 : 2; }
+__host__ __device__ constexpr int a8_q_bytes(int dim) { return dim == 256 ? A8_ROWS * dim * 2 : 0; }  // else in registers
+// a warp's ring, query fragments, scales and barriers; where the pieces begin
 __host__ __device__ constexpr int a8_smem(int dim) {
-  return A8_WARPS * (A8_RING + a8_stages(dim) * 16) + A8_ROWS * dim * 2 + A8_ROWS * dim * 4 + 4096;
+  return 1024 + A8_WARPS * (a8_stages(dim) * (a8_stage(dim) + 24) + a8_q_bytes(dim)) + 1024;
 }
-__host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows = A8_ROWS) { return (size_t)rows * (dim + 2); }
+__host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
 struct A8Split {  // an item that begins in a piece and ends in a later one
   int b, h, block, last;
   int first_slot;
   int pad[3];
 };
-__host__ __device__ constexpr size_t a8_workspace_bytes(int dim, int rows) {
-  return A8_PIECES * sizeof(A8Split) + 2 * A8_PIECES * a8_partial_floats(dim, rows) * sizeof(float);
+// `subs` pieces a thread block, of blocks of `rows` rows
+__host__ __device__ constexpr size_t a8_workspace_bytes(int dim, int subs, int rows) {
+  return A8_BLOCKS * subs * (sizeof(A8Split) + 2 * a8_partial_floats(dim, rows) * sizeof(float));
 }
 
 // A request, its rows in blocks of ROWS; n = 0 if its lengths are out of range.
@@ -148,12 +151,16 @@ struct A8Walk {
   __device__ __forceinline__ int base(int tile) const { return (tile < s.lead ? tile : s.first + tile - s.lead) * TILE; }
 };
 
-// Where a thread block's piece of the line begins: item and tile (`from`), where that item begins on the line (`begin`), where the
-// piece ends (w1) and how long pieces are (step). An item is its tiles and `cost` more; a piece holds at least one tile. Every
-// thread of the block calls it, with room for THREADS / 32 + 3 numbers; false: nothing is left for this piece.
-template <int ROWS, int TILE, int THREADS>
-__device__ __forceinline__ bool a8_piece(const Attn8Args& a, int G, int cost, int piece, int64_t* room, A8At& from, int64_t& begin,
-                                         int64_t& w1, int64_t& step) {
+// A piece of the line: where it begins (item and tile), where that item begins on the line, and where the piece ends. An item is
+// its tiles and `cost` more; a piece holds at least one tile, or nothing (b < 0).
+struct A8Lot {
+  A8At from;
+  int64_t begin, end;
+};
+// The pieces of a thread block, SUBS of them: piece s * A8_BLOCKS + block. Every thread of the block calls it, with room for
+// THREADS / 32 numbers. Returns how long pieces are.
+template <int ROWS, int TILE, int THREADS, int SUBS>
+__device__ __forceinline__ int64_t a8_lots(const Attn8Args& a, int G, int cost, int block, int64_t* room, A8Lot* lots) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (a.rows + THREADS - 1) / THREADS, rb0 = min(a.rows, tid * per), rb1 = min(a.rows, rb0 + per);
   auto units_of = [&](const A8Req& r) {  // of one key head
@@ -162,7 +169,7 @@ __device__ __forceinline__ bool a8_piece(const Attn8Args& a, int G, int cost, in
     return u;
   };
   int64_t mine = 0;
-  for (int b = rb0; b < rb1; ++b) mine += units_of(a8_request<ROWS>(a, G, b, piece == 0)) * a.hkv;
+  for (int b = rb0; b < rb1; ++b) mine += units_of(a8_request<ROWS>(a, G, b, block == 0)) * a.hkv;
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -170,44 +177,40 @@ __device__ __forceinline__ bool a8_piece(const Attn8Args& a, int G, int cost, in
     if (lane >= o) upto += y;
   }
   if (lane == 31) room[warp] = upto;
+  if (tid < SUBS) lots[tid].from.b = -1;
   __syncthreads();
   int64_t before = upto - mine, units = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += room[w];
     units += room[w];
   }
-  step = max((int64_t)(cost + 1), (units + A8_PIECES - 1) / A8_PIECES);
-  const int64_t w0 = min(units, piece * step);
-  w1 = min(units, w0 + step);
-  if (w0 >= w1) return false;
-  int64_t* found = room + THREADS / 32;
-  A8At* at_found = reinterpret_cast<A8At*>(found + 1);
-  if (w0 >= before && w0 < before + mine) {
+  const int64_t step = max((int64_t)(cost + 1), (units + SUBS * A8_BLOCKS - 1) / (SUBS * A8_BLOCKS));
+  // the first piece of this block that begins at or after this thread's first unit
+  int64_t s0 = before > block * step ? ((before + step - 1) / step - block + A8_BLOCKS - 1) / A8_BLOCKS : 0;
+  if (mine > 0 && s0 < SUBS && (s0 * A8_BLOCKS + block) * step < before + mine) {
     int64_t at = before;
     for (int b = rb0; b < rb1; ++b) {
       const A8Req r = a8_request<ROWS>(a, G, b, false);
       const int64_t one = units_of(r), all = one * a.hkv;
-      if (w0 >= at && w0 < at + all) {
+      for (; s0 < SUBS; ++s0) {
+        const int64_t w0 = (s0 * A8_BLOCKS + block) * step;
+        if (w0 >= at + all) break;
         const int h = (int)((w0 - at) / one);
         int64_t u = at + h * one;
         for (int k = 0; k < r.blocks; ++k) {
           const int n = a8_span<ROWS, TILE>(a, r, G, k).n + cost;
           if (w0 < u + n) {
-            *at_found = A8At{b, h, k, (int)max((int64_t)0, w0 - u - cost)};
-            *found = u;
+            lots[s0] = A8Lot{A8At{b, h, k, (int)max((int64_t)0, w0 - u - cost)}, u, min(units, w0 + step)};
             break;
           }
           u += n;
         }
-        break;
       }
       at += all;
     }
   }
   __syncthreads();
-  from = *at_found;
-  begin = *found;
-  return true;
+  return step;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
@@ -219,15 +222,14 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool th
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Byte offset of 16-byte piece ch of key k of a warp's 16 keys, so that neither way of reading meets a bank twice: K by
-// (key n, piece c) for eight n and four c, V by (keys 2 c, dims of piece x) for four c and two or four x at a time.
-template <int D> __device__ __forceinline__ uint32_t a8_k_at(int k, int ch) {
-  return k * D + ((D == 64 ? ch : ch ^ ((k & 1) << 2)) << 4);
-}
-template <int D> __device__ __forceinline__ uint32_t a8_v_at(int k, int ch) {
-  if constexpr (D == 64) return (k >> 1) * 128 + ((((k & 1) << 2 | ch) ^ ((k >> 1 & 3) << 1)) << 4);
-  else if constexpr (D == 128) return k * 128 + ((ch ^ (k & 6)) << 4);
-  else return k * 256 + ((ch ^ ((k >> 1 & 1) | (k & 4))) << 4);
+// Of the 8 keys of a product, the one that stands in column n; of a key's 16-byte pieces, the one that lane group x takes for P V
+// (of each 128 bytes; at head dim 64 the x-th 8 bytes). Swizzled places differ in the bits that pairs of lanes would share.
+template <int D> __device__ __forceinline__ int a8_key(int n) { return D == 64 ? n : (n & 1) << 2 | n >> 1; }
+__device__ __forceinline__ int a8_piece_of(int x) { return (x & 1) << 2 | x >> 1; }
+// Byte offset of 16-byte piece ch of key k in a slice of 16 keys, as TMA writes it: blocks of 128 bytes a key (64 at head dim 64)
+template <int D> __device__ __forceinline__ uint32_t a8_at(int k, int ch) {
+  if constexpr (D == 64) return sw64_off(k, ch);
+  else return (ch >> 3) * (A8_SLICE * 128) + sw128_off(k, ch & 7);
 }
 
 // Four codes as fp16, two pairs.
@@ -265,97 +267,109 @@ __device__ __forceinline__ bool a8_sees(const Attn8Args& a, const A8Req& r, int 
 
 template <int D, typename T>
 __global__ void __launch_bounds__(A8_THREADS, 1)
-attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partials) {
-  constexpr int STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 8;
-  extern __shared__ __align__(128) uint8_t a8_smem_raw[];
-  uint8_t* rings = a8_smem_raw;                                        // [warps][ST][K 16 x D, V 16 x D]
-  float* ring_scales = reinterpret_cast<float*>(rings + A8_WARPS * A8_RING);  // [warps][ST][ks 2, vs 2]
-  uint4* s_q = reinterpret_cast<uint4*>(ring_scales + A8_WARPS * ST * 4);     // [steps][32 lanes] fragments of 16 rows
-  float* s_o = reinterpret_cast<float*>(s_q + STEPS * 32);              // [16][D]
-  float* s_m = s_o + A8_ROWS * D;                                       // [warps][16]
-  float* s_l = s_m + A8_WARPS * A8_ROWS;                                // [warps][16]
-  float* s_rowscale = s_l + A8_WARPS * A8_ROWS;                         // [16]
-  int64_t* s_scan = reinterpret_cast<int64_t*>(s_rowscale + 16);        // a8_piece's
+attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Attn8Args a,
+             int box, A8Split* splits, float* partials) {
+  constexpr int STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 8, BLOCKS = D == 256 ? 2 : 1;
+  extern __shared__ __align__(1024) uint8_t a8_smem_raw[];
+  uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a8_smem_raw) + 1023) & ~uintptr_t(1023));  // [warps][ST][K, V]
+  uint4* q_frags = reinterpret_cast<uint4*>(rings + A8_WARPS * ST * STAGE);               // [warps][steps][32 lanes], head dim 256
+  float* ring_scales = reinterpret_cast<float*>(q_frags + A8_WARPS * a8_q_bytes(D) / 16);  // [warps][ST][ks 2, vs 2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + A8_WARPS * ST * 4);           // [warps][ST] a slice has landed
+  A8Lot* lots = reinterpret_cast<A8Lot*>(bars + A8_WARPS * ST);                            // [warps]
+  int64_t* scan = reinterpret_cast<int64_t*>(lots + A8_WARPS);
 
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, piece = blockIdx.x;
-  const int G = a.hq / a.hkv, quad = lane & 3, x8 = lane >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int piece = warp * A8_BLOCKS + blockIdx.x, G = a.hq / a.hkv, quad = lane & 3, x8 = lane >> 2;
+  if (tid < A8_WARPS * ST) {
+    mbar_init(bars + tid, 1);
+    fence_barrier_init();
+  }
+  if (tid == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
   pdl_wait();
-  if (tid == 0) splits[piece].last = -1;
+  if (lane == 0) splits[piece].last = -1;
+  const int64_t step = a8_lots<A8_ROWS, A8_SLICE, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
+  const A8Lot lot = lots[warp];
+  if (lot.from.b < 0) return;
+  // of an item that begins at `unit` on the line, slices up to this lie in the piece
+  auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, lot.end - unit - A8_COST)); };
 
-  int64_t begin, w1, step;
-  A8At from;
-  if (!a8_piece<A8_ROWS, A8_TILE, A8_THREADS>(a, G, A8_COST, piece, s_scan, from, begin, w1, step)) return;  // nobody waits for this block
-
-  // What of an item lies in this piece, from where the item begins on the line: tiles [i0, i1).
-  auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, w1 - unit - A8_COST)); };
-
-  // ---- the copying side of a warp: a walk of its own, ahead by ST stages ----
-  A8Walk<A8_ROWS, A8_TILE> put;
-  put.start(a, G, from);
-  int64_t put_unit = begin;
+  // ---- the copying side: a walk of its own, ahead by the ring's stages ----
+  A8Walk<A8_ROWS, A8_SLICE> put;
+  put.start(a, G, lot.from);
+  int64_t put_unit = lot.begin;
   int put_i = put.at.i, put_i1 = part_end(put_unit, put.s.n);
-  bool put_more = true;
-  uint8_t* ring = rings + warp * A8_RING;
+  bool put_more = true, asked = false;
+  uint8_t* ring = rings + warp * ST * STAGE;
   float* scales = ring_scales + warp * ST * 4;
-  const uint32_t ring_u = smem_u32(ring), scales_u = smem_u32(scales);
-  int put_slot = 0;
-  int put_base = 0, put_page = -1;  // of the tile to be copied next: this warp's first key; lanes 0 and 1: its groups' pages
-  bool put_asked = false;           // (if the item can see one of the group's keys)
-  auto settle = [&]() {  // to the next tile that exists, and ask for its pages
-    while (put_more && put_i >= put_i1) {
+  uint64_t* full = bars + warp * ST;
+  int put_slot = 0, put_base = 0, page = 0, within = 0;  // of the slice to be copied next; lane i < 2: of keys 8 i .. 8 i + 7
+  auto settle = [&]() {  // to the next slice that exists, and ask for its pages
+    while (put_i >= put_i1) {
       put_unit += put.s.n + A8_COST;
-      if (put_unit + A8_COST >= w1) {  // no tile of the next item lies in this piece
+      if (put_unit + A8_COST >= lot.end) {  // no slice of the next item lies in this piece
         put_more = false;
-        break;
+        return;
       }
       put.next_item(a, G);
       put_i = 0;
       put_i1 = part_end(put_unit, put.s.n);
     }
-    if (!put_more) return;
-    put_base = put.base(put_i) + warp * 16;
-    put_page = -1;
-    const int j = put_base + (lane & 1) * 8;
-    put_asked = lane < 2 && j < put.s.hi && (j > put.s.lo - 8 || j < put.s.ahead);
-    if (put_asked) put_page = a.table[put.at.b * a.table_stride + a.cache.page_div.div(j)];
+    put_base = put.base(put_i);
+    const int j = put_base + lane * 8;
+    asked = lane < 2 && j < put.s.hi && (j > put.s.lo - 8 || j < put.s.ahead);
+    if (asked) {
+      const int p = a.cache.page_div.div(j);
+      within = j - p * a.cache.page;
+      page = a.table[put.at.b * a.table_stride + p];
+    }
   };
   settle();
+  int issued = 0;
   auto copy = [&]() {
     if (put_more) {
       const Cache8& c = a.cache;
-      int off[2];
-      const uint8_t *kb[2], *vb[2];
-      bool good[2];
-      int pages[2];
-      if (put_asked && (put_page < 0 || put_page >= c.pages)) set_error(a.err, ERR_BAD_PAGE);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int page = __shfl_sync(0xffffffffu, put_page, g);
-        const int j = put_base + 8 * g;
-        pages[g] = page;
-        good[g] = page >= 0 && page < c.pages;
-        off[g] = j - (int)c.page_div.div(j) * c.page;
-        const int64_t at = good[g] ? (int64_t)page * c.page_stride + off[g] * c.token_stride + put.at.h * c.head_stride : 0;
-        kb[g] = c.k + at;
-        vb[g] = c.v + at;
+      const bool good = asked && page >= 0 && page < c.pages;
+      if (asked && !good) set_error(a.err, ERR_BAD_PAGE);
+      // a box of 16 keys is fetched if one of its two groups is asked for (both are of one page)
+      const unsigned groups = __ballot_sync(0xffffffffu, good);
+      if (box == 16) {
+        const int from = groups & 1 ? 0 : 1;
+        page = __shfl_sync(0xffffffffu, page, from);
+        within = __shfl_sync(0xffffffffu, within, from) - 8 * from + 8 * (lane & 1);
       }
-      const uint32_t dst = ring_u + put_slot * STAGE;
+      const bool bring = box == 16 ? lane == 0 && groups : lane < 2 && good;
+      if (lane == 0)
+        mbar_arrive_expect_tx(&full[put_slot], (box == 16 ? (groups ? 2 : 0) : __popc(groups)) * 8 * 2 * D);
+      __syncwarp();
+      if (bring) {
+        uint8_t* dst = ring + put_slot * STAGE + (D == 64 ? lane * 8 * 64 : lane * 8 * 128);
+        if constexpr (D == 256) {
+          if (box == 8) {  // a box of 8 keys would pack its blocks of 128 bytes closer than a slice of 16 does
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int e = lane + 32 * i, k = e / (D / 16), ch = e % (D / 16), g = k >> 3, j = put_base + k;
-        const bool there = good[g] && j < put.s.hi && (j >= put.s.lo || j < put.s.ahead);
-        const int64_t o = (k & 7) * c.token_stride + ch * 16;
-        cp_async16(dst + a8_k_at<D>(k, ch), there ? kb[g] + o : c.k, there);
-        cp_async16(dst + 16 * D + a8_v_at<D>(k, ch), there ? vb[g] + o : c.v, there);
+            for (int e = 0; e < 2; ++e) {
+              tma_load_5d(dst + e * (A8_SLICE * 128), &tm_k, 0, within, e, put.at.h, page, &full[put_slot]);
+              tma_load_5d(dst + A8_SLICE * D + e * (A8_SLICE * 128), &tm_v, 0, within, e, put.at.h, page, &full[put_slot]);
+            }
+          } else {
+            tma_load_5d(dst, &tm_k, 0, within, 0, put.at.h, page, &full[put_slot]);
+            tma_load_5d(dst + A8_SLICE * D, &tm_v, 0, within, 0, put.at.h, page, &full[put_slot]);
+          }
+        } else {
+          tma_load_5d(dst, &tm_k, 0, within, 0, put.at.h, page, &full[put_slot]);
+          tma_load_5d(dst + A8_SLICE * D, &tm_v, 0, within, 0, put.at.h, page, &full[put_slot]);
+        }
       }
+      // the scales of two groups, lanes 0 and 1 for K and 2 and 3 for V
+      const int g = lane & 1, pg = __shfl_sync(0xffffffffu, page, g), in = __shfl_sync(0xffffffffu, within, g);
       if (lane < 4) {
-        const int g = lane & 1;
-        const int page = g ? pages[1] : pages[0], from_row = g ? off[1] : off[0];
-        const bool there = g ? good[1] : good[0];
-        const float* from = lane < 2 ? c.ks : c.vs;
-        const int64_t at = there ? ((int64_t)page * c.blocks + c.block_div.div(from_row)) * a.hkv + put.at.h : 0;
-        cp_async4(scales_u + (put_slot * 4 + lane) * 4, from + at, there);
+        const bool there = groups >> g & 1;
+        const int64_t at = there ? ((int64_t)pg * c.blocks + c.block_div.div(in)) * a.hkv + put.at.h : 0;
+        cp_async4(smem_u32(scales + put_slot * 4 + lane), (lane < 2 ? c.ks : c.vs) + at, there);
       }
+      ++issued;
       if (++put_slot == ST) put_slot = 0;
       ++put_i;
       settle();
@@ -366,61 +380,81 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
   for (int s = 0; s < ST; ++s) copy();
 
   // ---- items ----
-  A8Walk<A8_ROWS, A8_TILE> get;
-  get.start(a, G, from);
-  int64_t unit = begin;
-  int slot = 0;
+  A8Walk<A8_ROWS, A8_SLICE> get;
+  get.start(a, G, lot.from);
+  int64_t unit = lot.begin;
+  int slot = 0, taken = 0;
+  uint32_t phase = 0;
+  bool ok = true;
   const float to_log2 = a.scale * 1.4426950408889634f;
   for (int item = 0;; ++item) {
     const int i0 = get.at.i, i1 = part_end(unit, get.s.n);
     const A8Req r = get.r;
     const A8Span sp = get.s;
-    const int row0 = get.at.block * A8_ROWS;
-    // queries as fragments: step s of a lane takes dims 16 (quad + 4 (s / 4)) + 4 (s % 4) + 0 .. 3 of rows x8 and x8 + 8
+    const int row0 = get.at.block * A8_ROWS, old = r.len - r.n;
+    const int ta = (row0 + x8) / G, tb = (row0 + x8 + 8) / G;
+    const bool valid_a = ta < r.n, valid_b = tb < r.n;
+    // queries as fragments: step s takes dims 16 (quad + 4 (s / 4)) + 4 (s % 4) + 0 .. 3 of rows x8 and x8 + 8
+    uint4 qf[D == 256 ? 1 : STEPS];
+    uint4* const q_mine = q_frags + (warp * STEPS) * 32 + lane;
+    float scale_a = to_log2, scale_b = to_log2;
     {
-      const int row = tid >> 4, sub = tid & 15;  // 16 threads a row, D / 16 dims each
-      const int at = row0 + row, t = at / G, g = at - t * G;
-      constexpr int N = D / 16;
-      float v[N];
-      const bool there = t < r.n;
-      const T* src = (const T*)a.q + (int64_t)(r.t0 + t) * a.q_ts + (int64_t)(get.at.h * G + g) * a.q_hs + sub * N;
+      uint32_t w[2][D / 64][8];
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = there ? (float)src[e] : 0.f;
-      float back = 1.f;
-      if constexpr (!std::is_same<T, __half>::value) {
-        float most = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        const int t = e ? tb : ta, g = row0 + x8 + 8 * e - t * G;
+        const T* src = (const T*)a.q + (int64_t)(r.t0 + t) * a.q_ts + (int64_t)(get.at.h * G + g) * a.q_hs + quad * 16;
 #pragma unroll
-        for (int e = 0; e < N; ++e) most = fmaxf(most, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        float up;
-        a8_row_scale(most, up, back);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] *= up;
+        for (int i = 0; i < D / 64; ++i) {
+          uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+          if (e ? valid_b : valid_a) {
+            lo = reinterpret_cast<const uint4*>(src + 64 * i)[0];
+            hi = reinterpret_cast<const uint4*>(src + 64 * i)[1];
+          }
+          w[e][i][0] = lo.x; w[e][i][1] = lo.y; w[e][i][2] = lo.z; w[e][i][3] = lo.w;
+          w[e][i][4] = hi.x; w[e][i][5] = hi.y; w[e][i][6] = hi.z; w[e][i][7] = hi.w;
+        }
       }
-      if (sub == 0) s_rowscale[row] = back * to_log2;
-      // dims d, d + 1 (d even) are half a register of lane (row % 8) * 4 + c of step s: d = 16 (c + 4 i) + 4 q + 2 hi, s = 4 i + q
-      uint32_t* frag = reinterpret_cast<uint32_t*>(s_q);
+      if constexpr (!std::is_same<T, __half>::value) {
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const int d = sub * N + e, ch = d >> 4, cq = ch & 3, st = (ch >> 2) * 4 + ((d >> 2) & 3), up = d >> 1 & 1;
-        frag[(st * 32 + (row & 7) * 4 + cq) * 4 + up * 2 + (row >> 3)] = pack_half2(v[e], v[e + 1]);
+        for (int e = 0; e < 2; ++e) {
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float x = fabsf(__uint_as_float(w[e][i][k] << 16)), y = fabsf(__uint_as_float(w[e][i][k] & 0xffff0000u));
+              most = fmaxf(most, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+            }
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+          float up, back;
+          a8_row_scale(most, up, back);
+          (e ? scale_b : scale_a) *= back;
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              w[e][i][k] = pack_half2(__uint_as_float(w[e][i][k] << 16) * up, __uint_as_float(w[e][i][k] & 0xffff0000u) * up);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const uint4 f = make_uint4(w[0][s / 4][2 * (s % 4)], w[1][s / 4][2 * (s % 4)], w[0][s / 4][2 * (s % 4) + 1], w[1][s / 4][2 * (s % 4) + 1]);
+        if constexpr (D == 256) q_mine[s * 32] = f;
+        else qf[s] = f;
       }
     }
-    __syncthreads();
-    const int ta = (row0 + x8) / G, tb = (row0 + x8 + 8) / G;
-    const float scale_a = s_rowscale[x8], scale_b = s_rowscale[x8 + 8];
-    const int old = r.len - r.n;
     int pa = 0, pb = 0;
     if (a.window) {
-      pa = ta < r.n ? (a.positions ? a.positions[r.t0 + ta] : old + ta) : 0;
-      pb = tb < r.n ? (a.positions ? a.positions[r.t0 + tb] : old + tb) : 0;
+      pa = valid_a ? (a.positions ? a.positions[r.t0 + ta] : old + ta) : 0;
+      pb = valid_b ? (a.positions ? a.positions[r.t0 + tb] : old + tb) : 0;
     }
     // keys below `sure` and above `low` are seen by every row
     const int sure = a.mask ? old : old + row0 / G + 1;
     int low = -1;
     if (a.window) {
-      low = max(ta < r.n ? pa - a.window : -1, tb < r.n ? pb - a.window : -1);
+      low = max(valid_a ? pa - a.window : -1, valid_b ? pb - a.window : -1);
       low = __reduce_max_sync(0xffffffffu, low);
     }
     float o[NT][4];
@@ -429,117 +463,118 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
     float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+#pragma unroll 1
     for (int i = i0; i < i1; ++i) {
       cp_async_wait<ST - 1>();
-      __syncwarp();
-      const int base = get.base(i) + warp * 16;
-      const bool any = base < sp.hi && (base > sp.lo - 16 || base < sp.ahead);
-      if (any) {
-        float s[2][4];
+      ok = da_wait(&full[slot], phase, a.err, ERR_TIMEOUT_TMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      __syncwarp();  // the scales that four lanes have waited for
+      ++taken;
+      const int base = get.base(i);
+      const uint8_t* kb = ring + slot * STAGE;
+      const uint8_t* vb = kb + A8_SLICE * D;
+      float s[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
 #pragma unroll
-        for (int i4 = 0; i4 < D / 64; ++i4) {
-          uint4 kw[2];
+      for (int i4 = 0; i4 < D / 64; ++i4) {
+        uint4 kw[2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-            kw[n] = *reinterpret_cast<const uint4*>(ring + slot * STAGE + a8_k_at<D>(n * 8 + x8, quad + 4 * i4));
+        for (int n = 0; n < 2; ++n)
+          kw[n] = *reinterpret_cast<const uint4*>(kb + a8_at<D>(n * 8 + a8_key<D>(x8), quad + 4 * i4));
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint4 f = s_q[(i4 * 4 + q) * 32 + lane];
+        for (int q = 0; q < 4; ++q) {
+          uint4 f;
+          if constexpr (D == 256) f = q_mine[(i4 * 4 + q) * 32];
+          else f = qf[i4 * 4 + q];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t w = q == 0 ? kw[n].x : q == 1 ? kw[n].y : q == 2 ? kw[n].z : kw[n].w;
-              mma16<T>(s[n], f, f8_half2(w & 0xffffu), f8_half2(w >> 16));
-            }
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t w = q == 0 ? kw[n].x : q == 1 ? kw[n].y : q == 2 ? kw[n].z : kw[n].w;
+            mma16<T>(s[n], f, f8_half2(w & 0xffffu), f8_half2(w >> 16));
           }
         }
-        const float4 sc = *reinterpret_cast<const float4*>(scales + slot * 4);  // ks 0, 1, vs 0, 1
-        const float ks[2] = {sc.x, sc.y};
-        // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write; NaN stays
-        const float vs[2] = {sc.z != sc.z ? sc.z : fminf(fmaxf(sc.z, 0x1p-100f), 0x1p120f),
-                             sc.w != sc.w ? sc.w : fminf(fmaxf(sc.w, 0x1p-100f), 0x1p120f)};
-        const bool special = base > sure - 16 || (a.window && base <= low);
-        uint32_t seen = 0xff;
-        if (special) {
-          seen = 0;
+      }
+      const float4 sc = *reinterpret_cast<const float4*>(scales + slot * 4);  // ks 0, 1, vs 0, 1
+      const float ks[2] = {sc.x, sc.y};
+      // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write
+      const float vs[2] = {fminf(fmaxf(sc.z, 0x1p-100f), 0x1p120f), fminf(fmaxf(sc.w, 0x1p-100f), 0x1p120f)};
+      const bool special = base > sure - A8_SLICE || (a.window && base <= low);
+      uint32_t seen = 0xff;
+      if (special) {
+        seen = 0;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (a8_sees(a, r, e < 2 ? ta : tb, e < 2 ? pa : pb, base + n * 8 + 2 * quad + (e & 1))) seen |= 1u << (4 * n + e);
+          for (int e = 0; e < 4; ++e)
+            if (a8_sees(a, r, e < 2 ? ta : tb, e < 2 ? pa : pb, base + n * 8 + a8_key<D>(2 * quad + (e & 1)))) seen |= 1u << (4 * n + e);
+      }
+      float top_a = -INFINITY, top_b = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float lv = __log2f(vs[n]), fa = scale_a * ks[n], fb = scale_b * ks[n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = fmaf(s[n][e], e < 2 ? fa : fb, lv);
+          if (special && !(seen >> (4 * n + e) & 1)) s[n][e] = -INFINITY;
         }
-        float top_a = -INFINITY, top_b = -INFINITY;
+        top_a = fmaxf(top_a, fmaxf(s[n][0], s[n][1]));
+        top_b = fmaxf(top_b, fmaxf(s[n][2], s[n][3]));
+      }
+      // the maximum is raised only when a score exceeds it by 2^A8_SLACK
+      if (__any_sync(0xffffffffu, top_a > ma + A8_SLACK || top_b > mb + A8_SLACK)) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float lv = __log2f(vs[n]), fa = scale_a * ks[n], fb = scale_b * ks[n];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[n][e] = fmaf(s[n][e], e < 2 ? fa : fb, lv);
-            if (special && !(seen >> (4 * n + e) & 1)) s[n][e] = -INFINITY;
-          }
-          top_a = fmaxf(top_a, fmaxf(s[n][0], s[n][1]));
-          top_b = fmaxf(top_b, fmaxf(s[n][2], s[n][3]));
+        for (int d = 1; d < 4; d <<= 1) {
+          top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, d));
+          top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, d));
         }
-        // the maximum is raised only when a score exceeds it by 2^A8_SLACK
-        if (__any_sync(0xffffffffu, top_a > ma + A8_SLACK || top_b > mb + A8_SLACK)) {
-#pragma unroll
-          for (int d = 1; d < 4; d <<= 1) {
-            top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, d));
-            top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, d));
-          }
-          float by_a = 1.f, by_b = 1.f;
-          if (top_a > ma + A8_SLACK) {
-            by_a = ma == -INFINITY ? 0.f : ex2_approx(ma - top_a);
-            ma = top_a;
-          }
-          if (top_b > mb + A8_SLACK) {
-            by_b = mb == -INFINITY ? 0.f : ex2_approx(mb - top_b);
-            mb = top_b;
-          }
-          la *= by_a;
-          lb *= by_b;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            o[j][0] *= by_a;
-            o[j][1] *= by_a;
-            o[j][2] *= by_b;
-            o[j][3] *= by_b;
-          }
+        float by_a = 1.f, by_b = 1.f;
+        if (top_a > ma + A8_SLACK) {
+          by_a = ma == -INFINITY ? 1.f : ex2_approx(ma - top_a);  // from -inf: sums are 0, or NaN
+          ma = top_a;
         }
-        const float off_a = ma == -INFINITY ? 0.f : A8_LIFT - ma, off_b = mb == -INFINITY ? 0.f : A8_LIFT - mb;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float rv = 1.0f / vs[n];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (e < 2 ? off_a : off_b));
-          // a block that a row sees nothing of must not count by its scale either
-          const float wa = s[n][0] + s[n][1], wb = s[n][2] + s[n][3];
-          la += !special || (seen >> (4 * n) & 3) ? wa * rv : 0.f;
-          lb += !special || (seen >> (4 * n + 2) & 3) ? wb * rv : 0.f;
+        if (top_b > mb + A8_SLACK) {
+          by_b = mb == -INFINITY ? 1.f : ex2_approx(mb - top_b);
+          mb = top_b;
         }
-        const uint4 p = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
-                                   pack_half2(s[1][2], s[1][3]));
-        // O += P V: dims x8 * D / 8 + j of keys 2 quad, 2 quad + 1 and those 8 further on
-        constexpr int BYTES = D / 8;  // of a key that a lane reads
-        constexpr int WORDS = BYTES / 4;
+        la *= by_a;
+        lb *= by_b;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          o[j][0] *= by_a;
+          o[j][1] *= by_a;
+          o[j][2] *= by_b;
+          o[j][3] *= by_b;
+        }
+      }
+      const float off_a = ma == -INFINITY ? 0.f : A8_LIFT - ma, off_b = mb == -INFINITY ? 0.f : A8_LIFT - mb;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float rv = 1.0f / vs[n];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (e < 2 ? off_a : off_b));
+        la = fmaf(s[n][0] + s[n][1], rv, la);
+        lb = fmaf(s[n][2] + s[n][3], rv, lb);
+      }
+      const uint4 p = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
+                                 pack_half2(s[1][2], s[1][3]));
+      // O += P V: of the keys in columns 2 quad and 2 quad + 1 of both halves, the dims of piece a8_piece_of(x8) of each 128
+      constexpr int WORDS = D == 64 ? 2 : 4;
+#pragma unroll
+      for (int blk = 0; blk < BLOCKS; ++blk) {
         uint32_t vw[4][WORDS];
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
-          const int k = 2 * quad + (k4 & 1) + (k4 >> 1) * 8;
+          const int k = a8_key<D>(2 * quad + (k4 & 1)) + (k4 >> 1) * 8;
           if constexpr (D == 64) {
-            const uint2 y = *reinterpret_cast<const uint2*>(ring + slot * STAGE + 16 * D + a8_v_at<D>(k, x8 >> 1) + (x8 & 1) * 8);
+            const uint2 y = *reinterpret_cast<const uint2*>(vb + a8_at<D>(k, x8 >> 1) + (x8 & 1) * 8);
             vw[k4][0] = y.x;
             vw[k4][1] = y.y;
           } else {
-#pragma unroll
-            for (int e = 0; e < D / 128; ++e) {
-              const uint4 y = *reinterpret_cast<const uint4*>(ring + slot * STAGE + 16 * D + a8_v_at<D>(k, x8 * (D / 128) + e));
-              vw[k4][4 * e] = y.x;
-              vw[k4][4 * e + 1] = y.y;
-              vw[k4][4 * e + 2] = y.z;
-              vw[k4][4 * e + 3] = y.w;
-            }
+            const uint4 y = *reinterpret_cast<const uint4*>(vb + a8_at<D>(k, a8_piece_of(x8) + 8 * blk));
+            vw[k4][0] = y.x;
+            vw[k4][1] = y.y;
+            vw[k4][2] = y.z;
+            vw[k4][3] = y.w;
           }
         }
         bool nan = false;
@@ -573,7 +608,7 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
               mma16<T>(hits, see, f8_half2(e & 1 ? b0 >> 16 : b0 & 0xffffu), f8_half2(e & 1 ? b1 >> 16 : b1 & 0xffffu));
 #pragma unroll
               for (int z = 0; z < 4; ++z)
-                if (hits[z] > 0.f) o[4 * w + e][z] = __int_as_float(0x7fffffff);
+                if (hits[z] > 0.f) o[16 * blk + 4 * w + e][z] = __int_as_float(0x7fffffff);
             }
           }
         }
@@ -583,98 +618,72 @@ attn8_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* partia
           for (int pr = 0; pr < 2; ++pr) {
             const uint32_t sel = pr == 0 ? 0x5140u : 0x7362u;
             const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], sel), b1 = __byte_perm(vw[2][w], vw[3][w], sel);
-            mma16<T>(o[4 * w + 2 * pr], p, f8_half2(b0 & 0xffffu), f8_half2(b1 & 0xffffu));
-            mma16<T>(o[4 * w + 2 * pr + 1], p, f8_half2(b0 >> 16), f8_half2(b1 >> 16));
+            mma16<T>(o[16 * blk + 4 * w + 2 * pr], p, f8_half2(b0 & 0xffffu), f8_half2(b1 & 0xffffu));
+            mma16<T>(o[16 * blk + 4 * w + 2 * pr + 1], p, f8_half2(b0 >> 16), f8_half2(b1 >> 16));
           }
         }
       }
-      __syncwarp();  // every lane has read the stage
+      __syncwarp();  // every lane has read the slice
       copy();
-      if (++slot == ST) slot = 0;
+      if (++slot == ST) {
+        slot = 0;
+        phase ^= 1u;
+      }
     }
-    // ---- the item's warps meet ----
+    if (!__all_sync(0xffffffffu, ok)) break;
+    // ---- the item, or this piece's part of it ----
 #pragma unroll
     for (int d = 1; d < 4; d <<= 1) {
       la += __shfl_xor_sync(0xffffffffu, la, d);
       lb += __shfl_xor_sync(0xffffffffu, lb, d);
     }
-    if (quad == 0) {
-      s_m[warp * 16 + x8] = ma;
-      s_m[warp * 16 + x8 + 8] = mb;
-      s_l[warp * 16 + x8] = la;
-      s_l[warp * 16 + x8 + 8] = lb;
-    }
-    __syncthreads();
-    float top_a = -INFINITY, top_b = -INFINITY;
+    const bool whole = i0 == 0 && i1 == sp.n;
+    const int part_slot = 2 * piece + (item > 0 ? 1 : 0);
+    float* part = partials + (size_t)part_slot * a8_partial_floats(D, A8_ROWS);
 #pragma unroll
-    for (int w = 0; w < A8_WARPS; ++w) {
-      top_a = fmaxf(top_a, s_m[w * 16 + x8]);
-      top_b = fmaxf(top_b, s_m[w * 16 + x8 + 8]);
-    }
-    const float by_a = ma == -INFINITY ? 0.f : ex2_approx(ma - top_a), by_b = mb == -INFINITY ? 0.f : ex2_approx(mb - top_b);
-    const bool none_a = ma == -INFINITY && la == 0.f, none_b = mb == -INFINITY && lb == 0.f;  // saw nothing: O may be 0 times junk
-    for (int w = 0; w < A8_WARPS; ++w) {
-      if (warp == w) {
-        // dims 2 quad D / 8 + j and the next D / 8 of row x8 and of row x8 + 8
-        float* to = s_o + x8 * D + 2 * quad * (D / 8);
+    for (int e = 0; e < 2; ++e) {
+      const int t = e ? tb : ta, row = x8 + 8 * e, g = row0 + row - t * G;
+      const float m = e ? mb : ma, l = e ? lb : la;
+      if (!(e ? valid_b : valid_a)) continue;
+      // columns 2 quad and 2 quad + 1 are dims D / 8 (or 16 of each 128) from these on
+      const int64_t orow = (int64_t)(r.t0 + t) * a.hq + get.at.h * G + g;
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float* at = to + (e >> 1) * 8 * D + (e & 1) * (D / 8);
-          const float by = e < 2 ? by_a : by_b;
-          const bool none = e < 2 ? none_a : none_b;
+      for (int z = 0; z < 2; ++z)
 #pragma unroll
-          for (int j = 0; j < NT; j += 4) {
-            float4 y = w ? *reinterpret_cast<float4*>(at + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-            if (!none) {
-              y.x += o[j][e] * by;
-              y.y += o[j + 1][e] * by;
-              y.z += o[j + 2][e] * by;
-              y.w += o[j + 3][e] * by;
+        for (int blk = 0; blk < BLOCKS; ++blk) {
+          constexpr int RUN = D == 64 ? 8 : 16;
+          const int d0 = D == 64 ? (2 * quad + z) * 8 : 128 * blk + 16 * a8_piece_of(2 * quad + z);
+#pragma unroll
+          for (int j = 0; j < RUN; j += 8) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = o[16 * blk + j + k][2 * e + z];
+            if (whole) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) y[k] *= inv;
+              store8((T*)a.out + orow * D + d0 + j, y);
+            } else {
+              float4* to = reinterpret_cast<float4*>(part + row * D + d0 + j);
+              to[0] = make_float4(y[0], y[1], y[2], y[3]);
+              to[1] = make_float4(y[4], y[5], y[6], y[7]);
             }
-            *reinterpret_cast<float4*>(at + j) = y;
           }
         }
+      if (quad == 0) {
+        if (!whole) *reinterpret_cast<float2*>(part + A8_ROWS * D + 2 * row) = make_float2(m, l);
+        else if (a.lse) a.lse[orow] = l > 0.f || l != l ? (m - A8_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
       }
-      __syncthreads();
     }
-    {
-      const int row = tid >> 4, sub = tid & 15, at = row0 + row, t = at / G, g = at - t * G;
-      constexpr int N = D / 16;
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < A8_WARPS; ++w) m = fmaxf(m, s_m[w * 16 + row]);
-#pragma unroll
-      for (int w = 0; w < A8_WARPS; ++w) {
-        const float mw = s_m[w * 16 + row], lw = s_l[w * 16 + row];
-        l += mw == -INFINITY ? lw : lw * ex2_approx(mw - m);
-      }
-      const bool whole = i0 == 0 && i1 == sp.n;
-      float* part = partials + (size_t)(2 * piece + (item > 0 ? 1 : 0)) * a8_partial_floats(D);
-      if (t < r.n) {
-        if (whole) {
-          const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-          const int64_t orow = (int64_t)(r.t0 + t) * a.hq + get.at.h * G + g;
-          T* dst = (T*)a.out + orow * D + sub * N;
-#pragma unroll
-          for (int e = 0; e < N; e += 2)
-            *reinterpret_cast<uint32_t*>(dst + e) = pack2(s_o[row * D + sub * N + e] * inv, s_o[row * D + sub * N + e + 1] * inv, dst);
-          if (sub == 0 && a.lse) a.lse[orow] = l > 0.f || l != l ? (m - A8_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) part[row * D + sub * N + e] = s_o[row * D + sub * N + e];
-          if (sub == 0) *reinterpret_cast<float2*>(part + A8_ROWS * D + 2 * row) = make_float2(m, l);
-        }
-      }
-      if (tid == 0 && i0 == 0 && i1 < sp.n)
-        splits[piece] = A8Split{get.at.b, get.at.h, get.at.block, (int)((unit + A8_COST + sp.n - 1) / step),
-                                2 * piece + (item > 0 ? 1 : 0), {0, 0, 0}};
-    }
+    if (lane == 0 && i0 == 0 && i1 < sp.n)
+      splits[piece] = A8Split{get.at.b, get.at.h, get.at.block, (int)((unit + A8_COST + sp.n - 1) / step), part_slot, {0, 0, 0}};
     unit += sp.n + A8_COST;
-    if (unit + A8_COST >= w1) break;
+    if (unit + A8_COST >= lot.end) break;
     get.next_item(a, G);
-    __syncthreads();  // queries, maxima and sums are free
   }
   cp_async_wait<0>();
+  // after a wait that gave up: what is still on its way lands before the memory goes
+  for (int s = taken; s < issued && !ok; ++s) da_wait(&full[s % ST], (s / ST) & 1, nullptr, 0);
 }
 
 // Tokens from .. to - 1 as if they saw nothing, by `count` threads of which this is number `me`.
@@ -694,21 +703,21 @@ template <int D, int ROWS, typename T>
 __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_constant__ Attn8Args a, const A8Split* splits,
                                                                 const float* partials) {
   pdl_wait();
-  const int c = blockIdx.x, lane = threadIdx.x & 31, G = a.hq / a.hkv;
+  const int c = blockIdx.x, lane = threadIdx.x & 31, G = a.hq / a.hkv, pieces = gridDim.x;
   const A8Split s = splits[c];
   const int lead = a.cu[0], trail = a.cu[a.rows];
   if (lead > 0 || trail < a.tokens) {
-    const int64_t me = ((int64_t)blockIdx.y * A8_PIECES + c) * A8J_THREADS + threadIdx.x,
-                  all = (int64_t)gridDim.y * A8_PIECES * A8J_THREADS;
+    const int64_t me = ((int64_t)blockIdx.y * pieces + c) * A8J_THREADS + threadIdx.x,
+                  all = (int64_t)gridDim.y * pieces * A8J_THREADS;
     a8_blank<D, T>(a, 0, min(lead, a.tokens), me, all);
     a8_blank<D, T>(a, max(trail, 0), a.tokens, me, all);
   }
   if (blockIdx.y == 0) {
-    for (int b0 = c + A8_PIECES * (threadIdx.x & ~31); b0 < a.rows; b0 += A8_PIECES * A8J_THREADS) {
-      const int b = b0 + A8_PIECES * lane;
+    for (int b0 = c + pieces * (threadIdx.x & ~31); b0 < a.rows; b0 += pieces * A8J_THREADS) {
+      const int b = b0 + pieces * lane;
       const bool out = b < a.rows && a.cu[b + 1] > a.cu[b] && a8_request<ROWS>(a, G, b, false).n == 0;
       for (unsigned rest = __ballot_sync(0xffffffffu, out); rest; rest &= rest - 1) {
-        const int r = b0 + A8_PIECES * (__ffs(rest) - 1);
+        const int r = b0 + pieces * (__ffs(rest) - 1);
         a8_blank<D, T>(a, max(a.cu[r], 0), min(a.cu[r + 1], a.tokens), lane, 32);
       }
     }

@@ -141,8 +141,9 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
   uint64_t* ml_full = item_empty + 2;            // [2] the group without an item's last tile is through with it
   uint64_t* o_free = ml_full + 2;                // O has been read
   constexpr int N_BARS = 12 + 4 + 12 + 16 + 2 + 8 + 6 + 1;
-  int64_t* scan = reinterpret_cast<int64_t*>(bars + N_BARS);        // [16 + 3] a8_piece's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + 20);
+  int64_t* scan = reinterpret_cast<int64_t*>(bars + N_BARS);        // [16] a8_lots'
+  A8Lot* lot_here = reinterpret_cast<A8Lot*>(scan + 16);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(lot_here + 1);
   int* poison = reinterpret_cast<int*>(tmem_slot + 2);              // [4] of item & 3: item + 1 if a NaN of V was zeroed
   uint32_t* k_info = reinterpret_cast<uint32_t*>(poison + 4);       // [NB], [NB] bit 0: first of its item here, 1: last, 2: the piece's last
   uint32_t* v_info = k_info + 3;
@@ -162,10 +163,10 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
   if (tid < 4) poison[tid] = 0;
   pdl_wait();
   if (tid == 0) splits[piece].last = -1;
-  A8At from;
-  int64_t begin, w1, step;
-  const bool work = a8_piece<W8_ROWS, KT, W8_THREADS>(a, G, W8_COST, piece, scan, from, begin, w1, step);
-  if (!work) return;  // the whole block
+  const int64_t step = a8_lots<W8_ROWS, KT, W8_THREADS, 1>(a, G, W8_COST, piece, scan, lot_here);
+  const A8At from = lot_here->from;
+  const int64_t begin = lot_here->begin, w1 = lot_here->end;
+  if (from.b < 0) return;  // the whole block
   if (warp == 3) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -258,7 +259,6 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
     };
 #pragma unroll 1
     for (int b = 0; b < 3; ++b) copy(b);
-    DaRing ring;
 #pragma unroll 1
     for (int b = 0;; ++b) {
       const bool is_v = b & 1;
