@@ -82,7 +82,9 @@ int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   }
   constexpr int PIECES = A8_BLOCKS * A8_WARPS;
   float* partials = reinterpret_cast<float*>(splits + PIECES);
-  const int box = p.cache.page % A8_SLICE == 0 ? A8_SLICE : 8, cols = D == 256 && box == A8_SLICE ? 2 : 1;
+  int box = a8_slice(D);  // tokens of a TMA box: all of one page
+  while (p.cache.page % box) box /= 2;
+  const int cols = D == 256 && box == a8_slice(D) ? 2 : 1;
   CUtensorMap k, v;
   int rc;
   if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||

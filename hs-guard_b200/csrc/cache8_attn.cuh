@@ -33,10 +33,9 @@ struct Attn8Args {
 
 // This kernel is for few rows a key head, where reading the cache is all that counts; products are warp-level (16 rows by 8
 // keys by 16 dims), since the 128 rows of a tcgen05 product would be padding. A request's rows of a key head, row r = (token
-// r / G, query head r % G), in blocks of 16, and the slices of 16 keys that such a block can see are an item; all items are one
+// r / G, query head r % G), in blocks of 16, and the slices of 32 keys (16 at head dim 256) that such a block can see are an item; all items are one
 // line that is cut into equal pieces, one a warp, eight warps an SM, whatever the requests' lengths. Warps do not meet: each has
-// its ring of slices, which it fills itself ahead of its use (TMA, one box of 16 keys, or two of 8 where pages divide into nothing
-// longer), its own running maximum, sums and accumulators. An item that lies in one piece is written out; of one that is cut, each
+// its ring of slices, which it fills itself ahead of its use (TMA, one box, or as many as a page's size takes), its own running maximum, sums and accumulators. An item that lies in one piece is written out; of one that is cut, each
 // piece leaves its sums in the workspace, and attn8_join_kernel joins them in piece order, so results do not depend on timing.
 //
 // Codes become fp16 exactly in registers. Queries are fp16 as well: an fp16 q as it is, a bf16 q times a power of two for
@@ -52,17 +51,17 @@ struct Attn8Args {
 constexpr int A8_THREADS = 256;
 constexpr int A8_WARPS = 8;
 constexpr int A8_ROWS = 16;
-constexpr int A8_SLICE = 16;        // keys
 constexpr int A8_BLOCKS = 148;      // one thread block an SM
 constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
 constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
 
-__host__ __device__ constexpr int a8_stage(int dim) { return 2 * A8_SLICE * dim; }
-__host__ __device__ constexpr int a8_stages(int dim) { return dim == 64 ? 12 : dim == 128 ? 6 : 2; }
+__host__ __device__ constexpr int a8_slice(int dim) { return dim == 256 ? 16 : 32; }  // keys
+__host__ __device__ constexpr int a8_stage(int dim) { return 2 * a8_slice(dim) * dim; }
+__host__ __device__ constexpr int a8_stages(int dim) { return dim == 64 ? 6 : dim == 128 ? 3 : 2; }
 __host__ __device__ constexpr int a8_q_bytes(int dim) { return dim == 256 ? A8_ROWS * dim * 2 : 0; }  // else in registers
 // a warp's ring, query fragments, scales and barriers; where the pieces begin
 __host__ __device__ constexpr int a8_smem(int dim) {
-  return 1024 + A8_WARPS * (a8_stages(dim) * (a8_stage(dim) + 24) + a8_q_bytes(dim)) + 1024;
+  return 1024 + A8_WARPS * (a8_stages(dim) * (a8_stage(dim) + 40) + a8_q_bytes(dim)) + 1024;
 }
 __host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
 struct A8Split {  // an item that begins in a piece and ends in a later one
@@ -226,10 +225,10 @@ template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile(
 // (of each 128 bytes; at head dim 64 the x-th 8 bytes). Swizzled places differ in the bits that pairs of lanes would share.
 template <int D> __device__ __forceinline__ int a8_key(int n) { return D == 64 ? n : (n & 1) << 2 | n >> 1; }
 __device__ __forceinline__ int a8_piece_of(int x) { return (x & 1) << 2 | x >> 1; }
-// Byte offset of 16-byte piece ch of key k in a slice of 16 keys, as TMA writes it: blocks of 128 bytes a key (64 at head dim 64)
+// Byte offset of 16-byte piece ch of key k in a slice, as TMA writes it: blocks of 128 bytes a key (64 at head dim 64)
 template <int D> __device__ __forceinline__ uint32_t a8_at(int k, int ch) {
   if constexpr (D == 64) return sw64_off(k, ch);
-  else return (ch >> 3) * (A8_SLICE * 128) + sw128_off(k, ch & 7);
+  else return (ch >> 3) * (a8_slice(D) * 128) + (k >> 3) * 1024 + sw128_off(k & 7, ch & 7);
 }
 
 // Four codes as fp16, two pairs.
@@ -269,12 +268,13 @@ template <int D, typename T>
 __global__ void __launch_bounds__(A8_THREADS, 1)
 attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Attn8Args a,
              int box, A8Split* splits, float* partials) {
-  constexpr int STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 8, BLOCKS = D == 256 ? 2 : 1;
+  constexpr int KEYS = a8_slice(D), GROUPS = KEYS / 8, STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 8,
+                BLOCKS = D == 256 ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t a8_smem_raw[];
   uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a8_smem_raw) + 1023) & ~uintptr_t(1023));  // [warps][ST][K, V]
   uint4* q_frags = reinterpret_cast<uint4*>(rings + A8_WARPS * ST * STAGE);               // [warps][steps][32 lanes], head dim 256
-  float* ring_scales = reinterpret_cast<float*>(q_frags + A8_WARPS * a8_q_bytes(D) / 16);  // [warps][ST][ks 2, vs 2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + A8_WARPS * ST * 4);           // [warps][ST] a slice has landed
+  float* ring_scales = reinterpret_cast<float*>(q_frags + A8_WARPS * a8_q_bytes(D) / 16);  // [warps][ST][ks, vs]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + A8_WARPS * ST * 8);           // [warps][ST] a slice has landed
   A8Lot* lots = reinterpret_cast<A8Lot*>(bars + A8_WARPS * ST);                            // [warps]
   int64_t* scan = reinterpret_cast<int64_t*>(lots + A8_WARPS);
 
@@ -290,22 +290,22 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   }
   pdl_wait();
   if (lane == 0) splits[piece].last = -1;
-  const int64_t step = a8_lots<A8_ROWS, A8_SLICE, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
+  const int64_t step = a8_lots<A8_ROWS, KEYS, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
   const A8Lot lot = lots[warp];
   if (lot.from.b < 0) return;
   // of an item that begins at `unit` on the line, slices up to this lie in the piece
   auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, lot.end - unit - A8_COST)); };
 
   // ---- the copying side: a walk of its own, ahead by the ring's stages ----
-  A8Walk<A8_ROWS, A8_SLICE> put;
+  A8Walk<A8_ROWS, KEYS> put;
   put.start(a, G, lot.from);
   int64_t put_unit = lot.begin;
   int put_i = put.at.i, put_i1 = part_end(put_unit, put.s.n);
   bool put_more = true, asked = false;
   uint8_t* ring = rings + warp * ST * STAGE;
-  float* scales = ring_scales + warp * ST * 4;
+  float* scales = ring_scales + warp * ST * 8;
   uint64_t* full = bars + warp * ST;
-  int put_slot = 0, put_base = 0, page = 0, within = 0;  // of the slice to be copied next; lane i < 2: of keys 8 i .. 8 i + 7
+  int put_slot = 0, put_base = 0, page = 0, within = 0;  // of the slice to be copied next; lane i < GROUPS: of keys 8 i .. 8 i + 7
   auto settle = [&]() {  // to the next slice that exists, and ask for its pages
     while (put_i >= put_i1) {
       put_unit += put.s.n + A8_COST;
@@ -319,7 +319,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     }
     put_base = put.base(put_i);
     const int j = put_base + lane * 8;
-    asked = lane < 2 && j < put.s.hi && (j > put.s.lo - 8 || j < put.s.ahead);
+    asked = lane < GROUPS && j < put.s.hi && (j > put.s.lo - 8 || j < put.s.ahead);
     if (asked) {
       const int p = a.cache.page_div.div(j);
       within = j - p * a.cache.page;
@@ -333,41 +333,31 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       const Cache8& c = a.cache;
       const bool good = asked && page >= 0 && page < c.pages;
       if (asked && !good) set_error(a.err, ERR_BAD_PAGE);
-      // a box of 16 keys is fetched if one of its two groups is asked for (both are of one page)
+      // lane i brings the i-th box of K and of V if it has a group that is asked for (a box is of one page), and knows where from
+      // by that group's lane
       const unsigned groups = __ballot_sync(0xffffffffu, good);
-      if (box == 16) {
-        const int from = groups & 1 ? 0 : 1;
-        page = __shfl_sync(0xffffffffu, page, from);
-        within = __shfl_sync(0xffffffffu, within, from) - 8 * from + 8 * (lane & 1);
-      }
-      const bool bring = box == 16 ? lane == 0 && groups : lane < 2 && good;
-      if (lane == 0)
-        mbar_arrive_expect_tx(&full[put_slot], (box == 16 ? (groups ? 2 : 0) : __popc(groups)) * 8 * 2 * D);
+      const int per = box >> 3, g0 = lane * per;  // groups a box; this lane's box's first
+      const unsigned mine = g0 < GROUPS ? groups >> g0 & ((1u << per) - 1u) : 0u;
+      const int from = mine ? g0 + __ffs(mine) - 1 : 0;
+      const int box_page = __shfl_sync(0xffffffffu, page, from), box_row = __shfl_sync(0xffffffffu, within, from) - 8 * (from - g0);
+      const unsigned boxes = __ballot_sync(0xffffffffu, mine != 0);
+      if (lane == 0) mbar_arrive_expect_tx(&full[put_slot], __popc(boxes) * box * 2 * D);
       __syncwarp();
-      if (bring) {
-        uint8_t* dst = ring + put_slot * STAGE + (D == 64 ? lane * 8 * 64 : lane * 8 * 128);
-        if constexpr (D == 256) {
-          if (box == 8) {  // a box of 8 keys would pack its blocks of 128 bytes closer than a slice of 16 does
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              tma_load_5d(dst + e * (A8_SLICE * 128), &tm_k, 0, within, e, put.at.h, page, &full[put_slot]);
-              tma_load_5d(dst + A8_SLICE * D + e * (A8_SLICE * 128), &tm_v, 0, within, e, put.at.h, page, &full[put_slot]);
-            }
-          } else {
-            tma_load_5d(dst, &tm_k, 0, within, 0, put.at.h, page, &full[put_slot]);
-            tma_load_5d(dst + A8_SLICE * D, &tm_v, 0, within, 0, put.at.h, page, &full[put_slot]);
-          }
-        } else {
-          tma_load_5d(dst, &tm_k, 0, within, 0, put.at.h, page, &full[put_slot]);
-          tma_load_5d(dst + A8_SLICE * D, &tm_v, 0, within, 0, put.at.h, page, &full[put_slot]);
+      if (mine) {
+        uint8_t* dst = ring + put_slot * STAGE + lane * box * (D == 64 ? 64 : 128);
+        const int cols = D == 256 && box < KEYS ? 2 : 1;  // a box of fewer keys would pack its blocks of 128 bytes closer
+#pragma unroll 1
+        for (int e = 0; e < cols; ++e) {
+          tma_load_5d(dst + e * (KEYS * 128), &tm_k, 0, box_row, e, put.at.h, box_page, &full[put_slot]);
+          tma_load_5d(dst + KEYS * D + e * (KEYS * 128), &tm_v, 0, box_row, e, put.at.h, box_page, &full[put_slot]);
         }
       }
-      // the scales of two groups, lanes 0 and 1 for K and 2 and 3 for V
-      const int g = lane & 1, pg = __shfl_sync(0xffffffffu, page, g), in = __shfl_sync(0xffffffffu, within, g);
-      if (lane < 4) {
+      // the groups' scales: K's by lanes 0 .. GROUPS - 1, V's by lanes 4 ..
+      const int g = lane & 3, pg = __shfl_sync(0xffffffffu, page, g), in = __shfl_sync(0xffffffffu, within, g);
+      if (lane < 8 && g < GROUPS) {
         const bool there = groups >> g & 1;
         const int64_t at = there ? ((int64_t)pg * c.blocks + c.block_div.div(in)) * a.hkv + put.at.h : 0;
-        cp_async4(smem_u32(scales + put_slot * 4 + lane), (lane < 2 ? c.ks : c.vs) + at, there);
+        cp_async4(smem_u32(scales + put_slot * 8 + lane), (lane < 4 ? c.ks : c.vs) + at, there);
       }
       ++issued;
       if (++put_slot == ST) put_slot = 0;
@@ -380,7 +370,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   for (int s = 0; s < ST; ++s) copy();
 
   // ---- items ----
-  A8Walk<A8_ROWS, A8_SLICE> get;
+  A8Walk<A8_ROWS, KEYS> get;
   get.start(a, G, lot.from);
   int64_t unit = lot.begin;
   int slot = 0, taken = 0;
@@ -472,15 +462,17 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       ++taken;
       const int base = get.base(i);
       const uint8_t* kb = ring + slot * STAGE;
-      const uint8_t* vb = kb + A8_SLICE * D;
-      float s[2][4];
+      const uint8_t* vb = kb + KEYS * D;
+      float s[GROUPS][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+      for (int n = 0; n < GROUPS; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
       for (int i4 = 0; i4 < D / 64; ++i4) {
-        uint4 kw[2];
+        uint4 kw[GROUPS];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < GROUPS; ++n)
           kw[n] = *reinterpret_cast<const uint4*>(kb + a8_at<D>(n * 8 + a8_key<D>(x8), quad + 4 * i4));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -488,29 +480,32 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
           if constexpr (D == 256) f = q_mine[(i4 * 4 + q) * 32];
           else f = qf[i4 * 4 + q];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int n = 0; n < GROUPS; ++n) {
             const uint32_t w = q == 0 ? kw[n].x : q == 1 ? kw[n].y : q == 2 ? kw[n].z : kw[n].w;
             mma16<T>(s[n], f, f8_half2(w & 0xffffu), f8_half2(w >> 16));
           }
         }
       }
-      const float4 sc = *reinterpret_cast<const float4*>(scales + slot * 4);  // ks 0, 1, vs 0, 1
-      const float ks[2] = {sc.x, sc.y};
-      // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write
-      const float vs[2] = {fminf(fmaxf(sc.z, 0x1p-100f), 0x1p120f), fminf(fmaxf(sc.w, 0x1p-100f), 0x1p120f)};
-      const bool special = base > sure - A8_SLICE || (a.window && base <= low);
-      uint32_t seen = 0xff;
+      float ks[GROUPS], vs[GROUPS];
+#pragma unroll
+      for (int n = 0; n < GROUPS; ++n) {
+        ks[n] = scales[slot * 8 + n];
+        // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write
+        vs[n] = fminf(fmaxf(scales[slot * 8 + 4 + n], 0x1p-100f), 0x1p120f);
+      }
+      const bool special = base > sure - KEYS || (a.window && base <= low);
+      uint32_t seen = ~0u;
       if (special) {
         seen = 0;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < GROUPS; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (a8_sees(a, r, e < 2 ? ta : tb, e < 2 ? pa : pb, base + n * 8 + a8_key<D>(2 * quad + (e & 1)))) seen |= 1u << (4 * n + e);
       }
       float top_a = -INFINITY, top_b = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < GROUPS; ++n) {
         const float lv = __log2f(vs[n]), fa = scale_a * ks[n], fb = scale_b * ks[n];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -548,23 +543,24 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       }
       const float off_a = ma == -INFINITY ? 0.f : A8_LIFT - ma, off_b = mb == -INFINITY ? 0.f : A8_LIFT - mb;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < GROUPS; ++n) {
         const float rv = 1.0f / vs[n];
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (e < 2 ? off_a : off_b));
         la = fmaf(s[n][0] + s[n][1], rv, la);
         lb = fmaf(s[n][2] + s[n][3], rv, lb);
       }
-      const uint4 p = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
-                                 pack_half2(s[1][2], s[1][3]));
       // O += P V: of the keys in columns 2 quad and 2 quad + 1 of both halves, the dims of piece a8_piece_of(x8) of each 128
       constexpr int WORDS = D == 64 ? 2 : 4;
 #pragma unroll
-      for (int blk = 0; blk < BLOCKS; ++blk) {
+      for (int part = 0; part < KEYS / 16 * BLOCKS; ++part) {
+        const int blk = part % BLOCKS, kh = part / BLOCKS;  // of 128 dims, of 16 keys
+        const uint4 p = make_uint4(pack_half2(s[2 * kh][0], s[2 * kh][1]), pack_half2(s[2 * kh][2], s[2 * kh][3]),
+                                   pack_half2(s[2 * kh + 1][0], s[2 * kh + 1][1]), pack_half2(s[2 * kh + 1][2], s[2 * kh + 1][3]));
         uint32_t vw[4][WORDS];
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
-          const int k = a8_key<D>(2 * quad + (k4 & 1)) + (k4 >> 1) * 8;
+          const int k = a8_key<D>(2 * quad + (k4 & 1)) + (k4 >> 1) * 8 + 16 * kh;
           if constexpr (D == 64) {
             const uint2 y = *reinterpret_cast<const uint2*>(vb + a8_at<D>(k, x8 >> 1) + (x8 & 1) * 8);
             vw[k4][0] = y.x;
@@ -590,7 +586,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
           uint4 see;  // 1 where a row sees a key
           uint32_t* f = reinterpret_cast<uint32_t*>(&see);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = (seen >> (2 * e) & 1 ? 0x3c00u : 0u) | (seen >> (2 * e + 1) & 1 ? 0x3c000000u : 0u);
+          for (int e = 0; e < 4; ++e) f[e] = (seen >> (8 * kh + 2 * e) & 1 ? 0x3c00u : 0u) | (seen >> (8 * kh + 2 * e + 1) & 1 ? 0x3c000000u : 0u);
 #pragma unroll
           for (int w = 0; w < WORDS; ++w) {
             uint32_t ind[4];  // 1.0 where a code is NaN, which becomes 0

@@ -491,10 +491,14 @@ def test_attention_no_request_and_bad_lengths(D):
     assert int(err.item()) == 5
     blank = [0, 1, 2, 3] + [4 + 2, 4 + 3, 4 + 4] + [4 + 6, 4 + 7] + list(range(12, 21))
     assert bool((out[blank] == 0).all()) and bool(torch.isneginf(lse[blank]).all())
-    for i in (0, 1, 5):
-        assert torch.equal(out[4 + i], good[0][i]) and torch.equal(lse[4 + i], good[1][i])
+    # where a request's keys are cut, and so the order of its sums, goes by all requests of a call
+    ref = attention_reference(s, 0.125)
+    keep = [0, 1, 5]
+    check_attention((out[4:][keep], lse[4:][keep]), [x[keep] for x in ref], F16)
+    check_attention(good, ref, F16)
     out, lse = D.attention_8bit(s["q"], s["kc"], s["vc"], s["ks"], s["vs"], s["table"], s["lens"], s["cu"], 0.125, 2, err=err.zero_())
-    assert int(err.item()) == 5 and bool((out[2:5] == 0).all()) and torch.equal(out[:2], good[0][:2])
+    assert int(err.item()) == 5 and bool((out[2:5] == 0).all())
+    check_attention((out[:2], lse[:2]), [x[:2] for x in ref], F16)
     out, lse = D.attention_8bit(s["q"], s["kc"], s["vc"], s["ks"], s["vs"], s["table"][:0], s["lens"][:0], s["cu"][:1], 0.125, 2)
     assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
 
