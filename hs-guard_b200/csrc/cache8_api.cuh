@@ -62,7 +62,8 @@ int make_codes_map(CUtensorMap* map, const uint8_t* base, const Cache8& c, int d
   const cuuint32_t box[5] = {(cuuint32_t)wide, (cuuint32_t)keys, (cuuint32_t)cols, 1, 1}, one[5] = {1, 1, 1, 1, 1};
   CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<uint8_t*>(base), dims, strides, box, one,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        // (256 bytes at a time brought 337 MB for 195 where a row has 64 and the heads of a token lie together)
+                        dim == 64 ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (codes) failed (%d)", (int)r);
   return HSG_OK;
 }
@@ -91,9 +92,14 @@ int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
       (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
     return rc;
   CU(cudaFuncSetAttribute(attn8_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
-  CU(launch_k(attn8_kernel<D, T>, dim3(A8_BLOCKS), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box, splits, partials));
-  const int64_t most = std::min<int64_t>(A8_ROWS, (int64_t)p.max_new * (p.hq / p.hkv));  // rows of an item
-  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3(PIECES, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),
+  // as many thread blocks as can have a piece: items, and the slices that one can see at most
+  const int64_t group = p.hq / p.hkv, reach = std::min<int64_t>((int64_t)p.width * p.cache.page, p.window ? (int64_t)p.window + p.sinks + p.max_new : INT64_MAX);
+  const int64_t items = std::min<int64_t>(p.tokens * group, (p.tokens * group) / A8_ROWS + p.rows) * p.hkv;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(PIECES, items * (reach / a8_slice(D) + 4 + A8_COST) / (A8_COST + 1) + 1));
+  CU(launch_k(attn8_kernel<D, T>, dim3((unsigned)std::min<int64_t>(A8_BLOCKS, pieces)), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box,
+              splits, partials));
+  const int64_t most = std::min<int64_t>(A8_ROWS, p.max_new * group);  // rows of an item
+  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3((unsigned)pieces, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),
               dim3(A8J_THREADS), 0, st, true, p, (const A8Split*)splits, (const float*)partials));
   return HSG_OK;
 }

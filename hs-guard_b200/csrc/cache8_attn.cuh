@@ -231,10 +231,15 @@ template <int D> __device__ __forceinline__ uint32_t a8_at(int k, int ch) {
   else return (ch >> 3) * (a8_slice(D) * 128) + (k >> 3) * 1024 + sw128_off(k & 7, ch & 7);
 }
 
-// Four codes as fp16, two pairs.
-__device__ __forceinline__ uint32_t f8_half2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Four codes as fp16: the lower two and the upper two.
+__device__ __forceinline__ void f8_halves(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(four));
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // What brings a row whose largest element is `most` to [2^14, 2^15), and back. A row of zeros, or of values below 2^-100, stays.
@@ -482,7 +487,9 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
 #pragma unroll
           for (int n = 0; n < GROUPS; ++n) {
             const uint32_t w = q == 0 ? kw[n].x : q == 1 ? kw[n].y : q == 2 ? kw[n].z : kw[n].w;
-            mma16<T>(s[n], f, f8_half2(w & 0xffffu), f8_half2(w >> 16));
+            uint32_t b0, b1;
+            f8_halves(w, b0, b1);
+            mma16<T>(s[n], f, b0, b1);
           }
         }
       }
@@ -508,10 +515,16 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       for (int n = 0; n < GROUPS; ++n) {
         const float lv = __log2f(vs[n]), fa = scale_a * ks[n], fb = scale_b * ks[n];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = fmaf(s[n][e], e < 2 ? fa : fb, lv);
-          if (special && !(seen >> (4 * n + e) & 1)) s[n][e] = -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], e < 2 ? fa : fb, lv);
+      }
+      if (special) {
+#pragma unroll
+        for (int n = 0; n < GROUPS; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = seen >> (4 * n + e) & 1 ? s[n][e] : -INFINITY;
+      }
+#pragma unroll
+      for (int n = 0; n < GROUPS; ++n) {
         top_a = fmaxf(top_a, fmaxf(s[n][0], s[n][1]));
         top_b = fmaxf(top_b, fmaxf(s[n][2], s[n][3]));
       }
@@ -544,7 +557,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       const float off_a = ma == -INFINITY ? 0.f : A8_LIFT - ma, off_b = mb == -INFINITY ? 0.f : A8_LIFT - mb;
 #pragma unroll
       for (int n = 0; n < GROUPS; ++n) {
-        const float rv = 1.0f / vs[n];
+        const float rv = rcp_approx(vs[n]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (e < 2 ? off_a : off_b));
         la = fmaf(s[n][0] + s[n][1], rv, la);
@@ -601,7 +614,10 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
               const uint32_t sel = e < 2 ? 0x5140u : 0x7362u;
               const uint32_t b0 = __byte_perm(ind[0], ind[1], sel), b1 = __byte_perm(ind[2], ind[3], sel);
               float hits[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16<T>(hits, see, f8_half2(e & 1 ? b0 >> 16 : b0 & 0xffffu), f8_half2(e & 1 ? b1 >> 16 : b1 & 0xffffu));
+              uint32_t x0, x1, y0, y1;
+              f8_halves(b0, x0, x1);
+              f8_halves(b1, y0, y1);
+              mma16<T>(hits, see, e & 1 ? x1 : x0, e & 1 ? y1 : y0);
 #pragma unroll
               for (int z = 0; z < 4; ++z)
                 if (hits[z] > 0.f) o[16 * blk + 4 * w + e][z] = __int_as_float(0x7fffffff);
@@ -614,8 +630,11 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
           for (int pr = 0; pr < 2; ++pr) {
             const uint32_t sel = pr == 0 ? 0x5140u : 0x7362u;
             const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], sel), b1 = __byte_perm(vw[2][w], vw[3][w], sel);
-            mma16<T>(o[16 * blk + 4 * w + 2 * pr], p, f8_half2(b0 & 0xffffu), f8_half2(b1 & 0xffffu));
-            mma16<T>(o[16 * blk + 4 * w + 2 * pr + 1], p, f8_half2(b0 >> 16), f8_half2(b1 >> 16));
+            uint32_t x0, x1, y0, y1;
+            f8_halves(b0, x0, x1);
+            f8_halves(b1, y0, y1);
+            mma16<T>(o[16 * blk + 4 * w + 2 * pr], p, x0, y0);
+            mma16<T>(o[16 * blk + 4 * w + 2 * pr + 1], p, x1, y1);
           }
         }
       }
@@ -627,6 +646,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       }
     }
     if (!__all_sync(0xffffffffu, ok)) break;
+    if (!put_more) pdl_trigger();  // the join's blocks may come while the last sums are written
     // ---- the item, or this piece's part of it ----
 #pragma unroll
     for (int d = 1; d < 4; d <<= 1) {
@@ -729,14 +749,20 @@ __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_co
   float l = 0.f, o[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
-  for (int p = c; p <= s.last; ++p) {
-    const float* x = part(p);
-    const float2 ml = *reinterpret_cast<const float2*>(x + ROWS * D + 2 * row);
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
-    const float w = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - m);  // -inf with a sum: NaN, which stays
-    l += ml.y * w;
+  for (int p0 = c; p0 <= s.last; p0 += 32) {
+    // lane i: what the i-th of these parts counts (one that saw nothing: 0; -inf with a sum is NaN, which stays)
+    const int p1 = p0 + lane;
+    const float2 ml = p1 <= s.last ? *reinterpret_cast<const float2*>(part(p1) + ROWS * D + 2 * row) : make_float2(-INFINITY, 0.f);
+    const float by = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2_approx(ml.x - m);
+    l += warp_sum(by * ml.y);
+    const int n = min(32, s.last + 1 - p0);
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float w = __shfl_sync(0xffffffffu, by, k);
+      const float* x = part(p0 + k) + row * D + lane;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] += w * x[row * D + e * 32 + lane];
+      for (int e = 0; e < D / 32; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e * 32], o[e]);
+    }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   const int64_t orow = (int64_t)(t0 + tok) * a.hq + s.h * G + at - tok * G;

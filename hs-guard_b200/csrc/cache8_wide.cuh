@@ -288,8 +288,7 @@ attn8_wide_kernel(const __grid_constant__ Attn8Args a, A8Split* splits, float* p
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[2 * e] = f8_half2(w[e] & 0xffffu);
-          y[2 * e + 1] = f8_half2(w[e] >> 16);
+          f8_halves(w[e], y[2 * e], y[2 * e + 1]);
         }
         *reinterpret_cast<uint4*>(to + at0 + n * (STRIDE / 8 * NC * 1024)) = make_uint4(y[0], y[1], y[2], y[3]);
         *reinterpret_cast<uint4*>(to + at1 + n * (STRIDE / 8 * NC * 1024)) = make_uint4(y[4], y[5], y[6], y[7]);
