@@ -150,6 +150,11 @@ struct A8Walk {
   __device__ __forceinline__ int base(int tile) const { return (tile < s.lead ? tile : s.first + tile - s.lead) * TILE; }
 };
 
+// Quotient of numbers that are not negative; mostly both are short.
+__device__ __forceinline__ int64_t a8_div(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
 // A piece of the line: where it begins (item and tile), where that item begins on the line, and where the piece ends. An item is
 // its tiles and `cost` more; a piece holds at least one tile, or nothing (b < 0).
 struct A8Lot {
@@ -183,9 +188,9 @@ __device__ __forceinline__ int64_t a8_lots(const Attn8Args& a, int G, int cost, 
     if (w < warp) before += room[w];
     units += room[w];
   }
-  const int64_t step = max((int64_t)(cost + 1), (units + SUBS * A8_BLOCKS - 1) / (SUBS * A8_BLOCKS));
+  const int64_t step = max((int64_t)(cost + 1), a8_div(units + SUBS * A8_BLOCKS - 1, SUBS * A8_BLOCKS));
   // the first piece of this block that begins at or after this thread's first unit
-  int64_t s0 = before > block * step ? ((before + step - 1) / step - block + A8_BLOCKS - 1) / A8_BLOCKS : 0;
+  int64_t s0 = before > block * step ? a8_div(a8_div(before + step - 1, step) - block + A8_BLOCKS - 1, A8_BLOCKS) : 0;
   if (mine > 0 && s0 < SUBS && (s0 * A8_BLOCKS + block) * step < before + mine) {
     int64_t at = before;
     for (int b = rb0; b < rb1; ++b) {
@@ -194,7 +199,7 @@ __device__ __forceinline__ int64_t a8_lots(const Attn8Args& a, int G, int cost, 
       for (; s0 < SUBS; ++s0) {
         const int64_t w0 = (s0 * A8_BLOCKS + block) * step;
         if (w0 >= at + all) break;
-        const int h = (int)((w0 - at) / one);
+        const int h = (int)a8_div(w0 - at, one);
         int64_t u = at + h * one;
         for (int k = 0; k < r.blocks; ++k) {
           const int n = a8_span<ROWS, TILE>(a, r, G, k).n + cost;
@@ -294,6 +299,9 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     prefetch_tmap(&tm_v);
   }
   pdl_wait();
+  // the join's blocks may come: at once where most of the device is idle, else when this warp's last slice is on its way (352
+  // conversations take 61 and 64 us, one 21.5 and 15.5)
+  if (gridDim.x < A8_BLOCKS) pdl_trigger();
   if (lane == 0) splits[piece].last = -1;
   const int64_t step = a8_lots<A8_ROWS, KEYS, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
   const A8Lot lot = lots[warp];
@@ -646,7 +654,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       }
     }
     if (!__all_sync(0xffffffffu, ok)) break;
-    if (!put_more) pdl_trigger();  // the join's blocks may come while the last sums are written
+    if (!put_more) pdl_trigger();
     // ---- the item, or this piece's part of it ----
 #pragma unroll
     for (int d = 1; d < 4; d <<= 1) {
@@ -692,7 +700,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       }
     }
     if (lane == 0 && i0 == 0 && i1 < sp.n)
-      splits[piece] = A8Split{get.at.b, get.at.h, get.at.block, (int)((unit + A8_COST + sp.n - 1) / step), part_slot, {0, 0, 0}};
+      splits[piece] = A8Split{get.at.b, get.at.h, get.at.block, (int)a8_div(unit + A8_COST + sp.n - 1, step), part_slot, {0, 0, 0}};
     unit += sp.n + A8_COST;
     if (unit + A8_COST >= lot.end) break;
     get.next_item(a, G);
@@ -743,25 +751,36 @@ __global__ void __launch_bounds__(A8J_THREADS) attn8_join_kernel(const __grid_co
   if (tok >= a.cu[s.b + 1] - t0) return;
   const size_t size = a8_partial_floats(D, ROWS);
   auto part = [&](int p) { return partials + (p == c ? (size_t)s.first_slot : 2 * (size_t)p) * size; };
-  float m = -INFINITY;
-  for (int p = c + lane; p <= s.last; p += 32) m = fmaxf(m, part(p)[ROWS * D + 2 * row]);
+  auto sums = [&](int p) {
+    return p <= s.last ? *reinterpret_cast<const float2*>(part(p) + ROWS * D + 2 * row) : make_float2(-INFINITY, 0.f);
+  };
+  const float2 first = sums(c + lane);
+  float m = first.x;
+  for (int p = c + 32 + lane; p <= s.last; p += 32) m = fmaxf(m, sums(p).x);
   m = warp_max(m);
   float l = 0.f, o[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
   for (int p0 = c; p0 <= s.last; p0 += 32) {
-    // lane i: what the i-th of these parts counts (one that saw nothing: 0; -inf with a sum is NaN, which stays)
-    const int p1 = p0 + lane;
-    const float2 ml = p1 <= s.last ? *reinterpret_cast<const float2*>(part(p1) + ROWS * D + 2 * row) : make_float2(-INFINITY, 0.f);
+    // lane i: what the i-th of these parts counts (-inf with a sum is NaN, which stays)
+    const float2 ml = p0 == c ? first : sums(p0 + lane);
     const float by = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2_approx(ml.x - m);
     l += warp_sum(by * ml.y);
     const int n = min(32, s.last + 1 - p0);
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const float w = __shfl_sync(0xffffffffu, by, k);
-      const float* x = part(p0 + k) + row * D + lane;
+    for (int k0 = 0; k0 < n; k0 += 8) {  // parts beyond the last: the last again, for nothing
+      float x[8][D / 32];
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, x[e * 32], o[e]);
+      for (int k = 0; k < 8; ++k) {
+        const float* from = part(min(p0 + k0 + k, s.last)) + row * D + lane;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) x[k][e] = from[e * 32];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, by, k0 + k);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) o[e] = k0 + k < n ? fmaf(w, x[k][e], o[e]) : o[e];
+      }
     }
   }
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
