@@ -68,6 +68,30 @@ int make_codes_map(CUtensorMap* map, const uint8_t* base, const Cache8& c, int d
   return HSG_OK;
 }
 
+template <int D, int NR, typename T>
+int launch_attn8_narrow(const Attn8Args& p, A8Split* splits, cudaStream_t st) {
+  constexpr int PIECES = A8_BLOCKS * A8_WARPS;
+  float* partials = reinterpret_cast<float*>(splits + PIECES);
+  int box = a8_slice(D);  // tokens of a TMA box: all of one page
+  while (p.cache.page % box) box /= 2;
+  const int cols = D == 256 && box == a8_slice(D) ? 2 : 1;
+  CUtensorMap k, v;
+  int rc;
+  if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||
+      (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
+    return rc;
+  CU(cudaFuncSetAttribute(attn8_kernel<D, NR, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
+  // as many thread blocks as can have a piece: items, and the slices that one can see at most
+  const int64_t group = p.hq / p.hkv, reach = std::min<int64_t>((int64_t)p.width * p.cache.page, p.window ? (int64_t)p.window + p.sinks + p.max_new : INT64_MAX);
+  const int64_t items = std::min<int64_t>(p.tokens * group, (p.tokens * group) / (8 * NR) + p.rows) * p.hkv;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(PIECES, items * (reach / a8_slice(D) + 4 + A8_COST) / (A8_COST + 1) + 1));
+  CU(launch_k(attn8_kernel<D, NR, T>, dim3((unsigned)std::min<int64_t>(A8_BLOCKS, pieces)), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box,
+              splits, partials));
+  const int64_t most = std::min<int64_t>(8 * NR, p.max_new * group);  // rows of an item
+  CU(launch_k(attn8_join_kernel<D, 8 * NR, T>, dim3((unsigned)pieces, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),
+              dim3(A8J_THREADS), 0, st, true, p, (const A8Split*)splits, (const float*)partials));
+  return HSG_OK;
+}
 template <int D, typename T>
 int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   A8Split* splits = static_cast<A8Split*>(workspace);
@@ -81,27 +105,8 @@ int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
                 (const A8Split*)splits, (const float*)partials));
     return HSG_OK;
   }
-  constexpr int PIECES = A8_BLOCKS * A8_WARPS;
-  float* partials = reinterpret_cast<float*>(splits + PIECES);
-  int box = a8_slice(D);  // tokens of a TMA box: all of one page
-  while (p.cache.page % box) box /= 2;
-  const int cols = D == 256 && box == a8_slice(D) ? 2 : 1;
-  CUtensorMap k, v;
-  int rc;
-  if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||
-      (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
-    return rc;
-  CU(cudaFuncSetAttribute(attn8_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
-  // as many thread blocks as can have a piece: items, and the slices that one can see at most
-  const int64_t group = p.hq / p.hkv, reach = std::min<int64_t>((int64_t)p.width * p.cache.page, p.window ? (int64_t)p.window + p.sinks + p.max_new : INT64_MAX);
-  const int64_t items = std::min<int64_t>(p.tokens * group, (p.tokens * group) / A8_ROWS + p.rows) * p.hkv;
-  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(PIECES, items * (reach / a8_slice(D) + 4 + A8_COST) / (A8_COST + 1) + 1));
-  CU(launch_k(attn8_kernel<D, T>, dim3((unsigned)std::min<int64_t>(A8_BLOCKS, pieces)), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box,
-              splits, partials));
-  const int64_t most = std::min<int64_t>(A8_ROWS, p.max_new * group);  // rows of an item
-  CU(launch_k(attn8_join_kernel<D, A8_ROWS, T>, dim3((unsigned)pieces, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),
-              dim3(A8J_THREADS), 0, st, true, p, (const A8Split*)splits, (const float*)partials));
-  return HSG_OK;
+  // blocks of 8 rows where none has more
+  return (int64_t)p.max_new * (p.hq / p.hkv) <= 8 ? launch_attn8_narrow<D, 1, T>(p, splits, st) : launch_attn8_narrow<D, 2, T>(p, splits, st);
 }
 template <typename T>
 int launch_attn8_dim(const Attn8Args& p, int dim, void* ws, cudaStream_t st) {

@@ -31,9 +31,11 @@ struct Attn8Args {
   int* err;
 };
 
-// This kernel is for few rows a key head, where reading the cache is all that counts; products are warp-level (16 rows by 8
-// keys by 16 dims), since the 128 rows of a tcgen05 product would be padding. A request's rows of a key head, row r = (token
-// r / G, query head r % G), in blocks of 16, and the slices of 32 keys (16 at head dim 256) that such a block can see are an item; all items are one
+// This kernel is for few rows a key head, where reading the cache is all that counts; products are warp-level, since the 128 rows
+// of a tcgen05 product would be padding, and have keys or dims as their 16 rows (S^T = K Q^T, O^T = V^T P^T) and 8 queries as
+// their columns, so that 8 rows or fewer waste nothing (with queries as the 16 rows it took twice the products, accumulators and
+// exponentials: 352 conversations 63 us). A request's rows of a key head, row r = (token
+// r / G, query head r % G), in blocks of 8 or 16, and the slices of 32 keys (16 at head dim 256) that such a block can see are an item; all items are one
 // line that is cut into equal pieces, one a warp, eight warps an SM, whatever the requests' lengths. Warps do not meet: each has
 // its ring of slices, which it fills itself ahead of its use (TMA, one box, or as many as a page's size takes), its own running maximum, sums and accumulators. An item that lies in one piece is written out; of one that is cut, each
 // piece leaves its sums in the workspace, and attn8_join_kernel joins them in piece order, so results do not depend on timing.
@@ -50,7 +52,7 @@ struct Attn8Args {
 // 128 and 256 (twice at 64, for V).
 constexpr int A8_THREADS = 256;
 constexpr int A8_WARPS = 8;
-constexpr int A8_ROWS = 16;
+constexpr int A8_ROWS = 16;         // of a block, at most
 constexpr int A8_BLOCKS = 148;      // one thread block an SM
 constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
 constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
@@ -58,10 +60,9 @@ constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
 __host__ __device__ constexpr int a8_slice(int dim) { return dim == 256 ? 16 : 32; }  // keys
 __host__ __device__ constexpr int a8_stage(int dim) { return 2 * a8_slice(dim) * dim; }
 __host__ __device__ constexpr int a8_stages(int dim) { return dim == 64 ? 6 : dim == 128 ? 3 : 2; }
-__host__ __device__ constexpr int a8_q_bytes(int dim) { return dim == 256 ? A8_ROWS * dim * 2 : 0; }  // else in registers
-// a warp's ring, query fragments, scales and barriers; where the pieces begin
+// a warp's ring, scales and barriers; where the pieces begin
 __host__ __device__ constexpr int a8_smem(int dim) {
-  return 1024 + A8_WARPS * (a8_stages(dim) * (a8_stage(dim) + 40) + a8_q_bytes(dim)) + 1024;
+  return 1024 + A8_WARPS * a8_stages(dim) * (a8_stage(dim) + 40) + 1024;
 }
 __host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
 struct A8Split {  // an item that begins in a piece and ends in a later one
@@ -254,7 +255,14 @@ __device__ __forceinline__ void a8_row_scale(float most, float& up, float& back)
   back = __int_as_float((127 - by) << 23);
 }
 
-template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+// An 8 x 8 matrix of 16-bit numbers, a row of two numbers a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   mma_f16_16816(d, a.x, a.y, a.z, a.w, b0, b1);
 }
 
@@ -274,16 +282,15 @@ __device__ __forceinline__ bool a8_sees(const Attn8Args& a, const A8Req& r, int 
   return !a.window || at > p - a.window || at < a.sinks;
 }
 
-template <int D, typename T>
+template <int D, int NR, typename T>
 __global__ void __launch_bounds__(A8_THREADS, 1)
 attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Attn8Args a,
              int box, A8Split* splits, float* partials) {
-  constexpr int KEYS = a8_slice(D), GROUPS = KEYS / 8, STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 8,
-                BLOCKS = D == 256 ? 2 : 1;
+  constexpr int KEYS = a8_slice(D), GROUPS = KEYS / 8, STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 16,
+                BLOCKS = D == 256 ? 2 : 1, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t a8_smem_raw[];
   uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a8_smem_raw) + 1023) & ~uintptr_t(1023));  // [warps][ST][K, V]
-  uint4* q_frags = reinterpret_cast<uint4*>(rings + A8_WARPS * ST * STAGE);               // [warps][steps][32 lanes], head dim 256
-  float* ring_scales = reinterpret_cast<float*>(q_frags + A8_WARPS * a8_q_bytes(D) / 16);  // [warps][ST][ks, vs]
+  float* ring_scales = reinterpret_cast<float*>(rings + A8_WARPS * ST * STAGE);            // [warps][ST][ks, vs]
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + A8_WARPS * ST * 8);           // [warps][ST] a slice has landed
   A8Lot* lots = reinterpret_cast<A8Lot*>(bars + A8_WARPS * ST);                            // [warps]
   int64_t* scan = reinterpret_cast<int64_t*>(lots + A8_WARPS);
@@ -303,14 +310,14 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   // conversations take 61 and 64 us, one 21.5 and 15.5)
   if (gridDim.x < A8_BLOCKS) pdl_trigger();
   if (lane == 0) splits[piece].last = -1;
-  const int64_t step = a8_lots<A8_ROWS, KEYS, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
+  const int64_t step = a8_lots<ROWS, KEYS, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
   const A8Lot lot = lots[warp];
   if (lot.from.b < 0) return;
   // of an item that begins at `unit` on the line, slices up to this lie in the piece
   auto part_end = [&](int64_t unit, int n) { return (int)min((int64_t)n, max((int64_t)0, lot.end - unit - A8_COST)); };
 
   // ---- the copying side: a walk of its own, ahead by the ring's stages ----
-  A8Walk<A8_ROWS, KEYS> put;
+  A8Walk<ROWS, KEYS> put;
   put.start(a, G, lot.from);
   int64_t put_unit = lot.begin;
   int put_i = put.at.i, put_i1 = part_end(put_unit, put.s.n);
@@ -383,7 +390,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   for (int s = 0; s < ST; ++s) copy();
 
   // ---- items ----
-  A8Walk<A8_ROWS, KEYS> get;
+  A8Walk<ROWS, KEYS> get;
   get.start(a, G, lot.from);
   int64_t unit = lot.begin;
   int slot = 0, taken = 0;
@@ -394,78 +401,74 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     const int i0 = get.at.i, i1 = part_end(unit, get.s.n);
     const A8Req r = get.r;
     const A8Span sp = get.s;
-    const int row0 = get.at.block * A8_ROWS, old = r.len - r.n;
-    const int ta = (row0 + x8) / G, tb = (row0 + x8 + 8) / G;
-    const bool valid_a = ta < r.n, valid_b = tb < r.n;
-    // queries as fragments: step s takes dims 16 (quad + 4 (s / 4)) + 4 (s % 4) + 0 .. 3 of rows x8 and x8 + 8
-    uint4 qf[D == 256 ? 1 : STEPS];
-    uint4* const q_mine = q_frags + (warp * STEPS) * 32 + lane;
-    float scale_a = to_log2, scale_b = to_log2;
-    {
-      uint32_t w[2][D / 64][8];
+    const int row0 = get.at.block * ROWS, old = r.len - r.n;
+    // queries as columns: step s takes dims 16 (quad + 4 (s / 4)) + 4 (s % 4) + 0 .. 3 of row x8 of each 8
+    uint2 qf[STEPS][NR];
+    // what a lane's scores belong to: rows 2 quad and 2 quad + 1 of each 8
+    float scale[NR][2];
+    int tok[NR][2], pos[NR][2];
+    int low = -1;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      const int at = row0 + 8 * nr + x8, t = at / G;
+      const T* src = (const T*)a.q + (int64_t)(r.t0 + t) * a.q_ts + (int64_t)(get.at.h * G + at - t * G) * a.q_hs + quad * 16;
+      uint32_t w[D / 64][8];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+        if (t < r.n) {
+          lo = reinterpret_cast<const uint4*>(src + 64 * i)[0];
+          hi = reinterpret_cast<const uint4*>(src + 64 * i)[1];
+        }
+        w[i][0] = lo.x; w[i][1] = lo.y; w[i][2] = lo.z; w[i][3] = lo.w;
+        w[i][4] = hi.x; w[i][5] = hi.y; w[i][6] = hi.z; w[i][7] = hi.w;
+      }
+      float back = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float x = fabsf(__uint_as_float(w[i][k] << 16)), y = fabsf(__uint_as_float(w[i][k] & 0xffff0000u));
+            most = fmaxf(most, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+          }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        float up;
+        a8_row_scale(most, up, back);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            w[i][k] = pack_half2(__uint_as_float(w[i][k] << 16) * up, __uint_as_float(w[i][k] & 0xffff0000u) * up);
+      }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) qf[s][nr] = make_uint2(w[s / 4][2 * (s % 4)], w[s / 4][2 * (s % 4) + 1]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int t = e ? tb : ta, g = row0 + x8 + 8 * e - t * G;
-        const T* src = (const T*)a.q + (int64_t)(r.t0 + t) * a.q_ts + (int64_t)(get.at.h * G + g) * a.q_hs + quad * 16;
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-          if (e ? valid_b : valid_a) {
-            lo = reinterpret_cast<const uint4*>(src + 64 * i)[0];
-            hi = reinterpret_cast<const uint4*>(src + 64 * i)[1];
-          }
-          w[e][i][0] = lo.x; w[e][i][1] = lo.y; w[e][i][2] = lo.z; w[e][i][3] = lo.w;
-          w[e][i][4] = hi.x; w[e][i][5] = hi.y; w[e][i][6] = hi.z; w[e][i][7] = hi.w;
+        scale[nr][e] = to_log2 * __shfl_sync(0xffffffffu, back, (2 * quad + e) * 4);
+        tok[nr][e] = (row0 + 8 * nr + 2 * quad + e) / G;
+        pos[nr][e] = 0;
+        if (a.window && tok[nr][e] < r.n) {
+          pos[nr][e] = a.positions ? a.positions[r.t0 + tok[nr][e]] : old + tok[nr][e];
+          low = max(low, pos[nr][e] - a.window);
         }
       }
-      if constexpr (!std::is_same<T, __half>::value) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float most = 0.f;
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float x = fabsf(__uint_as_float(w[e][i][k] << 16)), y = fabsf(__uint_as_float(w[e][i][k] & 0xffff0000u));
-              most = fmaxf(most, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
-            }
-#pragma unroll
-          for (int d = 1; d < 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-          float up, back;
-          a8_row_scale(most, up, back);
-          (e ? scale_b : scale_a) *= back;
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              w[e][i][k] = pack_half2(__uint_as_float(w[e][i][k] << 16) * up, __uint_as_float(w[e][i][k] & 0xffff0000u) * up);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const uint4 f = make_uint4(w[0][s / 4][2 * (s % 4)], w[1][s / 4][2 * (s % 4)], w[0][s / 4][2 * (s % 4) + 1], w[1][s / 4][2 * (s % 4) + 1]);
-        if constexpr (D == 256) q_mine[s * 32] = f;
-        else qf[s] = f;
-      }
-    }
-    int pa = 0, pb = 0;
-    if (a.window) {
-      pa = valid_a ? (a.positions ? a.positions[r.t0 + ta] : old + ta) : 0;
-      pb = valid_b ? (a.positions ? a.positions[r.t0 + tb] : old + tb) : 0;
     }
     // keys below `sure` and above `low` are seen by every row
     const int sure = a.mask ? old : old + row0 / G + 1;
-    int low = -1;
-    if (a.window) {
-      low = max(valid_a ? pa - a.window : -1, valid_b ? pb - a.window : -1);
-      low = __reduce_max_sync(0xffffffffu, low);
+    if (a.window) low = __reduce_max_sync(0xffffffffu, low);
+    float o[NT][NR][4], m[NR][2], l[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][nr][e] = 0.f;
+      m[nr][0] = m[nr][1] = -INFINITY;
+      l[nr][0] = l[nr][1] = 0.f;
     }
-    float o[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-    float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
       cp_async_wait<ST - 1>();
@@ -476,108 +479,111 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       const int base = get.base(i);
       const uint8_t* kb = ring + slot * STAGE;
       const uint8_t* vb = kb + KEYS * D;
-      float s[GROUPS][4];
+      // S^T: element e of a lane is key a8_key(x8) (+ 8 from e = 2 on) of 16, row 2 quad + e % 2
+      float s[KEYS / 16][NR][4];
 #pragma unroll
-      for (int n = 0; n < GROUPS; ++n)
+      for (int kh = 0; kh < KEYS / 16; ++kh)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[kh][nr][e] = 0.f;
 #pragma unroll
       for (int i4 = 0; i4 < D / 64; ++i4) {
-        uint4 kw[GROUPS];
 #pragma unroll
-        for (int n = 0; n < GROUPS; ++n)
-          kw[n] = *reinterpret_cast<const uint4*>(kb + a8_at<D>(n * 8 + a8_key<D>(x8), quad + 4 * i4));
+        for (int kh = 0; kh < KEYS / 16; ++kh) {
+          const uint4 k0 = *reinterpret_cast<const uint4*>(kb + a8_at<D>(16 * kh + a8_key<D>(x8), quad + 4 * i4));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(kb + a8_at<D>(16 * kh + 8 + a8_key<D>(x8), quad + 4 * i4));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4 f;
-          if constexpr (D == 256) f = q_mine[(i4 * 4 + q) * 32];
-          else f = qf[i4 * 4 + q];
+          for (int q = 0; q < 4; ++q) {
+            uint4 f;
+            f8_halves(w0[q], f.x, f.z);
+            f8_halves(w1[q], f.y, f.w);
 #pragma unroll
-          for (int n = 0; n < GROUPS; ++n) {
-            const uint32_t w = q == 0 ? kw[n].x : q == 1 ? kw[n].y : q == 2 ? kw[n].z : kw[n].w;
-            uint32_t b0, b1;
-            f8_halves(w, b0, b1);
-            mma16<T>(s[n], f, b0, b1);
+            for (int nr = 0; nr < NR; ++nr) mma16(s[kh][nr], f, qf[i4 * 4 + q][nr].x, qf[i4 * 4 + q][nr].y);
           }
         }
       }
-      float ks[GROUPS], vs[GROUPS];
+      float vs[GROUPS];
 #pragma unroll
       for (int n = 0; n < GROUPS; ++n) {
-        ks[n] = scales[slot * 8 + n];
         // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write
         vs[n] = fminf(fmaxf(scales[slot * 8 + 4 + n], 0x1p-100f), 0x1p120f);
+        const float ks = scales[slot * 8 + n], lv = __log2f(vs[n]);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[n / 2][nr][2 * (n & 1) + e] = fmaf(s[n / 2][nr][2 * (n & 1) + e], scale[nr][e] * ks, lv);
       }
       const bool special = base > sure - KEYS || (a.window && base <= low);
-      uint32_t seen = ~0u;
+      uint32_t seen = ~0u;  // bit 8 of a half, 4 of 8 rows, element
       if (special) {
         seen = 0;
 #pragma unroll
-        for (int n = 0; n < GROUPS; ++n)
+        for (int kh = 0; kh < KEYS / 16; ++kh)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (a8_sees(a, r, e < 2 ? ta : tb, e < 2 ? pa : pb, base + n * 8 + a8_key<D>(2 * quad + (e & 1)))) seen |= 1u << (4 * n + e);
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool see = a8_sees(a, r, tok[nr][e & 1], pos[nr][e & 1], base + 16 * kh + 8 * (e >> 1) + a8_key<D>(x8));
+              seen |= see ? 1u << (8 * kh + 4 * nr + e) : 0u;
+              s[kh][nr][e] = see ? s[kh][nr][e] : -INFINITY;
+            }
       }
-      float top_a = -INFINITY, top_b = -INFINITY;
+      float top[NR][2];
+      bool raise = false;
 #pragma unroll
-      for (int n = 0; n < GROUPS; ++n) {
-        const float lv = __log2f(vs[n]), fa = scale_a * ks[n], fb = scale_b * ks[n];
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], e < 2 ? fa : fb, lv);
-      }
-      if (special) {
-#pragma unroll
-        for (int n = 0; n < GROUPS; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = seen >> (4 * n + e) & 1 ? s[n][e] : -INFINITY;
-      }
-#pragma unroll
-      for (int n = 0; n < GROUPS; ++n) {
-        top_a = fmaxf(top_a, fmaxf(s[n][0], s[n][1]));
-        top_b = fmaxf(top_b, fmaxf(s[n][2], s[n][3]));
-      }
+        for (int e = 0; e < 2; ++e) {
+          top[nr][e] = fmaxf(s[0][nr][e], s[0][nr][e + 2]);
+          if constexpr (KEYS == 32) top[nr][e] = fmaxf(top[nr][e], fmaxf(s[1][nr][e], s[1][nr][e + 2]));
+          raise |= top[nr][e] > m[nr][e] + A8_SLACK;
+        }
       // the maximum is raised only when a score exceeds it by 2^A8_SLACK
-      if (__any_sync(0xffffffffu, top_a > ma + A8_SLACK || top_b > mb + A8_SLACK)) {
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-          top_a = fmaxf(top_a, __shfl_xor_sync(0xffffffffu, top_a, d));
-          top_b = fmaxf(top_b, __shfl_xor_sync(0xffffffffu, top_b, d));
-        }
-        float by_a = 1.f, by_b = 1.f;
-        if (top_a > ma + A8_SLACK) {
-          by_a = ma == -INFINITY ? 1.f : ex2_approx(ma - top_a);  // from -inf: sums are 0, or NaN
-          ma = top_a;
-        }
-        if (top_b > mb + A8_SLACK) {
-          by_b = mb == -INFINITY ? 1.f : ex2_approx(mb - top_b);
-          mb = top_b;
-        }
-        la *= by_a;
-        lb *= by_b;
+        for (int nr = 0; nr < NR; ++nr) {
+          float by[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          o[j][0] *= by_a;
-          o[j][1] *= by_a;
-          o[j][2] *= by_b;
-          o[j][3] *= by_b;
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top[nr][e] = fmaxf(top[nr][e], __shfl_xor_sync(0xffffffffu, top[nr][e], d));
+            by[e] = 1.f;
+            if (top[nr][e] > m[nr][e] + A8_SLACK) {
+              by[e] = m[nr][e] == -INFINITY ? 1.f : ex2_approx(m[nr][e] - top[nr][e]);  // from -inf: sums are 0, or NaN
+              m[nr][e] = top[nr][e];
+            }
+            l[nr][e] *= by[e];
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][nr][e] *= by[e & 1];
         }
       }
-      const float off_a = ma == -INFINITY ? 0.f : A8_LIFT - ma, off_b = mb == -INFINITY ? 0.f : A8_LIFT - mb;
+      // weights, and as P^T: keys as rows become keys as columns
+      uint2 p[KEYS / 16][NR];
 #pragma unroll
-      for (int n = 0; n < GROUPS; ++n) {
-        const float rv = rcp_approx(vs[n]);
+      for (int nr = 0; nr < NR; ++nr) {
+        const float off[2] = {m[nr][0] == -INFINITY ? 0.f : A8_LIFT - m[nr][0], m[nr][1] == -INFINITY ? 0.f : A8_LIFT - m[nr][1]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = ex2_approx(s[n][e] + (e < 2 ? off_a : off_b));
-        la = fmaf(s[n][0] + s[n][1], rv, la);
-        lb = fmaf(s[n][2] + s[n][3], rv, lb);
+        for (int n = 0; n < GROUPS; ++n) {
+          float* x = &s[n / 2][nr][2 * (n & 1)];
+          const float rv = rcp_approx(vs[n]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[e] = ex2_approx(x[e] + off[e]);
+            l[nr][e] = fmaf(x[e], rv, l[nr][e]);
+          }
+          (n & 1 ? p[n / 2][nr].y : p[n / 2][nr].x) = transposed(pack_half2(x[0], x[1]));
+        }
       }
-      // O += P V: of the keys in columns 2 quad and 2 quad + 1 of both halves, the dims of piece a8_piece_of(x8) of each 128
+      // O^T += V^T P^T: of the keys in columns 2 quad and 2 quad + 1 of both halves, the dims of piece a8_piece_of(x8) of each 128
       constexpr int WORDS = D == 64 ? 2 : 4;
 #pragma unroll
       for (int part = 0; part < KEYS / 16 * BLOCKS; ++part) {
         const int blk = part % BLOCKS, kh = part / BLOCKS;  // of 128 dims, of 16 keys
-        const uint4 p = make_uint4(pack_half2(s[2 * kh][0], s[2 * kh][1]), pack_half2(s[2 * kh][2], s[2 * kh][3]),
-                                   pack_half2(s[2 * kh + 1][0], s[2 * kh + 1][1]), pack_half2(s[2 * kh + 1][2], s[2 * kh + 1][3]));
         uint32_t vw[4][WORDS];
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
@@ -604,10 +610,13 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
           nan = __any_sync(0xffffffffu, bad != 0);
         }
         if (nan) {
-          uint4 see;  // 1 where a row sees a key
-          uint32_t* f = reinterpret_cast<uint32_t*>(&see);
+          uint2 see[NR];  // 1 where a row sees a key
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = (seen >> (8 * kh + 2 * e) & 1 ? 0x3c00u : 0u) | (seen >> (8 * kh + 2 * e + 1) & 1 ? 0x3c000000u : 0u);
+          for (int nr = 0; nr < NR; ++nr) {
+            const uint32_t bits = seen >> (8 * kh + 4 * nr);
+            see[nr].x = transposed((bits & 1 ? 0x3c00u : 0u) | (bits & 2 ? 0x3c000000u : 0u));
+            see[nr].y = transposed((bits & 4 ? 0x3c00u : 0u) | (bits & 8 ? 0x3c000000u : 0u));
+          }
 #pragma unroll
           for (int w = 0; w < WORDS; ++w) {
             uint32_t ind[4];  // 1.0 where a code is NaN, which becomes 0
@@ -618,17 +627,19 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
               vw[k4][w] &= ~(hit * 0xffu);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t sel = e < 2 ? 0x5140u : 0x7362u;
-              const uint32_t b0 = __byte_perm(ind[0], ind[1], sel), b1 = __byte_perm(ind[2], ind[3], sel);
-              float hits[4] = {0.f, 0.f, 0.f, 0.f};
-              uint32_t x0, x1, y0, y1;
-              f8_halves(b0, x0, x1);
-              f8_halves(b1, y0, y1);
-              mma16<T>(hits, see, e & 1 ? x1 : x0, e & 1 ? y1 : y0);
+            for (int pr = 0; pr < 2; ++pr) {
+              const uint32_t sel = pr == 0 ? 0x5140u : 0x7362u;
+              uint4 f;
+              f8_halves(__byte_perm(ind[0], ind[1], sel), f.x, f.y);
+              f8_halves(__byte_perm(ind[2], ind[3], sel), f.z, f.w);
 #pragma unroll
-              for (int z = 0; z < 4; ++z)
-                if (hits[z] > 0.f) o[16 * blk + 4 * w + e][z] = __int_as_float(0x7fffffff);
+              for (int nr = 0; nr < NR; ++nr) {
+                float hits[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16(hits, f, see[nr].x, see[nr].y);
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  if (hits[z] > 0.f) o[8 * blk + 2 * w + pr][nr][z] = __int_as_float(0x7fffffff);
+              }
             }
           }
         }
@@ -637,12 +648,11 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
 #pragma unroll
           for (int pr = 0; pr < 2; ++pr) {
             const uint32_t sel = pr == 0 ? 0x5140u : 0x7362u;
-            const uint32_t b0 = __byte_perm(vw[0][w], vw[1][w], sel), b1 = __byte_perm(vw[2][w], vw[3][w], sel);
-            uint32_t x0, x1, y0, y1;
-            f8_halves(b0, x0, x1);
-            f8_halves(b1, y0, y1);
-            mma16<T>(o[16 * blk + 4 * w + 2 * pr], p, x0, y0);
-            mma16<T>(o[16 * blk + 4 * w + 2 * pr + 1], p, x1, y1);
+            uint4 f;
+            f8_halves(__byte_perm(vw[0][w], vw[1][w], sel), f.x, f.y);
+            f8_halves(__byte_perm(vw[2][w], vw[3][w], sel), f.z, f.w);
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma16(o[8 * blk + 2 * w + pr][nr], f, p[kh][nr].x, p[kh][nr].y);
           }
         }
       }
@@ -656,36 +666,32 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     if (!__all_sync(0xffffffffu, ok)) break;
     if (!put_more) pdl_trigger();
     // ---- the item, or this piece's part of it ----
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      la += __shfl_xor_sync(0xffffffffu, la, d);
-      lb += __shfl_xor_sync(0xffffffffu, lb, d);
-    }
     const bool whole = i0 == 0 && i1 == sp.n;
     const int part_slot = 2 * piece + (item > 0 ? 1 : 0);
-    float* part = partials + (size_t)part_slot * a8_partial_floats(D, A8_ROWS);
+    float* part = partials + (size_t)part_slot * a8_partial_floats(D, ROWS);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int t = e ? tb : ta, row = x8 + 8 * e, g = row0 + row - t * G;
-      const float m = e ? mb : ma, l = e ? lb : la;
-      if (!(e ? valid_b : valid_a)) continue;
-      // columns 2 quad and 2 quad + 1 are dims D / 8 (or 16 of each 128) from these on
-      const int64_t orow = (int64_t)(r.t0 + t) * a.hq + get.at.h * G + g;
-      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-      for (int z = 0; z < 2; ++z)
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nr][e];
 #pragma unroll
-        for (int blk = 0; blk < BLOCKS; ++blk) {
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const int row = 8 * nr + 2 * quad + e, t = tok[nr][e];
+        if (t >= r.n) continue;
+        const int64_t orow = (int64_t)(r.t0 + t) * a.hq + get.at.h * G + row0 + row - t * G;
+        const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+#pragma unroll
+        for (int blk = 0; blk < BLOCKS; ++blk) {  // 8 or 16 dims of each 128
           constexpr int RUN = D == 64 ? 8 : 16;
-          const int d0 = D == 64 ? (2 * quad + z) * 8 : 128 * blk + 16 * a8_piece_of(2 * quad + z);
+          const int d0 = D == 64 ? 8 * x8 : 128 * blk + 16 * a8_piece_of(x8);
 #pragma unroll
           for (int j = 0; j < RUN; j += 8) {
             float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = o[16 * blk + j + k][2 * e + z];
+            for (int z = 0; z < 8; ++z) y[z] = o[8 * blk + j / 2 + z / 2][nr][2 * (z & 1) + e];
             if (whole) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) y[k] *= inv;
+              for (int z = 0; z < 8; ++z) y[z] *= inv;
               store8((T*)a.out + orow * D + d0 + j, y);
             } else {
               float4* to = reinterpret_cast<float4*>(part + row * D + d0 + j);
@@ -694,11 +700,11 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
             }
           }
         }
-      if (quad == 0) {
-        if (!whole) *reinterpret_cast<float2*>(part + A8_ROWS * D + 2 * row) = make_float2(m, l);
-        else if (a.lse) a.lse[orow] = l > 0.f || l != l ? (m - A8_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        if (x8 == 0) {
+          if (!whole) *reinterpret_cast<float2*>(part + ROWS * D + 2 * row) = make_float2(m[nr][e], sum);
+          else if (a.lse) a.lse[orow] = sum > 0.f || sum != sum ? (m[nr][e] - A8_LIFT + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        }
       }
-    }
     if (lane == 0 && i0 == 0 && i1 < sp.n)
       splits[piece] = A8Split{get.at.b, get.at.h, get.at.block, (int)a8_div(unit + A8_COST + sp.n - 1, step), part_slot, {0, 0, 0}};
     unit += sp.n + A8_COST;
