@@ -37,12 +37,16 @@ constexpr int A8_WIDE_ROWS = 32;  // rows of a key head up to which warp-level p
 
 template <int D, typename T>
 int launch_append8(const Append8Args& p, cudaStream_t st) {
-  // entries a thread block: one where that leaves few blocks idle, else eight, of which most continue a run
-  const int per = p.count <= 16 * SM_COUNT ? 1 : 8;
-  const int smem = A8R_CHUNK * (p.rot / 2) * (int)sizeof(float2) + 2 * p.hkv * (int)sizeof(float);
-  if (smem > 48 * 1024) return fail(HSG_ERR_INVALID, "too many key heads (%d)", p.hkv);
-  append8_kernel<D, T><<<(p.count + per - 1) / per, A8R_THREADS, smem, st>>>(p, per);
-  CU(cudaGetLastError());
+  // entries a thread block: one where that leaves few blocks idle, else up to a block's, of which most continue a run
+  const int per = p.count <= 16 * SM_COUNT ? 1 : std::min(32, p.cache.block), kv_blocks = (p.count + per - 1) / per;
+  // warps that share a token's query heads: as few as leave four blocks an SM
+  constexpr int WARPS = A8R_THREADS / 32, RPW = 256 / D;
+  int split = 1;
+  while (split < WARPS && (int64_t)(p.count + WARPS / split * RPW - 1) / (WARPS / split * RPW) < 4 * SM_COUNT) split *= 2;
+  const int per_q = WARPS / split * RPW, q_blocks = p.hq ? (p.count + per_q - 1) / per_q : 0;
+  const int smem = 2 * p.hkv * (int)sizeof(uint32_t);
+  if (smem > 40 * 1024) return fail(HSG_ERR_INVALID, "too many key heads (%d)", p.hkv);
+  CU(launch_k(append8_kernel<D, T>, dim3((unsigned)(kv_blocks + q_blocks)), dim3(A8R_THREADS), smem, st, true, p, kv_blocks, per, split));
   return HSG_OK;
 }
 template <typename T>

@@ -43,7 +43,7 @@ struct Append8Args {
 };
 
 constexpr int A8R_THREADS = 256;
-constexpr int A8R_CHUNK = 16;     // tokens whose angles lie in shared memory at once
+constexpr int A8R_LIVE = 4;       // 16-byte pieces a lane has under way
 constexpr float F8_MAX = 448.f;
 constexpr int SCALE_MIN_EXP = -100, SCALE_MAX_EXP = 120;
 
@@ -61,54 +61,309 @@ __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
   b = fabsf(b) < INFINITY ? b : __int_as_float(0x7fffffff);
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint2 f8_eight(const float (&x)[8], float by) {
+  return make_uint2(f8_pair(x[0] * by, x[1] * by) | f8_pair(x[2] * by, x[3] * by) << 16,
+                    f8_pair(x[4] * by, x[5] * by) | f8_pair(x[6] * by, x[7] * by) << 16);
+}
 __device__ __forceinline__ float2 f8_values(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
   return __half22float2(__half2(h));
 }
 
-// One run of entries at a time: ones whose slots ascend within one block, with entries that are not kept between them at most (each
-// of which is a run by itself). A block that takes `per` entries does the runs that begin there. Units of a warp are heads:
-//   1  keys and values: the run's bound, the block's scale (from the run alone if it holds the block's first token, else at
-//      least what it was), rows that were there rounded to a risen scale;
-//   2  angles of up to 16 tokens into shared memory, then rows of q, k and v: rotated, scaled, written.
-// Rows are read twice, the second time mostly from L1 or L2. dim / 8 lanes share a row, eight elements each.
+// Eight 16-bit numbers as fp32.
+template <typename T> __device__ __forceinline__ void unpack8(const uint4& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = unpack_half2(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// How a lane turns the eight elements from d on of a row that dim / 8 lanes share: the other element of a pair is among its own
+// eight (pairs) or rot / 16 lanes away. A lane keeps the angles of its row while it goes through the row's heads: read from shared
+// memory for every head they took 64 bytes for 16 of data, at a fourth of the banks' rate (37,500 tokens of 40 heads 326 and
+// 190 us).
+//
+// A frequency is the 64-bit fraction of a turn that one position adds, made once a block in fp64 (2^-53 of itself); a position
+// times it, modulo 2^64, is where the position stands within the turn, whatever its size. The 32 upper bits of that go to fp32
+// and sincospif: the angle is off by less than 2e-7.
+struct A8Turn {
+  int half, d, partner;
+  bool in_rot, first_half, pairs;
+  float2 cs[8];  // (cos, sin) times rope_scale of the lane's elements; pairs: the first four, of its pairs
+  __device__ __forceinline__ A8Turn(const Append8Args& a, int lane, int dim)
+      : half(a.rot / 2), d(lane % (dim / 8) * 8), in_rot(d < a.rot), first_half(d < half), pairs(a.pairs) {
+    partner = in_rot && !pairs ? (first_half ? lane + half / 8 : lane - half / 8) : lane;
+  }
+  __device__ __forceinline__ void at(const Append8Args& a, int position, const uint64_t* steps) {
+    if (!in_rot) return;
+    const uint64_t* mine = steps + (pairs ? d / 2 : first_half ? d : d - half);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e >= 4 && pairs) break;
+      const int within = (int)((uint64_t)((int64_t)position * (int64_t)mine[e]) >> 32);
+      float s, c;
+      sincospif((float)within * 4.6566128730773926e-10f, &s, &c);  // half turns: 2^-31
+      cs[e] = make_float2(c * a.rope_scale, (first_half || pairs ? s : -s) * a.rope_scale);
+    }
+  }
+  // every lane of the warp calls both
+  __device__ __forceinline__ uint4 others(const uint4& raw) const {
+    if (pairs) return raw;
+    return make_uint4(__shfl_sync(0xffffffffu, raw.x, partner), __shfl_sync(0xffffffffu, raw.y, partner),
+                      __shfl_sync(0xffffffffu, raw.z, partner), __shfl_sync(0xffffffffu, raw.w, partner));
+  }
+  template <typename T> __device__ __forceinline__ void apply(const uint4& raw, bool turn, float (&x)[8]) const {
+    unpack8<T>(raw, x);
+    if (!turn || !half) return;
+    if (pairs) {
+      if (!in_rot) return;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p = x[e], q = x[e + 1];
+        x[e] = fmaf(-q, cs[e / 2].y, p * cs[e / 2].x);
+        x[e + 1] = fmaf(p, cs[e / 2].y, q * cs[e / 2].x);
+      }
+      return;
+    }
+    float y[8];
+    unpack8<T>(others(raw), y);
+    if (!in_rot) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(-y[e], cs[e].y, x[e] * cs[e].x);
+  }
+  // what the eight elements ask of the scale: pairs that turn count with the sum of their magnitudes
+  template <typename T> __device__ __forceinline__ float bound(const uint4& raw, float factor, bool turns) const {
+    float x[8], y[8], most = 0.f;
+    unpack8<T>(raw, x);
+    if (turns && half) unpack8<T>(others(raw), y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float z = turns && in_rot ? (fabsf(x[e]) + fabsf(y[pairs ? e ^ 1 : e])) * factor : fabsf(x[e]);
+      most = fmaxf(most, z < INFINITY ? z : 0.f);
+    }
+    return most;
+  }
+};
+
+__device__ __forceinline__ void append8_steps(const Append8Args& a, uint64_t* steps) {
+  for (int e = threadIdx.x; e < a.rot / 2; e += A8R_THREADS) {
+    const double turns = (double)a.inv_freq[e] * 0.15915494309189533577;
+    steps[e] = (uint64_t)__double2ll_rn((turns - rint(turns)) * 9223372036854775808.0) << 1;
+  }
+}
+
+// Queries: `tokens` entries from the first-th on. A warp takes as many tokens as it has rows of lanes; `split` warps share those
+// tokens' heads, of which A8R_LIVE are under way at a time.
 template <int D, typename T>
-__global__ void __launch_bounds__(A8R_THREADS) append8_kernel(const __grid_constant__ Append8Args a, int per) {
-  extern __shared__ __align__(16) float2 s_angles[];  // [chunk][rot / 2] (cos, sin) times rope_scale
+__device__ __forceinline__ void append8_queries(const Append8Args& a, int first, int tokens, int split, const uint64_t* steps) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = warp / split * RPW + lane / LPR, i = first + t;
+  A8Turn turn(a, lane, D);
+  if (__all_sync(0xffffffffu, t >= tokens)) return;
+  const bool mine = t < tokens;
+  const T* src = (const T*)a.q + i * a.q_ts + turn.d;
+  uint4 raw[A8R_LIVE];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < A8R_LIVE; ++u) {
+      raw[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (mine && h0 + u * split < a.hq) raw[u] = *reinterpret_cast<const uint4*>(src + (h0 + u * split) * a.q_hs);
+    }
+  };
+  load(warp % split);
+  if (mine && a.rot) turn.at(a, a.positions[i], steps);  // while the first heads are on their way
+  T* dst = (T*)a.q_out + (int64_t)i * a.hq * D + turn.d;
+  for (int h0 = warp % split; h0 < a.hq; h0 += A8R_LIVE * split) {
+#pragma unroll
+    for (int u = 0; u < A8R_LIVE; ++u) {
+      const int h = h0 + u * split, next = h + A8R_LIVE * split;
+      float x[8];
+      turn.apply<T>(raw[u], true, x);
+      if (mine && next < a.hq) raw[u] = *reinterpret_cast<const uint4*>(src + next * a.q_hs);
+      if (mine && h < a.hq) store8(dst + h * D, x);
+    }
+  }
+}
+
+// Keys and values, one run of entries at a time: ones whose slots ascend within one block, with entries that are not kept between
+// them at most. Warps take tokens and share their heads of K and V like those of queries:
+//   1  the heads' bounds, joined in shared memory;
+//   2  the block's scales (from the run alone if it holds the block's first token, else at least what they were), rows that were
+//      there rounded to a risen scale;
+//   3  rows, read again (mostly from L2), turned, scaled and written.
+template <int D, typename T>
+__device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n, int slot0, bool same, const uint64_t* steps, uint32_t* s_units) {
   constexpr int LPR = D / 8, RPW = 32 / LPR, WARPS = A8R_THREADS / 32;
-  float* s_scale = reinterpret_cast<float*>(s_angles + A8R_CHUNK * (a.rot / 2));  // [2 hkv] inverse scales of the run
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane % LPR * 8, sub = lane / LPR, half = a.rot / 2;
-  const bool in_rot = d < a.rot, first_half = d < half;
-  const int partner = in_rot && !a.pairs ? (first_half ? lane + half / 8 : lane - half / 8) : lane;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPR;
+  A8Turn turn(a, lane, D);
   const float factor = fabsf(a.rope_scale);
   const Cache8& c = a.cache;
-  auto row_of = [&](int i) {  // of k and v; -1: not kept, -2: not there
-    if (a.slots[i] < 0) return -1;
-    const int r = a.source ? a.source[i] : i;
-    return r >= 0 && r < a.rows ? r : -2;
-  };
-  const int end = min(a.count, (int)(blockIdx.x + 1) * per);
-  for (int i0 = blockIdx.x * per; i0 < end; ++i0) {
-    const int slot0 = a.slots[i0], blk = slot0 >= 0 ? slot0 / c.block : -1;
-    // the kept entry before this one
-    int before = -1;
-    if (slot0 >= 0) {
-      for (int j = i0 - 1 - lane;; j -= 32) {
-        const int s = j >= 0 ? a.slots[j] : -1;
-        const unsigned kept = __ballot_sync(0xffffffffu, s >= 0);
-        if (kept) before = __shfl_sync(0xffffffffu, s, __ffs(kept) - 1);
-        if (kept || j + lane - 31 <= 0) break;
+  const int blk = c.block_div.div(slot0), page = blk / c.blocks, inner = blk - page * c.blocks, first = slot0 - blk * c.block;
+  if (same || page >= c.pages) {  // a slot that does not ascend, or no page
+    if (threadIdx.x == 0) set_error(a.err, ERR_BAD_SLOT);
+    return;
+  }
+  const int64_t base = (int64_t)page * c.page_stride + (int64_t)inner * c.block * c.token_stride;
+  const int units = 2 * a.hkv, groups = (n + RPW - 1) / RPW;
+  const int split = groups >= WARPS ? 1 : WARPS / groups, teams = WARPS / split, team = warp / split, u_first = warp % split;
+  for (int u = threadIdx.x; u < units; u += A8R_THREADS) s_units[u] = 0u;
+  __syncthreads();
+  int row = -1, at = 0;  // of K and V, and within the block; -1: not kept or not there
+  auto token = [&](int g) {
+    const int t = g * RPW + sub, i = i0 + t;
+    row = -1;
+    if (t < n) {
+      const int slot = a.slots[i];
+      if (slot >= 0) {
+        at = slot - blk * c.block;
+        row = a.source ? a.source[i] : i;
+        if (row < 0 || row >= a.rows) {
+          set_error(a.err, ERR_BAD_SLOT);
+          row = -1;
+        }
       }
     }
-    const bool same = before >= 0 && before / c.block == blk;
-    if (same && slot0 > before) continue;  // inside a run that began earlier
+  };
+  uint4 raw[A8R_LIVE];
+  auto load = [&](int u0) {
+#pragma unroll
+    for (int v = 0; v < A8R_LIVE; ++v) {
+      const int u = u0 + v * split, h = u < a.hkv ? u : u - a.hkv;
+      raw[v] = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= 0 && u < units)
+        raw[v] = *reinterpret_cast<const uint4*>(u < a.hkv ? (const T*)a.k + row * a.k_ts + h * a.k_hs + turn.d
+                                                           : (const T*)a.v + row * a.v_ts + h * a.v_hs + turn.d);
+    }
+  };
+  if (team < teams) {
+    for (int g = team; g < groups; g += teams) {
+      token(g);
+      for (int u0 = u_first; u0 < units; u0 += A8R_LIVE * split) {
+        load(u0);
+#pragma unroll
+        for (int v = 0; v < A8R_LIVE; ++v) {
+          const int u = u0 + v * split;
+          if (u >= units) break;
+          const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(turn.bound<T>(raw[v], factor, u < a.hkv)));
+          if (lane == 0) atomicMax(&s_units[u], most);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int u = warp; u < units; u += WARPS) {
+    const bool is_k = u < a.hkv;
+    const int h = is_k ? u : u - a.hkv;
+    float* where = (is_k ? c.ks : c.vs) + ((int64_t)page * c.blocks + inner) * a.hkv + h;
+    float scale = scale8_of(__uint_as_float(s_units[u]));
+    if (first) {
+      const float old = *where;
+      scale = fmaxf(scale, old);
+      if (scale > old) {  // rows that are there, to the new scale
+        const float ratio = old / scale;
+        uint8_t* rows = (is_k ? c.k : c.v) + base + h * c.head_stride;
+        for (int e = lane; e < first * (D / 16); e += 32) {
+          uint4* to = reinterpret_cast<uint4*>(rows + e / (D / 16) * c.token_stride + e % (D / 16) * 16);
+          uint4 w = *to;
+          uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 lo = f8_values(x[q] & 0xffffu), hi = f8_values(x[q] >> 16);
+            x[q] = f8_pair(lo.x * ratio, lo.y * ratio) | f8_pair(hi.x * ratio, hi.y * ratio) << 16;
+          }
+          *to = w;
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the bound and the old scale
+    if (lane == 0) {
+      *where = scale;
+      s_units[u] = __float_as_uint(1.0f / scale);
+    }
+  }
+  __syncthreads();
+  if (team < teams) {
+    for (int g = team; g < groups; g += teams) {
+      token(g);
+      if (row >= 0 && a.rot) turn.at(a, a.positions[i0 + g * RPW + sub], steps);
+      for (int u0 = u_first; u0 < units; u0 += A8R_LIVE * split) {
+        load(u0);
+#pragma unroll
+        for (int v = 0; v < A8R_LIVE; ++v) {
+          const int u = u0 + v * split, h = u < a.hkv ? u : u - a.hkv;
+          if (u >= units) break;
+          float x[8];
+          turn.apply<T>(raw[v], u < a.hkv, x);
+          if (row >= 0)
+            *reinterpret_cast<uint2*>((u < a.hkv ? c.k : c.v) + base + at * c.token_stride + h * c.head_stride + turn.d) =
+                f8_eight(x, __uint_as_float(s_units[u]));
+        }
+      }
+    }
+  }
+}
+
+// Blocks 0 .. kv_blocks - 1 take `per` entries each, of which they write the runs that begin there; the others queries, whose heads
+// `split` warps share.
+template <int D, typename T>
+__global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_constant__ Append8Args a, int kv_blocks, int per, int split) {
+  __shared__ uint64_t s_steps[128];      // [rot / 2]
+  extern __shared__ uint32_t s_units[];  // [2 hkv] bounds, then inverse scales
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x >= kv_blocks) {
+    append8_steps(a, s_steps);
+    __syncthreads();
+    const int per_q = A8R_THREADS / 32 / split * (256 / D), first = (blockIdx.x - kv_blocks) * per_q;
+    append8_queries<D, T>(a, first, min(per_q, a.count - first), split, s_steps);
+    return;
+  }
+  const Cache8& c = a.cache;
+  const int lane = threadIdx.x & 31, begin = blockIdx.x * per;
+  // lane l has entry begin + l, and of the entries before them the l-th
+  const int slot = lane < per && begin + lane < a.count ? a.slots[begin + lane] : -1;
+  int ahead = begin - 1 - lane >= 0 ? a.slots[begin - 1 - lane] : -1;
+  // the kept entry before each
+  int before = -1;
+  for (int j = begin - 1 - lane;;) {
+    const unsigned kept = __ballot_sync(0xffffffffu, ahead >= 0);
+    if (kept) before = __shfl_sync(0xffffffffu, ahead, __ffs(kept) - 1);
+    if (kept || j + lane - 31 <= 0) break;
+    j -= 32;
+    ahead = j >= 0 ? a.slots[j] : -1;
+  }
+  {
+    const unsigned below = __ballot_sync(0xffffffffu, slot >= 0) & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, slot, below ? 31 - __clz(below) : 0);
+    if (below) before = prev;
+  }
+  const bool joined = slot >= 0 && before >= 0 && c.block_div.div(slot) == c.block_div.div(before);
+  // those that are not inside a run that began earlier
+  unsigned leaders = __ballot_sync(0xffffffffu, slot >= 0 && !(joined && slot > before));
+  if (!leaders) return;
+  append8_steps(a, s_steps);
+  for (; leaders; leaders &= leaders - 1) {
+    const int l = __ffs(leaders) - 1, i0 = begin + l;
+    const int slot0 = __shfl_sync(0xffffffffu, slot, l), blk = c.block_div.div(slot0);
+    const bool same = __shfl_sync(0xffffffffu, (int)joined, l);
+    int next = i0 + 1 + lane < a.count ? a.slots[i0 + 1 + lane] : -1;
+    auto in_block = [&](int s) { return s >= blk * c.block && s - blk * c.block < c.block; };
     // the run's end: its slots ascend, so it holds at most a block of entries that are kept
     int n = 1;
-    for (int j0 = i0 + 1, last = slot0; slot0 >= 0 && j0 < a.count && last % c.block != c.block - 1; j0 += 32) {
-      const int j = j0 + lane, s = j < a.count ? a.slots[j] : -1;
+    for (int j0 = i0 + 1, last = slot0; j0 < a.count && last - blk * c.block != c.block - 1;) {
+      const int j = j0 + lane, s = next;
       const unsigned kept = __ballot_sync(0xffffffffu, s >= 0), below = kept & ((1u << lane) - 1u);
       const int prev = __shfl_sync(0xffffffffu, s, below ? 31 - __clz(below) : 0);
-      const bool fits = s < 0 || (s / c.block == blk && s > (below ? prev : last));
+      const bool fits = s < 0 || (in_block(s) && s > (below ? prev : last));
       const unsigned stop = __ballot_sync(0xffffffffu, j >= a.count || !fits);
       const unsigned in = kept & (stop ? (stop & -stop) - 1u : ~0u);
       const int top = in ? 31 - __clz(in) : 0, newest = __shfl_sync(0xffffffffu, s, top);
@@ -117,146 +372,10 @@ __global__ void __launch_bounds__(A8R_THREADS) append8_kernel(const __grid_const
         last = newest;
       }
       if (stop) break;
+      j0 += 32;
+      next = j0 + lane < a.count ? a.slots[j0 + lane] : -1;
     }
-    const int per_page = c.page / c.block, page = blk >= 0 ? blk / per_page : 0;
-    bool keep = slot0 >= 0;
-    if (keep && (same || page >= c.pages)) {  // a slot that does not ascend, or no page
-      keep = false;
-      if (threadIdx.x == 0) set_error(a.err, ERR_BAD_SLOT);
-    }
-    const int inner = keep ? blk - page * per_page : 0, first = keep ? slot0 - blk * c.block : 0;  // block and row
-    const int64_t base = (int64_t)page * c.page_stride + (int64_t)inner * c.block * c.token_stride;
-    if (keep) {
-      for (int u = warp; u < 2 * a.hkv; u += WARPS) {
-        const bool is_k = u < a.hkv;
-        const int h = is_k ? u : u - a.hkv;
-        const T* src = (const T*)(is_k ? a.k : a.v) + h * (is_k ? a.k_hs : a.v_hs) + d;
-        const int64_t ts = is_k ? a.k_ts : a.v_ts;
-        float* where = (is_k ? c.ks : c.vs) + ((int64_t)page * per_page + inner) * a.hkv + h;
-        const float old = first ? *where : 0.f;
-        float bound = 0.f;
-#pragma unroll 2
-        for (int t = sub; t < n + sub; t += RPW) {  // every lane of a row's lanes takes part in the shuffles
-          const int r = t < n ? row_of(i0 + t) : -1;
-          float x[8];
-          if (r >= 0) {
-            load8(src + r * ts, x);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-          }
-          if (is_k && half) {
-            float y[8];
-            if (a.pairs) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
-            }
-            if (in_rot) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = (fabsf(x[e]) + fabsf(y[e])) * factor;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) bound = fmaxf(bound, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
-        }
-        bound = warp_max(bound);
-        float scale = scale8_of(bound);
-        if (first) scale = fmaxf(scale, old);
-        if (first && scale > old) {  // rows that are there, to the new scale
-          const float ratio = old / scale;
-          uint8_t* rows = (is_k ? c.k : c.v) + base + h * c.head_stride;
-          for (int e = lane; e < first * (D / 16); e += 32) {
-            uint4* at = reinterpret_cast<uint4*>(rows + e / (D / 16) * c.token_stride + e % (D / 16) * 16);
-            uint4 w = *at;
-            uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float2 lo = f8_values(x[q] & 0xffffu), hi = f8_values(x[q] >> 16);
-              x[q] = f8_pair(lo.x * ratio, lo.y * ratio) | f8_pair(hi.x * ratio, hi.y * ratio) << 16;
-            }
-            *at = w;
-          }
-        }
-        if (lane == 0) {
-          *where = scale;
-          s_scale[u] = 1.0f / scale;
-        }
-      }
-    }
-    for (int t0 = 0; t0 < n; t0 += A8R_CHUNK) {
-      const int tokens = min(A8R_CHUNK, n - t0);
-      __syncthreads();
-      for (int e = threadIdx.x; e < tokens * half; e += A8R_THREADS) {
-        const int t = e / half;
-        float s, co;
-        rotation(a.positions[i0 + t0 + t], a.inv_freq[e - t * half], s, co);
-        s_angles[e] = make_float2(co * a.rope_scale, s * a.rope_scale);
-      }
-      __syncthreads();
-      for (int u = warp; u < a.hq + (keep ? 2 * a.hkv : 0); u += WARPS) {
-        const bool is_q = u < a.hq, is_k = !is_q && u < a.hq + a.hkv;
-        const int h = is_q ? u : is_k ? u - a.hq : u - a.hq - a.hkv;
-        const T* src = (const T*)(is_q ? a.q : is_k ? a.k : a.v) + h * (is_q ? a.q_hs : is_k ? a.k_hs : a.v_hs) + d;
-        const int64_t ts = is_q ? a.q_ts : is_k ? a.k_ts : a.v_ts;
-        const float inv = is_q ? 1.f : s_scale[u - a.hq];
-#pragma unroll 2
-        for (int t = sub; t < tokens + sub; t += RPW) {
-          const int i = i0 + t0 + t, r = t >= tokens ? -1 : !is_q ? row_of(i) : a.slots[i] >= 0 || n == 1 ? i : -1;
-          float x[8];
-          if (r >= 0) {
-            load8(src + r * ts, x);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
-          }
-          if ((is_q || is_k) && half) {
-            if (a.pairs) {
-              if (in_rot && r >= 0) {
-                const float4* cs = reinterpret_cast<const float4*>(s_angles + t * half + d / 2);
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                  const float4 w = cs[e / 4];
-                  const float p = x[e], q = x[e + 1], p2 = x[e + 2], q2 = x[e + 3];
-                  x[e] = fmaf(-q, w.y, p * w.x);
-                  x[e + 1] = fmaf(p, w.y, q * w.x);
-                  x[e + 2] = fmaf(-q2, w.w, p2 * w.z);
-                  x[e + 3] = fmaf(p2, w.w, q2 * w.z);
-                }
-              }
-            } else {
-              float y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
-              if (in_rot && r >= 0) {
-                const float4* cs = reinterpret_cast<const float4*>(s_angles + t * half + (first_half ? d : d - half));
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                  const float4 w = cs[e / 2];
-                  x[e] = fmaf(first_half ? -y[e] : y[e], w.y, x[e] * w.x);
-                  x[e + 1] = fmaf(first_half ? -y[e + 1] : y[e + 1], w.w, x[e + 1] * w.z);
-                }
-              }
-            }
-          }
-          if (r < 0) {
-            if (r == -2 && d == 0) set_error(a.err, ERR_BAD_SLOT);
-            continue;
-          }
-          if (is_q) {
-            store8((T*)a.q_out + ((int64_t)i * a.hq + h) * D + d, x);
-          } else {
-            const int at = a.slots[i] - blk * c.block;
-            uint2 w;
-            w.x = f8_pair(x[0] * inv, x[1] * inv) | f8_pair(x[2] * inv, x[3] * inv) << 16;
-            w.y = f8_pair(x[4] * inv, x[5] * inv) | f8_pair(x[6] * inv, x[7] * inv) << 16;
-            *reinterpret_cast<uint2*>((is_k ? c.k : c.v) + base + at * c.token_stride + h * c.head_stride + d) = w;
-          }
-        }
-      }
-    }
+    append8_run<D, T>(a, i0, n, slot0, same, s_steps, s_units);
     __syncthreads();  // shared memory is free for the next run
   }
 }
