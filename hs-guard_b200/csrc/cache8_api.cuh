@@ -44,7 +44,7 @@ int launch_append8(const Append8Args& p, cudaStream_t st) {
   int split = 1;
   while (split < WARPS && (int64_t)(p.count + WARPS / split * RPW - 1) / (WARPS / split * RPW) < 4 * SM_COUNT) split *= 2;
   const int per_q = WARPS / split * RPW, q_blocks = p.hq ? (p.count + per_q - 1) / per_q : 0;
-  const int smem = 2 * p.hkv * (int)sizeof(uint32_t);
+  const int smem = 4 * p.hkv * (int)sizeof(uint32_t);
   if (smem > 40 * 1024) return fail(HSG_ERR_INVALID, "too many key heads (%d)", p.hkv);
   CU(launch_k(append8_kernel<D, T>, dim3((unsigned)(kv_blocks + q_blocks)), dim3(A8R_THREADS), smem, st, true, p, kv_blocks, per, split));
   return HSG_OK;

@@ -61,9 +61,15 @@ __device__ __forceinline__ uint32_t f8_pair(float a, float b) {
   b = fabsf(b) < INFINITY ? b : __int_as_float(0x7fffffff);
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ uint2 f8_eight(const float (&x)[8], float by) {
-  return make_uint2(f8_pair(x[0] * by, x[1] * by) | f8_pair(x[2] * by, x[3] * by) << 16,
-                    f8_pair(x[4] * by, x[5] * by) | f8_pair(x[6] * by, x[7] * by) << 16);
+// Eight values times `by`; infinities may be among them if `checked`.
+__device__ __forceinline__ uint2 f8_eight(const float (&x)[8], float by, bool checked) {
+  if (checked)
+    return make_uint2(f8_pair(x[0] * by, x[1] * by) | f8_pair(x[2] * by, x[3] * by) << 16,
+                      f8_pair(x[4] * by, x[5] * by) | f8_pair(x[6] * by, x[7] * by) << 16);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * by, x[2 * i + 1] * by), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 __device__ __forceinline__ float2 f8_values(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
@@ -139,15 +145,17 @@ struct A8Turn {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(-y[e], cs[e].y, x[e] * cs[e].x);
   }
-  // what the eight elements ask of the scale: pairs that turn count with the sum of their magnitudes
-  template <typename T> __device__ __forceinline__ float bound(const uint4& raw, float factor, bool turns) const {
+  // what the eight elements ask of the scale but for |rope_scale|: pairs that turn count with the sum of their magnitudes. Without
+  // NaN; infinite if one is, unless `finite` leaves those out
+  template <typename T, bool finite> __device__ __forceinline__ float bound(const uint4& raw, bool turns) const {
     float x[8], y[8], most = 0.f;
     unpack8<T>(raw, x);
     if (turns && half) unpack8<T>(others(raw), y);
+    const bool both = turns && in_rot;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float z = turns && in_rot ? (fabsf(x[e]) + fabsf(y[pairs ? e ^ 1 : e])) * factor : fabsf(x[e]);
-      most = fmaxf(most, z < INFINITY ? z : 0.f);
+      const float z = both ? fabsf(x[e]) + fabsf(y[pairs ? e ^ 1 : e]) : fabsf(x[e]);
+      most = fmaxf(most, finite && !(z < INFINITY) ? 0.f : z);
     }
     return most;
   }
@@ -215,7 +223,7 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
   const int64_t base = (int64_t)page * c.page_stride + (int64_t)inner * c.block * c.token_stride;
   const int units = 2 * a.hkv, groups = (n + RPW - 1) / RPW;
   const int split = groups >= WARPS ? 1 : WARPS / groups, teams = WARPS / split, team = warp / split, u_first = warp % split;
-  for (int u = threadIdx.x; u < units; u += A8R_THREADS) s_units[u] = 0u;
+  for (int u = threadIdx.x; u < 2 * units; u += A8R_THREADS) s_units[u] = 0u;
   __syncthreads();
   int row = -1, at = 0;  // of K and V, and within the block; -1: not kept or not there
   auto token = [&](int g) {
@@ -234,29 +242,72 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
     }
   };
   uint4 raw[A8R_LIVE];
-  auto load = [&](int u0) {
-#pragma unroll
-    for (int v = 0; v < A8R_LIVE; ++v) {
-      const int u = u0 + v * split, h = u < a.hkv ? u : u - a.hkv;
-      raw[v] = make_uint4(0u, 0u, 0u, 0u);
-      if (row >= 0 && u < units)
-        raw[v] = *reinterpret_cast<const uint4*>(u < a.hkv ? (const T*)a.k + row * a.k_ts + h * a.k_hs + turn.d
-                                                           : (const T*)a.v + row * a.v_ts + h * a.v_hs + turn.d);
+  auto load = [&](int v, int u0) {  // the v-th of the units from u0 on
+    const int u = u0 + v * split, h = u < a.hkv ? u : u - a.hkv;
+    raw[v] = make_uint4(0u, 0u, 0u, 0u);
+    if (row >= 0 && u < units)
+      raw[v] = *reinterpret_cast<const uint4*>(u < a.hkv ? (const T*)a.k + row * a.k_ts + h * a.k_hs + turn.d
+                                                         : (const T*)a.v + row * a.v_ts + h * a.v_hs + turn.d);
+  };
+  auto bound_of = [&](int u, float most, bool wild) {  // (times |rope_scale| where the pair turns: rounding keeps the order)
+    const float z = u < a.hkv && turn.in_rot ? most * factor : most;
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(z < INFINITY ? z : 0x1.fffffep127f));
+    if (lane == 0) {
+      atomicMax(&s_units[u], bits);
+      if (wild) s_units[units + u] = 1u;
     }
   };
-  if (team < teams) {
-    for (int g = team; g < groups; g += teams) {
-      token(g);
-      for (int u0 = u_first; u0 < units; u0 += A8R_LIVE * split) {
-        load(u0);
+  // bounds: of a few groups of tokens several heads are under way, else several groups of one head
+  const bool few = groups <= 2 * teams;
+  for (int g = team; few && g < groups && team < teams; g += teams) {
+    token(g);
 #pragma unroll
-        for (int v = 0; v < A8R_LIVE; ++v) {
-          const int u = u0 + v * split;
-          if (u >= units) break;
-          const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(turn.bound<T>(raw[v], factor, u < a.hkv)));
-          if (lane == 0) atomicMax(&s_units[u], most);
-        }
+    for (int v = 0; v < A8R_LIVE; ++v) load(v, u_first);
+    for (int u0 = u_first; u0 < units; u0 += A8R_LIVE * split) {
+#pragma unroll
+      for (int v = 0; v < A8R_LIVE; ++v) {
+        const int u = u0 + v * split;
+        if (u >= units) break;
+        float most = turn.bound<T, false>(raw[v], u < a.hkv);
+        const bool wild = __any_sync(0xffffffffu, most == INFINITY);
+        if (wild) most = turn.bound<T, true>(raw[v], u < a.hkv);
+        load(v, u0 + A8R_LIVE * split);
+        bound_of(u, most, wild);
       }
+    }
+  }
+  for (int g0 = team; !few && g0 < groups && team < teams; g0 += A8R_LIVE * teams) {
+    int rows[A8R_LIVE];
+#pragma unroll
+    for (int v = 0; v < A8R_LIVE; ++v) {
+      token(g0 + v * teams);
+      rows[v] = row;
+    }
+    auto fetch = [&](int u, uint4 (&x)[A8R_LIVE]) {
+      const int h = u < a.hkv ? u : u - a.hkv;
+      const T* src = (u < a.hkv ? (const T*)a.k + h * a.k_hs : (const T*)a.v + h * a.v_hs) + turn.d;
+#pragma unroll
+      for (int v = 0; v < A8R_LIVE; ++v) {
+        x[v] = make_uint4(0u, 0u, 0u, 0u);
+        if (rows[v] >= 0 && u < units) x[v] = *reinterpret_cast<const uint4*>(src + rows[v] * (u < a.hkv ? a.k_ts : a.v_ts));
+      }
+    };
+    uint4 ahead[A8R_LIVE];
+    fetch(u_first, ahead);
+    for (int u = u_first; u < units; u += split) {
+#pragma unroll
+      for (int v = 0; v < A8R_LIVE; ++v) raw[v] = ahead[v];
+      fetch(u + split, ahead);
+      float most = 0.f;
+#pragma unroll
+      for (int v = 0; v < A8R_LIVE; ++v) most = fmaxf(most, turn.bound<T, false>(raw[v], u < a.hkv));
+      const bool wild = __any_sync(0xffffffffu, most == INFINITY);
+      if (wild) {
+        most = 0.f;
+#pragma unroll 1
+        for (int v = 0; v < A8R_LIVE; ++v) most = fmaxf(most, turn.bound<T, true>(v == 0 ? raw[0] : v == 1 ? raw[1] : v == 2 ? raw[2] : raw[3], u < a.hkv));
+      }
+      bound_of(u, most, wild);
     }
   }
   __syncthreads();
@@ -294,18 +345,20 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
   if (team < teams) {
     for (int g = team; g < groups; g += teams) {
       token(g);
+#pragma unroll
+      for (int v = 0; v < A8R_LIVE; ++v) load(v, u_first);
       if (row >= 0 && a.rot) turn.at(a, a.positions[i0 + g * RPW + sub], steps);
       for (int u0 = u_first; u0 < units; u0 += A8R_LIVE * split) {
-        load(u0);
 #pragma unroll
         for (int v = 0; v < A8R_LIVE; ++v) {
           const int u = u0 + v * split, h = u < a.hkv ? u : u - a.hkv;
           if (u >= units) break;
           float x[8];
           turn.apply<T>(raw[v], u < a.hkv, x);
+          load(v, u0 + A8R_LIVE * split);
           if (row >= 0)
             *reinterpret_cast<uint2*>((u < a.hkv ? c.k : c.v) + base + at * c.token_stride + h * c.head_stride + turn.d) =
-                f8_eight(x, __uint_as_float(s_units[u]));
+                f8_eight(x, __uint_as_float(s_units[u]), s_units[units + u]);
         }
       }
     }
@@ -313,22 +366,23 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
 }
 
 // Blocks 0 .. kv_blocks - 1 take `per` entries each, of which they write the runs that begin there; the others queries, whose heads
-// `split` warps share.
+// `split` warps share. (Queries first, or both spread among each other, took 1.2 times as long.)
 template <int D, typename T>
 __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_constant__ Append8Args a, int kv_blocks, int per, int split) {
   __shared__ uint64_t s_steps[128];      // [rot / 2]
-  extern __shared__ uint32_t s_units[];  // [2 hkv] bounds, then inverse scales
+  extern __shared__ uint32_t s_units[];  // [2 hkv] bounds, then inverse scales; [2 hkv] whether infinities are among the rows
   pdl_wait();
   pdl_trigger();
+  const int kv = min((int)blockIdx.x, kv_blocks);
   if ((int)blockIdx.x >= kv_blocks) {
     append8_steps(a, s_steps);
     __syncthreads();
-    const int per_q = A8R_THREADS / 32 / split * (256 / D), first = (blockIdx.x - kv_blocks) * per_q;
+    const int per_q = A8R_THREADS / 32 / split * (256 / D), first = (blockIdx.x - kv) * per_q;
     append8_queries<D, T>(a, first, min(per_q, a.count - first), split, s_steps);
     return;
   }
   const Cache8& c = a.cache;
-  const int lane = threadIdx.x & 31, begin = blockIdx.x * per;
+  const int lane = threadIdx.x & 31, begin = kv * per;
   // lane l has entry begin + l, and of the entries before them the l-th
   const int slot = lane < per && begin + lane < a.count ? a.slots[begin + lane] : -1;
   int ahead = begin - 1 - lane >= 0 ? a.slots[begin - 1 - lane] : -1;
