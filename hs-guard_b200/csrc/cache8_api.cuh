@@ -117,13 +117,23 @@ int launch_attn8_dim(const Attn8Args& p, int dim, void* ws, cudaStream_t st) {
   return dim == 64 ? launch_attn8<64, T>(p, ws, st) : dim == 128 ? launch_attn8<128, T>(p, ws, st) : launch_attn8<256, T>(p, ws, st);
 }
 
+template <typename T, int THREADS>
+int launch_logprobs_of(const LogprobsArgs& p, int size, cudaStream_t st) {
+  if (size > 8) CU(cudaFuncSetAttribute(logprobs_kernel<T, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  CU(launch_cluster(logprobs_kernel<T, THREADS>, dim3((unsigned)(p.rows * size)), dim3(THREADS), size, 0, st, true, p));
+  return HSG_OK;
+}
 template <typename T>
 int launch_logprobs(const LogprobsArgs& p, cudaStream_t st) {
-  // blocks a row: as many as it takes to give every SM two, up to a cluster's eight
+  static const int force = getenv("LP") ? atoi(getenv("LP")) : 0;
+  if (force) {
+    const int s = force % 100;
+    return force / 100 == 1 ? launch_logprobs_of<T, 1024>(p, s, st) : force / 100 == 2 ? launch_logprobs_of<T, 512>(p, s, st) : launch_logprobs_of<T, 256>(p, s, st);
+  }
+  // blocks a row: as many as it takes to give every SM two, up to a cluster's sixteen
   int size = 1;
-  while (size < LP_CLUSTER && (int64_t)p.rows * size < 2 * SM_COUNT) size *= 2;
-  CU(launch_cluster(logprobs_kernel<T>, dim3((unsigned)(p.rows * size)), dim3(LP_THREADS), size, 0, st, false, p));
-  return HSG_OK;
+  while (size < 8 && (int64_t)p.rows * size < 2 * SM_COUNT) size *= 2;
+  return launch_logprobs_of<T, 512>(p, size, st);
 }
 
 }  // namespace

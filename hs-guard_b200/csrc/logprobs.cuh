@@ -9,14 +9,14 @@
 // Alternatives: a thread also remembers the largest value that it met. A value tau that at least `top` threads' largest reach
 // (a bisection over its bits, threads counted by a block-wide vote) is no larger than the top-th value of the block's share,
 // so every alternative is at least tau and lies with a thread whose largest is: only what those few threads read is read
-// again, by whole warps, and what reaches tau becomes a candidate (about as many as are asked for), ranked by counting.
+// again, by all threads, and what reaches tau becomes a candidate (about as many as are asked for), ranked by counting.
 // Equal values rank by token, the lowest first. If too many values reach tau (long runs of equal or ascending values), the
 // alternatives are taken one by one instead: the block's largest, after which its owner's warp looks for that thread's next.
 //
-// A row is shared by a cluster of up to 8 blocks, whose parts meet in the first one's shared memory.
+// A row is shared by a cluster of up to 16 blocks, whose parts meet in the first one's shared memory.
 #pragma once
 #include "draft_rows.cuh"
-#include "ring_prefill_tc.cuh"  // ex2_approx
+#include "draft_attn.cuh"  // ex2_approx, add2, fma2
 
 namespace hsg {
 
@@ -34,12 +34,10 @@ struct LogprobsArgs {
   int* err;
 };
 
-constexpr int LP_THREADS = 512;
-constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_MAX_TOP = 64;
-constexpr int LP_CLUSTER = 8;
+constexpr int LP_CLUSTER = 16;
 constexpr int LP_CAND = 512;      // candidates that are ranked by counting
-constexpr int LP_OWNERS = 96;     // threads whose values are read again, as far as the bisection can tell
+constexpr int LP_MORE = 12;       // threads beyond `top` whose values are read again, as far as the bisection can tell
 constexpr int LP_LIVE = 4;        // 16-byte pieces a thread has under way
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
@@ -79,6 +77,21 @@ struct LpSum {
     u = f * fmaf(d, s, u);
     s *= f;
     m = to;
+  }
+  // four or eight at a time, two in an instruction
+  template <int N> __device__ __forceinline__ void add_all(const float (&x)[N], float off, float c) {
+    float2 s2 = make_float2(s, 0.f), u2 = make_float2(u, 0.f);
+    const float2 less = make_float2(-off, -off), by = make_float2(c, c), zero = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float2 d = fma2(add2(make_float2(x[i], x[i + 1]), less), by, zero);
+      d = make_float2(max_nan(d.x, -200.f), max_nan(d.y, -200.f));
+      const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+      s2 = add2(s2, e);
+      u2 = fma2(e, d, u2);
+    }
+    s = s2.x + s2.y;
+    u = u2.x + u2.y;
   }
   __device__ __forceinline__ void add(float x, float off, float c) {
     const float d = max_nan((x - off) * c, -200.f), e = ex2_approx(d);
@@ -134,16 +147,17 @@ __device__ __forceinline__ float cluster_load32(uint32_t addr) {
   return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_constant__ LogprobsArgs a) {
-  constexpr int V = 16 / sizeof(T);  // elements of a 16-byte piece
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const __grid_constant__ LogprobsArgs a) {
+  constexpr int V = 16 / sizeof(T), WARPS = THREADS / 32;  // elements of a 16-byte piece
   __shared__ uint64_t s_top[LP_MAX_TOP];           // the block's alternatives, best first; 0: none
   __shared__ uint64_t s_cand[LP_CAND];
-  __shared__ uint64_t s_all[LP_CLUSTER * LP_MAX_TOP];
+  __shared__ uint64_t s_all[THREADS < 1024 ? 8 * LP_MAX_TOP : LP_CLUSTER * LP_MAX_TOP];
   __shared__ float s_sum[3];                       // the block's (m, S, U)
-  __shared__ float s_warp[3][LP_WARPS];
-  __shared__ uint64_t s_key[LP_WARPS];
-  __shared__ int s_owner[LP_THREADS];
+  __shared__ float s_warp[3][WARPS];
+  __shared__ uint32_t s_best[WARPS];
+  __shared__ uint64_t s_key[WARPS];
+  __shared__ int s_owner[THREADS];
   __shared__ int s_n[2];                           // candidates, owners
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), size = (int)cluster_size(), row = blockIdx.x / size;
@@ -157,6 +171,15 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
   // one more element for some threads: of the head with the first block, of the tail with the last
   const int extra = rank == 0 && tid < head ? tid : rank == size - 1 && tid >= 32 && tid < 32 + tail ? a.vocab - tail + tid - 32 : -1;
 
+  pdl_wait();
+  pdl_trigger();
+  // the first given token and its logit, by the block that writes it, ahead of the row
+  int given = -1;
+  float given_x = 0.f;
+  if (rank == 0 && tid < a.n_given) {
+    given = a.given[(int64_t)row * a.n_given + tid];
+    if (given >= 0 && given < a.vocab) given_x = (float)x[given];
+  }
   LpSum sum;
   float best = -INFINITY;  // largest value met, and the piece that had it first (-1: the single element, -2: none)
   int best_at = -2;
@@ -167,27 +190,28 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     best = v;
     best_at = -1;
   }
-  for (int p = p0 + tid; p < p1; p += LP_THREADS * LP_LIVE) {
+  for (int p = p0 + tid; p < p1; p += THREADS * LP_LIVE) {
     float v[LP_LIVE][V];
 #pragma unroll
     for (int u = 0; u < LP_LIVE; ++u)
-      if (p + u * LP_THREADS < p1) lp_load(body + (int64_t)(p + u * LP_THREADS) * V, v[u]);
+      if (p + u * THREADS < p1) lp_load(body + (int64_t)(p + u * THREADS) * V, v[u]);
 #pragma unroll
     for (int u = 0; u < LP_LIVE; ++u) {
-      if (p + u * LP_THREADS >= p1) break;
+      if (p + u * THREADS >= p1) break;
       float t = v[u][0];
 #pragma unroll
       for (int e = 1; e < V; ++e) t = fmaxf(t, v[u][e]);
       if (t > best || best_at == -2) {
         best = t;
-        best_at = p + u * LP_THREADS;
+        best_at = p + u * THREADS;
       }
       if (t > sum.m) sum.raise(t, c);
       const float off = sum.m == -INFINITY ? 0.f : sum.m;
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum.add(v[u][e], off, c);
+      sum.add_all(v[u], off, c);
     }
   }
+  const uint32_t mine = best_at == -2 ? 0u : max(1u, lp_order(best == 0.f ? 0.f : best));
+  const uint32_t warp_best = __reduce_max_sync(0xffffffffu, mine);
   // ---- the block's sums ----
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -199,19 +223,20 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     s_warp[0][warp] = sum.m;
     s_warp[1][warp] = sum.s;
     s_warp[2][warp] = sum.u;
+    s_best[warp] = warp_best;
   }
   if (tid < LP_MAX_TOP) s_top[tid] = 0;
   if (tid < 2) s_n[tid] = 0;
   __syncthreads();
   if (warp == 0) {
     LpSum all;
-    if (lane < LP_WARPS) {
+    if (lane < WARPS) {
       all.m = s_warp[0][lane];
       all.s = s_warp[1][lane];
       all.u = s_warp[2][lane];
     }
 #pragma unroll
-    for (int o = LP_WARPS / 2; o > 0; o >>= 1)
+    for (int o = WARPS / 2; o > 0; o >>= 1)
       all.join(__shfl_xor_sync(0xffffffffu, all.m, o), __shfl_xor_sync(0xffffffffu, all.s, o),
                __shfl_xor_sync(0xffffffffu, all.u, o), c);
     if (lane == 0) {
@@ -222,10 +247,16 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
   }
   // ---- the block's alternatives ----
   if (a.top) {
-    const uint32_t mine = best_at == -2 ? 0u : max(1u, lp_order(best == 0.f ? 0.f : best));
-    uint32_t lo = 0, hi = ~0u;  // at least `top` threads reach lo (or all that have anything), fewer reach hi
-    int reach = LP_THREADS;
-    while (hi - lo > 1 && reach > LP_OWNERS) {
+    // at least `top` threads reach lo (or all that have anything), fewer reach hi; values of an eighth of the largest or more first
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) hi = max(hi, s_best[w]);
+    const uint32_t near = hi > 1u << 24 ? hi - (1u << 24) : 0u;
+    hi = hi == ~0u ? hi : hi + 1;
+    int reach = __syncthreads_count(mine >= near);
+    if (reach >= a.top) lo = near;
+    else reach = THREADS, hi = near;
+    while (hi - lo > 1 && reach > a.top + LP_MORE) {
       const uint32_t mid = lo + (hi - lo) / 2;
       const int n = __syncthreads_count(mine >= mid);
       if (n >= a.top) {
@@ -238,7 +269,6 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     const uint32_t tau = max(1u, lo);
     if (mine >= tau) s_owner[atomicAdd(&s_n[1], 1)] = tid;
     __syncthreads();
-    const int owners = s_n[1];
     auto consider = [&](float v, int i) {
       if (lp_order(v == 0.f ? 0.f : v) >= tau) {
         const int at = atomicAdd(&s_n[0], 1);
@@ -246,14 +276,14 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
       }
     };
     if (extra >= 0) consider((float)x[extra], extra);
-    for (int w = warp; w < owners; w += LP_WARPS) {
-      const int t = s_owner[w];
-      for (int p = p0 + t + lane * LP_THREADS; p < p1; p += 32 * LP_THREADS) {
-        float v[V];
-        lp_load(body + (int64_t)p * V, v);
+    const int each = (p1 - p0 + THREADS - 1) / THREADS, again = s_n[1] * each;  // pieces of a thread, to be read again
+    for (int j = tid; j < again; j += THREADS) {
+      const int o = j / each, p = p0 + s_owner[o] + (j - o * each) * THREADS;
+      if (p >= p1) continue;
+      float v[V];
+      lp_load(body + (int64_t)p * V, v);
 #pragma unroll
-        for (int e = 0; e < V; ++e) consider(v[e], head + p * V + e);
-      }
+      for (int e = 0; e < V; ++e) consider(v[e], head + p * V + e);
     }
     __syncthreads();
     const int n = s_n[0];
@@ -268,7 +298,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
       // one by one: `next` is this thread's best that has not been taken
       uint64_t next = 0;
       if (extra >= 0) next = lp_key((float)x[extra], extra);
-      for (int p = p0 + tid; p < p1; p += LP_THREADS) {
+      for (int p = p0 + tid; p < p1; p += THREADS) {
         float v[V];
         lp_load(body + (int64_t)p * V, v);
 #pragma unroll
@@ -287,7 +317,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
         if (lane == 0) s_key[warp] = most;
         __syncthreads();
         uint64_t taken = 0;
-        for (int w = 0; w < LP_WARPS; ++w) taken = s_key[w] > taken ? s_key[w] : taken;
+        for (int w = 0; w < WARPS; ++w) taken = s_key[w] > taken ? s_key[w] : taken;
         if (taken == 0) break;
         if (tid == 0) s_top[k] = taken;
         const unsigned owns = __ballot_sync(0xffffffffu, next == taken);
@@ -298,7 +328,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
             const uint64_t key = lp_key((float)x[ex], ex);
             if (key < taken) found = key;
           }
-          for (int p = p0 + t + lane * LP_THREADS; p < p1; p += 32 * LP_THREADS) {
+          for (int p = p0 + t + lane * THREADS; p < p1; p += 32 * THREADS) {
             float v[V];
             lp_load(body + (int64_t)p * V, v);
 #pragma unroll
@@ -339,7 +369,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
           s_warp[2][0] = all.u;
         }
       }
-      for (int j = tid; j < size * a.top; j += LP_THREADS) {
+      for (int j = tid; j < size * a.top; j += THREADS) {
         const int r = j / a.top;
         s_all[j] = cluster_load64(cluster_addr(&s_top[j - r * a.top], r));
       }
@@ -349,7 +379,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     if (tid < 3) s_sum[tid] = s_warp[tid][0];
     if (tid < a.top) s_top[tid] = 0;
     __syncthreads();
-    for (int j = tid; j < size * a.top; j += LP_THREADS) {
+    for (int j = tid; j < size * a.top; j += THREADS) {
       const uint64_t key = s_all[j];
       if (!key) continue;
       const int r = j / a.top;
@@ -376,18 +406,18 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const __grid_const
     a.lse[row] = good ? fmaf(m, a.inv_t, log_s) : s == 0.f ? -INFINITY : nan;
     a.entropy[row] = good ? log_s - kLn2 * (u / s) : nan;
   }
-  for (int j = tid; j < a.n_given; j += LP_THREADS) {
-    const int i = a.given[(int64_t)row * a.n_given + j];
+  for (int j = tid; j < a.n_given; j += THREADS) {
+    const int i = j == tid ? given : a.given[(int64_t)row * a.n_given + j];
     float y = 0.f;
     if (i >= a.vocab) {
       set_error(a.err, ERR_BAD_TOKEN);
       y = nan;
     } else if (i >= 0) {
-      y = good ? fmaf((float)x[i] - m, a.inv_t, -log_s) : nan;
+      y = good ? fmaf((j == tid ? given_x : (float)x[i]) - m, a.inv_t, -log_s) : nan;
     }
     a.logprobs[(int64_t)row * a.n_given + j] = y;
   }
-  for (int j = tid; j < a.top; j += LP_THREADS) {
+  for (int j = tid; j < a.top; j += THREADS) {
     const uint64_t key = s_top[j];
     a.top_logprobs[(int64_t)row * a.top + j] = good ? fmaf(lp_value(key) - m, a.inv_t, -log_s) : nan;
     a.top_ids[(int64_t)row * a.top + j] = good ? lp_token(key) : -1;
