@@ -119,20 +119,18 @@ int launch_attn8_dim(const Attn8Args& p, int dim, void* ws, cudaStream_t st) {
 
 template <typename T, int THREADS>
 int launch_logprobs_of(const LogprobsArgs& p, int size, cudaStream_t st) {
-  if (size > 8) CU(cudaFuncSetAttribute(logprobs_kernel<T, THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   CU(launch_cluster(logprobs_kernel<T, THREADS>, dim3((unsigned)(p.rows * size)), dim3(THREADS), size, 0, st, true, p));
   return HSG_OK;
 }
 template <typename T>
 int launch_logprobs(const LogprobsArgs& p, cudaStream_t st) {
-  static const int force = getenv("LP") ? atoi(getenv("LP")) : 0;
-  if (force) {
-    const int s = force % 100;
-    return force / 100 == 1 ? launch_logprobs_of<T, 1024>(p, s, st) : force / 100 == 2 ? launch_logprobs_of<T, 512>(p, s, st) : launch_logprobs_of<T, 256>(p, s, st);
-  }
-  // blocks a row: as many as it takes to give every SM two, up to a cluster's sixteen
+  // Rows that fill the device with four blocks an SM have 256 threads each, so that one row's selection overlaps others' reading;
+  // fewer have 512, and as many blocks a row as two an SM leave room for, up to eight. 2,500 rows of 50,001 fp16: 71 us with 256
+  // threads, 91 with 512; 352 of 248,320 bf16: 63 and 46 (51 with two blocks a row); one of 248,320 fp32: 12.1 with eight blocks of
+  // 256, 10.7 of 512, 11.9 of 1,024 (sixteen of those: 13.7).
+  if (p.rows >= 4 * SM_COUNT) return launch_logprobs_of<T, 256>(p, 1, st);
   int size = 1;
-  while (size < 8 && (int64_t)p.rows * size < 2 * SM_COUNT) size *= 2;
+  while (size < LP_CLUSTER && (int64_t)p.rows * size * 2 <= 2 * SM_COUNT) size *= 2;
   return launch_logprobs_of<T, 512>(p, size, st);
 }
 
