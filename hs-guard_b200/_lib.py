@@ -99,7 +99,7 @@ def lib():
         L.hsg_slot_state_bytes.argtypes, L.hsg_slot_state_bytes.restype = [P], C.c_size_t
         L.hsg_stream.argtypes, L.hsg_stream.restype = [P], P
         L.hsg_tree_attention_workspace.argtypes, L.hsg_tree_attention_workspace.restype = [I], C.c_size_t
-        L.hsg_attention8_workspace.argtypes, L.hsg_attention8_workspace.restype = [I], C.c_size_t
+        L.hsg_attention8_workspace.argtypes, L.hsg_attention8_workspace.restype = [I, I, I], C.c_size_t
         L.hsg_device_error_text.argtypes, L.hsg_device_error_text.restype = [I], C.c_char_p
         L.hsg_last_error.argtypes, L.hsg_last_error.restype = [], C.c_char_p
         L.hsg_version.argtypes, L.hsg_version.restype = [], C.c_char_p

@@ -72,6 +72,11 @@ int make_codes_map(CUtensorMap* map, const uint8_t* base, const Cache8& c, int d
   return HSG_OK;
 }
 
+// Workspace: partial results of either kernel, then what the wide one makes of the queries
+size_t attn8_fixed_bytes(int dim) {
+  return (std::max(a8_workspace_bytes(dim, A8_WARPS, A8_ROWS), a8_workspace_bytes(dim, 1, W8_ROWS)) + 127) / 128 * 128;
+}
+
 template <int D, int NR, typename T>
 int launch_attn8_narrow(const Attn8Args& p, A8Split* splits, cudaStream_t st) {
   constexpr int PIECES = A8_BLOCKS * A8_WARPS;
@@ -103,8 +108,35 @@ int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   const int64_t rows = std::min<int64_t>(p.max_new, (p.tokens + p.rows - 1) / p.rows) * (p.hq / p.hkv);
   if (rows > A8_WIDE_ROWS) {
     float* partials = reinterpret_cast<float*>(splits + A8_BLOCKS);
-    CU(cudaFuncSetAttribute(attn8_wide_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, w8_smem(D)));
-    CU(launch_k(attn8_wide_kernel<D, T>, dim3(A8_BLOCKS), dim3(W8_THREADS), w8_smem(D), st, true, p, splits, partials));
+    int box = w8_tile(D);  // tokens of a TMA box: all of one page
+    while (p.cache.page % box) box /= 2;
+    const int cols = D == 256 && box == w8_tile(D) ? 2 : 1, smem = w8_smem(D, std::is_same<T, __half>::value ? 3 : 2);
+    CUtensorMap k, v;
+    int rc;
+    if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||
+        (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
+      return rc;
+    // queries as sums of e4m3 numbers, behind the partial results
+    constexpr int PARTS = std::is_same<T, __half>::value ? 3 : 2;
+    const int64_t q_rows = (int64_t)p.tokens * p.hq;
+    uint8_t* parts = static_cast<uint8_t*>(workspace) + attn8_fixed_bytes(D);
+    float* q_scales = reinterpret_cast<float*>(parts + 3 * q_rows * D);
+    CUtensorMap q;
+    {
+      const int wide = std::min(D, 128);
+      const cuuint64_t dims[4] = {(cuuint64_t)wide, (cuuint64_t)q_rows, (cuuint64_t)(D / wide), PARTS};
+      const cuuint64_t strides[3] = {(cuuint64_t)D, 128, (cuuint64_t)q_rows * D};
+      const cuuint32_t boxes[4] = {(cuuint32_t)wide, W8_ROWS, (cuuint32_t)(D / wide), 1}, one[4] = {1, 1, 1, 1};
+      CUresult r = g_encode(&q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, parts, dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (r != CUDA_SUCCESS) return fail(HSG_ERR_CUDA, "cuTensorMapEncodeTiled (queries) failed (%d)", (int)r);
+    }
+    constexpr int ROWS_A_BLOCK = 8 * 256 / D;
+    CU(launch_k(attn8_split_kernel<D, T>, dim3((unsigned)((q_rows + ROWS_A_BLOCK - 1) / ROWS_A_BLOCK)), dim3(256), 0, st, true, (const T*)p.q, p.q_ts,
+                p.q_hs, p.tokens, p.hq, p.hq / p.hkv, parts, q_scales));
+    CU(cudaFuncSetAttribute(attn8_wide_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CU(launch_k(attn8_wide_kernel<D, T>, dim3(A8_BLOCKS), dim3(W8_THREADS), smem, st, true, q, k, v, p, box, (const float*)q_scales, splits, partials));
     CU(launch_k(attn8_join_kernel<D, W8_ROWS, T>, dim3(A8_BLOCKS, W8_ROWS / (A8J_THREADS / 32)), dim3(A8J_THREADS), 0, st, true, p,
                 (const A8Split*)splits, (const float*)partials));
     return HSG_OK;
@@ -162,7 +194,9 @@ extern "C" int hsg_append8(const hsg_append8_args* a) {
   return a->dtype == HSG_DT_F16 ? launch_append8_dim<__half>(p, a->dim, st) : launch_append8_dim<__nv_bfloat16>(p, a->dim, st);
 }
 
-extern "C" size_t hsg_attention8_workspace(int head_dim) { return head_dim_ok(head_dim) ? std::max(a8_workspace_bytes(head_dim, A8_WARPS, A8_ROWS), a8_workspace_bytes(head_dim, 1, W8_ROWS)) : 0; }
+extern "C" size_t hsg_attention8_workspace(int head_dim, int tokens, int hq) {
+  return head_dim_ok(head_dim) && tokens >= 0 && hq > 0 ? attn8_fixed_bytes(head_dim) + (size_t)tokens * hq * (3 * head_dim + 4) : 0;
+}
 
 extern "C" int hsg_attention8(const hsg_attention8_args* a) {
   DRAFT_ARGS(a);
@@ -180,8 +214,9 @@ extern "C" int hsg_attention8(const hsg_attention8_args* a) {
   if (a->window < 0 || a->sinks < 0) return fail(HSG_ERR_INVALID, "window and sinks must not be negative, got %d and %d", a->window, a->sinks);
   if (a->rows == 0 || a->tokens == 0) return HSG_OK;
   if (!a->q || !a->table || !a->lens || !a->cu || !a->out) return fail(HSG_ERR_INVALID, "NULL argument");
-  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)hsg_attention8_workspace(a->dim))
-    return fail(HSG_ERR_INVALID, "the workspace must have %zu bytes on a 16-byte boundary", hsg_attention8_workspace(a->dim));
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < (int64_t)hsg_attention8_workspace(a->dim, a->tokens, a->hq))
+    return fail(HSG_ERR_INVALID, "the workspace must have %zu bytes on a 16-byte boundary",
+                hsg_attention8_workspace(a->dim, a->tokens, a->hq));
   if (a->width < 1 || a->table_stride < a->width)
     return fail(HSG_ERR_INVALID, "bad table shape (width %d, stride %lld)", a->width, (long long)a->table_stride);
   int rc;
@@ -190,7 +225,7 @@ extern "C" int hsg_attention8(const hsg_attention8_args* a) {
     return fail(HSG_ERR_INVALID, "%d pages of %d tokens are beyond 32-bit positions", a->width, a->cache.page_size);
   if (!aligned16(a->q) || !aligned16(a->out) || !rows16(a->q_token_stride, a->q_head_stride, 2))
     return fail(HSG_ERR_INVALID, "q rows must lie on 16-byte boundaries");
-  if ((int64_t)a->max_new * (a->hq / a->hkv) > INT32_MAX / 2) return fail(HSG_ERR_INVALID, "too many rows a key head");
+  if ((int64_t)a->tokens * a->hq > INT32_MAX || (int64_t)a->max_new * (a->hq / a->hkv) > INT32_MAX / 2) return fail(HSG_ERR_INVALID, "too many rows a key head");
   Attn8Args p{a->q, a->q_token_stride, a->q_head_stride, cache8(a->cache), a->table, a->table_stride, a->lens, a->cu,
               a->positions, a->mask, a->rows, a->width, a->tokens, a->words, a->max_new, a->hq, a->hkv, a->window, a->sinks,
               a->scale, a->out, a->lse, a->err};

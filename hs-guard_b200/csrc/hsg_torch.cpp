@@ -574,7 +574,7 @@ PyObject* attention_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.window = whole(a[12], "window", 0, INT32_MAX);
     s.sinks = whole(a[13], "sinks", 0, INT32_MAX);
     Tensor workspace;
-    if (a[14] == Py_None) workspace = empty({(int64_t)hsg_attention8_workspace(s.dim)}, at::kByte, device);
+    if (a[14] == Py_None) workspace = empty({(int64_t)hsg_attention8_workspace(s.dim, s.tokens, s.hq)}, at::kByte, device);
     else workspace = shaped(a[14], "workspace", 1, at::kByte, device);
     s.workspace = workspace.data_ptr();
     s.workspace_bytes = workspace.numel();

@@ -151,9 +151,9 @@ def append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source=None, po
                                  rope_scale, q, err)
 
 
-def attention_8bit_workspace(dim):
-    """Bytes of workspace an ``attention_8bit`` call of this head dim uses."""
-    return int(_lib.lib().hsg_attention8_workspace(dim))
+def attention_8bit_workspace(dim, tokens, heads):
+    """Bytes of workspace that an ``attention_8bit`` call of this head dim and up to so many query tokens and heads uses."""
+    return int(_lib.lib().hsg_attention8_workspace(dim, tokens, heads))
 
 
 def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask=None, positions=None, window=0,
@@ -168,7 +168,7 @@ def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale
     minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (None: their places in the cache) are
     read only then. Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets
     0 and -inf, as do tokens outside cu[0] .. cu[rows] - 1 and those of a request whose lengths are out of range (which ``err``
-    records). ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim)`` bytes, for one call at a time) is allocated when it
+    records). ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim, tokens, hq)`` bytes, for one call at a time) is allocated when it
     is not given."""
     return tensors().attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask, positions, window,
                                     sinks, workspace, err)

@@ -107,8 +107,9 @@ def test_a_call_without_work_does_nothing(L):
 
 
 def test_workspace(L):
-    assert drafts.attention_8bit_workspace(96) == 0
-    assert 0 < drafts.attention_8bit_workspace(64) <= drafts.attention_8bit_workspace(256)
+    assert drafts.attention_8bit_workspace(96, 1, 8) == 0
+    small, large = drafts.attention_8bit_workspace(64, 1, 8), drafts.attention_8bit_workspace(256, 1, 8)
+    assert 0 < small <= large < drafts.attention_8bit_workspace(256, 2, 8) == drafts.attention_8bit_workspace(256, 1, 16)
 
 
 def test_host_tensors_are_refused():

@@ -543,7 +543,7 @@ def test_attention_streams_and_graphs(D):
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
-    ws = torch.empty(D.attention_8bit_workspace(128), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(D.attention_8bit_workspace(128, 4, 8), dtype=torch.uint8, device="cuda")
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         o = attend(D, s, 0.1, 2, workspace=ws)
