@@ -33,7 +33,11 @@ Cache8 cache8(const hsg_cache8& c) {
 }
 
 static_assert(A8_BLOCKS == SM_COUNT, "one piece an SM");
-constexpr int A8_WIDE_ROWS = 32;  // rows of a key head up to which warp-level products are taken
+// Rows of a key head, on average over the requests, up to which warp-level products are taken. Narrow and wide, us: head dim 128, 40
+// requests of 6,000 tokens, 8 query heads a key head: 16 rows 60 and 77, 24 rows 79 and 78, 48 rows 115 and 82; 5 requests of
+// 50,000: 12 rows 87 and 92, 24 rows 138 and 93; head dim 256, 352 requests, window 512: 12 rows 104 and 145, 24 rows 151 and
+// 148, 48 rows 252 and 162; head dim 64, 64 requests of 2,100: 12 rows 104 and 160, 24 rows 175 and 162.
+constexpr int A8_WIDE_ROWS = 20;
 
 template <int D, typename T>
 int launch_append8(const Append8Args& p, cudaStream_t st) {
