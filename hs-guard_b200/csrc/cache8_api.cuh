@@ -109,7 +109,7 @@ template <int D, typename T>
 int launch_attn8(const Attn8Args& p, void* workspace, cudaStream_t st) {
   A8Split* splits = static_cast<A8Split*>(workspace);
   // rows of a key head, as far as the host can tell: no request has more than max_new tokens, all have `tokens` together
-  const int64_t rows = std::min<int64_t>(p.max_new, (p.tokens + p.rows - 1) / p.rows) * (p.hq / p.hkv);
+  const int64_t rows = std::min<int64_t>(p.max_new, ((int64_t)p.tokens + p.rows - 1) / p.rows) * (p.hq / p.hkv);
   if (rows > A8_WIDE_ROWS) {
     float* partials = reinterpret_cast<float*>(splits + A8_BLOCKS);
     int box = w8_tile(D);  // tokens of a TMA box: all of one page

@@ -236,6 +236,42 @@ def test_append_a_scale_that_rises_and_one_that_stays(D):
         check_append(s, ref, False)
 
 
+@pytest.mark.parametrize("pad", [1, 31, 33, 200])
+def test_append_of_a_padded_batch(D, pad):
+    """Entries that are skipped before, within and after a block's: queries of all of them are turned, the block is one."""
+    page, hkv, hq, dim = 64, 2, 6, 128
+    s = append_state(5, page, 32, hkv, dim, False, 20)
+    slots = [-1] * pad + [64, 65] + [-1] * pad + [66, 67, 96] + [-1] * pad + [130] + [-1] * pad + [131] * 1 + [-1] * pad
+    n = len(slots)
+    g = torch.Generator().manual_seed(pad)
+    x = torch.randn(n, hq + 2 * hkv, dim, generator=g).bfloat16().cuda()
+    q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+    inv = 10000.0 ** (-torch.arange(0, 64, 2).float() / 64)
+    p = torch.arange(n, dtype=torch.int32) * 7
+    ref = append_reference(s, k, v, slots, None, p, inv, False, 1.0)
+    err = err_word()
+    got = D.append_8bit(k, v, s["kc"], s["vc"], s["ks"], s["vs"], dev(slots), positions=p.cuda(), inv_freq=inv.cuda(), q=q, err=err)
+    assert int(err.item()) == 0
+    check_append(s, ref, True)
+    y, _ = turned(q.cpu(), p, inv, False, 1.0)
+    assert bool(((got.cpu().double() - y).abs() <= U[BF16] * y.abs() + 1e-5 * y.abs().amax(-1, keepdim=True)).all())
+
+
+def test_append_far_positions(D):
+    """Angles of positions up to 2^31 - 1, and of negative ones, to fp32's own exactness."""
+    page, dim = 16, 64
+    s = append_state(2, page, 16, 1, dim, False, 21)
+    p = torch.tensor([0, 1, 65537, 1 << 24, (1 << 24) + 1, 1 << 30, 2 ** 31 - 1, -5], dtype=torch.int32)
+    inv = torch.cat([torch.tensor([1.0, 0.9999999, 3.1, 7.5, 100.25]), 500000.0 ** (-torch.arange(0, 54, 2).float() / 64)])
+    x = torch.randn(8, 3, dim, generator=torch.Generator().manual_seed(2)).half().cuda()
+    q = D.append_8bit(x[:, :1], x[:, 1:2], s["kc"], s["vc"], s["ks"], s["vs"], dev(range(8)), positions=p.cuda(), inv_freq=inv.cuda(), q=x[:, 2:])
+    y, _ = turned(x[:, 2:].cpu(), p, inv, False, 1.0)
+    # 2^31 positions times 2^-53 of a frequency of up to 100 / (2 pi) turns: below 2^-18 of a turn there, 1e-6 at ordinary ones
+    angle = p.double().abs()[:, None, None] * inv.double().abs() * 2.0 ** -52
+    slack = 1e-6 + torch.cat([angle, angle], -1)
+    assert bool(((q.cpu().double() - y).abs() <= U[F16] * y.abs() + slack * 8 + 1e-6).all())
+
+
 def test_append_refuses_slots_on_the_device(D):
     """Slots beyond the pages, ones that do not ascend in a block, sources outside the rows: recorded, the rest is written."""
     page, hkv, dim = 16, 2, 64
