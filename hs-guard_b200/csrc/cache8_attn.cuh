@@ -46,6 +46,13 @@ struct Attn8Args {
 // that sum, so that weights use fp16's range however the scales differ, and the row sum takes w_j / vs_j. Weights are rounded to
 // fp16 (2^-11, the largest between 2^11 and 2^15, as in the 16-bit attention); sums, maxima and accumulators are fp32.
 //
+// Measured on B200: 352 requests of one or two tokens, 512-token window and 4 first tokens, 8 / 2 heads of 256: 186 MB in 56 us,
+// 3.3 TB/s: 6 us until the first slice is there, HBM at 4 to 5 TB/s, then the last pieces (they end up to 14% after the mean) and 5
+// for the join. 5 requests of up to 50,001 tokens, 3 tokens, 32 / 8 heads of 128: 360 MB in 75 to 96 us (the clock), 64 requests of
+// up to 2,100 tokens, 16 / 16 heads of 64, pages of 8: 195 MB in 80 us. Instructions of few warps bound those (1.3 a clock and SM,
+// waits for results of the ones before): codes to fp16, and at pages of 8 the copies, of which each costs a warp about 30. One
+// token: 14 us of latencies.
+//
 // The order of dims and keys within a product is free as long as both factors agree: a lane reads 16 consecutive bytes of a key,
 // which are its elements of four steps of 16 dims, and for P V consecutive dims of two keys, interleaved bytewise. Which keys
 // (a8_key) and which dims (a8_piece_of) a lane takes is chosen so that reading the swizzled slices meets no bank twice at head dims
