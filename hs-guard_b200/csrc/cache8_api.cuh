@@ -78,12 +78,13 @@ int make_codes_map(CUtensorMap* map, const uint8_t* base, const Cache8& c, int d
 
 // Workspace: partial results of either kernel, then what the wide one makes of the queries
 size_t attn8_fixed_bytes(int dim) {
-  return (std::max(a8_workspace_bytes(dim, A8_WARPS, A8_ROWS), a8_workspace_bytes(dim, 1, W8_ROWS)) + 127) / 128 * 128;
+  const size_t one = a8_workspace_bytes(dim, a8_warps(dim, 1), 8), two = a8_workspace_bytes(dim, a8_warps(dim, 2), 16);
+  return (std::max(std::max(one, two), a8_workspace_bytes(dim, 1, W8_ROWS)) + 127) / 128 * 128;
 }
 
 template <int D, int NR, typename T>
 int launch_attn8_narrow(const Attn8Args& p, A8Split* splits, cudaStream_t st) {
-  constexpr int PIECES = A8_BLOCKS * A8_WARPS;
+  constexpr int PIECES = A8_BLOCKS * a8_warps(D, NR);
   float* partials = reinterpret_cast<float*>(splits + PIECES);
   int box = a8_slice(D);  // tokens of a TMA box: all of one page
   while (p.cache.page % box) box /= 2;
@@ -93,12 +94,12 @@ int launch_attn8_narrow(const Attn8Args& p, A8Split* splits, cudaStream_t st) {
   if ((rc = make_codes_map(&k, p.cache.k, p.cache, D, p.hkv, box, cols)) != HSG_OK ||
       (rc = make_codes_map(&v, p.cache.v, p.cache, D, p.hkv, box, cols)) != HSG_OK)
     return rc;
-  CU(cudaFuncSetAttribute(attn8_kernel<D, NR, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D)));
+  CU(cudaFuncSetAttribute(attn8_kernel<D, NR, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, a8_smem(D, NR)));
   // as many thread blocks as can have a piece: items, and the slices that one can see at most
   const int64_t group = p.hq / p.hkv, reach = std::min<int64_t>((int64_t)p.width * p.cache.page, p.window ? (int64_t)p.window + p.sinks + p.max_new : INT64_MAX);
   const int64_t items = std::min<int64_t>(p.tokens * group, (p.tokens * group) / (8 * NR) + p.rows) * p.hkv;
   const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(PIECES, items * (reach / a8_slice(D) + 4 + A8_COST) / (A8_COST + 1) + 1));
-  CU(launch_k(attn8_kernel<D, NR, T>, dim3((unsigned)std::min<int64_t>(A8_BLOCKS, pieces)), dim3(A8_THREADS), a8_smem(D), st, true, k, v, p, box,
+  CU(launch_k(attn8_kernel<D, NR, T>, dim3((unsigned)std::min<int64_t>(A8_BLOCKS, pieces)), dim3(32 * a8_warps(D, NR)), a8_smem(D, NR), st, true, k, v, p, box,
               splits, partials));
   const int64_t most = std::min<int64_t>(8 * NR, p.max_new * group);  // rows of an item
   CU(launch_k(attn8_join_kernel<D, 8 * NR, T>, dim3((unsigned)pieces, (unsigned)((most + A8J_THREADS / 32 - 1) / (A8J_THREADS / 32))),

@@ -36,7 +36,7 @@ struct Attn8Args {
 // their columns, so that 8 rows or fewer waste nothing (with queries as the 16 rows it took twice the products, accumulators and
 // exponentials: 352 conversations 63 us). A request's rows of a key head, row r = (token
 // r / G, query head r % G), in blocks of 8 or 16, and the slices of 32 keys (16 at head dim 256) that such a block can see are an item; all items are one
-// line that is cut into equal pieces, one a warp, eight warps an SM, whatever the requests' lengths. Warps do not meet: each has
+// line that is cut into equal pieces, one a warp, eight warps an SM (16 for 8 rows of 64 dims), whatever the requests' lengths. Warps do not meet: each has
 // its ring of slices, which it fills itself ahead of its use (TMA, one box, or as many as a page's size takes), its own running maximum, sums and accumulators. An item that lies in one piece is written out; of one that is cut, each
 // piece leaves its sums in the workspace, and attn8_join_kernel joins them in piece order, so results do not depend on timing.
 //
@@ -49,7 +49,7 @@ struct Attn8Args {
 // Measured on B200: 352 requests of one or two tokens, 512-token window and 4 first tokens, 8 / 2 heads of 256: 186 MB in 56 us,
 // 3.3 TB/s: 6 us until the first slice is there, HBM at 4 to 5 TB/s, then the last pieces (they end up to 14% after the mean) and 5
 // for the join. 5 requests of up to 50,001 tokens, 3 tokens, 32 / 8 heads of 128: 360 MB in 75 to 96 us (the clock), 64 requests of
-// up to 2,100 tokens, 16 / 16 heads of 64, pages of 8: 195 MB in 80 us. Instructions of few warps bound those (1.3 a clock and SM,
+// up to 2,100 tokens, 16 / 16 heads of 64, pages of 8: 195 MB in 59 us. Instructions of few warps bound those (1.3 a clock and SM,
 // waits for results of the ones before): codes to fp16, and at pages of 8 the copies, of which each costs a warp about 30. One
 // token: 14 us of latencies.
 //
@@ -57,8 +57,10 @@ struct Attn8Args {
 // which are its elements of four steps of 16 dims, and for P V consecutive dims of two keys, interleaved bytewise. Which keys
 // (a8_key) and which dims (a8_piece_of) a lane takes is chosen so that reading the swizzled slices meets no bank twice at head dims
 // 128 and 256 (twice at 64, for V).
-constexpr int A8_THREADS = 256;
-constexpr int A8_WARPS = 8;
+// Warps of a thread block, each with its own ring. The accumulators of 8 rows of 64 dims leave room for 16 warps of 128 registers: the
+// 64 requests above take 59 us, with 8 warps 80. The others need up to 255 registers: with 12 warps of 168, up to 2 KB a thread would
+// go to local memory.
+__host__ __device__ constexpr int a8_warps(int dim, int nr) { return dim == 64 && nr == 1 ? 16 : 8; }
 constexpr int A8_ROWS = 16;         // of a block, at most
 constexpr int A8_BLOCKS = 148;      // one thread block an SM
 constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
@@ -66,10 +68,10 @@ constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
 
 __host__ __device__ constexpr int a8_slice(int dim) { return dim == 256 ? 16 : 32; }  // keys
 __host__ __device__ constexpr int a8_stage(int dim) { return 2 * a8_slice(dim) * dim; }
-__host__ __device__ constexpr int a8_stages(int dim) { return dim == 64 ? 6 : dim == 128 ? 3 : 2; }
+__host__ __device__ constexpr int a8_stages(int dim, int nr) { return dim == 64 ? (nr == 1 ? 3 : 6) : dim == 128 ? 3 : 2; }
 // a warp's ring, scales and barriers; where the pieces begin
-__host__ __device__ constexpr int a8_smem(int dim) {
-  return 1024 + A8_WARPS * a8_stages(dim) * (a8_stage(dim) + 40) + 1024;
+__host__ __device__ constexpr int a8_smem(int dim, int nr) {
+  return 1024 + a8_warps(dim, nr) * a8_stages(dim, nr) * (a8_stage(dim) + 40) + 2048;
 }
 __host__ __device__ constexpr size_t a8_partial_floats(int dim, int rows) { return (size_t)rows * (dim + 2); }
 struct A8Split {  // an item that begins in a piece and ends in a later one
@@ -225,9 +227,6 @@ __device__ __forceinline__ int64_t a8_lots(const Attn8Args& a, int G, int cost, 
   return step;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
@@ -290,21 +289,21 @@ __device__ __forceinline__ bool a8_sees(const Attn8Args& a, const A8Req& r, int 
 }
 
 template <int D, int NR, typename T>
-__global__ void __launch_bounds__(A8_THREADS, 1)
+__global__ void __launch_bounds__(32 * a8_warps(D, NR), 1)
 attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Attn8Args a,
              int box, A8Split* splits, float* partials) {
-  constexpr int KEYS = a8_slice(D), GROUPS = KEYS / 8, STAGE = a8_stage(D), ST = a8_stages(D), STEPS = D / 16, NT = D / 16,
-                BLOCKS = D == 256 ? 2 : 1, ROWS = 8 * NR;
+  constexpr int KEYS = a8_slice(D), GROUPS = KEYS / 8, STAGE = a8_stage(D), ST = a8_stages(D, NR), WARPS = a8_warps(D, NR), STEPS = D / 16,
+                NT = D / 16, BLOCKS = D == 256 ? 2 : 1, ROWS = 8 * NR;
   extern __shared__ __align__(1024) uint8_t a8_smem_raw[];
   uint8_t* rings = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a8_smem_raw) + 1023) & ~uintptr_t(1023));  // [warps][ST][K, V]
-  float* ring_scales = reinterpret_cast<float*>(rings + A8_WARPS * ST * STAGE);            // [warps][ST][ks, vs]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + A8_WARPS * ST * 8);           // [warps][ST] a slice has landed
-  A8Lot* lots = reinterpret_cast<A8Lot*>(bars + A8_WARPS * ST);                            // [warps]
-  int64_t* scan = reinterpret_cast<int64_t*>(lots + A8_WARPS);
+  float* ring_scales = reinterpret_cast<float*>(rings + WARPS * ST * STAGE);            // [warps][ST][ks, vs]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + WARPS * ST * 8);           // [warps][ST] a slice has landed
+  A8Lot* lots = reinterpret_cast<A8Lot*>(bars + WARPS * ST);                            // [warps]
+  int64_t* scan = reinterpret_cast<int64_t*>(lots + WARPS);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int piece = warp * A8_BLOCKS + blockIdx.x, G = a.hq / a.hkv, quad = lane & 3, x8 = lane >> 2;
-  if (tid < A8_WARPS * ST) {
+  if (tid < WARPS * ST) {
     mbar_init(bars + tid, 1);
     fence_barrier_init();
   }
@@ -317,7 +316,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   // conversations take 61 and 64 us, one 21.5 and 15.5)
   if (gridDim.x < A8_BLOCKS) pdl_trigger();
   if (lane == 0) splits[piece].last = -1;
-  const int64_t step = a8_lots<ROWS, KEYS, A8_THREADS, A8_WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
+  const int64_t step = a8_lots<ROWS, KEYS, 32 * WARPS, WARPS>(a, G, A8_COST, blockIdx.x, scan, lots);
   const A8Lot lot = lots[warp];
   if (lot.from.b < 0) return;
   // of an item that begins at `unit` on the line, slices up to this lie in the piece

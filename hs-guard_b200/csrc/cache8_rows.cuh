@@ -48,7 +48,6 @@ struct Append8Args {
 
 constexpr int A8R_THREADS = 256;
 constexpr int A8R_LIVE = 4;       // 16-byte pieces a lane has under way
-constexpr float F8_MAX = 448.f;
 constexpr int SCALE_MIN_EXP = -100, SCALE_MAX_EXP = 120;
 
 // The smallest power of two that brings `bound` to at most 448 = 1.75 * 2^8, from its bits.
@@ -99,7 +98,7 @@ template <typename T> __device__ __forceinline__ void unpack8(const uint4& r, fl
 // How a lane turns the eight elements from d on of a row that dim / 8 lanes share: the other element of a pair is among its own
 // eight (pairs) or rot / 16 lanes away. A lane keeps the angles of its row while it goes through the row's heads: read from shared
 // memory for every head they took 64 bytes for 16 of data, at a fourth of the banks' rate (37,500 tokens of 40 heads 326 and
-// 190 us).
+// 264 us, before the other steps).
 //
 // A frequency is the 64-bit fraction of a turn that one position adds, made once a block in fp64 (2^-53 of itself); a position
 // times it, modulo 2^64, is where the position stands within the turn, whatever its size. The 32 upper bits of that go to fp32
