@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     __syncthreads();
     const int n = s_n[0];
     if (n <= LP_CAND) {
-      if (tid < n) {
-        const uint64_t key = s_cand[tid];
+      for (int i = tid; i < n; i += THREADS) {  // as many as twice the threads
+        const uint64_t key = s_cand[i];
         int ahead = 0;
         for (int j = 0; j < n; ++j) ahead += s_cand[j] > key;
         if (ahead < a.top) s_top[ahead] = key;
