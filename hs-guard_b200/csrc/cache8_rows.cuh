@@ -206,28 +206,31 @@ __device__ __forceinline__ void append8_queries(const Append8Args& a, int first,
 }
 
 // Keys and values, one run of entries at a time: ones whose slots ascend within one block, with entries that are not kept between
-// them at most. Warps take tokens and share their heads of K and V like those of queries:
+// them at most. (In a list that has others between, a block's entries are several runs, one after the other.) Warps take tokens and share their heads of K and V like those of queries:
 //   1  the heads' bounds, joined in shared memory;
 //   2  the block's scales (from the run alone if it holds the block's first token, else at least what they were), rows that were
 //      there rounded to a risen scale;
 //   3  rows, read again (mostly from L2), turned, scaled and written.
+// Returns whether there is such a page; then (odd, last) are in s_odd, for all threads after a barrier.
 template <int D, typename T>
-__device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n, int slot0, bool same, const uint64_t* steps, uint32_t* s_units) {
+__device__ __forceinline__ bool append8_run(const Append8Args& a, int i0, int n, int slot0, const uint64_t* steps, uint32_t* s_units, int odd,
+                                            int last, int* s_odd) {
   constexpr int LPR = D / 8, RPW = 32 / LPR, WARPS = A8R_THREADS / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPR;
   A8Turn turn(a, lane, D);
   const float factor = fabsf(a.rope_scale);
   const Cache8& c = a.cache;
   const int blk = c.block_div.div(slot0), page = blk / c.blocks, inner = blk - page * c.blocks, first = slot0 - blk * c.block;
-  if (same || page >= c.pages) {  // a slot that does not ascend, or no page
+  if (page >= c.pages) {
     if (threadIdx.x == 0) set_error(a.err, ERR_BAD_SLOT);
-    return;
+    return false;
   }
   const int64_t base = (int64_t)page * c.page_stride + (int64_t)inner * c.block * c.token_stride;
   const int units = 2 * a.hkv, groups = (n + RPW - 1) / RPW;
   const int split = groups >= WARPS ? 1 : WARPS / groups, teams = WARPS / split, team = warp / split, u_first = warp % split;
   for (int u = threadIdx.x; u < 2 * units; u += A8R_THREADS) s_units[u] = 0u;
   __syncthreads();
+  if (threadIdx.x < 2) s_odd[threadIdx.x] = threadIdx.x ? last : odd;  // what is read after this run does not take a register through it
   int row = -1, at = 0;  // of K and V, and within the block; -1: not kept or not there
   auto token = [&](int g) {
     const int t = g * RPW + sub, i = i0 + t;
@@ -366,6 +369,19 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
       }
     }
   }
+  return true;
+}
+
+// From entry j on, the next of last's block whose slot is above `last`, before any of another block; -1: none.
+__device__ __noinline__ int append8_above(const Append8Args& a, int j, int last) {
+  const int lane = threadIdx.x & 31, blk = a.cache.block_div.div(last);
+  for (; j < a.count; j += 32) {
+    const int s = j + lane < a.count ? a.slots[j + lane] : -1;
+    const bool other = s < blk * a.cache.block || s - blk * a.cache.block >= a.cache.block;
+    const unsigned hit = __ballot_sync(0xffffffffu, s >= 0 && (other || s > last));
+    if (hit) return __shfl_sync(0xffffffffu, (int)other, __ffs(hit) - 1) ? -1 : j + __ffs(hit) - 1;
+  }
+  return -1;
 }
 
 // Blocks 0 .. kv_blocks - 1 take `per` entries each, of which they write the runs that begin there; the others queries, whose heads
@@ -373,6 +389,7 @@ __device__ __forceinline__ void append8_run(const Append8Args& a, int i0, int n,
 template <int D, typename T>
 __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_constant__ Append8Args a, int kv_blocks, int per, int split) {
   __shared__ uint64_t s_steps[128];      // [rot / 2]
+  __shared__ int s_odd[2];
   extern __shared__ uint32_t s_units[];  // [2 hkv] bounds, then inverse scales; [2 hkv] whether infinities are among the rows
   pdl_wait();
   pdl_trigger();
@@ -404,36 +421,46 @@ __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_co
     if (below) before = prev;
   }
   const bool joined = slot >= 0 && before >= 0 && c.block_div.div(slot) == c.block_div.div(before);
-  // those that are not inside a run that began earlier
-  unsigned leaders = __ballot_sync(0xffffffffu, slot >= 0 && !(joined && slot > before));
+  if (joined && slot <= before && threadIdx.x < 32) set_error(a.err, ERR_BAD_SLOT);
+  // a block's entries are its first one's
+  unsigned leaders = __ballot_sync(0xffffffffu, slot >= 0 && !joined);
   if (!leaders) return;
   append8_steps(a, s_steps);
   for (; leaders; leaders &= leaders - 1) {
-    const int l = __ffs(leaders) - 1, i0 = begin + l;
-    const int slot0 = __shfl_sync(0xffffffffu, slot, l), blk = c.block_div.div(slot0);
-    const bool same = __shfl_sync(0xffffffffu, (int)joined, l);
-    int next = i0 + 1 + lane < a.count ? a.slots[i0 + 1 + lane] : -1;
-    auto in_block = [&](int s) { return s >= blk * c.block && s - blk * c.block < c.block; };
-    // the run's end: its slots ascend, so it holds at most a block of entries that are kept
-    int n = 1;
-    for (int j0 = i0 + 1, last = slot0; j0 < a.count && last - blk * c.block != c.block - 1;) {
-      const int j = j0 + lane, s = next;
-      const unsigned kept = __ballot_sync(0xffffffffu, s >= 0), below = kept & ((1u << lane) - 1u);
-      const int prev = __shfl_sync(0xffffffffu, s, below ? 31 - __clz(below) : 0);
-      const bool fits = s < 0 || (in_block(s) && s > (below ? prev : last));
-      const unsigned stop = __ballot_sync(0xffffffffu, j >= a.count || !fits);
-      const unsigned in = kept & (stop ? (stop & -stop) - 1u : ~0u);
-      const int top = in ? 31 - __clz(in) : 0, newest = __shfl_sync(0xffffffffu, s, top);
-      if (in) {
-        n = j0 + top + 1 - i0;
-        last = newest;
+    const int l = __ffs(leaders) - 1;
+    int i = begin + l, slot0 = __shfl_sync(0xffffffffu, slot, l);
+    do {
+      const int blk = c.block_div.div(slot0);
+      auto in_block = [&](int s) { return s >= blk * c.block && s - blk * c.block < c.block; };
+      // the run's end: its slots ascend, so it holds at most a block of entries that are kept
+      int n = 1, last = slot0, odd = -1;  // odd: where an entry of the block comes next that does not ascend
+      int next = i + 1 + lane < a.count ? a.slots[i + 1 + lane] : -1;
+      for (int j0 = i + 1; j0 < a.count && last - blk * c.block != c.block - 1;) {
+        const int s = next;
+        const unsigned kept = __ballot_sync(0xffffffffu, s >= 0), below = kept & ((1u << lane) - 1u);
+        const int prev = __shfl_sync(0xffffffffu, s, below ? 31 - __clz(below) : 0);
+        const unsigned stop = __ballot_sync(0xffffffffu, s >= 0 && !(in_block(s) && s > (below ? prev : last)));
+        const unsigned in = kept & (stop ? (stop & -stop) - 1u : ~0u);
+        const int top = in ? 31 - __clz(in) : 0, newest = __shfl_sync(0xffffffffu, s, top);
+        if (in) {
+          n = j0 + top + 1 - i;
+          last = newest;
+        }
+        if (stop) {
+          if (in_block(__shfl_sync(0xffffffffu, s, __ffs(stop) - 1))) odd = j0 + __ffs(stop) - 1;
+          break;
+        }
+        j0 += 32;
+        next = j0 + lane < a.count ? a.slots[j0 + lane] : -1;
       }
-      if (stop) break;
-      j0 += 32;
-      next = j0 + lane < a.count ? a.slots[j0 + lane] : -1;
-    }
-    append8_run<D, T>(a, i0, n, slot0, same, s_steps, s_units);
-    __syncthreads();  // shared memory is free for the next run
+      if (!append8_run<D, T>(a, i, n, slot0, s_steps, s_units, odd, last, s_odd)) break;
+      __syncthreads();  // shared memory is free for the next run, and what this one wrote is there
+      i = s_odd[0];
+      if (i >= 0) {
+        i = append8_above(a, i, s_odd[1]);
+        if (i >= 0) slot0 = a.slots[i];
+      }
+    } while (i >= 0);
   }
 }
 

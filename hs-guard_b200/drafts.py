@@ -145,8 +145,8 @@ def append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source=None, po
     Entries of one block must stand together (but for skipped ones), in ascending slots (as ``advance_tables`` lists them). A block's scale becomes the
     power of two that its largest appended element asks for (a pair that turns counts with the sum of its magnitudes, so that
     rounding decides nothing); unless its first token is among the entries it does not fall, and when it rises the tokens that
-    were there are rounded again. Elements that are not finite become NaN. Slots that do not ascend within a block or lie beyond
-    the pages, and sources outside the rows, are skipped and recorded in ``err``."""
+    were there are rounded again. Elements that are not finite become NaN. Slots that do not stand above all of their block's
+    before them or lie beyond the pages, and sources outside the rows, are skipped and recorded in ``err``."""
     return tensors().append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, slots, source, positions, inv_freq, interleaved,
                                  rope_scale, q, err)
 

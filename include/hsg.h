@@ -376,8 +376,8 @@ typedef struct hsg_cache8 {
  * skipped ones) with ascending slots; the block's scales become 2^e, e the smallest integer (in [-100, 120]) with b <= 448 * 2^e, b the largest of: |x| of V's
  * elements and of K's that do not turn, (|x| + |y|) |rope_scale| of K's pairs that do, computed in fp32 without those that are not finite; but if the
  * block's first token is not among the entries, at least the scale that it had, and if that rises, tokens before the first
- * entry are rounded again. Codes are x / scale to nearest even, NaN for what is not finite. A slot that does not ascend beyond
- * the entry before it within a block, or beyond the pages, or a source outside the rows, is skipped and sets err. An entry of
+ * entry are rounded again. Codes are x / scale to nearest even, NaN for what is not finite. A slot that does not stand
+ * above all of its block's entries before it, or beyond the pages, or a source outside the rows, is skipped and sets err. An entry of
  * a block that other entries, apart from these, have been listed for gives that block's tokens and scales some value. */
 typedef struct hsg_append8_args {
   int64_t size;

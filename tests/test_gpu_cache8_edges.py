@@ -1,0 +1,37 @@
+"""The 8-bit cache on a B200 where it can go wrong: slot lists that do not ascend or are mostly padding, sums beyond fp32, pages
+outside the cache, positions that repeat, V of zeros over long caches, outliers in queries, chunks beside single tokens.
+
+Tolerances are those of test_gpu_cache8.py unless a test says otherwise; all were derived before the first run."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_cache8 import (BF16, D, F16, F8, U, append_reference, append_state, attend, attention_reference, attention_state,  # noqa: F401
+                             check_append, check_attention, dev, err_word, pool, turned)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- append_8bit: lists that are wrong, lists of padding --------------------------------------------------------------
+@pytest.mark.parametrize("slots,good", [
+    ([5, 4, 6, 7], [0, 2, 3]), ([5, 5, 6], [0, 2]), ([5, 4, 5, 6], [0, 3]), ([0, 3, 2, 4, 1, 9, 15, 15, 3, 16, 17], [0, 1, 3, 5, 6, 9, 10]),
+    ([20, 16, 17, 21, 32, 33, 32, 40], [0, 3, 4, 5, 7]), ([9, 3, -1, 10, -1, -1, 8, -1, 12, 13], [0, 3, 8, 9]),
+    ([0, 1] + [0] * 70 + [2, 3], [0, 1, 72, 73]), ([0, -1] + [-1] * 300 + [0] + [-1] * 3000 + [7, 8, 7, 9], [0, 3303, 3304, 3306])])
+def test_append_skips_only_the_slots_that_do_not_ascend(D, slots, good):
+    """Of a block's entries those that stand above all before them are written, whatever is between them."""
+    page, hkv, dim, n = 16, 2, 64, len(slots)
+    g = torch.Generator().manual_seed(n)
+    k = torch.randn(n, hkv, dim, generator=g)
+    k[0] *= 16  # the first entries' scale holds for all: no code is rounded twice
+    k[[i for i in good if slots[i] % 16 == 0]] *= 16
+    k = k.half().cuda()
+    s = append_state(4, page, 16, hkv, dim, False, 30)
+    if slots[0] % 16:
+        s["ks"][0], s["vs"][0], s["ks"][1], s["vs"][1] = 1.0, 1.0, 1.0, 1.0
+    kept = [x if i in good else -1 for i, x in enumerate(slots)]
+    ref = append_reference(s, k, k, kept, None, torch.zeros(n), torch.zeros(0), False, 1.0)
+    err = err_word()
+    D.append_8bit(k, k, s["kc"], s["vc"], s["ks"], s["vs"], dev(slots), err=err)
+    assert int(err.item()) == 3
+    check_append(s, ref, False)
