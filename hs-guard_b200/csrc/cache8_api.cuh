@@ -177,6 +177,7 @@ extern "C" int hsg_append8(const hsg_append8_args* a) {
   DRAFT_ARGS(a);
   if (a->count < 0 || a->rows < 0 || a->hkv < 1 || a->hq < 0)
     return fail(HSG_ERR_INVALID, "bad shape (count %d, rows %d, heads %d / %d)", a->count, a->rows, a->hq, a->hkv);
+  if (a->count > INT32_MAX - 2 * A8R_WALK * A8R_THREADS) return fail(HSG_ERR_INVALID, "too many entries (%d)", a->count);
   if (!head_dim_ok(a->dim)) return fail(HSG_ERR_INVALID, "head_dim must be 64, 128 or 256, got %d", a->dim);
   if (a->rot < 0 || a->rot > a->dim || a->rot % 16)
     return fail(HSG_ERR_INVALID, "the rotated dims must be a multiple of 16 up to head_dim, got %d", a->rot);

@@ -372,10 +372,39 @@ __device__ __forceinline__ bool append8_run(const Append8Args& a, int i0, int n,
   return true;
 }
 
-// From entry j on, the next of last's block whose slot is above `last`, before any of another block; -1: none.
-__device__ __noinline__ int append8_above(const Append8Args& a, int j, int last) {
+// The first entry that is kept from j on (Dir 1; count: none) or from j back (Dir -1; below 0: none). Lists are padded to what a
+// captured call has room for. With walks of 32 entries a step, a load's latency each, and made by blocks of padding too, ten tokens in a
+// list of 2^17 entries took 3,800 us; 53 with these, 11 unpadded. Called by the whole block.
+constexpr int A8R_WALK = 16;  // entries of a thread under way
+template <int Dir>
+__device__ __noinline__ int append8_kept(const Append8Args& a, int j, int* s_warps) {
+  const int none = Dir > 0 ? a.count : -1;
+  while (Dir > 0 ? j < a.count : j >= 0) {
+    int slots[A8R_WALK], found = Dir > 0 ? INT_MAX : INT_MIN;
+#pragma unroll
+    for (int u = 0; u < A8R_WALK; ++u) {
+      const int at = j + Dir * (u * A8R_THREADS + (int)threadIdx.x);
+      slots[u] = (Dir > 0 ? at < a.count : at >= 0) ? a.slots[at] : -1;
+    }
+#pragma unroll
+    for (int u = A8R_WALK - 1; u >= 0; --u)
+      if (slots[u] >= 0) found = j + Dir * (u * A8R_THREADS + (int)threadIdx.x);
+    found = Dir > 0 ? __reduce_min_sync(0xffffffffu, found) : __reduce_max_sync(0xffffffffu, found);
+    __syncthreads();  // the last ones have been read
+    if ((threadIdx.x & 31) == 0) s_warps[threadIdx.x >> 5] = found;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < A8R_THREADS / 32; ++w) found = Dir > 0 ? min(found, s_warps[w]) : max(found, s_warps[w]);
+    if (found != (Dir > 0 ? INT_MAX : INT_MIN)) return found;
+    j += Dir * A8R_WALK * A8R_THREADS;
+  }
+  return none;
+}
+
+// From entry j on, the next of last's block whose slot is above `last`, before any of another block; -1: none. Called by the whole block.
+__device__ __noinline__ int append8_above(const Append8Args& a, int j, int last, int* s_warps) {
   const int lane = threadIdx.x & 31, blk = a.cache.block_div.div(last);
-  for (; j < a.count; j += 32) {
+  for (; j < a.count; j = append8_kept<1>(a, j + 32, s_warps)) {
     const int s = j + lane < a.count ? a.slots[j + lane] : -1;
     const bool other = s < blk * a.cache.block || s - blk * a.cache.block >= a.cache.block;
     const unsigned hit = __ballot_sync(0xffffffffu, s >= 0 && (other || s > last));
@@ -389,7 +418,7 @@ __device__ __noinline__ int append8_above(const Append8Args& a, int j, int last)
 template <int D, typename T>
 __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_constant__ Append8Args a, int kv_blocks, int per, int split) {
   __shared__ uint64_t s_steps[128];      // [rot / 2]
-  __shared__ int s_odd[2];
+  __shared__ int s_odd[2], s_warps[A8R_THREADS / 32];
   extern __shared__ uint32_t s_units[];  // [2 hkv] bounds, then inverse scales; [2 hkv] whether infinities are among the rows
   pdl_wait();
   pdl_trigger();
@@ -405,18 +434,20 @@ __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_co
   const int lane = threadIdx.x & 31, begin = kv * per;
   // lane l has entry begin + l, and of the entries before them the l-th
   const int slot = lane < per && begin + lane < a.count ? a.slots[begin + lane] : -1;
-  int ahead = begin - 1 - lane >= 0 ? a.slots[begin - 1 - lane] : -1;
+  const int ahead = begin - 1 - lane >= 0 ? a.slots[begin - 1 - lane] : -1;
+  const unsigned own = __ballot_sync(0xffffffffu, slot >= 0);
+  if (!own) return;  // padding, say: what is before it does not matter
   // the kept entry before each
   int before = -1;
-  for (int j = begin - 1 - lane;;) {
-    const unsigned kept = __ballot_sync(0xffffffffu, ahead >= 0);
-    if (kept) before = __shfl_sync(0xffffffffu, ahead, __ffs(kept) - 1);
-    if (kept || j + lane - 31 <= 0) break;
-    j -= 32;
-    ahead = j >= 0 ? a.slots[j] : -1;
-  }
   {
-    const unsigned below = __ballot_sync(0xffffffffu, slot >= 0) & ((1u << lane) - 1u);
+    const unsigned kept = __ballot_sync(0xffffffffu, ahead >= 0);
+    if (kept) {
+      before = __shfl_sync(0xffffffffu, ahead, __ffs(kept) - 1);
+    } else if (begin > 32) {
+      const int at = append8_kept<-1>(a, begin - 33, s_warps);
+      if (at >= 0) before = a.slots[at];
+    }
+    const unsigned below = own & ((1u << lane) - 1u);
     const int prev = __shfl_sync(0xffffffffu, slot, below ? 31 - __clz(below) : 0);
     if (below) before = prev;
   }
@@ -450,14 +481,14 @@ __global__ void __launch_bounds__(A8R_THREADS, 3) append8_kernel(const __grid_co
           if (in_block(__shfl_sync(0xffffffffu, s, __ffs(stop) - 1))) odd = j0 + __ffs(stop) - 1;
           break;
         }
-        j0 += 32;
+        j0 = kept ? j0 + 32 : append8_kept<1>(a, j0 + 32, s_warps);
         next = j0 + lane < a.count ? a.slots[j0 + lane] : -1;
       }
       if (!append8_run<D, T>(a, i, n, slot0, s_steps, s_units, odd, last, s_odd)) break;
       __syncthreads();  // shared memory is free for the next run, and what this one wrote is there
       i = s_odd[0];
       if (i >= 0) {
-        i = append8_above(a, i, s_odd[1]);
+        i = append8_above(a, i, s_odd[1], s_warps);
         if (i >= 0) slot0 = a.slots[i];
       }
     } while (i >= 0);

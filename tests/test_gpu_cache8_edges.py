@@ -35,3 +35,44 @@ def test_append_skips_only_the_slots_that_do_not_ascend(D, slots, good):
     D.append_8bit(k, k, s["kc"], s["vc"], s["ks"], s["vs"], dev(slots), err=err)
     assert int(err.item()) == 3
     check_append(s, ref, False)
+
+
+@pytest.mark.parametrize("gap", [31, 1000, 4095, 4096, 5000, 20000])
+def test_append_over_long_padding(D, gap):
+    """Entries far apart in a padded list: runs that go on behind the padding, and ones that begin there."""
+    page, hkv, dim = 64, 2, 64
+    slots = [-1] * gap + [64, 65] + [-1] * gap + [66, 67, 96] + [-1] * gap + [130] + [-1] * gap + [131, 192] + [-1] * gap
+    n = len(slots)
+    k = torch.randn(n, hkv, dim, generator=torch.Generator().manual_seed(gap)).bfloat16().cuda()
+    s = append_state(5, page, 32, hkv, dim, False, 31)
+    at = [i for i, x in enumerate(slots) if x >= 0]
+    ref = append_reference(s, k[at], k[at], [slots[i] for i in at], None, torch.zeros(len(at)), torch.zeros(0), False, 1.0)
+    err = err_word()
+    D.append_8bit(k, k, s["kc"], s["vc"], s["ks"], s["vs"], dev(slots), err=err)
+    assert int(err.item()) == 0
+    check_append(s, ref, False)
+
+
+def test_append_time_goes_by_tokens_not_by_padding(D):
+    """Ten tokens in a list of 2^17 entries, as a captured call with room for many has them: tens of us more than in one of 16. Where
+    every block of padding looked for the entry before it, they took 3,650."""
+    page, hkv, dim, n = 64, 2, 64, 1 << 17
+    s = append_state(2, page, 64, hkv, dim, False, 32)
+    k = torch.randn(n, hkv, dim, device="cuda").half()
+
+    def us(slots):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            D.append_8bit(k, k, s["kc"], s["vc"], s["ks"], s["vs"], slots)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        return sorted(times)[4]
+
+    few = dev(list(range(10)) + [-1] * 6)
+    for where in (0, n // 2, n - 10):
+        many = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+        many[where:where + 10] = torch.arange(10, device="cuda")
+        assert us(many) < us(few) + 200, where
