@@ -148,8 +148,8 @@ struct A8Turn {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(-y[e], cs[e].y, x[e] * cs[e].x);
   }
-  // what the eight elements ask of the scale but for |rope_scale|: pairs that turn count with the sum of their magnitudes. Without
-  // NaN; infinite if one is, unless `finite` leaves those out
+  // what the eight elements ask of the scale but for |rope_scale|: pairs that turn count with the sum of their magnitudes, at most
+  // fp32's largest number. Without NaN; infinite if one is or such a sum is, unless `finite` leaves infinite elements out
   template <typename T, bool finite> __device__ __forceinline__ float bound(const uint4& raw, bool turns) const {
     float x[8], y[8], most = 0.f;
     unpack8<T>(raw, x);
@@ -157,8 +157,8 @@ struct A8Turn {
     const bool both = turns && in_rot;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float z = both ? fabsf(x[e]) + fabsf(y[pairs ? e ^ 1 : e]) : fabsf(x[e]);
-      most = fmaxf(most, finite && !(z < INFINITY) ? 0.f : z);
+      const float p = fabsf(x[e]), q = both ? fabsf(y[pairs ? e ^ 1 : e]) : 0.f, z = p + q;
+      most = fmaxf(most, !finite ? z : p < INFINITY && q < INFINITY ? fminf(z, 0x1.fffffep127f) : 0.f);
     }
     return most;
   }

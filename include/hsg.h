@@ -374,7 +374,8 @@ typedef struct hsg_cache8 {
  * (j, j + rot / 2), or (2 j, 2 j + 1) if interleaved. With hq > 0, q [count][hq][dim] is turned likewise into q_out
  * [count][hq][dim], contiguous, whatever its slot (source is NULL then). Entries of one block must stand together (but for
  * skipped ones) with ascending slots; the block's scales become 2^e, e the smallest integer (in [-100, 120]) with b <= 448 * 2^e, b the largest of: |x| of V's
- * elements and of K's that do not turn, (|x| + |y|) |rope_scale| of K's pairs that do, computed in fp32 without those that are not finite; but if the
+ * elements and of K's that do not turn, (|x| + |y|) |rope_scale| of K's pairs that do, computed in fp32 without elements and pairs that are not
+ * finite (a sum or product beyond fp32 counts as its largest number); but if the
  * block's first token is not among the entries, at least the scale that it had, and if that rises, tokens before the first
  * entry are rounded again. Codes are x / scale to nearest even, NaN for what is not finite. A slot that does not stand
  * above all of its block's entries before it, or beyond the pages, or a source outside the rows, is skipped and sets err. An entry of

@@ -76,3 +76,23 @@ def test_append_time_goes_by_tokens_not_by_padding(D):
         many = torch.full((n,), -1, dtype=torch.int32, device="cuda")
         many[where:where + 10] = torch.arange(10, device="cuda")
         assert us(many) < us(few) + 200, where
+
+
+def test_append_pairs_whose_sum_is_beyond_fp32(D):
+    """Two finite elements that turn together and whose magnitudes add up to more than fp32 has count as the largest number, not as
+    infinite ones, which count for nothing."""
+    page, dim = 16, 64
+    k = torch.zeros(4, 1, dim)
+    k[0, 0, 3], k[0, 0, 3 + 32] = 2e38, -3e38
+    k[1, 0, 3], k[1, 0, 3 + 32], k[1, 0, 5] = 2e38, math.inf, 1.0
+    k[2, 0, 4], k[2, 0, 4 + 32], k[2, 0, 5] = 3e38, 3e38, math.nan
+    k[3, 0, 7] = 1.0
+    k = k.bfloat16().cuda()
+    s = append_state(5, page, 16, 1, dim, False, 33)
+    p = torch.zeros(4, dtype=torch.int32, device="cuda")
+    D.append_8bit(k, k, s["kc"], s["vc"], s["ks"], s["vs"], dev([0, 16, 32, 48]), positions=p, inv_freq=torch.ones(32, device="cuda"))
+    assert s["ks"][:4, 0, 0].tolist() == [2.0 ** 120, 2.0 ** -8, 2.0 ** 120, 2.0 ** -8]
+    got, x = s["kc"][:4, 0, 0].double() * s["ks"][:4, 0].double(), k[:, 0].double()
+    for r, d in ((0, 3), (0, 35), (2, 4), (2, 36), (1, 5), (3, 7)):
+        assert abs(float(got[r, d] - x[r, d])) <= 2.0 ** -4 * abs(float(x[r, d]))
+    assert bool(torch.isnan(got[1, [3, 35]]).all()) and bool(torch.isnan(got[2, [5, 37]]).all())
