@@ -7,7 +7,7 @@
 //   token len_b - n_b + u       iff bit u of its mask is set (without a mask: u <= t), and likewise for position p_u
 // and its output is sum_j softmax_j(scale ks_j q.k_j) vs_j v_j over what it sees, its log-sum-exp that of the same scores.
 // A token that sees nothing has output 0 and log-sum-exp -inf. What is not seen is never part of a result, whatever its codes
-// and scales are.
+// and scales are. Tokens of a page that the cache does not have (which is recorded) are not seen.
 #pragma once
 #include "cache8_rows.cuh"
 #include "draft_attn.cuh"  // pack2, ex2_approx
@@ -65,6 +65,7 @@ constexpr int A8_ROWS = 16;         // of a block, at most
 constexpr int A8_BLOCKS = 148;      // one thread block an SM
 constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
 constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;
+constexpr int A8_LOST = -(1 << 30);  // below every key: each slice is looked at key by key
 
 __host__ __device__ constexpr int a8_slice(int dim) { return dim == 256 ? 16 : 32; }  // keys
 __host__ __device__ constexpr int a8_stage(int dim) { return 2 * a8_slice(dim) * dim; }
@@ -300,6 +301,8 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring_scales + WARPS * ST * 8);           // [warps][ST] a slice has landed
   A8Lot* lots = reinterpret_cast<A8Lot*>(bars + WARPS * ST);                            // [warps]
   int64_t* scan = reinterpret_cast<int64_t*>(lots + WARPS);
+  // [warps][ST] groups of a slice whose page the cache does not have: their place holds what was there before
+  uint32_t* lost = reinterpret_cast<uint32_t*>(scan + WARPS) + (threadIdx.x >> 5) * ST;
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int piece = warp * A8_BLOCKS + blockIdx.x, G = a.hq / a.hkv, quad = lane & 3, x8 = lane >> 2;
@@ -307,6 +310,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     mbar_init(bars + tid, 1);
     fence_barrier_init();
   }
+  if (lane < ST) lost[lane] = 0;
   if (tid == 0) {
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
@@ -328,6 +332,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
   int64_t put_unit = lot.begin;
   int put_i = put.at.i, put_i1 = part_end(put_unit, put.s.n);
   bool put_more = true, asked = false;
+  int sure = 0;  // keys below this, and above `low`, are seen by every row of the item; A8_LOST once a page was not there
   uint8_t* ring = rings + warp * ST * STAGE;
   float* scales = ring_scales + warp * ST * 8;
   uint64_t* full = bars + warp * ST;
@@ -358,7 +363,12 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
     if (put_more) {
       const Cache8& c = a.cache;
       const bool good = asked && page >= 0 && page < c.pages;
-      if (asked && !good) set_error(a.err, ERR_BAD_PAGE);
+      if (__any_sync(0xffffffffu, asked && !good) || sure == A8_LOST) {
+        const unsigned gone = __ballot_sync(0xffffffffu, asked && !good);
+        if (lane == 0) lost[put_slot] = gone;
+        if (asked && !good) set_error(a.err, ERR_BAD_PAGE);
+        sure = A8_LOST;
+      }
       // lane i brings the i-th box of K and of V if it has a group that is asked for (a box is of one page), and knows where from
       // by that group's lane
       const unsigned groups = __ballot_sync(0xffffffffu, good);
@@ -462,8 +472,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
         }
       }
     }
-    // keys below `sure` and above `low` are seen by every row
-    const int sure = a.mask ? old : old + row0 / G + 1;
+    if (sure != A8_LOST) sure = a.mask ? old : old + row0 / G + 1;
     if (a.window) low = __reduce_max_sync(0xffffffffu, low);
     float o[NT][NR][4], m[NR][2], l[NR][2];
 #pragma unroll
@@ -524,6 +533,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       const bool special = base > sure - KEYS || (a.window && base <= low);
       uint32_t seen = ~0u;  // bit 8 of a half, 4 of 8 rows, element
       if (special) {
+        const unsigned gone = lost[slot];
         seen = 0;
 #pragma unroll
         for (int kh = 0; kh < KEYS / 16; ++kh)
@@ -531,7 +541,8 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
           for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const bool see = a8_sees(a, r, tok[nr][e & 1], pos[nr][e & 1], base + 16 * kh + 8 * (e >> 1) + a8_key<D>(x8));
+              const int j = gone >> (2 * kh + (e >> 1)) & 1 ? INT_MAX : base + 16 * kh + 8 * (e >> 1) + a8_key<D>(x8);
+              const bool see = a8_sees(a, r, tok[nr][e & 1], pos[nr][e & 1], j);
               seen |= see ? 1u << (8 * kh + 4 * nr + e) : 0u;
               s[kh][nr][e] = see ? s[kh][nr][e] : -INFINITY;
             }

@@ -340,7 +340,7 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     struct Tile {
       W8Tile t;
       int h, page, within;
-      bool asked;
+      bool asked, lost;  // lost: the cache has no such page
       float ksc, vsc;
     };
     // warp 3: what an item is, and its rows' scales (lane l: rows l, l + 32 ...), as its first tile is taken
@@ -364,7 +364,7 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     };
     auto take = [&](bool begins) {  // the walk's tile, and the walk to the next one
       const int old = walk.r.len - walk.r.n, sure = a.mask ? old : old + walk.at.block * W8_ROWS / G + 1, base = walk.base(i);
-      Tile x{{base, walk.s.lo, walk.s.hi, walk.s.ahead, begins || i == 0 ? 1u : 0u, 0u, item}, walk.at.h, 0, 0, false, 0.f, 1.f};
+      Tile x{{base, walk.s.lo, walk.s.hi, walk.s.ahead, begins || i == 0 ? 1u : 0u, 0u, item}, walk.at.h, 0, 0, false, false, 0.f, 1.f};
       if (is_v && (x.t.what & 1u)) describe();
       if (base > sure - KT || a.window) x.t.what |= 8u;
       if (base < x.t.lo || base > x.t.hi - KT) x.t.what |= 16u;
@@ -391,11 +391,9 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     };
     auto resolve = [&](Tile& x) {  // its page has come: which groups can be brought, and their scales
       const bool good = x.asked && x.page >= 0 && x.page < c.pages;
-      if (x.asked && !good) {
-        set_error(a.err, ERR_BAD_PAGE);
-        x.t.what |= 16u;
-      }
-      x.t.what |= __any_sync(0xffffffffu, x.asked && !good) ? 16u : 0u;
+      x.lost = x.asked && !good;
+      if (x.lost) set_error(a.err, ERR_BAD_PAGE);
+      x.t.what |= __any_sync(0xffffffffu, x.lost) ? 16u : 0u;
       x.t.groups = __ballot_sync(0xffffffffu, good);
       if (good && !is_v) {
         const int64_t at = ((int64_t)x.page * c.blocks + c.block_div.div(x.within)) * a.hkv + x.h;
@@ -456,12 +454,21 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (is_v) tiles[ring.at] = cur.t;
         else k_info[ring.at] = cur.t.what;
       }
+      if (!is_v && __any_sync(0xffffffffu, cur.lost)) {
+        // keys of no page: codes of 0 in place of what was there before, and a scale of V that leaves their weights at 0
+        if (cur.lost)
+#pragma unroll 1
+          for (int e = 0; e < 8 * D / 16; ++e)
+            *reinterpret_cast<uint4*>(bufs + ring.at * CODES + (e / (ROW / 2)) * (KT * 128) + lane * (8 * ROW) + e % (ROW / 2) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async();
+        __syncwarp();
+      }
       bring(bufs + ring.at * CODES, cur, &full[ring.at]);
       ++issued;
       if (!is_v) {
         // scales of 0 or beyond what append_8bit writes are taken as the nearest that it would write
         const float v = fminf(fmaxf(cur.vsc, 0x1p-100f), 0x1p120f);
-        if (lane < GROUPS) group_scales[(g % W8_PLACES) * 16 + lane] = make_float4(cur.ksc, __log2f(v), rcp_approx(v), 0.f);
+        if (lane < GROUPS) group_scales[(g % W8_PLACES) * 16 + lane] = make_float4(cur.ksc, cur.lost ? -INFINITY : __log2f(v), rcp_approx(v), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_full[g % W8_PLACES]);
       }

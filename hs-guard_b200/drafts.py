@@ -168,7 +168,7 @@ def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale
     minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (None: their places in the cache) are
     read only then. Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets
     0 and -inf, as do tokens outside cu[0] .. cu[rows] - 1 and those of a request whose lengths are out of range (which ``err``
-    records). ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim, tokens, hq)`` bytes, for one call at a time) is allocated when it
+    records). Tokens of a page outside the cache (recorded as well) are not seen. ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim, tokens, hq)`` bytes, for one call at a time) is allocated when it
     is not given."""
     return tensors().attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask, positions, window,
                                     sinks, workspace, err)

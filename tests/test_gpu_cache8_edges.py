@@ -96,3 +96,43 @@ def test_append_pairs_whose_sum_is_beyond_fp32(D):
     for r, d in ((0, 3), (0, 35), (2, 4), (2, 36), (1, 5), (3, 7)):
         assert abs(float(got[r, d] - x[r, d])) <= 2.0 ** -4 * abs(float(x[r, d]))
     assert bool(torch.isnan(got[1, [3, 35]]).all()) and bool(torch.isnan(got[2, [5, 37]]).all())
+
+
+# ---- attention_8bit ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,hq,hkv,page,block,heads_first", [(64, 4, 2, 16, 16, False), (64, 4, 2, 8, 8, True), (128, 8, 2, 32, 8, False),
+                                                               (128, 8, 2, 128, 32, True), (256, 8, 2, 16, 8, False), (256, 8, 2, 64, 64, True)])
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("bad", [-1, 1 << 20])
+def test_attention_skips_pages_outside_the_cache(D, dim, hq, hkv, page, block, heads_first, n, bad, dtype):
+    """Tokens of a page that the cache does not have are not seen, as if the request were without them: shared memory that holds
+    NaN from another call does not show."""
+    lens = [20 * page + 3, 9 * page, 11 * page + page // 2]
+    lens = [x + n for x in lens]
+    s = attention_state(dim, hq, hkv, page, block, lens, [n] * 3, dtype, heads_first, seed=40 + n)
+    nan = dict(s, kc=pool(s["kc"].shape[0], page, hkv, dim, heads_first, fill=0x7f), vc=pool(s["kc"].shape[0], page, hkv, dim, heads_first, fill=0x7f))
+    wrong, without = dict(s, table=s["table"].clone()), dict(s, table=s["table"].clone(), lens=s["lens"].clone())
+    for b, pages in ((0, (3, 4, 11)), (2, (0,))):
+        for p in pages:
+            wrong["table"][b, p] = bad
+        rest = [x for i, x in enumerate(s["table"][b].tolist()) if i not in pages]
+        without["table"][b] = dev(rest + [-7] * len(pages))
+        without["lens"][b] -= len(pages) * page
+    ref = attention_reference(without, dim ** -0.5)
+    for _ in range(3):
+        attend(D, nan, dim ** -0.5, n)
+        err = err_word()
+        got = attend(D, wrong, dim ** -0.5, n, err=err)
+        assert int(err.item()) == 6
+        check_attention(got, ref, dtype)
+
+
+def test_attention_of_a_request_without_a_page(D):
+    """Every page outside the cache: nothing is seen."""
+    for n in (1, 40):
+        s = attention_state(128, 8, 2, 16, 16, [50, 60], [n, n], F16, seed=45)
+        good = attention_reference(s, 0.1)
+        s["table"][0] = -1
+        out, lse = attend(D, s, 0.1, n)
+        assert bool((out[:n] == 0).all()) and bool(torch.isneginf(lse[:n]).all())
+        check_attention((out[n:], lse[n:]), [x[n:] for x in good], F16)
