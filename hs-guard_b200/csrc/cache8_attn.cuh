@@ -126,6 +126,12 @@ __device__ __forceinline__ A8Span a8_span(const Attn8Args& a, const A8Req& r, in
   return s;
 }
 
+// Of a block that begins with new token t: tokens below this are seen by all its rows, but for a window. A window that goes by given
+// positions may leave any of the new ones out, also ones whose places are behind its end.
+__device__ __forceinline__ int a8_sure(const Attn8Args& a, int old, int t) {
+  return a.mask || (a.window && a.positions) ? old : old + t + 1;
+}
+
 // A place on the line of tiles: item (request, key head, block of rows) and tile.
 struct A8At {
   int b, h, block, i;
@@ -472,7 +478,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
         }
       }
     }
-    if (sure != A8_LOST) sure = a.mask ? old : old + row0 / G + 1;
+    if (sure != A8_LOST) sure = a8_sure(a, old, row0 / G);
     if (a.window) low = __reduce_max_sync(0xffffffffu, low);
     float o[NT][NR][4], m[NR][2], l[NR][2];
 #pragma unroll

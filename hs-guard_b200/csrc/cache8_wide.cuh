@@ -355,7 +355,7 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           lows = max(lows, (a.positions ? a.positions[walk.r.t0 + t] : old + t) - a.window);
         lows = __reduce_max_sync(0xffffffffu, lows);
       }
-      next_item = W8Item{walk.r, walk.s, walk.at.b, walk.at.h, walk.at.block, i, i1, a.mask ? old : old + row0 / G + 1, lows,
+      next_item = W8Item{walk.r, walk.s, walk.at.b, walk.at.h, walk.at.block, i, i1, a8_sure(a, old, row0 / G), lows,
                          (int)a8_div(unit + W8_COST + walk.s.n - 1, step), unit + walk.s.n + 2 * W8_COST >= w1};
       const int64_t first = (int64_t)walk.at.h * a.tokens * G + (int64_t)walk.r.t0 * G + row0;
 #pragma unroll
@@ -363,7 +363,7 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         next_scale[e] = row0 + lane + 32 * e < walk.r.n * G ? q_scales[first + lane + 32 * e] : 1.f;
     };
     auto take = [&](bool begins) {  // the walk's tile, and the walk to the next one
-      const int old = walk.r.len - walk.r.n, sure = a.mask ? old : old + walk.at.block * W8_ROWS / G + 1, base = walk.base(i);
+      const int old = walk.r.len - walk.r.n, sure = a8_sure(a, old, walk.at.block * W8_ROWS / G), base = walk.base(i);
       Tile x{{base, walk.s.lo, walk.s.hi, walk.s.ahead, begins || i == 0 ? 1u : 0u, 0u, item}, walk.at.h, 0, 0, false, false, 0.f, 1.f};
       if (is_v && (x.t.what & 1u)) describe();
       if (base > sure - KT || a.window) x.t.what |= 8u;

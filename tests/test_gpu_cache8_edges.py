@@ -136,3 +136,17 @@ def test_attention_of_a_request_without_a_page(D):
         out, lse = attend(D, s, 0.1, n)
         assert bool((out[:n] == 0).all()) and bool(torch.isneginf(lse[:n]).all())
         check_attention((out[n:], lse[n:]), [x[n:] for x in good], F16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,hq,hkv", [(64, 4, 4), (128, 4, 2), (256, 2, 1)])
+@pytest.mark.parametrize("lens,counts", [([420, 33, 1, 60, 60, 60, 60, 60, 60, 60], [150, 1, 1, 1, 1, 1, 1, 1, 1, 1]), ([700, 500], [600, 300])])
+@pytest.mark.parametrize("step,window,sinks", [(0.125, 10, 0), (0.125, 10, 300), (0.02, 5, 2), (3, 40, 0)])
+def test_attention_positions_without_a_mask(D, lens, counts, dim, hq, hkv, step, window, sinks, dtype):
+    """A chain whose positions repeat (parts of a picture, say) or leave some out: the window goes by them, not by the places."""
+    s = attention_state(dim, hq, hkv, 16, 16, lens, counts, dtype, seed=46)
+    s["positions"] = dev([n - c + int(t * step) for n, c in zip(lens, counts) for t in range(c)])
+    err = err_word()
+    got = attend(D, s, dim ** -0.5, max(counts), window=window, sinks=sinks, err=err)
+    assert int(err.item()) == 0
+    check_attention(got, attention_reference(s, dim ** -0.5, window, sinks), dtype)
