@@ -250,6 +250,10 @@ template <int D> __device__ __forceinline__ uint32_t a8_at(int k, int ch) {
   else return (ch >> 3) * (a8_slice(D) * 128) + (k >> 3) * 1024 + sw128_off(k & 7, ch & 7);
 }
 
+// V scales are taken within [2^-80, 2^120]. The row sums of weights over them, up to 2^15 each, so stay below 2^128 over 2^31 keys (with
+// 2^-100, which blocks of zeros have, the sum over 150,000 keys did not); what codes of smaller scales stand for is below 4e-22 either way.
+__device__ __forceinline__ float a8_v_scale(float scale) { return fminf(fmaxf(scale, 0x1p-80f), 0x1p120f); }
+
 // Four codes as fp16: the lower two and the upper two.
 __device__ __forceinline__ void f8_halves(uint32_t four, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
@@ -528,8 +532,7 @@ attn8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ C
       float vs[GROUPS];
 #pragma unroll
       for (int n = 0; n < GROUPS; ++n) {
-        // a V scale of 0 or beyond what append_8bit writes is taken as the nearest that it would write
-        vs[n] = fminf(fmaxf(scales[slot * 8 + 4 + n], 0x1p-100f), 0x1p120f);
+        vs[n] = a8_v_scale(scales[slot * 8 + 4 + n]);
         const float ks = scales[slot * 8 + n], lv = __log2f(vs[n]);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)

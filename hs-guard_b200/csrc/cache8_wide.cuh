@@ -466,8 +466,7 @@ attn8_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       bring(bufs + ring.at * CODES, cur, &full[ring.at]);
       ++issued;
       if (!is_v) {
-        // scales of 0 or beyond what append_8bit writes are taken as the nearest that it would write
-        const float v = fminf(fmaxf(cur.vsc, 0x1p-100f), 0x1p120f);
+        const float v = a8_v_scale(cur.vsc);
         if (lane < GROUPS) group_scales[(g % W8_PLACES) * 16 + lane] = make_float4(cur.ksc, cur.lost ? -INFINITY : __log2f(v), rcp_approx(v), 0.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_full[g % W8_PLACES]);

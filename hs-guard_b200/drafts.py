@@ -161,8 +161,8 @@ def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale
     """Attention of each request's newest tokens over its pages of an 8-bit cache.
 
     q [tokens, hq, dim] (fp16 or bf16, hq a multiple of hkv, at most 128 query heads a key head, dim 64, 128 or 256; any strides
-    that keep rows on 16-byte boundaries); cache and scales as in ``append_8bit`` (any positive scales); table [rows, width], lens
-    [rows], cu [rows + 1] int32. Request b has lens[b] tokens in its pages, the last cu[b + 1] - cu[b] (at most max_new) being
+    that keep rows on 16-byte boundaries); cache and scales as in ``append_8bit`` (any positive scales; of v_scale what is below
+    2^-80 or above 2^120 is taken as those); table [rows, width], lens [rows], cu [rows + 1] int32. Request b has lens[b] tokens in its pages, the last cu[b + 1] - cu[b] (at most max_new) being
     those of q. They see all tokens before them, and among themselves the earlier ones and their own, or the ones whose bits
     mask [tokens, words] int32 has set (as ``plan_tree`` makes it). With window > 0 only tokens at positions above the query's own
     minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (None: their places in the cache) are

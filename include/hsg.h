@@ -406,7 +406,8 @@ int hsg_append8(const hsg_append8_args* args);
  * window and must be at least lens[b] - n. out [tokens][hq][dim] = softmax(scale q.k) v in dtype (q's: HSG_DT_F16 or _BF16), lse
  * [tokens][hq] = the log-sum-exp (may be NULL). A token that sees nothing, or only scores of -inf, gets 0 and -inf, and so do
  * tokens of no request and those of a request whose lengths are out of range; what is not seen does not enter a result whatever
- * its codes, nor do scales of blocks of which nothing is seen. cu must not descend; no request has more than max_new query tokens. Table entries of pages that no query
+ * its codes, nor do scales of blocks of which nothing is seen. V scales
+ * below 2^-80 or above 2^120 are taken as those. cu must not descend; no request has more than max_new query tokens. Table entries of pages that no query
  * token sees are not read; tokens of an entry outside the pages are not seen, and err is set. `workspace`: hsg_attention8_workspace(dim, tokens, hq) bytes on a 16-byte boundary, not shared by calls that
  * overlap in time. */
 typedef struct hsg_attention8_args {

@@ -150,3 +150,25 @@ def test_attention_positions_without_a_mask(D, lens, counts, dim, hq, hkv, step,
     got = attend(D, s, dim ** -0.5, max(counts), window=window, sinks=sinks, err=err)
     assert int(err.item()) == 0
     check_attention(got, attention_reference(s, dim ** -0.5, window, sinks), dtype)
+
+
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("values", ["zeros", "some"])
+def test_attention_over_many_values_of_zero(D, n, values):
+    """Blocks of zeros have the smallest scale there is: the sum of the weights over it stays a number, over 150,000 keys too."""
+    page, dim, keys = 128, 64, 150000
+    pages = -(-keys // page)
+    k, v = (torch.zeros(pages, page, 1, dim, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2))
+    ks, vs = torch.ones(pages, 1, 1, device="cuda"), torch.full((pages, 1, 1), 2.0 ** -100, device="cuda")
+    share = 0.0
+    if values == "some":  # a page of ones
+        v.view(torch.uint8)[7] = 0x38
+        vs[7] = 1.0
+        share = page / keys
+    q = torch.zeros(n, 1, dim, device="cuda").half()
+    table = torch.arange(pages, device="cuda").int()[None]
+    mask = torch.full((n, 1), -1, dtype=torch.int32, device="cuda")  # all of them see all
+    out, lse = D.attention_8bit(q, k, v, ks, vs, table, dev([keys]), dev([0, n]), 0.125, n, mask=mask)
+    more = (keys / 8 + 32) * 2.0 ** -23
+    assert float((lse.double() - math.log(keys)).abs().max()) <= more + 4e-6 * (1 + math.log(keys))
+    assert float((out.double() - share).abs().max()) <= (U[F16] + 2.0 ** -11 + more) * share + 2.0 ** -25
