@@ -5,11 +5,13 @@
 // can see are an item; all items are one line, cut into equal pieces, one a thread block. Per tile S = Q K^T (TMEM), softmax with
 // a running maximum in registers (a row a thread), P in fp16 over S in TMEM, O += P V (A = P from TMEM, B = V, N-major).
 //
-// S takes K's codes as they are (kind::f8f6f4): a query is scaled by a power of two for each row and written as a sum of e4m3
-// numbers, each the rounding of what the ones before left: two for bf16 (8 bits), three for fp16 (12). Elements below 2^-14 of the
-// row's largest lose bits to e4m3's smallest step, 2^-18.8 of that largest, far below what rounding that one to 16 bits has cost. P V
-// is a product of fp16 (weights rounded once; e4m3 weights would have to be two or three numbers each): V's codes become fp16 on
-// the way, which is exact. K converted as well (1,316 us for 2,000-token chunks) kept four warps longer than the softmax takes. Keys
+// S takes K's codes as they are (kind::f8f6f4): a query is scaled by a power of two for each row, which brings its largest element to
+// (224, 448], and written as a sum of e4m3 numbers, each the rounding of what the ones before left: two for bf16 (8 bits), three for
+// fp16 (11). e4m3's last step there is 2^-9: a bf16 element is exact from 2^-2 on (2^-10.8 to 2^-9.8 of the row's largest), an fp16
+// element from 2 on (2^-7.8 to 2^-6.8 of it), and smaller ones are off by at most 2^-10, which is up to 2^-17.8 of the largest: a score
+// by that times scale sum |k| beside a query with an outlier. P V is a product of fp16 (weights rounded once; e4m3 weights would have to
+// be two or three numbers each): V's codes become fp16 on the way, which is exact. K converted as well (1,316 us for 2,000-token chunks)
+// kept four warps longer than the softmax takes. Keys
 // that the item cannot see have V written as zeros. A NaN of V in a tile that not every row sees alike is written as zero as well,
 // and put back for the rows that see it at the end. Scales, and log2 and reciprocal of V's, of each 8 keys go to the softmax through
 // a ring of their own: a weight is 2^(s ks + log2 vs - m), m the running maximum of that exponent, and adds itself over vs to the

@@ -172,3 +172,26 @@ def test_attention_over_many_values_of_zero(D, n, values):
     more = (keys / 8 + 32) * 2.0 ** -23
     assert float((lse.double() - math.log(keys)).abs().max()) <= more + 4e-6 * (1 + math.log(keys))
     assert float((out.double() - share).abs().max()) <= (U[F16] + 2.0 ** -11 + more) * share + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("largest", [230.0, 447.0])
+def test_attention_queries_with_an_outlier(D, dim, dtype, largest):
+    """One element of a query hundreds of times the others, over keys that are small there, so that the others decide.
+
+    For many rows a query is a sum of e4m3 numbers, its largest element brought to (224, 448], e4m3's last step there 2^-9: an
+    element is off by at most 2^-10 / 224 of the largest. Scores by that times scale sum |k| more than otherwise, twice in a weight."""
+    n = 40
+    s = attention_state(dim, 4, 2, 16, 16, [500, 300], [n, n], dtype, seed=47)
+    q = torch.empty(2 * n, 4, dim, device="cuda").uniform_(-1.5, 1.5, generator=torch.Generator(device="cuda").manual_seed(1))
+    q[..., 5] = largest
+    s["q"] = q.to(dtype)
+    s["kc"].view(torch.uint8)[:, :, :, 5] = torch.where(torch.isnan(s["kc"][:, :, :, 5].float()), 0x7f, 0).to(torch.uint8)
+    scale = 0.02
+    out, lse, tol, ltol = attention_reference(s, scale)
+    keys = torch.where(torch.isnan(s["ks"]), 0.0, s["ks"])[..., None].repeat_interleave(16, 1)[..., 0]
+    sums = (torch.nan_to_num(s["kc"].float()).abs().sum(-1) * keys).max()
+    ds = scale * 2.0 ** -10 / 224 * largest * float(sums)
+    most = torch.nan_to_num(s["vc"].float()).abs().mul(torch.nan_to_num(s["vs"]).repeat_interleave(16, 1)[..., None]).max()
+    check_attention(attend(D, s, scale, n), (out, lse, tol + 2 * ds * float(most), ltol + ds), dtype)
