@@ -195,3 +195,14 @@ def test_attention_queries_with_an_outlier(D, dim, dtype, largest):
     ds = scale * 2.0 ** -10 / 224 * largest * float(sums)
     most = torch.nan_to_num(s["vc"].float()).abs().mul(torch.nan_to_num(s["vs"]).repeat_interleave(16, 1)[..., None]).max()
     check_attention(attend(D, s, scale, n), (out, lse, tol + 2 * ds * float(most), ltol + ds), dtype)
+
+
+@pytest.mark.parametrize("singles", [9, 300])
+def test_attention_of_a_chunk_beside_single_tokens(D, singles):
+    """A prompt's chunk first, in the middle and last among requests of one token, in one call."""
+    for at in (0, singles // 2, singles):
+        lens, counts = [31 + 7 * (i % 40) for i in range(singles)], [1] * singles
+        lens.insert(at, 900)
+        counts.insert(at, 700)
+        s = attention_state(128, 8, 2, 16, 16, lens, counts, BF16, seed=48)
+        check_attention(attend(D, s, 0.09, 700), attention_reference(s, 0.09), BF16)
