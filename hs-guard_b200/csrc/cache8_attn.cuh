@@ -46,12 +46,12 @@ struct Attn8Args {
 // that sum, so that weights use fp16's range however the scales differ, and the row sum takes w_j / vs_j. Weights are rounded to
 // fp16 (2^-11, the largest between 2^11 and 2^15, as in the 16-bit attention); sums, maxima and accumulators are fp32.
 //
-// Measured on B200: 352 requests of one or two tokens, 512-token window and 4 first tokens, 8 / 2 heads of 256: 186 MB in 56 us,
+// Measured on B200: 352 requests of one or two tokens, 512-token window and 4 first tokens, 8 / 2 heads of 256: 186 MB in 57 us,
 // 3.3 TB/s: 6 us until the first slice is there, HBM at 4 to 5 TB/s, then the last pieces (they end up to 14% after the mean) and 5
-// for the join. 5 requests of up to 50,001 tokens, 3 tokens, 32 / 8 heads of 128: 360 MB in 75 to 96 us (the clock), 64 requests of
-// up to 2,100 tokens, 16 / 16 heads of 64, pages of 8: 195 MB in 59 us. Instructions of few warps bound those (1.3 a clock and SM,
-// waits for results of the ones before): codes to fp16, and at pages of 8 the copies, of which each costs a warp about 30. One
-// token: 14 us of latencies.
+// for the join. 4 requests of up to 50,001 tokens, 3 tokens, 32 / 8 heads of 128: 228 MB in 87 to 94 us (with queries as the products'
+// 16 rows these 12 rows a key head took 74), 64 requests of up to 2,100 tokens, 16 / 16 heads of 64, pages of 8: 195 MB in 60 us.
+// Instructions of few warps bound those (1.3 a clock and SM, waits for results of the ones before): codes to fp16, and at pages of 8 the
+// copies, of which each costs a warp about 30. One token: 14 us of latencies.
 //
 // The order of dims and keys within a product is free as long as both factors agree: a lane reads 16 consecutive bytes of a key,
 // which are its elements of four steps of 16 dims, and for P V consecutive dims of two keys, interleaved bytewise. Which keys
@@ -61,7 +61,6 @@ struct Attn8Args {
 // 64 requests above take 59 us, with 8 warps 80. The others need up to 255 registers: with 12 warps of 168, up to 2 KB a thread would
 // go to local memory.
 __host__ __device__ constexpr int a8_warps(int dim, int nr) { return dim == 64 && nr == 1 ? 16 : 8; }
-constexpr int A8_ROWS = 16;         // of a block, at most
 constexpr int A8_BLOCKS = 148;      // one thread block an SM
 constexpr int A8_COST = 2;          // what an item costs besides its slices, in slices
 constexpr float A8_LIFT = 11.f, A8_SLACK = 4.f;

@@ -27,8 +27,8 @@
 //   12-15  V from the staging ring to fp16
 // Codes lie as [dim / 128][keys][128 B] (64 bytes a key at head dim 64), V as [8 keys][dim / 64][8][128 B], both swizzled.
 //
-// Measured on B200: 40 requests of up to 6,000 tokens, trees of 64, 32 / 4 heads of 128, bf16: 258 to 271 us (the products 82 at the
-// measured bf16 rate, the cache 27); chunks of 2,000 tokens over up to 8,000, 32 / 8 heads of 128: 698 to 719 (products 225). A tile
+// Measured on B200: 40 requests of up to 6,000 tokens, trees of 64, 32 / 4 heads of 128, bf16: 258 to 279 us (the products 82 at the
+// measured bf16 rate, the cache 27); chunks of 2,000 tokens over up to 8,000, 32 / 8 heads of 128: 635 to 698 (products 225). A tile
 // takes 2,650 clocks where one follows the other, of which the softmax of one group takes 4,000 for its every second one (maximum
 // 950, hand-over and rescaling 600, weights 2,450: three clocks an instruction), the products 1,024, the conversion of V 1,100.
 //

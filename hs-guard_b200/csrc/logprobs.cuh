@@ -10,8 +10,11 @@
 // (a bisection over its bits, threads counted by a block-wide vote) is no larger than the top-th value of the block's share,
 // so every alternative is at least tau and lies with a thread whose largest is: only what those few threads read is read
 // again, by all threads, and what reaches tau becomes a candidate (about as many as are asked for), ranked by counting.
-// Equal values rank by token, the lowest first. If too many values reach tau (long runs of equal or ascending values), the
-// alternatives are taken one by one instead: the block's largest, after which its owner's warp looks for that thread's next.
+// Equal values rank by token, the lowest first. If too many values reach tau, the alternatives
+// are taken one by one instead: the block's largest, after which its owner's warp looks for that thread's next. That happens in long
+// runs of equal or ascending values, and where fewer threads than alternatives meet anything but -inf (a grammar that leaves a
+// few tokens or a run of them): 30 allowed tokens and 20 alternatives take one row of 248,320 fp32 43 us, 352 rows of bf16 351, 2,500
+// rows of 50,001 fp16 415.
 //
 // A row is shared by a cluster of up to 8 blocks, whose parts meet in the first one's shared memory.
 //

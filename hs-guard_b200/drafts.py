@@ -165,11 +165,12 @@ def attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale
     2^-80 or above 2^120 is taken as those); table [rows, width], lens [rows], cu [rows + 1] int32. Request b has lens[b] tokens in its pages, the last cu[b + 1] - cu[b] (at most max_new) being
     those of q. They see all tokens before them, and among themselves the earlier ones and their own, or the ones whose bits
     mask [tokens, words] int32 has set (as ``plan_tree`` makes it). With window > 0 only tokens at positions above the query's own
-    minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (None: their places in the cache) are
-    read only then. Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets
+    minus window, or below ``sinks``, are seen; positions [tokens] int32 of q's tokens (at least as many as there are
+    tokens before q's; None: their places in the cache) are read only then. Returns out [tokens, hq, dim] in q's type and the log-sum-exp [tokens, hq] fp32; a token that sees nothing gets
     0 and -inf, as do tokens outside cu[0] .. cu[rows] - 1 and those of a request whose lengths are out of range (which ``err``
-    records). Tokens of a page outside the cache (recorded as well) are not seen. ``workspace`` (a uint8 tensor of ``attention_8bit_workspace(dim, tokens, hq)`` bytes, for one call at a time) is allocated when it
-    is not given."""
+    records). Tokens of a page outside the cache (recorded as well) are not seen. One kernel is taken for all requests, by their mean number
+    of new tokens: chunks of prompts and single tokens are faster in a call each. ``workspace`` (a uint8 tensor of
+    ``attention_8bit_workspace(dim, tokens, hq)`` bytes, for one call at a time) is allocated when it is not given."""
     return tensors().attention_8bit(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, max_new, mask, positions, window,
                                     sinks, workspace, err)
 
