@@ -208,7 +208,8 @@ __device__ __forceinline__ void append8_queries(const Append8Args& a, int first,
 }
 
 // Keys and values, one run of entries at a time: ones whose slots ascend within one block, with entries that are not kept between
-// them at most. (In a list that has others between, a block's entries are several runs, one after the other.) Warps take tokens and share their heads of K and V like those of queries:
+// them at most. (In a list that has others between, a block's entries are several runs, one after the other.) Warps take tokens and
+// share their heads of K and V like those of queries:
 //   1  the heads' bounds, joined in shared memory;
 //   2  the block's scales (from the run alone if it holds the block's first token, else at least what they were), rows that were
 //      there rounded to a risen scale;
